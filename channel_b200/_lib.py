@@ -66,6 +66,41 @@ class ChStreamStep(C.Structure):
                 ("active", P(u32)), ("sliding", P(u32)), ("n_active", u32), ("n_sliding", u32)]
 
 
+i64 = C.c_int64
+CH_F32, CH_F16, CH_BF16 = 0, 1, 2
+
+
+class ChPagePlanArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("lens", "new_tokens", "free_pages", "table", "lens_out", "starts", "slots",
+                                  "positions", "rows", "counts")] + \
+               [("table_stride", i64)] + \
+               [(n, u32) for n in ("n_streams", "table_cols", "n_free", "page_size", "max_tokens", "prefix_len")] + \
+               [("status", vp)]
+
+
+class ChKvWriteArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("k", "v", "k_pool", "v_pool", "slots")] + \
+               [(n, i64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride",
+                                   "page_stride", "token_stride", "head_stride")] + \
+               [(n, u32) for n in ("n_tokens", "n_kv", "head_dim", "page_size", "n_pages")] + \
+               [("src_dtype", C.c_int32), ("dst_dtype", C.c_int32), ("status", vp)]
+
+
+class ChPrefixAttnArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k_pool", "v_pool", "out", "prefix_table", "table", "lens")] + \
+               [(n, i64) for n in ("q_stream_stride", "q_head_stride", "out_stream_stride", "out_head_stride",
+                                   "page_stride", "token_stride", "head_stride", "table_stride")] + \
+               [(n, u32) for n in ("n_streams", "n_q", "n_kv", "head_dim", "page_size", "n_pages", "table_cols",
+                                   "prefix_len", "window")] + \
+               [("scale", f32), ("dtype", C.c_int32), ("status", vp)]
+
+
+class ChSampleRowsArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "uniform", "temperature", "top_p", "min_p", "top_k", "tokens", "kept",
+                                  "logprobs")] + \
+               [("row_stride", i64), ("n_rows", u32), ("vocab", u32), ("softcap", f32), ("dtype", C.c_int32)]
+
+
 PROGRESS_FN = C.CFUNCTYPE(None, sz, sz, vp)
 
 # name -> (restype, argtypes); every symbol declared in include/channel_cuda.h
@@ -156,6 +191,11 @@ SIGNATURES = {
     "ch_ring_dev_lists": (i32, [vp, u32, i32, sz, vp, vp, vp, vp, vp]),
     "ch_ring_dev_prefill_prev": (i32, [vp, u32, u32, vp, vp]),
     "ch_decode_run_ring": (i32, [vp, vp, vp, u32, u32, u32]),
+    "ch_page_plan": (i32, [P(ChPagePlanArgs), vp]),
+    "ch_paged_kv_write": (i32, [P(ChKvWriteArgs), vp]),
+    "ch_prefix_attention_workspace": (sz, [P(ChPrefixAttnArgs)]),
+    "ch_prefix_attention": (i32, [P(ChPrefixAttnArgs), vp, sz, vp]),
+    "ch_sample_rows": (i32, [P(ChSampleRowsArgs), vp]),
 }
 
 _lib = None

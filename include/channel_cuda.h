@@ -57,7 +57,8 @@ int ch_ctx_synchronize(ch_ctx *ctx);
 void *ch_ctx_stream(ch_ctx *ctx); /* cudaStream_t */
 /* Reads and clears the device status word (bit 0 bulk-copy wait timeout,
  * bit 1 bad slot, bit 2 bad slot-list entry, bit 3 peer wait timeout, bit 4 a Q4
- * block scale with |d| >= 16, outside the tensor-core GEMM's exact range). */
+ * block scale with |d| >= 16, outside the tensor-core GEMM's exact range, bit 5 a page
+ * plan that ran out of pages, table columns or token rows). */
 int ch_ctx_device_status(ch_ctx *ctx, uint32_t *flags);
 
 /* ------------------------------------------------------------------------
@@ -394,6 +395,110 @@ int ch_ring_dev_prefill_prev(ch_ring_dev *r, uint32_t start_clock, uint32_t chun
  * ch_decode_plan. */
 int ch_decode_run_ring(ch_model *m, ch_ring_dev *r, ch_ring *host, uint32_t first_token, uint32_t first_clock,
                        uint32_t n_steps);
+
+/* ------------------------------------------------------------------------
+ * Streams that share a prompt (no reference counterpart: the reference serves one
+ * stream).  K and V of a layer live in pools of pages, element (page, token, head, d) at
+ * page * page_stride + token * token_stride + head * head_stride + d; a stream owns the
+ * pages of its block-table row, and all streams share the pages of prefix_table in front.
+ * Every pointer is a device pointer.  The calls take no context: they run on the current
+ * device, asynchronously on `stream` (a cudaStream_t; NULL = default stream), allocate
+ * nothing, may be captured into a graph, and read all their arguments before they
+ * return.  status, if not NULL, is a device word into which bits of ch_ctx_device_status
+ * are ORed (never cleared); NULL discards them.
+ * ---------------------------------------------------------------------- */
+typedef enum { CH_F32 = 0, CH_F16 = 1, CH_BF16 = 2 } ch_dtype;
+
+/* Block tables and slot map of a step that appends new_tokens[b] >= 0 tokens to stream
+ * b, which holds lens[b] >= 0 of its own (n_streams <= 8192, page_size a power of two).
+ * Fresh pages are taken from free_pages in order, stream by stream:
+ *   table      (n_streams x table_cols, row stride table_stride; in place) columns
+ *              ceil(lens/page) .. ceil((lens+new)/page)-1 of each row get their pages
+ *   lens_out   [n_streams]     lens + new_tokens (not the same array as lens)
+ *   starts     [n_streams + 1] first packed token of each stream; the last is the total
+ *   slots, positions, rows [max_tokens]  per packed token: page * page_size + offset,
+ *              prefix_len + index in the stream, stream; -1 past the total
+ *   counts     [2]             packed tokens, pages taken
+ * Status bit 5: the pages, the table's columns or max_tokens did not suffice, or a length
+ * was negative (taken as 0).  A missing page is -1 in the table and its tokens' slots are
+ * -1, which ch_paged_kv_write skips; counts[1] still says how many pages were needed. */
+typedef struct {
+  const int32_t *lens, *new_tokens, *free_pages;
+  int32_t *table, *lens_out, *starts, *slots, *positions, *rows, *counts;
+  int64_t table_stride;
+  uint32_t n_streams, table_cols, n_free, page_size, max_tokens, prefix_len;
+  uint32_t *status;
+} ch_page_plan_args;
+int ch_page_plan(const ch_page_plan_args *args, void *stream);
+
+/* New K and V rows (element (t, head, d) at t * token_stride + head * head_stride + d of
+ * its tensor) into the pages: row t goes to slots[t]; a negative slot is skipped, one past
+ * n_pages * page_size too (status bit 1).  Slots of one call are distinct.  src_dtype
+ * CH_F32 (rounded to nearest) or dst_dtype; dst_dtype CH_F16 or CH_BF16.  Strides are
+ * multiples of 8 elements, k, v and the pools 16-byte aligned, head_dim % 8 == 0. */
+typedef struct {
+  const void *k, *v;
+  void *k_pool, *v_pool;
+  const int32_t *slots;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t page_stride, token_stride, head_stride;
+  uint32_t n_tokens, n_kv, head_dim, page_size, n_pages;
+  int32_t src_dtype, dst_dtype;
+  uint32_t *status;
+} ch_kv_write_args;
+int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
+
+/* Attention of one query token per stream: stream b's keys are the prefix_len shared
+ * tokens followed by its own lens[b]; with T = prefix_len + lens[b] it attends to
+ * positions [max(0, T - window), T) (window 0 = all), q head h to kv head
+ * h / (n_q / n_kv):  out = softmax(scale q.k) v, zeros when no position is visible.
+ * q / out element (b, head, d) at b * stream_stride + head * head_stride + d.
+ * head_dim 64, 128 or 256; n_q / n_kv at most 16; page_size a power of two from 8 to 256;
+ * dtype (of q, out and both pools) CH_F16 or CH_BF16, sums in f32.  Strides are multiples
+ * of 8 elements, q, out and the pools 16-byte aligned.  Positions whose page index is not
+ * in [0, n_pages) are left out (status bit 2), as are own positions past table_cols pages.
+ * The shared pages are read once for the whole batch.  workspace: at least
+ * ch_prefix_attention_workspace(args) bytes (0 when a size is invalid), 16-byte aligned,
+ * contents irrelevant; calls that may overlap need one each. */
+typedef struct {
+  const void *q, *k_pool, *v_pool;
+  void *out;
+  const int32_t *prefix_table, *table, *lens;
+  int64_t q_stream_stride, q_head_stride, out_stream_stride, out_head_stride;
+  int64_t page_stride, token_stride, head_stride, table_stride;
+  uint32_t n_streams, n_q, n_kv, head_dim, page_size, n_pages, table_cols, prefix_len, window;
+  float scale;
+  int32_t dtype;
+  uint32_t *status;
+} ch_prefix_attn_args;
+size_t ch_prefix_attention_workspace(const ch_prefix_attn_args *args);
+int ch_prefix_attention(const ch_prefix_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token per row of logits (n_rows x vocab, vocab <= 262144, row stride row_stride
+ * elements).  With x = softcap * tanh(logit / softcap) (softcap 0: the logit; NaN counts
+ * as -inf), m = max x, T = temperature[row], token i weighs e_i = exp((x_i - m) / T),
+ * held as floor(2^44 e_i); tokens of weight 0 are never drawn.  Kept are, in the order of
+ * falling e (equal ones by index):  e_i >= min_p (and every e_i = 1);  of those the first
+ * top_k (0 = all);  of those the first whose weights before them sum to less than top_p of
+ * the whole (top_p >= 1 = all).  The row's token is the first kept one, in index order, at
+ * which the running sum of weights exceeds uniform[row] * sum, uniform in [0, 1).
+ * T <= 0: the lowest index of the largest x.  temperature NULL = 1, top_k / top_p / min_p
+ * NULL = off.  logprobs (may be NULL): log of the token's share of the kept weight, 0 when
+ * greedy; kept (may be NULL): how many tokens were kept.  A row without a finite or +inf
+ * logit gives token -1, logprob -inf, kept 0.  The sums are exact integers: the result
+ * does not depend on how the work is split. */
+typedef struct {
+  const void *logits;
+  const float *uniform, *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  int32_t *tokens, *kept;
+  float *logprobs;
+  int64_t row_stride;
+  uint32_t n_rows, vocab;
+  float softcap;
+  int32_t dtype;
+} ch_sample_rows_args;
+int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
 
 #ifdef __cplusplus
 }
