@@ -15,8 +15,6 @@ namespace ch {
 int set_last_error(int code, const std::string &msg);
 
 namespace {
-constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
-
 struct PrefixArgs {
   const void *q, *k, *v;
   void *out;
@@ -24,90 +22,479 @@ struct PrefixArgs {
   long long qs, qh, os, oh;
   long long page, token, head, ts;
   uint32_t n, nq, nkv, group, shift, n_pages, cols, prefix, window;
+  uint32_t from;  // first position read stream by stream
   float scale;
   uint32_t *status;
 };
 
 CH_DEV float to_f32(__half v) { return __half2float(v); }
 CH_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-CH_DEV T from_f32(float v);
-template <>
-CH_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-CH_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 // own tokens of stream b, limited to what its table can hold
 CH_DEV uint32_t own_len(const PrefixArgs &a, uint32_t b) {
-  const int32_t len = a.lens[b];
-  if (len <= 0) return 0;
-  return (uint32_t)min((unsigned long long)len, (unsigned long long)a.cols << a.shift);
+  const long long len = a.lens[b];
+  return (uint32_t)min(max(len, 0ll), (long long)a.cols << a.shift);
 }
 
-// One (stream, q head) per CTA, a warp per key in turn: the plain form, no sharing.
-template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const PrefixArgs a) {
-  constexpr int EPL = D / 32;
-  __shared__ float s_o[kRowWarps][D], s_m[kRowWarps], s_l[kRowWarps];
-  const uint32_t b = blockIdx.y, h = blockIdx.x, kvh = h / a.group;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T *q = static_cast<const T *>(a.q) + b * a.qs + h * a.qh;
-  const T *kp = static_cast<const T *>(a.k) + kvh * a.head, *vp = static_cast<const T *>(a.v) + kvh * a.head;
-  float qr[EPL], o[EPL], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[lane * EPL + e]) * a.scale, o[e] = 0.f;
-  const unsigned long long end = (unsigned long long)a.prefix + own_len(a, b);
-  const unsigned long long begin = a.window && end > a.window ? end - a.window : 0;
-  for (unsigned long long j = begin + warp; j < end; j += kRowWarps) {
-    const bool shared = j < a.prefix;
-    const uint32_t i = (uint32_t)(shared ? j : j - a.prefix);
-    const int32_t page = shared ? a.prefix_table[i >> a.shift] : a.table[b * a.ts + (i >> a.shift)];
-    if (page < 0 || (uint32_t)page >= a.n_pages) {
-      if (lane == 0 && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
-      continue;
-    }
-    const long long at = page * a.page + (long long)(i & ((1u << a.shift) - 1)) * a.token + lane * EPL;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < EPL; e++) s = fmaf(qr[e], to_f32(kp[at + e]), s);
-    s = warp_sum(s);
-    if (s == -INFINITY) continue;
-    const float m1 = fmaxf(m, s), c = expf(m - m1), p = expf(s - m1);
-    l = l * c + p;
-#pragma unroll
-    for (int e = 0; e < EPL; e++) o[e] = fmaf(p, to_f32(vp[at + e]), o[e] * c);
-    m = m1;
+CH_DEV void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+CH_DEV void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+CH_DEV uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+CH_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const __half *) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const __nv_bfloat16 *) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+CH_DEV uint32_t pack2(float lo, float hi, const __half *) { return pack_half2(__float2half_rn(lo), __float2half_rn(hi)); }
+CH_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16 *) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// positions stream b attends to: [lo, hi)
+CH_DEV void visible(const PrefixArgs &a, uint32_t b, uint32_t &lo, uint32_t &hi) {
+  hi = a.prefix + own_len(a, b);  // both below 2^31
+  lo = a.window && hi > a.window ? hi - a.window : 0u;
+}
+// page and row inside it of position j of stream b; -1 when the page is not in the pool
+CH_DEV int32_t page_of(const PrefixArgs &a, uint32_t b, uint32_t j, uint32_t &row) {
+  const bool shared = j < a.prefix;
+  const uint32_t i = shared ? j : j - a.prefix;
+  row = i & ((1u << a.shift) - 1);
+  const int32_t page = shared ? a.prefix_table[i >> a.shift] : a.table[b * a.ts + (i >> a.shift)];
+  if (page < 0 || (uint32_t)page >= a.n_pages) {
+    if (a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
+    return -1;
   }
+  return page;
+}
+
+// ---------------------------------------------------------------------------
+// Positions read stream by stream.  HBM-bound: each K and V row is used by the `group`
+// query rows of its kv head only, so what counts is bytes in flight.  A warp is a unit of
+// its own: it takes an equal run of the 16-key tiles of all (stream, kv head) pairs, laid
+// end to end, and streams them through a private ring of row copies (lane l < 16 copies K
+// row l of a tile, lane 16 + l its V row), so no barrier couples the warps and tiles of the
+// next pair are in flight while one pair ends.  A tile takes
+//   S^T (16 keys x 8 rows) = K (16 x D) Q^T,   O^T (D x 8 rows) += V^T (D x 16 keys) P^T,
+// with K and V as the 16-row A operand of mma.m16n8k16 (the query rows, at most 8 or 16, are
+// its narrow side) and P^T from S^T by two 8 x 8 register transposes.  P is rounded to the
+// type of V (what the tensor core takes); its sum is kept in f32 before rounding.  The
+// running maximum, in units of log2, is per warp; each cut pair leaves (O, m, l) in the
+// workspace and attend_join_kernel adds the parts.
+constexpr uint32_t kTile = 16;  // keys
+template <int D>
+struct Own {
+  static constexpr int kWarps = D == 256 ? 4 : 8;
+  static constexpr int kStages = D == 64 ? 5 : 3;
+  static constexpr uint32_t kPitch = D * 2 + 16;  // 8 rows of a fragment load hit distinct banks
+  static constexpr uint32_t kStage = 2 * kTile * kPitch;
+  static constexpr uint32_t kRing = kWarps * kStages * kStage;
+};
+constexpr uint32_t kMaxStreams = 4096;
+
+struct Work {      // in the caller's workspace
+  uint32_t *start; // [n + 1] first tile of a stream, per kv head; [n + 1]: tiles per warp
+  float *o;        // [segments][group][D]; segment = warp + pair, pair = stream * n_kv + head
+  float2 *ml;      // [segments][group]: maximum, sum
+  uint32_t warps;  // of the whole grid
+};
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(const PrefixArgs a, const Work w) {
+  using O = Own<D>;
+  constexpr int kThreads = O::kWarps * 32, kSteps = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint32_t *start = reinterpret_cast<uint32_t *>(smem + O::kRing);  // [n + 1]
+  __shared__ __align__(8) uint64_t bars[O::kWarps][O::kStages];
+  __shared__ uint32_t masks[O::kWarps][O::kStages], sums[O::kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+
+  // ---- tiles per stream, summed over the streams ----
+  const uint32_t per_thread = (a.n + kThreads - 1) / kThreads, b0 = min(a.n, tid * per_thread), b1 = min(a.n, b0 + per_thread);
+  auto tiles_of = [&](uint32_t b) {
+    uint32_t lo, hi;
+    visible(a, b, lo, hi);
+    lo = max(lo, a.from);
+    return hi > lo ? (hi - lo + kTile - 1) / kTile : 0u;
+  };
+  uint32_t mine = 0;
+  for (uint32_t b = b0; b < b1; b++) mine += tiles_of(b);
+  uint32_t inc = mine;
 #pragma unroll
-  for (int e = 0; e < EPL; e++) s_o[warp][lane * EPL + e] = o[e];
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) sums[warp] = inc;
+  if (lane < O::kStages) mbar_init(&bars[warp][lane], 1);
+  fence_mbar_init();
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kRowWarps; w++) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < kRowWarps; w++)
-    if (s_m[w] != -INFINITY) sum += s_l[w] * expf(s_m[w] - top);
-  T *out = static_cast<T *>(a.out) + b * a.os + h * a.oh;
-  for (int d = threadIdx.x; d < D; d += kRowThreads) {
-    float v = 0.f;
-    for (int w = 0; w < kRowWarps; w++)
-      if (s_m[w] != -INFINITY) v += s_o[w][d] * expf(s_m[w] - top);
-    out[d] = from_f32<T>(sum == 0.f ? 0.f : v / sum);
+  uint32_t at = inc - mine, all = 0;
+  for (int k = 0; k < O::kWarps; k++) {
+    if (k < warp) at += sums[k];
+    all += sums[k];
+  }
+  for (uint32_t b = b0; b < b1; b++) {
+    start[b] = at;
+    at += tiles_of(b);
+  }
+  if (tid == 0) start[a.n] = all;
+  // 64-bit: n_kv times the tiles of all streams
+  const unsigned long long total = (unsigned long long)all * a.nkv;
+  const uint32_t per = (uint32_t)max(1ull, (total + w.warps - 1) / w.warps);
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (uint32_t b = tid; b <= a.n; b += kThreads) w.start[b] = start[b];
+    if (tid == 0) w.start[a.n + 1] = per;
+  }
+  grid_dep_launch();
+
+  // consecutive runs go to different SMs, so that few tiles spread over all of them
+  const uint32_t wid = warp * gridDim.x + blockIdx.x;
+  const unsigned long long first = (unsigned long long)wid * per;
+  if (first >= total) return;
+  uint32_t left = (uint32_t)min((unsigned long long)per, total - first);
+
+  struct Cursor {
+    uint32_t b, h, i, tiles, lo, hi;
+  };
+  auto enter = [&](Cursor &c) {  // the stream's bounds
+    visible(a, c.b, c.lo, c.hi);
+    c.lo = max(c.lo, a.from);
+    c.tiles = start[c.b + 1] - start[c.b];
+  };
+  Cursor ld;
+  {
+    uint32_t lo = 0, hi = a.n;
+    while (lo + 1 < hi) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if ((unsigned long long)start[mid] * a.nkv <= first) lo = mid; else hi = mid;
+    }
+    ld.b = lo;
+    while (start[ld.b + 1] == start[ld.b]) ld.b++;
+    enter(ld);
+    const uint32_t rem = (uint32_t)(first - (unsigned long long)start[ld.b] * a.nkv);
+    ld.h = rem / ld.tiles;
+    ld.i = rem % ld.tiles;
+  }
+  auto advance = [&](Cursor &c) {
+    if (++c.i < c.tiles) return;
+    c.i = 0;
+    if (++c.h < a.nkv) return;
+    c.h = 0;
+    do c.b++;
+    while (c.b < a.n && start[c.b + 1] == start[c.b]);
+    if (c.b < a.n) enter(c);
+  };
+  Cursor cu = ld;
+  uint8_t *ring = smem + warp * O::kStages * O::kStage;
+  const T *pool = static_cast<const T *>(lane < 16 ? a.k : a.v);
+  uint32_t to_load = left;
+  uint32_t row = 0;
+  auto look_up = [&]() {
+    const uint32_t j = ld.lo + ld.i * kTile + (lane & 15);
+    return j < ld.hi ? page_of(a, ld.b, j, row) : -1;
+  };
+  int32_t page = look_up();
+  auto issue = [&](int s) {
+    uint8_t *dst = ring + s * O::kStage + lane * O::kPitch;
+    const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+    if (page < 0) {  // not copied: zeros, so that a weight of 0 meets no stale bits
+      for (uint32_t c = 0; c < D * 2; c += 16) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+    }
+    if (lane == 0) {
+      masks[warp][s] = have & 0xFFFFu;
+      mbar_arrive_expect_tx(&bars[warp][s], __popc(have) * D * 2);
+    }
+    __syncwarp();
+    if (page >= 0)
+      bulk_g2s(dst, pool + page * a.page + (long long)row * a.token + ld.h * a.head, D * 2, &bars[warp][s]);
+    to_load--;
+    if (to_load) {
+      advance(ld);
+      page = look_up();
+    }
+  };
+  for (int s = 0; s < O::kStages; s++)
+    if (to_load) issue(s);
+
+  uint32_t qf[NR][kSteps][2];
+  float o[NR][kSteps][4], m[NR][2], l[NR][2];
+  const float scale2 = a.scale * 1.44269504088896341f;
+  const T *tag = nullptr;
+  bool fresh = true;
+  const uint32_t frag = smem_u32(ring);
+  // fragment addresses of this lane: K rows by key, V columns by key
+  const uint32_t k_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * O::kPitch + (lane >> 4) * 16;
+  const uint32_t v_at = (kTile + (lane & 7) + (lane >> 4) * 8) * O::kPitch + ((lane >> 3) & 1) * 16;
+  int stage = 0;
+  uint32_t parity = 0;
+  for (; left; left--) {
+    if (fresh) {  // the pair's query rows and empty sums
+      fresh = false;
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+        const uint32_t qr = r * 8 + g;
+        const T *q = static_cast<const T *>(a.q) + cu.b * a.qs + (cu.h * a.group + qr) * a.qh + 2 * t4;
+#pragma unroll
+        for (int k = 0; k < kSteps; k++) {
+          qf[r][k][0] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k) : 0u;
+          qf[r][k][1] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8) : 0u;
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[r][k][e] = 0.f;
+        }
+        m[r][0] = m[r][1] = -INFINITY;
+        l[r][0] = l[r][1] = 0.f;
+      }
+    }
+    const bool ok = mbar_wait_bounded(&bars[warp][stage], parity, a.status);
+    if (!__all_sync(0xffffffffu, ok)) {  // reported; the copies still in flight get a wait of their own
+      for (int k = 1; k < O::kStages && (uint32_t)k < left; k++) {
+        if (++stage == O::kStages) stage = 0, parity ^= 1;
+        mbar_wait_bounded(&bars[warp][stage], parity, a.status);
+      }
+      return;
+    }
+    const uint32_t base = frag + stage * O::kStage, mask = masks[warp][stage];
+    float s[NR][2][4];
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[r][0][e] = s[r][1][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; k++) {
+      uint32_t f[4];
+      ldsm_x4(base + k_at + k * 32, f);
+#pragma unroll
+      for (int r = 0; r < NR; r++) mma16(s[r][k & 1], f, qf[r][k][0], qf[r][k][1], tag);
+    }
+    const bool on0 = (mask >> g) & 1, on1 = (mask >> (g + 8)) & 1;
+    uint32_t p[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+#pragma unroll
+      for (int c = 0; c < 2; c++) {  // query row r * 8 + 2 * t4 + c, keys g and g + 8
+        const float s0 = on0 ? (s[r][0][c] + s[r][1][c]) * scale2 : -INFINITY;
+        const float s1 = on1 ? (s[r][0][c + 2] + s[r][1][c + 2]) * scale2 : -INFINITY;
+        float top = fmaxf(s0, s1);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float m1 = fmaxf(m[r][c], top), ref = m1 == -INFINITY ? 0.f : m1;
+        const float keep = exp2_approx(m[r][c] - ref);
+        m[r][c] = m1;
+        const float p0 = exp2_approx(s0 - ref), p1 = exp2_approx(s1 - ref);
+        l[r][c] = l[r][c] * keep + (p0 + p1);
+        s[r][0][c] = p0;
+        s[r][0][c + 2] = p1;
+        s[r][1][c] = keep;
+      }
+      p[r][0] = transpose8x8(pack2(s[r][0][0], s[r][0][1], tag));
+      p[r][1] = transpose8x8(pack2(s[r][0][2], s[r][0][3], tag));
+      if (__any_sync(0xffffffffu, s[r][1][0] != 1.f || s[r][1][1] != 1.f)) {
+#pragma unroll
+        for (int k = 0; k < kSteps; k++) {
+          o[r][k][0] *= s[r][1][0], o[r][k][1] *= s[r][1][1];
+          o[r][k][2] *= s[r][1][0], o[r][k][3] *= s[r][1][1];
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; k++) {
+      uint32_t f[4];
+      ldsm_x4_trans(base + v_at + k * 32, f);
+#pragma unroll
+      for (int r = 0; r < NR; r++) mma16(o[r][k], f, p[r][0], p[r][1], tag);
+    }
+    __syncwarp();
+    if (to_load) issue(stage);
+    if (++stage == O::kStages) stage = 0, parity ^= 1;
+
+    if (cu.i + 1 == cu.tiles || left == 1) {  // the pair, or this warp's run, ends
+      const unsigned long long seg = (unsigned long long)wid + cu.b * a.nkv + cu.h;
+      float *po = w.o + seg * a.group * D;
+      float2 *pm = w.ml + seg * a.group;
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float sum = l[r][c];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          const uint32_t qr = r * 8 + 2 * t4 + c;
+          if (qr >= a.group) continue;
+          if (g == 0) pm[qr] = make_float2(m[r][c], sum);
+#pragma unroll
+          for (int k = 0; k < kSteps; k++) {
+            po[qr * D + 16 * k + g] = o[r][k][c];
+            po[qr * D + 16 * k + 8 + g] = o[r][k][c + 2];
+          }
+        }
+      }
+      fresh = true;
+    }
+    advance(cu);
   }
 }
 
+// ---------------------------------------------------------------------------
+// out = sum over a row's parts of O 2^(m - M) / sum of l 2^(m - M); a warp per query row.
+// A weight of 0 times a non-finite V at a masked position of the same tile is NaN, so a row
+// that is not finite is computed again on its own, key by key, from its visible positions
+// only (ordinary rows never take this path).
+constexpr int kJoinWarps = 4;
 template <typename T, int D>
-cudaError_t launch_t(const PrefixArgs &a, cudaStream_t s) {
-  attend_row_kernel<T, D><<<dim3(a.nq, a.n), kRowThreads, 0, s>>>(a);
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const PrefixArgs a, const Work w) {
+  constexpr int EPL = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = blockIdx.x * kJoinWarps + warp;
+  if (row >= a.n * a.nq) return;
+  const uint32_t b = row / a.nq, hq = row % a.nq, h = hq / a.group, r = hq % a.group;
+  grid_dep_wait();
+  const uint32_t s0 = w.start[b], tiles = w.start[b + 1] - s0, per = w.start[a.n + 1];
+  const unsigned long long t0 = (unsigned long long)s0 * a.nkv + (unsigned long long)h * tiles;
+  const uint32_t w0 = (uint32_t)(t0 / per), parts = tiles ? (uint32_t)((t0 + tiles - 1) / per) - w0 + 1 : 0u;
+  const unsigned long long seg0 = (unsigned long long)w0 + b * a.nkv + h;
+  const float2 *ml = w.ml + seg0 * a.group + r;
+  const float *po = w.o + (seg0 * a.group + r) * D + lane * EPL;
+  float top = -INFINITY;
+  for (uint32_t p = lane; p < parts; p += 32) top = fmaxf(top, ml[(size_t)p * a.group].x);
+  top = warp_max(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float o[EPL], sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; e++) o[e] = 0.f;
+  for (uint32_t p = 0; p < parts; p++) {
+    const float2 v = ml[(size_t)p * a.group];
+    const float f = exp2_approx(v.x - ref);
+    sum = fmaf(v.y, f, sum);
+    const float *src = po + (size_t)p * a.group * D;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = fmaf(src[e], f, o[e]);
+  }
+  bool bad = !isfinite(sum);
+#pragma unroll
+  for (int e = 0; e < EPL; e++) {
+    o[e] = sum == 0.f ? 0.f : o[e] / sum;
+    bad |= !isfinite(o[e]);
+  }
+  if (__any_sync(0xffffffffu, bad)) {
+    const T *q = static_cast<const T *>(a.q) + b * a.qs + hq * a.qh + lane * EPL;
+    float qr[EPL], m = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[e]), o[e] = 0.f;
+    uint32_t lo, hi;
+    visible(a, b, lo, hi);
+    for (uint32_t j = lo; j < hi; j++) {
+      uint32_t in_page;
+      const int32_t page = page_of(a, b, j, in_page);
+      if (page < 0) continue;
+      const long long at = page * a.page + (long long)in_page * a.token + h * a.head + lane * EPL;
+      const T *k = static_cast<const T *>(a.k) + at, *v = static_cast<const T *>(a.v) + at;
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; e++) s = fmaf(qr[e], to_f32(k[e]), s);
+      s = warp_sum(s) * a.scale;
+      if (s == -INFINITY) continue;
+      const float m1 = fmaxf(m, s), c = expf(m - m1), p = expf(s - m1);
+      sum = sum * c + p;
+#pragma unroll
+      for (int e = 0; e < EPL; e++) o[e] = fmaf(p, to_f32(v[e]), o[e] * c);
+      m = m1;
+    }
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = sum == 0.f ? 0.f : o[e] / sum;
+  }
+  T *out = static_cast<T *>(a.out) + b * a.os + hq * a.oh + lane * EPL;
+  uint32_t packed[EPL / 2];
+#pragma unroll
+  for (int e = 0; e < EPL / 2; e++) packed[e] = pack2(o[2 * e], o[2 * e + 1], static_cast<const T *>(nullptr));
+  if constexpr (EPL == 8)
+    *reinterpret_cast<uint4 *>(out) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  else if constexpr (EPL == 4)
+    *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
+  else
+    *reinterpret_cast<uint32_t *>(out) = packed[0];
+}
+
+// workspace: w.start | w.ml | w.o
+uint32_t own_grid() { return (uint32_t)num_sms(); }
+uint32_t own_warps(uint32_t D) { return own_grid() * (D == 256 ? Own<256>::kWarps : Own<128>::kWarps); }
+static_assert(Own<64>::kWarps == Own<128>::kWarps, "own_warps");
+size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w) {
+  const uint32_t warps = own_warps(p->head_dim);
+  const size_t rows = ((size_t)warps + (size_t)p->n_streams * p->n_kv) * (p->n_q / p->n_kv);
+  size_t at = 0;
+  w->warps = warps;
+  w->start = reinterpret_cast<uint32_t *>(base);
+  at += aligned(((size_t)p->n_streams + 2) * sizeof(uint32_t));
+  w->ml = reinterpret_cast<float2 *>(base + at);
+  at += aligned(rows * sizeof(float2));
+  w->o = reinterpret_cast<float *>(base + at);
+  at += aligned(rows * p->head_dim * sizeof(float));
+  return at;
+}
+
+template <typename T, int D, int NR>
+cudaError_t launch_own(const PrefixArgs &a, const Work &w, cudaStream_t s) {
+  const size_t smem = Own<D>::kRing + ((size_t)a.n + 1) * sizeof(uint32_t);
+  const auto kernel = attend_own_kernel<T, D, NR>;
+  cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<own_grid(), Own<D>::kWarps * 32, smem, s>>>(a, w);
   return cudaGetLastError();
 }
+
+template <typename T, int D>
+cudaError_t launch_t(const PrefixArgs &a, const Work &w, cudaStream_t s) {
+  cudaError_t e = a.group <= 8 ? launch_own<T, D, 1>(a, w, s) : launch_own<T, D, 2>(a, w, s);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.n * a.nq + kJoinWarps - 1) / kJoinWarps);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D>, a, w);
+}
 template <typename T>
-cudaError_t launch(const PrefixArgs &a, uint32_t D, cudaStream_t s) {
-  return D == 64 ? launch_t<T, 64>(a, s) : D == 128 ? launch_t<T, 128>(a, s) : launch_t<T, 256>(a, s);
+cudaError_t launch(const PrefixArgs &a, const Work &w, uint32_t D, cudaStream_t s) {
+  return D == 64 ? launch_t<T, 64>(a, w, s) : D == 128 ? launch_t<T, 128>(a, w, s) : launch_t<T, 256>(a, w, s);
 }
 
 const char *check(const ch_prefix_attn_args *p) {
   if (!p) return "args is NULL";
-  if (p->n_streams > 65535) return "at most 65535 streams";
+  if (p->n_streams > kMaxStreams) return "at most 4096 streams";
   if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return "head_dim must be 64, 128 or 256";
   if (p->n_kv == 0 || p->n_q == 0 || p->n_q % p->n_kv || p->n_q / p->n_kv > 16)
     return "n_q must be n_kv times 1..16";
@@ -116,6 +503,8 @@ const char *check(const ch_prefix_attn_args *p) {
     return "page_size must be a power of two from 8 to 256";
   if (p->n_pages > 0x7FFFFFFFu || p->table_cols > 0x7FFFFFFFu || p->prefix_len > 0x7FFFFFFFu)
     return "a size is 2^31 or more";
+  const unsigned long long reach = p->prefix_len + (unsigned long long)p->table_cols * p->page_size;
+  if (reach >= 1ull << 32 || (reach / 16 + 1) * p->n_streams >= 1ull << 32) return "the positions of all streams exceed 2^36";
   if (p->dtype != CH_F16 && p->dtype != CH_BF16) return "dtype must be CH_F16 or CH_BF16";
   return nullptr;
 }
@@ -162,9 +551,12 @@ int prefix_attention(const ch_prefix_attn_args *p, void *workspace, size_t bytes
   a.window = p->window;
   a.scale = p->scale;
   a.status = p->status;
+  a.from = 0;
+  Work w;
+  carve(p, static_cast<uint8_t *>(workspace), &w);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
-      p->dtype == CH_F16 ? launch<__half>(a, p->head_dim, s) : launch<__nv_bfloat16>(a, p->head_dim, s);
+      p->dtype == CH_F16 ? launch<__half>(a, w, p->head_dim, s) : launch<__nv_bfloat16>(a, w, p->head_dim, s);
   if (e != cudaSuccess) return set_last_error(CH_ECUDA, std::string("prefix_attention: ") + cudaGetErrorString(e));
   return CH_OK;
 }
@@ -173,7 +565,8 @@ int prefix_attention(const ch_prefix_attn_args *p, void *workspace, size_t bytes
 
 extern "C" size_t ch_prefix_attention_workspace(const ch_prefix_attn_args *args) {
   if (ch::check(args)) return 0;
-  return 0;
+  ch::Work w;
+  return ch::carve(args, nullptr, &w);
 }
 extern "C" int ch_prefix_attention(const ch_prefix_attn_args *args, void *workspace, size_t workspace_bytes,
                                    void *stream) {
