@@ -3,38 +3,16 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - m),
 // over the visible positions j; m is the running maximum, and sums are f32.
-#include <cuda_bf16.h>
-
 #include <string>
+#include <type_traits>
 
 #include "../../include/channel_cuda.h"
-#include "common.cuh"
-#include "kernels.cuh"
+#include "prefix_attn.cuh"
 
 namespace ch {
 int set_last_error(int code, const std::string &msg);
 
 namespace {
-struct PrefixArgs {
-  const void *q, *k, *v;
-  void *out;
-  const int32_t *prefix_table, *table, *lens;
-  long long qs, qh, os, oh;
-  long long page, token, head, ts;
-  uint32_t n, nq, nkv, group, shift, n_pages, cols, prefix, window;
-  uint32_t from;  // first position read stream by stream
-  float scale;
-  uint32_t *status;
-};
-
-CH_DEV float to_f32(__half v) { return __half2float(v); }
-CH_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-// own tokens of stream b, limited to what its table can hold
-CH_DEV uint32_t own_len(const PrefixArgs &a, uint32_t b) {
-  const long long len = a.lens[b];
-  return (uint32_t)min(max(len, 0ll), (long long)a.cols << a.shift);
-}
-
 CH_DEV void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -52,11 +30,6 @@ CH_DEV uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-CH_DEV float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const __half *) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -69,30 +42,6 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-CH_DEV uint32_t pack2(float lo, float hi, const __half *) { return pack_half2(__float2half_rn(lo), __float2half_rn(hi)); }
-CH_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16 *) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
-
-// positions stream b attends to: [lo, hi)
-CH_DEV void visible(const PrefixArgs &a, uint32_t b, uint32_t &lo, uint32_t &hi) {
-  hi = a.prefix + own_len(a, b);  // both below 2^31
-  lo = a.window && hi > a.window ? hi - a.window : 0u;
-}
-// page and row inside it of position j of stream b; -1 when the page is not in the pool
-CH_DEV int32_t page_of(const PrefixArgs &a, uint32_t b, uint32_t j, uint32_t &row) {
-  const bool shared = j < a.prefix;
-  const uint32_t i = shared ? j : j - a.prefix;
-  row = i & ((1u << a.shift) - 1);
-  const int32_t page = shared ? a.prefix_table[i >> a.shift] : a.table[b * a.ts + (i >> a.shift)];
-  if (page < 0 || (uint32_t)page >= a.n_pages) {
-    if (a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
-    return -1;
-  }
-  return page;
-}
-
 // ---------------------------------------------------------------------------
 // Positions read stream by stream.  HBM-bound: each K and V row is used by the `group`
 // query rows of its kv head only, so what counts is bytes in flight.  A warp is a unit of
@@ -177,7 +126,10 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
   // consecutive runs go to different SMs, so that few tiles spread over all of them
   const uint32_t wid = warp * gridDim.x + blockIdx.x;
   const unsigned long long first = (unsigned long long)wid * per;
-  if (first >= total) return;
+  if (first >= total) {
+    grid_dep_wait();
+    return;
+  }
   uint32_t left = (uint32_t)min((unsigned long long)per, total - first);
 
   struct Cursor {
@@ -360,6 +312,7 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
     }
     advance(cu);
   }
+  grid_dep_wait();  // the join waits for this kernel, and through it for the prefix kernel
 }
 
 // ---------------------------------------------------------------------------
@@ -369,34 +322,68 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
 // only (ordinary rows never take this path).
 constexpr int kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const PrefixArgs a, const Work w) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const PrefixArgs a, const Work w, const PrefixParts pp) {
   constexpr int EPL = D / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t row = blockIdx.x * kJoinWarps + warp;
   if (row >= a.n * a.nq) return;
   const uint32_t b = row / a.nq, hq = row % a.nq, h = hq / a.group, r = hq % a.group;
   grid_dep_wait();
+  // the row's parts: one per split of the shared prefix, then one per warp whose run touched
+  // the pair (b, h)
   const uint32_t s0 = w.start[b], tiles = w.start[b + 1] - s0, per = w.start[a.n + 1];
   const unsigned long long t0 = (unsigned long long)s0 * a.nkv + (unsigned long long)h * tiles;
-  const uint32_t w0 = (uint32_t)(t0 / per), parts = tiles ? (uint32_t)((t0 + tiles - 1) / per) - w0 + 1 : 0u;
-  const unsigned long long seg0 = (unsigned long long)w0 + b * a.nkv + h;
-  const float2 *ml = w.ml + seg0 * a.group + r;
-  const float *po = w.o + (seg0 * a.group + r) * D + lane * EPL;
+  const uint32_t w0 = (uint32_t)(t0 / per), own = tiles ? (uint32_t)((t0 + tiles - 1) / per) - w0 + 1 : 0u;
+  const size_t rows = (size_t)a.n * a.group, at_prefix = (size_t)h * rows + (size_t)b * a.group + r;
+  const size_t at_own = ((size_t)w0 + (size_t)b * a.nkv + h) * a.group + r;
+  const uint32_t parts = pp.splits + own;
+  auto ml_of = [&](uint32_t p) {
+    return p < pp.splits ? pp.ml[at_prefix + (size_t)p * a.nkv * rows] : w.ml[at_own + (size_t)(p - pp.splits) * a.group];
+  };
+  auto o_of = [&](uint32_t p) {
+    return (p < pp.splits ? pp.o + (at_prefix + (size_t)p * a.nkv * rows) * D
+                          : w.o + (at_own + (size_t)(p - pp.splits) * a.group) * D) + lane * EPL;
+  };
   float top = -INFINITY;
-  for (uint32_t p = lane; p < parts; p += 32) top = fmaxf(top, ml[(size_t)p * a.group].x);
+  for (uint32_t p = lane; p < parts; p += 32) top = fmaxf(top, ml_of(p).x);
   top = warp_max(top);
   const float ref = top == -INFINITY ? 0.f : top;
   float o[EPL], sum = 0.f;
 #pragma unroll
   for (int e = 0; e < EPL; e++) o[e] = 0.f;
-  for (uint32_t p = 0; p < parts; p++) {
-    const float2 v = ml[(size_t)p * a.group];
-    const float f = exp2_approx(v.x - ref);
-    sum = fmaf(v.y, f, sum);
-    const float *src = po + (size_t)p * a.group * D;
+  for (uint32_t p0 = 0; p0 < parts; p0 += 32) {
+    const uint32_t n = min(32u, parts - p0);
+    float f = 0.f;
+    if ((uint32_t)lane < n) {
+      const float2 v = ml_of(p0 + lane);
+      f = exp2_approx(v.x - ref);
+      sum = fmaf(v.y, f, sum);
+    }
+    constexpr uint32_t kU = 4;  // parts whose loads are in flight together
+    for (uint32_t k = 0; k < n; k += kU) {
+      float v[kU][EPL], fk[kU];
 #pragma unroll
-    for (int e = 0; e < EPL; e++) o[e] = fmaf(src[e], f, o[e]);
+      for (uint32_t u = 0; u < kU; u++) {
+        fk[u] = __shfl_sync(0xffffffffu, f, (k + u) & 31);
+        if (k + u >= n) fk[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) v[u][e] = 0.f;
+        if (fk[u] == 0.f) continue;  // a part without a visible position has no O
+        const float *src = o_of(p0 + k + u);
+        if constexpr (EPL == 2) {
+          *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4 *>(&v[u][e]) = *reinterpret_cast<const float4 *>(src + e);
+        }
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kU; u++)
+#pragma unroll
+        for (int e = 0; e < EPL; e++) o[e] = fmaf(v[u][e], fk[u], o[e]);
+    }
   }
+  sum = warp_sum(sum);
   bool bad = !isfinite(sum);
 #pragma unroll
   for (int e = 0; e < EPL; e++) {
@@ -443,12 +430,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
     *reinterpret_cast<uint32_t *>(out) = packed[0];
 }
 
-// workspace: w.start | w.ml | w.o
+// The shared prefix has its own kernel when more than one stream can share it.
+bool shares(const ch_prefix_attn_args *p) { return p->prefix_len > 0 && p->n_streams > 1; }
+
+// workspace: w.start | w.ml | w.o | the prefix's ml | o
 uint32_t own_grid() { return (uint32_t)num_sms(); }
 uint32_t own_warps(uint32_t D) { return own_grid() * (D == 256 ? Own<256>::kWarps : Own<128>::kWarps); }
 static_assert(Own<64>::kWarps == Own<128>::kWarps, "own_warps");
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
-size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w) {
+size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w, PrefixParts *pp) {
   const uint32_t warps = own_warps(p->head_dim);
   const size_t rows = ((size_t)warps + (size_t)p->n_streams * p->n_kv) * (p->n_q / p->n_kv);
   size_t at = 0;
@@ -459,37 +449,54 @@ size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w) {
   at += aligned(rows * sizeof(float2));
   w->o = reinterpret_cast<float *>(base + at);
   at += aligned(rows * p->head_dim * sizeof(float));
+  pp->splits = shares(p) ? prefix_tc_splits(p->prefix_len, p->n_streams, p->n_q / p->n_kv, p->n_kv) : 0;
+  const size_t shared = (size_t)pp->splits * p->n_streams * p->n_q;
+  pp->ml = reinterpret_cast<float2 *>(base + at);
+  at += aligned(shared * sizeof(float2));
+  pp->o = reinterpret_cast<float *>(base + at);
+  at += aligned(shared * p->head_dim * sizeof(float));
   return at;
 }
 
-template <typename T, int D, int NR>
-cudaError_t launch_own(const PrefixArgs &a, const Work &w, cudaStream_t s) {
-  const size_t smem = Own<D>::kRing + ((size_t)a.n + 1) * sizeof(uint32_t);
-  const auto kernel = attend_own_kernel<T, D, NR>;
+// kernel<<<grid, block, smem, s>>>(args...); after: it may start before the kernel in front of
+// it ends
+template <typename K, typename... A>
+cudaError_t start_kernel(K kernel, uint32_t grid, uint32_t block, size_t smem, cudaStream_t s, bool after, const A &...args) {
   cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<own_grid(), Own<D>::kWarps * 32, smem, s>>>(a, w);
-  return cudaGetLastError();
-}
-
-template <typename T, int D>
-cudaError_t launch_t(const PrefixArgs &a, const Work &w, cudaStream_t s) {
-  cudaError_t e = a.group <= 8 ? launch_own<T, D, 1>(a, w, s) : launch_own<T, D, 2>(a, w, s);
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.n * a.nq + kJoinWarps - 1) / kJoinWarps);
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D>, a, w);
+  cfg.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int D>
+cudaError_t launch_t(PrefixArgs a, const Work &w, PrefixParts pp, cudaStream_t s) {
+  if (pp.splits) {
+    const cudaError_t e = launch_prefix_tc(a, pp, D, std::is_same<T, __nv_bfloat16>::value, s);
+    if (e == cudaErrorNotSupported)
+      pp.splits = 0;  // pools no tensor map can describe: stream by stream
+    else if (e != cudaSuccess)
+      return e;
+  }
+  a.from = pp.splits ? a.prefix : 0;
+  const size_t smem = Own<D>::kRing + ((size_t)a.n + 1) * sizeof(uint32_t);
+  const cudaError_t e = start_kernel(a.group <= 8 ? attend_own_kernel<T, D, 1> : attend_own_kernel<T, D, 2>, own_grid(),
+                                     Own<D>::kWarps * 32, smem, s, pp.splits != 0, a, w);
+  if (e != cudaSuccess) return e;
+  return start_kernel(attend_join_kernel<T, D>, (a.n * a.nq + kJoinWarps - 1) / kJoinWarps, kJoinWarps * 32, 0, s, true, a,
+                      w, pp);
 }
 template <typename T>
-cudaError_t launch(const PrefixArgs &a, const Work &w, uint32_t D, cudaStream_t s) {
-  return D == 64 ? launch_t<T, 64>(a, w, s) : D == 128 ? launch_t<T, 128>(a, w, s) : launch_t<T, 256>(a, w, s);
+cudaError_t launch(const PrefixArgs &a, const Work &w, const PrefixParts &pp, uint32_t D, cudaStream_t s) {
+  return D == 64 ? launch_t<T, 64>(a, w, pp, s) : D == 128 ? launch_t<T, 128>(a, w, pp, s) : launch_t<T, 256>(a, w, pp, s);
 }
 
 const char *check(const ch_prefix_attn_args *p) {
@@ -551,12 +558,12 @@ int prefix_attention(const ch_prefix_attn_args *p, void *workspace, size_t bytes
   a.window = p->window;
   a.scale = p->scale;
   a.status = p->status;
-  a.from = 0;
   Work w;
-  carve(p, static_cast<uint8_t *>(workspace), &w);
+  PrefixParts pp;
+  carve(p, static_cast<uint8_t *>(workspace), &w, &pp);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
-      p->dtype == CH_F16 ? launch<__half>(a, w, p->head_dim, s) : launch<__nv_bfloat16>(a, w, p->head_dim, s);
+      p->dtype == CH_F16 ? launch<__half>(a, w, pp, p->head_dim, s) : launch<__nv_bfloat16>(a, w, pp, p->head_dim, s);
   if (e != cudaSuccess) return set_last_error(CH_ECUDA, std::string("prefix_attention: ") + cudaGetErrorString(e));
   return CH_OK;
 }
@@ -566,7 +573,8 @@ int prefix_attention(const ch_prefix_attn_args *p, void *workspace, size_t bytes
 extern "C" size_t ch_prefix_attention_workspace(const ch_prefix_attn_args *args) {
   if (ch::check(args)) return 0;
   ch::Work w;
-  return ch::carve(args, nullptr, &w);
+  ch::PrefixParts pp;
+  return ch::carve(args, nullptr, &w, &pp);
 }
 extern "C" int ch_prefix_attention(const ch_prefix_attn_args *args, void *workspace, size_t workspace_bytes,
                                    void *stream) {
