@@ -3,11 +3,13 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - m),
 // over the visible positions j; m is the running maximum, and sums are f32.
+#include <algorithm>
+#include <cstring>
 #include <string>
 #include <type_traits>
 
 #include "../../include/channel_cuda.h"
-#include "prefix_attn.cuh"
+#include "prefix_tc.cuh"
 
 namespace ch {
 int set_last_error(int code, const std::string &msg);
@@ -63,36 +65,90 @@ struct Own {
   static constexpr uint32_t kPitch = D * 2 + 16;  // 8 rows of a fragment load hit distinct banks
   static constexpr uint32_t kStage = 2 * kTile * kPitch;
   static constexpr uint32_t kRing = kWarps * kStages * kStage;
+  static constexpr int kThreads = kWarps * 32 > kTcThreads ? kWarps * 32 : kTcThreads;
+  // shared memory: the prefix unit's or the rings, then start[n + 1]
+  static constexpr uint32_t kOffStart = Tc<D>::kBytes > kRing ? Tc<D>::kBytes : kRing;
 };
 constexpr uint32_t kMaxStreams = 4096;
 
-struct Work {      // in the caller's workspace
-  uint32_t *start; // [n + 1] first tile of a stream, per kv head; [n + 1]: tiles per warp
-  float *o;        // [segments][group][D]; segment = warp + pair, pair = stream * n_kv + head
-  float2 *ml;      // [segments][group]: maximum, sum
-  uint32_t warps;  // of the whole grid
+// How the work is dealt to the CTAs, the same in each (computed from lens by all of them).
+// The prefix is n_kv * row tiles * splits units for CTAs 0, 1, ...; the 16-key tiles of the
+// streams go to the warps in equal runs, longer ones (y tiles) to the CTAs without a unit and
+// shorter ones (x) to those with one, by the units' cost.
+struct Deal {
+  uint32_t splits;  // of the prefix
+  uint32_t units, unit_ctas;
+  uint32_t y_runs, y, x;  // runs 0 .. y_runs - 1 have y tiles, the rest x
 };
+struct Work {       // in the caller's workspace
+  uint32_t *start;  // [n + 1] first tile of a stream, per kv head
+  Deal *deal;
+  float *o;    // [segments][group][D]; segment = run + pair, pair = stream * n_kv + head
+  float2 *ml;  // [segments][group]: maximum, sum
+};
+// What a 128-key tile of the prefix and a unit's start and end cost, in 16-key tiles
+constexpr uint32_t kCostTile = 8, kCostUnit = 12;
+
+CH_DEV Deal deal_work(unsigned long long own, uint32_t ptiles, uint32_t per_split, uint32_t max_splits, uint32_t ctas,
+                      uint32_t warps) {
+  Deal d;
+  const unsigned long long prefix = (unsigned long long)ptiles * per_split * kCostTile;
+  d.splits = 0;
+  if (prefix) {
+    const unsigned long long all = own + prefix, step = all * per_split;
+    d.splits = (uint32_t)min((unsigned long long)min(max_splits, ptiles), (prefix * ctas + step - 1) / step);
+    d.splits = max(d.splits, 1u);
+  }
+  d.units = d.splits * per_split;
+  d.unit_ctas = min(d.units, ctas);
+  const uint32_t rest = ctas - d.unit_ctas;
+  // a CTA's cost of its units, and the even share of everything
+  const unsigned long long used =
+      d.units ? (prefix + (unsigned long long)d.units * kCostUnit + d.unit_ctas - 1) / d.unit_ctas : 0ull;
+  const unsigned long long share = (own + used * d.unit_ctas + ctas - 1) / ctas;
+  d.y_runs = rest * warps;
+  d.y = d.x = 0;
+  if (rest == 0) {
+    d.x = (uint32_t)((own + (unsigned long long)ctas * warps - 1) / ((unsigned long long)ctas * warps));
+  } else if (used >= share) {
+    d.y = (uint32_t)((own + d.y_runs - 1) / d.y_runs);
+  } else {
+    d.y = (uint32_t)((share + warps - 1) / warps);
+    d.x = (uint32_t)((share - used + warps - 1) / warps);
+  }
+  return d;
+}
 
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(const PrefixArgs a, const Work w) {
+__global__ void __launch_bounds__(Own<D>::kThreads, 1)
+    attend_kernel(const PrefixArgs a, const Work w, const PrefixParts pp, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap) {
   using O = Own<D>;
-  constexpr int kThreads = O::kWarps * 32, kSteps = D / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint32_t *start = reinterpret_cast<uint32_t *>(smem + O::kRing);  // [n + 1]
+  constexpr int kThreads = O::kThreads, kSteps = D / 16;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t *smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
+  uint32_t *start = reinterpret_cast<uint32_t *>(smem + O::kOffStart);  // [n + 1]
+  __shared__ TcBars tc_bars;
   __shared__ __align__(8) uint64_t bars[O::kWarps][O::kStages];
-  __shared__ uint32_t masks[O::kWarps][O::kStages], sums[O::kWarps];
+  __shared__ uint32_t masks[O::kWarps][O::kStages], sums[kThreads / 32], lo_min;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
 
-  // ---- tiles per stream, summed over the streams ----
+  // ---- tiles per stream, summed over the streams; the first position any stream sees ----
   const uint32_t per_thread = (a.n + kThreads - 1) / kThreads, b0 = min(a.n, tid * per_thread), b1 = min(a.n, b0 + per_thread);
+  uint32_t mine = 0, low = 0xFFFFFFFFu;
   auto tiles_of = [&](uint32_t b) {
     uint32_t lo, hi;
     visible(a, b, lo, hi);
+    low = min(low, lo);
     lo = max(lo, a.from);
     return hi > lo ? (hi - lo + kTile - 1) / kTile : 0u;
   };
-  uint32_t mine = 0;
-  for (uint32_t b = b0; b < b1; b++) mine += tiles_of(b);
+  if (tid == 0) lo_min = 0xFFFFFFFFu;
+  for (uint32_t b = b0; b < b1; b++) {
+    const uint32_t n = tiles_of(b);
+    start[b] = n;
+    mine += n;
+  }
   uint32_t inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -100,45 +156,64 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
     if (lane >= o) inc += u;
   }
   if (lane == 31) sums[warp] = inc;
-  if (lane < O::kStages) mbar_init(&bars[warp][lane], 1);
+  if (warp < O::kWarps && lane < O::kStages) mbar_init(&bars[warp][lane], 1);
   fence_mbar_init();
   __syncthreads();
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (lane == 0) atomicMin(&lo_min, low);
   uint32_t at = inc - mine, all = 0;
-  for (int k = 0; k < O::kWarps; k++) {
+  for (int k = 0; k < kThreads / 32; k++) {
     if (k < warp) at += sums[k];
     all += sums[k];
   }
   for (uint32_t b = b0; b < b1; b++) {
+    const uint32_t n = start[b];
     start[b] = at;
-    at += tiles_of(b);
+    at += n;
   }
   if (tid == 0) start[a.n] = all;
+  __syncthreads();
+  const uint32_t zlo = min(lo_min, a.prefix), tile0 = zlo / kKeys;
+  const uint32_t ptiles = pp.max_splits && zlo < a.prefix ? (a.prefix + kKeys - 1) / kKeys - tile0 : 0u;
+  const uint32_t row_tiles = (a.n * a.group + kRows - 1) / kRows;
   // 64-bit: n_kv times the tiles of all streams
   const unsigned long long total = (unsigned long long)all * a.nkv;
-  const uint32_t per = (uint32_t)max(1ull, (total + w.warps - 1) / w.warps);
-  __syncthreads();
-  if (blockIdx.x == 0) {
+  const Deal d = deal_work(total, ptiles, a.nkv * row_tiles, pp.max_splits, gridDim.x, O::kWarps);
+  if (blockIdx.x == gridDim.x - 1) {
     for (uint32_t b = tid; b <= a.n; b += kThreads) w.start[b] = start[b];
-    if (tid == 0) w.start[a.n + 1] = per;
+    if (tid == 0) *w.deal = d;
   }
   grid_dep_launch();
 
-  // consecutive runs go to different SMs, so that few tiles spread over all of them
-  const uint32_t wid = warp * gridDim.x + blockIdx.x;
-  const unsigned long long first = (unsigned long long)wid * per;
-  if (first >= total) {
-    grid_dep_wait();
-    return;
+  // ---- the shared prefix ----
+  for (uint32_t u = blockIdx.x; u < d.units; u += gridDim.x) {
+    const uint32_t h = u % a.nkv, rt = (u / a.nkv) % row_tiles, split = u / (a.nkv * row_tiles);
+    const uint32_t i0 = (uint32_t)((unsigned long long)split * ptiles / d.splits);
+    const uint32_t i1 = (uint32_t)((unsigned long long)(split + 1) * ptiles / d.splits);
+    prefix_unit<T, D>(a, pp, kmap, vmap, smem, tc_bars, h, rt, split, tile0 + i0, i1 - i0, zlo);
   }
+
+  // ---- this warp's run of the streams' own tiles; consecutive runs lie on different SMs, so
+  // that few tiles spread over all of them ----
+  if (warp >= O::kWarps) return;
+  const bool with_unit = blockIdx.x < d.unit_ctas;
+  const uint32_t run = with_unit ? d.y_runs + warp * d.unit_ctas + blockIdx.x
+                                 : warp * (gridDim.x - d.unit_ctas) + blockIdx.x - d.unit_ctas;
+  const uint32_t per = with_unit ? d.x : d.y;
+  const unsigned long long first =
+      with_unit ? (unsigned long long)d.y_runs * d.y + (unsigned long long)(run - d.y_runs) * d.x
+                : (unsigned long long)run * d.y;
+  if (per == 0 || first >= total) return;
   uint32_t left = (uint32_t)min((unsigned long long)per, total - first);
 
   struct Cursor {
     uint32_t b, h, i, tiles, lo, hi;
   };
-  auto enter = [&](Cursor &c) {  // the stream's bounds
+  auto enter = [&](Cursor &c, bool bounds) {
+    c.tiles = start[c.b + 1] - start[c.b];
+    if (!bounds) return;
     visible(a, c.b, c.lo, c.hi);
     c.lo = max(c.lo, a.from);
-    c.tiles = start[c.b + 1] - start[c.b];
   };
   Cursor ld;
   {
@@ -149,19 +224,19 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
     }
     ld.b = lo;
     while (start[ld.b + 1] == start[ld.b]) ld.b++;
-    enter(ld);
+    enter(ld, true);
     const uint32_t rem = (uint32_t)(first - (unsigned long long)start[ld.b] * a.nkv);
     ld.h = rem / ld.tiles;
     ld.i = rem % ld.tiles;
   }
-  auto advance = [&](Cursor &c) {
+  auto advance = [&](Cursor &c, bool bounds) {
     if (++c.i < c.tiles) return;
     c.i = 0;
     if (++c.h < a.nkv) return;
     c.h = 0;
     do c.b++;
     while (c.b < a.n && start[c.b + 1] == start[c.b]);
-    if (c.b < a.n) enter(c);
+    if (c.b < a.n) enter(c, bounds);
   };
   Cursor cu = ld;
   uint8_t *ring = smem + warp * O::kStages * O::kStage;
@@ -189,7 +264,7 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
       bulk_g2s(dst, pool + page * a.page + (long long)row * a.token + ld.h * a.head, D * 2, &bars[warp][s]);
     to_load--;
     if (to_load) {
-      advance(ld);
+      advance(ld, true);
       page = look_up();
     }
   };
@@ -288,7 +363,7 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
     if (++stage == O::kStages) stage = 0, parity ^= 1;
 
     if (cu.i + 1 == cu.tiles || left == 1) {  // the pair, or this warp's run, ends
-      const unsigned long long seg = (unsigned long long)wid + cu.b * a.nkv + cu.h;
+      const unsigned long long seg = (unsigned long long)run + cu.b * a.nkv + cu.h;
       float *po = w.o + seg * a.group * D;
       float2 *pm = w.ml + seg * a.group;
 #pragma unroll
@@ -310,9 +385,8 @@ __global__ void __launch_bounds__(Own<D>::kWarps * 32, 1) attend_own_kernel(cons
       }
       fresh = true;
     }
-    advance(cu);
+    advance(cu, false);
   }
-  grid_dep_wait();  // the join waits for this kernel, and through it for the prefix kernel
 }
 
 // ---------------------------------------------------------------------------
@@ -331,18 +405,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
   grid_dep_wait();
   // the row's parts: one per split of the shared prefix, then one per warp whose run touched
   // the pair (b, h)
-  const uint32_t s0 = w.start[b], tiles = w.start[b + 1] - s0, per = w.start[a.n + 1];
+  const uint32_t s0 = w.start[b], tiles = w.start[b + 1] - s0;
+  const Deal d = *w.deal;
   const unsigned long long t0 = (unsigned long long)s0 * a.nkv + (unsigned long long)h * tiles;
-  const uint32_t w0 = (uint32_t)(t0 / per), own = tiles ? (uint32_t)((t0 + tiles - 1) / per) - w0 + 1 : 0u;
+  const unsigned long long y_tiles = (unsigned long long)d.y_runs * d.y;
+  auto run_of = [&](unsigned long long t) {
+    return t < y_tiles ? (uint32_t)(t / d.y) : d.y_runs + (uint32_t)((t - y_tiles) / d.x);
+  };
+  const uint32_t w0 = tiles ? run_of(t0) : 0u, own = tiles ? run_of(t0 + tiles - 1) - w0 + 1 : 0u;
   const size_t rows = (size_t)a.n * a.group, at_prefix = (size_t)h * rows + (size_t)b * a.group + r;
   const size_t at_own = ((size_t)w0 + (size_t)b * a.nkv + h) * a.group + r;
-  const uint32_t parts = pp.splits + own;
+  const uint32_t parts = d.splits + own;
   auto ml_of = [&](uint32_t p) {
-    return p < pp.splits ? pp.ml[at_prefix + (size_t)p * a.nkv * rows] : w.ml[at_own + (size_t)(p - pp.splits) * a.group];
+    return p < d.splits ? pp.ml[at_prefix + (size_t)p * a.nkv * rows] : w.ml[at_own + (size_t)(p - d.splits) * a.group];
   };
   auto o_of = [&](uint32_t p) {
-    return (p < pp.splits ? pp.o + (at_prefix + (size_t)p * a.nkv * rows) * D
-                          : w.o + (at_own + (size_t)(p - pp.splits) * a.group) * D) + lane * EPL;
+    return (p < d.splits ? pp.o + (at_prefix + (size_t)p * a.nkv * rows) * D
+                          : w.o + (at_own + (size_t)(p - d.splits) * a.group) * D) + lane * EPL;
   };
   float top = -INFINITY;
   for (uint32_t p = lane; p < parts; p += 32) top = fmaxf(top, ml_of(p).x);
@@ -433,28 +512,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
 // The shared prefix has its own kernel when more than one stream can share it.
 bool shares(const ch_prefix_attn_args *p) { return p->prefix_len > 0 && p->n_streams > 1; }
 
-// workspace: w.start | w.ml | w.o | the prefix's ml | o
-uint32_t own_grid() { return (uint32_t)num_sms(); }
-uint32_t own_warps(uint32_t D) { return own_grid() * (D == 256 ? Own<256>::kWarps : Own<128>::kWarps); }
-static_assert(Own<64>::kWarps == Own<128>::kWarps, "own_warps");
+// As many splits as fit the SMs at once, at most one per key tile.
+uint32_t max_splits(const ch_prefix_attn_args *p) {
+  if (!shares(p)) return 0;
+  const unsigned long long rows = (unsigned long long)p->n_streams * (p->n_q / p->n_kv);
+  const unsigned long long per_split = (rows + kRows - 1) / kRows * p->n_kv;
+  return (uint32_t)std::max(1ull, std::min<unsigned long long>((unsigned)num_sms() / per_split,
+                                                               (p->prefix_len + kKeys - 1) / kKeys));
+}
+// workspace: w.start | w.deal | w.ml | w.o | the prefix's ml | o
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w, PrefixParts *pp) {
-  const uint32_t warps = own_warps(p->head_dim);
-  const size_t rows = ((size_t)warps + (size_t)p->n_streams * p->n_kv) * (p->n_q / p->n_kv);
+  const uint32_t runs = (uint32_t)num_sms() * (p->head_dim == 256 ? Own<256>::kWarps : Own<128>::kWarps);
+  static_assert(Own<64>::kWarps == Own<128>::kWarps, "runs");
+  const size_t rows = ((size_t)runs + (size_t)p->n_streams * p->n_kv) * (p->n_q / p->n_kv);
   size_t at = 0;
-  w->warps = warps;
-  w->start = reinterpret_cast<uint32_t *>(base);
-  at += aligned(((size_t)p->n_streams + 2) * sizeof(uint32_t));
-  w->ml = reinterpret_cast<float2 *>(base + at);
-  at += aligned(rows * sizeof(float2));
-  w->o = reinterpret_cast<float *>(base + at);
-  at += aligned(rows * p->head_dim * sizeof(float));
-  pp->splits = shares(p) ? prefix_tc_splits(p->prefix_len, p->n_streams, p->n_q / p->n_kv, p->n_kv) : 0;
-  const size_t shared = (size_t)pp->splits * p->n_streams * p->n_q;
-  pp->ml = reinterpret_cast<float2 *>(base + at);
-  at += aligned(shared * sizeof(float2));
-  pp->o = reinterpret_cast<float *>(base + at);
-  at += aligned(shared * p->head_dim * sizeof(float));
+  auto take = [&](size_t bytes) {
+    uint8_t *r = base + at;
+    at += aligned(bytes);
+    return r;
+  };
+  w->start = reinterpret_cast<uint32_t *>(take(((size_t)p->n_streams + 1) * sizeof(uint32_t)));
+  w->deal = reinterpret_cast<Deal *>(take(sizeof(Deal)));
+  w->ml = reinterpret_cast<float2 *>(take(rows * sizeof(float2)));
+  w->o = reinterpret_cast<float *>(take(rows * p->head_dim * sizeof(float)));
+  pp->max_splits = max_splits(p);
+  const size_t shared = (size_t)pp->max_splits * p->n_streams * p->n_q;
+  pp->ml = reinterpret_cast<float2 *>(take(shared * sizeof(float2)));
+  pp->o = reinterpret_cast<float *>(take(shared * p->head_dim * sizeof(float)));
   return at;
 }
 
@@ -479,17 +564,20 @@ cudaError_t start_kernel(K kernel, uint32_t grid, uint32_t block, size_t smem, c
 
 template <typename T, int D>
 cudaError_t launch_t(PrefixArgs a, const Work &w, PrefixParts pp, cudaStream_t s) {
-  if (pp.splits) {
-    const cudaError_t e = launch_prefix_tc(a, pp, D, std::is_same<T, __nv_bfloat16>::value, s);
-    if (e == cudaErrorNotSupported)
-      pp.splits = 0;  // pools no tensor map can describe: stream by stream
-    else if (e != cudaSuccess)
-      return e;
+  alignas(64) CUtensorMap kmap, vmap;
+  std::memset(&kmap, 0, sizeof(kmap));
+  std::memset(&vmap, 0, sizeof(vmap));
+  if (pp.max_splits) {
+    const uint32_t ps = 1u << a.shift;
+    // pools no tensor map can describe are read stream by stream
+    if (pool_map(&kmap, a.k, a, D, std::min(ps, kKeys)) != cudaSuccess ||
+        pool_map(&vmap, a.v, a, D, std::min(ps, Tc<D>::kVKeys)) != cudaSuccess)
+      pp.max_splits = 0;
   }
-  a.from = pp.splits ? a.prefix : 0;
-  const size_t smem = Own<D>::kRing + ((size_t)a.n + 1) * sizeof(uint32_t);
-  const cudaError_t e = start_kernel(a.group <= 8 ? attend_own_kernel<T, D, 1> : attend_own_kernel<T, D, 2>, own_grid(),
-                                     Own<D>::kWarps * 32, smem, s, pp.splits != 0, a, w);
+  a.from = pp.max_splits ? a.prefix : 0;
+  const size_t smem = 1024 + Own<D>::kOffStart + ((size_t)a.n + 1) * sizeof(uint32_t);
+  const cudaError_t e = start_kernel(a.group <= 8 ? attend_kernel<T, D, 1> : attend_kernel<T, D, 2>, num_sms(),
+                                     Own<D>::kThreads, smem, s, false, a, w, pp, kmap, vmap);
   if (e != cudaSuccess) return e;
   return start_kernel(attend_join_kernel<T, D>, (a.n * a.nq + kJoinWarps - 1) / kJoinWarps, kJoinWarps * 32, 0, s, true, a,
                       w, pp);
@@ -505,13 +593,14 @@ const char *check(const ch_prefix_attn_args *p) {
   if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return "head_dim must be 64, 128 or 256";
   if (p->n_kv == 0 || p->n_q == 0 || p->n_q % p->n_kv || p->n_q / p->n_kv > 16)
     return "n_q must be n_kv times 1..16";
-  if (p->n_q > 65535) return "at most 65535 q heads";
+  if (p->n_q > 1024) return "at most 1024 q heads";
   if (p->page_size < 8 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
     return "page_size must be a power of two from 8 to 256";
   if (p->n_pages > 0x7FFFFFFFu || p->table_cols > 0x7FFFFFFFu || p->prefix_len > 0x7FFFFFFFu)
     return "a size is 2^31 or more";
   const unsigned long long reach = p->prefix_len + (unsigned long long)p->table_cols * p->page_size;
-  if (reach >= 1ull << 32 || (reach / 16 + 1) * p->n_streams >= 1ull << 32) return "the positions of all streams exceed 2^36";
+  if (reach >= 1ull << 32 || (reach / 16 + 1) * p->n_streams >= 1ull << 32)
+    return "the positions of all streams exceed 2^36";
   if (p->dtype != CH_F16 && p->dtype != CH_BF16) return "dtype must be CH_F16 or CH_BF16";
   return nullptr;
 }

@@ -1,4 +1,4 @@
-// prefix_tc.cu -- the shared prefix of ch_prefix_attention on the 5th-generation tensor
+// prefix_tc.cuh -- the shared prefix of ch_prefix_attention on the 5th-generation tensor
 // cores: every shared K and V row is read once for all streams.
 //
 // The query rows of one kv head -- `group` per stream, row b * group + g -- are the M = 128
@@ -21,20 +21,78 @@
 // 4)).  Every wait is bounded; one that gives up sets the status word and the abort flag,
 // the roles leave their loops, and the MMA warp's last commit is waited for before tensor
 // memory is released.
+#pragma once
+#include <cuda_bf16.h>
 #include <cudaTypedefs.h>
 
-#include <algorithm>
 #include <type_traits>
 
-#include "prefix_attn.cuh"
+#include "common.cuh"
+#include "kernels.cuh"
 #include "tcgen05.cuh"
 
 namespace ch {
 
+struct PrefixArgs {
+  const void *q, *k, *v;
+  void *out;
+  const int32_t *prefix_table, *table, *lens;
+  long long qs, qh, os, oh;
+  long long page, token, head, ts;
+  uint32_t n, nq, nkv, group, shift, n_pages, cols, prefix, window;
+  uint32_t from;  // first position read stream by stream
+  float scale;
+  uint32_t *status;
+};
+
+CH_DEV float to_f32(__half v) { return __half2float(v); }
+CH_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// own tokens of stream b, limited to what its table can hold
+CH_DEV uint32_t own_len(const PrefixArgs &a, uint32_t b) {
+  const long long len = a.lens[b];
+  return (uint32_t)min(max(len, 0ll), (long long)a.cols << a.shift);
+}
+
+CH_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+CH_DEV uint32_t pack2(float lo, float hi, const __half *) { return pack_half2(__float2half_rn(lo), __float2half_rn(hi)); }
+CH_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16 *) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// positions stream b attends to: [lo, hi)
+CH_DEV void visible(const PrefixArgs &a, uint32_t b, uint32_t &lo, uint32_t &hi) {
+  hi = a.prefix + own_len(a, b);  // both below 2^31
+  lo = a.window && hi > a.window ? hi - a.window : 0u;
+}
+// page and row inside it of position j of stream b; -1 when the page is not in the pool
+CH_DEV int32_t page_of(const PrefixArgs &a, uint32_t b, uint32_t j, uint32_t &row) {
+  const bool shared = j < a.prefix;
+  const uint32_t i = shared ? j : j - a.prefix;
+  row = i & ((1u << a.shift) - 1);
+  const int32_t page = shared ? a.prefix_table[i >> a.shift] : a.table[b * a.ts + (i >> a.shift)];
+  if (page < 0 || (uint32_t)page >= a.n_pages) {
+    if (a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
+    return -1;
+  }
+  return page;
+}
+
+// The shared prefix's parts in the caller's workspace: per split and kv head the n * group
+// query rows (row b * group + g), unnormalised O, and the maximum (units of log2) and sum.
+struct PrefixParts {
+  float *o;             // [splits][n_kv][n * group][D]
+  float2 *ml;           // [splits][n_kv][n * group]
+  uint32_t max_splits;  // 0: the prefix is read stream by stream
+};
 namespace {
 constexpr uint32_t kKeys = 128, kRows = 128;
 constexpr uint32_t kPiece = 16384;
-constexpr int kThreads = 6 * 32, kSoft = 4 * 32;
+constexpr int kTcThreads = 6 * 32, kSoft = 4 * 32;
 constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. D - 1; S: 256 and 384
 constexpr int kMasks = 8;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
@@ -43,12 +101,10 @@ template <int D>
 struct Tc {
   static constexpr int kParts = D / 64;  // pieces of a K tile (64 dims each) and of a V tile
   static constexpr uint32_t kVKeys = kPiece / (2 * D);  // keys of a V piece
-  static constexpr int kSlots = D == 256 ? 10 : 12;
+  static constexpr int kSlots = D == 256 ? 9 : D == 128 ? 11 : 12;
   static constexpr uint32_t kOffRing = kRows * D * 2;
-  static constexpr uint32_t kOffEnd = kOffRing + kSlots * kPiece;
-  static constexpr size_t kSmem = kOffEnd + 1024;  // + alignment
+  static constexpr uint32_t kBytes = kOffRing + kSlots * kPiece;
 };
-static_assert(Tc<256>::kSmem <= 232448 - 1024, "shared memory per CTA");
 
 CH_DEV void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
   asm volatile(
@@ -101,22 +157,27 @@ CH_DEV uint64_t v_desc(uint32_t saddr, uint32_t vkeys) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// grid (splits, row tiles, n_kv)
+struct TcBars {
+  uint64_t full[12], empty[12], q_ready, s_full[2], p_ready[2], pv_done, done, mask_full[kMasks];
+  uint32_t masks[kMasks][4], tmem_slot, abort_flag;
+};
+
+// One unit: kv head h, row tile rt, key tiles [i0, i0 + nt) of the prefix, whose positions
+// below zlo no stream sees.  Leaves the rows' parts at split `split`.  All threads of the CTA
+// call it; sm (1024-byte aligned) is free before and after.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
-    prefix_tc_kernel(const PrefixArgs a, const PrefixParts w, const __grid_constant__ CUtensorMap kmap,
-                     const __grid_constant__ CUtensorMap vmap) {
+CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtensorMap &kmap, const CUtensorMap &vmap,
+                        uint8_t *sm, TcBars &bars, uint32_t h, uint32_t rt, uint32_t split, uint32_t i0, uint32_t nt,
+                        uint32_t zlo) {
   using C = Tc<D>;
-  extern __shared__ uint8_t smem_dyn[];
-  const uint32_t dyn = smem_u32(smem_dyn);
-  uint8_t *sm = smem_dyn + (((dyn + 1023u) & ~1023u) - dyn);
   const uint32_t sbase = smem_u32(sm), ring = sbase + C::kOffRing;
-  __shared__ __align__(8) uint64_t full[C::kSlots], empty[C::kSlots], q_ready, s_full[2], p_ready[2], pv_done, done,
-      mask_full[kMasks];
-  __shared__ uint32_t masks[kMasks][4], tmem_slot, lo_min;
-  __shared__ volatile uint32_t abort_flag;
+  uint64_t *full = bars.full, *empty = bars.empty, *s_full = bars.s_full, *p_ready = bars.p_ready,
+           *mask_full = bars.mask_full;
+  uint64_t &q_ready = bars.q_ready, &pv_done = bars.pv_done, &done = bars.done;
+  auto &masks = bars.masks;
+  volatile uint32_t &abort_flag = bars.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t h = blockIdx.z, rows = a.n * a.group;
+  const uint32_t rows = a.n * a.group;
 
   if (tid == 0) {
     for (int s = 0; s < C::kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
@@ -126,11 +187,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&pv_done, 1);
     mbar_init(&done, 1);
     abort_flag = 0u;
-    lo_min = a.window ? 0xFFFFFFFFu : 0u;
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_slot)),
                  "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -138,23 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  if (a.window) {  // the first position any stream sees
-    uint32_t low = 0xFFFFFFFFu;
-    for (uint32_t b = tid; b < a.n; b += kThreads) {
-      uint32_t lo, hi;
-      visible(a, b, lo, hi);
-      low = min(low, lo);
-    }
-    low = __reduce_min_sync(0xffffffffu, low);
-    if (lane == 0) atomicMin(&lo_min, low);
-    __syncthreads();
-  }
-  const uint32_t zlo = min(lo_min, a.prefix), tile_first = zlo / kKeys, tile_end = (a.prefix + kKeys - 1) / kKeys;
-  const uint32_t tiles = zlo < a.prefix ? tile_end - tile_first : 0u;
-  const uint32_t i0 = tile_first + (uint32_t)((unsigned long long)blockIdx.x * tiles / w.splits);
-  const uint32_t nt = tile_first + (uint32_t)((unsigned long long)(blockIdx.x + 1) * tiles / w.splits) - i0;
-  grid_dep_launch();
+  const uint32_t tmem = *(volatile uint32_t *)&bars.tmem_slot;
 
   if (warp == 0) {
     // ---- copies.  Lane l of a tile holds the page of its keys [l * kr, (l + 1) * kr) ----
@@ -179,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return s;
     };
     // a page index past the pool reads as zeros
-    int32_t page = nt ? look_up(i0) : -1, next = -1, prev = -1;
+    int32_t page = look_up(i0), next = -1, prev = -1;
     for (uint32_t i = 0; i <= nt && ok; i++) {
       if (i < nt) {
         const uint32_t tile = i0 + i, j0 = tile * kKeys;
@@ -228,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_idesc = idesc_of(kKeys, std::is_same<T, __nv_bfloat16>::value, false);
       const uint32_t o_idesc = idesc_of(D, std::is_same<T, __nv_bfloat16>::value, true);
       uint32_t seq = 0;
-      bool ok = nt == 0 || tc_wait(&q_ready, 0, &abort_flag, a.status);
+      bool ok = tc_wait(&q_ready, 0, &abort_flag, a.status);
       auto take = [&]() {  // the next piece of the ring
         const uint32_t s = seq % C::kSlots;
         ok = ok && tc_wait(&full[s], (seq / C::kSlots) & 1, &abort_flag, a.status);
@@ -236,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         seq++;
         return s;
       };
-      for (uint32_t i = 0; nt && i <= nt && ok; i++) {
+      for (uint32_t i = 0; i <= nt && ok; i++) {
         if (i < nt) {
           // S_i lies where P_{i-2} lay
           if (i >= 2) ok = tc_wait(&pv_done, (i - 2) & 1, &abort_flag, a.status);
@@ -269,18 +313,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(&done);  // every MMA issued (all of them, or those before an abort) is complete
     }
-  } else {
+  } else if (warp < 6) {
     // ---- softmax: thread = query row ----
-    const uint32_t quad = warp & 3, row = quad * 32 + lane, row0 = blockIdx.y * kRows;
+    const uint32_t quad = warp & 3, row = quad * 32 + lane, row0 = rt * kRows;
     const uint32_t lanes = (quad * 32u) << 16;
     constexpr uint32_t kVecs = D / 8;  // 16-byte pieces of a row
-    for (uint32_t x = lane; x < 32 * kVecs; x += 32) {
-      const uint32_t r = quad * 32 + x / kVecs, v = x % kVecs, gr = row0 + r;
-      uint4 val = make_uint4(0, 0, 0, 0);
-      if (gr < rows && nt)
-        val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (gr / a.group) * a.qs +
-                                               (h * a.group + gr % a.group) * a.qh + v * 8);
-      *reinterpret_cast<uint4 *>(sm + (v >> 3) * kRows * 128 + r * 128 + (((v & 7) ^ (r & 7)) << 4)) = val;
+    // the warp's 32 rows of Q, 16 loads of 16 bytes in flight per lane
+    constexpr uint32_t kAt = kVecs < 16 ? kVecs : 16;
+#pragma unroll 1
+    for (uint32_t x0 = 0; x0 < kVecs; x0 += kAt) {
+      uint4 val[kAt];
+#pragma unroll
+      for (uint32_t u = 0; u < kAt; u++) {
+        const uint32_t x = (x0 + u) * 32 + lane, v = x % kVecs, gr = row0 + quad * 32 + x / kVecs;
+        val[u] = make_uint4(0, 0, 0, 0);
+        if (gr < rows)
+          val[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (gr / a.group) * a.qs +
+                                                    (h * a.group + gr % a.group) * a.qh + v * 8);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kAt; u++) {
+        const uint32_t x = (x0 + u) * 32 + lane, v = x % kVecs, r = quad * 32 + x / kVecs;
+        *reinterpret_cast<uint4 *>(sm + (v >> 3) * kRows * 128 + r * 128 + (((v & 7) ^ (r & 7)) << 4)) = val[u];
+      }
     }
     fence_proxy_async();
     mbar_arrive(&q_ready);
@@ -408,9 +463,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     ok = __all_sync(0xffffffffu, ok && !abort_flag);
     if (ok) {
-      const size_t at = ((size_t)blockIdx.x * a.nkv + h) * rows + gr;
+      const size_t at = ((size_t)split * a.nkv + h) * rows + gr;
       if (gr < rows) w.ml[at] = make_float2(m, l);
-      if (nt) {
+      {
         float *po = w.o + at * D;
 #pragma unroll 1
         for (uint32_t c = 0; c < D; c += 32) {
@@ -428,11 +483,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncwarp();
   tc_fence_before();
-  __syncthreads();  // every role done with tensor memory
+  __syncthreads();  // every role done with tensor memory and the barriers
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
+  if (tid == 0) {  // the barriers' memory may be initialised again
+    auto drop = [](uint64_t *bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
+    for (int s = 0; s < C::kSlots; s++) drop(&full[s]), drop(&empty[s]);
+    for (int s = 0; s < 2; s++) drop(&s_full[s]), drop(&p_ready[s]);
+    for (int s = 0; s < kMasks; s++) drop(&mask_full[s]);
+    drop(&q_ready), drop(&pv_done), drop(&done);
+  }
+  __syncthreads();
 }
 
 // One layer's pool as a 4-D tensor: dim, token in the page, head, page; boxes of 64 dims of
@@ -457,36 +520,6 @@ cudaError_t pool_map(CUtensorMap *map, const void *pool, const PrefixArgs &a, ui
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorNotSupported;
 }
-
-template <typename T, int D>
-cudaError_t launch_t(const PrefixArgs &a, const PrefixParts &w, cudaStream_t s) {
-  alignas(64) CUtensorMap kmap, vmap;
-  const uint32_t ps = 1u << a.shift;
-  cudaError_t e = pool_map(&kmap, a.k, a, D, std::min(ps, kKeys));
-  if (e == cudaSuccess) e = pool_map(&vmap, a.v, a, D, std::min(ps, Tc<D>::kVKeys));
-  if (e == cudaSuccess) e = ensure_smem_attr((const void *)prefix_tc_kernel<T, D>, Tc<D>::kSmem);
-  if (e != cudaSuccess) return e;
-  const dim3 grid(w.splits, (a.n * a.group + kRows - 1) / kRows, a.nkv);
-  prefix_tc_kernel<T, D><<<grid, kThreads, Tc<D>::kSmem, s>>>(a, w, kmap, vmap);
-  return cudaGetLastError();
-}
 }  // namespace
-
-// As many splits as fit the SMs at once, at most one per key tile.
-uint32_t prefix_tc_splits(uint32_t prefix, uint32_t n, uint32_t group, uint32_t nkv) {
-  const unsigned long long ctas = (unsigned long long)((n * group + kRows - 1) / kRows) * nkv;
-  const uint32_t tiles = (prefix + kKeys - 1) / kKeys;
-  return (uint32_t)std::max(1ull, std::min<unsigned long long>((unsigned)num_sms() / ctas, tiles));
-}
-
-cudaError_t launch_prefix_tc(const PrefixArgs &a, const PrefixParts &w, uint32_t D, bool bf16, cudaStream_t s) {
-  if (bf16)
-    return D == 64    ? launch_t<__nv_bfloat16, 64>(a, w, s)
-           : D == 128 ? launch_t<__nv_bfloat16, 128>(a, w, s)
-                      : launch_t<__nv_bfloat16, 256>(a, w, s);
-  return D == 64    ? launch_t<__half, 64>(a, w, s)
-         : D == 128 ? launch_t<__half, 128>(a, w, s)
-                    : launch_t<__half, 256>(a, w, s);
-}
 
 }  // namespace ch

@@ -453,7 +453,7 @@ int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
  * positions [max(0, T - window), T) (window 0 = all), q head h to kv head
  * h / (n_q / n_kv):  out = softmax(scale q.k) v, zeros when no position is visible.
  * q / out element (b, head, d) at b * stream_stride + head * head_stride + d.
- * head_dim 64, 128 or 256; n_q / n_kv at most 16; n_streams at most 4096; page_size a power of two from 8 to 256;
+ * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096; page_size a power of two from 8 to 256;
  * dtype (of q, out and both pools) CH_F16 or CH_BF16, sums in f32.  Strides are multiples
  * of 8 elements, q, out and the pools 16-byte aligned.  Positions whose page index is not
  * in [0, n_pages) are left out (status bit 2), as are own positions past table_cols pages.
