@@ -60,8 +60,8 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
 constexpr uint32_t kTile = 16;  // keys
 template <int D>
 struct Own {
-  static constexpr int kWarps = D == 256 ? 4 : 8;
-  static constexpr int kStages = D == 64 ? 5 : 3;
+  static constexpr int kWarps = D == 256 ? 6 : 8;
+  static constexpr int kStages = D == 64 ? 5 : D == 128 ? 3 : 2;
   static constexpr uint32_t kPitch = D * 2 + 16;  // 8 rows of a fragment load hit distinct banks
   static constexpr uint32_t kStage = 2 * kTile * kPitch;
   static constexpr uint32_t kRing = kWarps * kStages * kStage;
@@ -242,16 +242,31 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   uint8_t *ring = smem + warp * O::kStages * O::kStage;
   const T *pool = static_cast<const T *>(lane < 16 ? a.k : a.v);
   uint32_t to_load = left;
-  uint32_t row = 0;
-  auto look_up = [&]() {
-    const uint32_t j = ld.lo + ld.i * kTile + (lane & 15);
-    return j < ld.hi ? page_of(a, ld.b, j, row) : -1;
+  // A tile on its way: its page index as read (looked at only when the copies go out, so that
+  // the reads of several tiles are in flight together)
+  struct Tile {
+    int32_t page;
+    uint32_t row, h;
+    bool in;
   };
-  int32_t page = look_up();
-  auto issue = [&](int s) {
+  auto look_up = [&]() {
+    Tile t;
+    const uint32_t j = ld.lo + ld.i * kTile + (lane & 15);
+    t.in = j < ld.hi;
+    t.h = ld.h;
+    const bool shared = j < a.prefix;
+    const uint32_t i = shared ? j : j - a.prefix;
+    t.row = i & ((1u << a.shift) - 1);
+    t.page = -1;
+    if (t.in) t.page = shared ? a.prefix_table[i >> a.shift] : a.table[ld.b * a.ts + (i >> a.shift)];
+    return t;
+  };
+  auto issue = [&](const Tile &t, int s) {
     uint8_t *dst = ring + s * O::kStage + lane * O::kPitch;
-    const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-    if (page < 0) {  // not copied: zeros, so that a weight of 0 meets no stale bits
+    const bool there = t.page >= 0 && (uint32_t)t.page < a.n_pages;
+    const uint32_t have = __ballot_sync(0xffffffffu, there);
+    if (!there) {  // not copied: zeros, so that a weight of 0 meets no stale bits
+      if (t.in && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
       for (uint32_t c = 0; c < D * 2; c += 16) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
       fence_proxy_async();
     }
@@ -260,16 +275,26 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
       mbar_arrive_expect_tx(&bars[warp][s], __popc(have) * D * 2);
     }
     __syncwarp();
-    if (page >= 0)
-      bulk_g2s(dst, pool + page * a.page + (long long)row * a.token + ld.h * a.head, D * 2, &bars[warp][s]);
-    to_load--;
-    if (to_load) {
-      advance(ld, true);
-      page = look_up();
-    }
+    if (there) bulk_g2s(dst, pool + t.page * a.page + (long long)t.row * a.token + t.h * a.head, D * 2, &bars[warp][s]);
   };
+  Tile ahead[O::kStages];
+#pragma unroll
   for (int s = 0; s < O::kStages; s++)
-    if (to_load) issue(s);
+    if ((uint32_t)s < to_load) {
+      ahead[s] = look_up();
+      advance(ld, true);
+    }
+#pragma unroll
+  for (int s = 0; s < O::kStages; s++)
+    if ((uint32_t)s < to_load) issue(ahead[s], s);
+  to_load -= min(to_load, (uint32_t)O::kStages);
+  Tile next;
+  auto read_ahead = [&]() {
+    if (!to_load) return;
+    next = look_up();
+    advance(ld, true);
+  };
+  read_ahead();
 
   uint32_t qf[NR][kSteps][2];
   float o[NR][kSteps][4], m[NR][2], l[NR][2];
@@ -359,7 +384,11 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
       for (int r = 0; r < NR; r++) mma16(o[r][k], f, p[r][0], p[r][1], tag);
     }
     __syncwarp();
-    if (to_load) issue(stage);
+    if (to_load) {
+      issue(next, stage);
+      to_load--;
+      read_ahead();
+    }
     if (++stage == O::kStages) stage = 0, parity ^= 1;
 
     if (cu.i + 1 == cu.tiles || left == 1) {  // the pair, or this warp's run, ends
@@ -570,8 +599,8 @@ cudaError_t launch_t(PrefixArgs a, const Work &w, PrefixParts pp, cudaStream_t s
   if (pp.max_splits) {
     const uint32_t ps = 1u << a.shift;
     // pools no tensor map can describe are read stream by stream
-    if (pool_map(&kmap, a.k, a, D, std::min(ps, kKeys)) != cudaSuccess ||
-        pool_map(&vmap, a.v, a, D, std::min(ps, Tc<D>::kVKeys)) != cudaSuccess)
+    if (pool_map(&kmap, a.k, a, D, std::min(ps, kKeys), false) != cudaSuccess ||
+        pool_map(&vmap, a.v, a, D, std::min(ps, Tc<D>::kVKeys), true) != cudaSuccess)
       pp.max_splits = 0;
   }
   a.from = pp.max_splits ? a.prefix : 0;

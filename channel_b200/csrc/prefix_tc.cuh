@@ -5,8 +5,8 @@
 // rows of a tile (a batch of 64 streams with two q heads per kv head fills it); a CTA takes
 // one row tile and a run of the prefix's 128-key tiles, and per key tile
 //   S (128 x 128) = Q K^T,   P = 2^(scale log2(e) S - m),   O (128 x D) += P V.
-// Q stays in shared memory; K and V come by TMA from the pages (one box per page and 64
-// dims, 128-byte swizzle) through one ring of 16 KB pieces in the order the products take
+// Q stays in shared memory; K and V come by TMA from the pages (K: a box per page and 64
+// dims, V: a box per page; 128-byte swizzle) through one ring of 16 KB pieces in the order the products take
 // them: K_0, K_1, V_0, K_2, V_1, ...; S (two buffers), P (over its S, as the TMEM operand A)
 // and O live in tensor memory (256 + 2 x 128 columns).  A softmax thread owns a row: no
 // shuffles.  O is rescaled only when a row's maximum has grown by more than 2^8 since its
@@ -106,6 +106,13 @@ struct Tc {
   static constexpr uint32_t kBytes = kOffRing + kSlots * kPiece;
 };
 
+CH_DEV void tma_load_5d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int u, int w, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(u), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
 CH_DEV void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
@@ -149,12 +156,16 @@ CH_DEV uint32_t idesc_of(uint32_t n, bool bf16, bool mn) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) |
          ((kRows >> 4) << 24);
 }
-// V piece as the N-major operand B in the 128-byte swizzle: 64 dims x 8 keys are 1024 bytes,
-// the next 8 keys follow (stride offset), the next 64 dims lie vkeys * 128 bytes on (leading
-// offset)
-CH_DEV uint64_t v_desc(uint32_t saddr, uint32_t vkeys) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(vkeys * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+// V as the N-major operand B in the 128-byte swizzle: 64 dims x 8 keys are 1024 bytes; the
+// next 8 keys lie `keys8` bytes on (stride offset), the next 64 dims `dims64` (leading offset)
+CH_DEV uint64_t v_desc(uint32_t saddr, uint32_t dims64, uint32_t keys8) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(dims64 >> 4) << 16) | ((uint64_t)(keys8 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+CH_DEV void st_global_32b(float *p, const uint32_t *v) {  // 32 bytes, 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 struct TcBars {
@@ -176,6 +187,9 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   uint64_t &q_ready = bars.q_ready, &pv_done = bars.pv_done, &done = bars.done;
   auto &masks = bars.masks;
   volatile uint32_t &abort_flag = bars.abort_flag;
+  // a V piece is boxes of vr keys, [D / 64][vr][64] each: 8 keys are 1024 bytes of a box, or
+  // (pages of 8) a box of their own
+  const uint32_t vr = min(1u << a.shift, C::kVKeys);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rows = a.n * a.group;
 
@@ -202,7 +216,7 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
 
   if (warp == 0) {
     // ---- copies.  Lane l of a tile holds the page of its keys [l * kr, (l + 1) * kr) ----
-    const uint32_t ps = 1u << a.shift, kr = min(ps, kKeys), vr = min(ps, C::kVKeys), boxes = kKeys / kr;
+    const uint32_t ps = 1u << a.shift, kr = min(ps, kKeys), boxes = kKeys / kr;
     auto look_up = [&](uint32_t i) {
       const uint32_t j = i * kKeys + lane * kr;
       if (lane >= (int)boxes || j >= a.prefix) return -1;
@@ -251,12 +265,11 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
         const uint32_t j0 = (i0 + i - 1) * kKeys;
         for (int c = 0; c < C::kParts && ok; c++) {
           const uint32_t s = claim();
-          const uint32_t per = C::kVKeys / vr, dc = lane % C::kParts, pi = lane / C::kParts;
-          const uint32_t key = c * C::kVKeys + min(pi, per - 1) * vr;
+          const uint32_t key = c * C::kVKeys + min((uint32_t)lane, C::kVKeys / vr - 1) * vr;
           const int32_t pg = __shfl_sync(0xffffffffu, prev, key / kr);
-          if (ok && pi < per)
-            tma_load_4d(ring + s * kPiece + (dc * C::kVKeys + pi * vr) * 128, &vmap, dc * 64,
-                        (int)((j0 + key) & (ps - 1)), (int)h, pg >= 0 ? pg : (int)a.n_pages, &full[s]);
+          if (ok && lane < (int)(C::kVKeys / vr))
+            tma_load_5d(ring + s * kPiece + lane * vr * 2 * D, &vmap, 0, (int)((j0 + key) & (ps - 1)), 0, (int)h,
+                        pg >= 0 ? pg : (int)a.n_pages, &full[s]);
         }
       }
       prev = page;
@@ -305,7 +318,9 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
 #pragma unroll
             for (uint32_t k = 0; k < C::kVKeys / 16; k++)
               mma_ts(tmem, tmem + kSCol + (j & 1) * kKeys + (c * C::kVKeys + k * 16) / 2,
-                     v_desc(ring + s * kPiece + k * 2048, C::kVKeys), o_idesc, (j | c | k) != 0);
+                     v_desc(ring + s * kPiece + k * 16 / vr * vr * 2 * D + k * 16 % vr * 128, vr * 128,
+                            vr > 8 ? 1024u : 16u * D),
+                     o_idesc, (j | c | k) != 0);
             commit(&empty[s]);
           }
           if (ok) commit(&pv_done);
@@ -318,35 +333,39 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     const uint32_t quad = warp & 3, row = quad * 32 + lane, row0 = rt * kRows;
     const uint32_t lanes = (quad * 32u) << 16;
     constexpr uint32_t kVecs = D / 8;  // 16-byte pieces of a row
-    // the warp's 32 rows of Q, 16 loads of 16 bytes in flight per lane
-    constexpr uint32_t kAt = kVecs < 16 ? kVecs : 16;
-#pragma unroll 1
-    for (uint32_t x0 = 0; x0 < kVecs; x0 += kAt) {
-      uint4 val[kAt];
-#pragma unroll
-      for (uint32_t u = 0; u < kAt; u++) {
-        const uint32_t x = (x0 + u) * 32 + lane, v = x % kVecs, gr = row0 + quad * 32 + x / kVecs;
-        val[u] = make_uint4(0, 0, 0, 0);
-        if (gr < rows)
-          val[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (gr / a.group) * a.qs +
-                                                    (h * a.group + gr % a.group) * a.qh + v * 8);
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < kAt; u++) {
-        const uint32_t x = (x0 + u) * 32 + lane, v = x % kVecs, r = quad * 32 + x / kVecs;
-        *reinterpret_cast<uint4 *>(sm + (v >> 3) * kRows * 128 + r * 128 + (((v & 7) ^ (r & 7)) << 4)) = val[u];
+    // the warp's 32 rows of Q, all copies in flight together; lane l knows row l's place
+    const uint32_t gr = row0 + row;
+    const T *mine = gr < rows ? static_cast<const T *>(a.q) + (gr / a.group) * a.qs + (h * a.group + gr % a.group) * a.qh
+                              : nullptr;
+#pragma unroll 8
+    for (uint32_t u = 0; u < kVecs; u++) {
+      const uint32_t x = u * 32 + lane, v = x % kVecs, r = x / kVecs;
+      const T *src = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+      uint8_t *dst = sm + (v >> 3) * kRows * 128 + (quad * 32 + r) * 128 + (((v & 7) ^ (r & 7)) << 4);
+      if (src)
+        cp_async16(dst, src + v * 8);
+      else
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+    }
+    cp_async_wait_all();
+    if (!(a.scale > 0.f)) {  // a scale that is not positive goes into Q: below it is |scale|
+      __syncwarp();
+      for (uint32_t u = 0; u < kVecs; u++) {
+        const uint32_t x = u * 32 + lane, v = x % kVecs, r = x / kVecs;
+        uint4 *q = reinterpret_cast<uint4 *>(sm + (v >> 3) * kRows * 128 + (quad * 32 + r) * 128 + ((v & 7) << 4));
+        const uint32_t keep = a.scale < 0.f ? 0xFFFFFFFFu : 0u, flip = a.scale < 0.f ? 0x80008000u : 0u;
+        *q = make_uint4((q->x & keep) ^ flip, (q->y & keep) ^ flip, (q->z & keep) ^ flip, (q->w & keep) ^ flip);
       }
     }
     fence_proxy_async();
     mbar_arrive(&q_ready);
 
     uint32_t lo = 0;
-    const uint32_t gr = row0 + row;
     if (a.window && gr < rows) {
       uint32_t hi;
       visible(a, gr / a.group, lo, hi);
     }
-    const float scale2 = a.scale * 1.44269504088896341f;
+    const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (uint32_t i = 0; i < nt; i++) {
@@ -375,26 +394,12 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
           for (int e = 0; e < 32; e++)
             if (!((mask[c] >> e) & 1)) s[c][e] = 0xFF800000u;  // -inf
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, low[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
-      if (scale2 >= 0.f) {
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 32; e++)
+      for (int e = 0; e < 32; e++)
 #pragma unroll
-          for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
-      } else {
-        // a negative scale turns the order round; masked scores stay -inf
-#pragma unroll
-        for (int e = 0; e < 32; e++)
-#pragma unroll
-          for (int c = 0; c < 4; c++)
-            if ((mask[c] >> e) & 1) low[c] = fminf(low[c], __uint_as_float(s[c][e]));
-      }
-      float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-      if (scale2 < 0.f) {
-        const float mn = fminf(fminf(low[0], low[1]), fminf(low[2], low[3]));
-        mx = mn == INFINITY ? -INFINITY : mn * scale2;
-      }
-      if (!(mx > -INFINITY)) mx = -INFINITY;  // nothing visible (or 0 * -inf)
+        for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
       const bool grow = mx > m + kGrow || (m == -INFINITY && mx > -INFINITY);
       const float m1 = grow ? mx : m, ref = m1 == -INFINITY ? 0.f : m1;
       if (__any_sync(0xffffffffu, grow)) {
@@ -423,13 +428,8 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
 #pragma unroll
         for (int e = 0; e < 32; e++) {
           const uint32_t b0 = s[c + (e >> 4)][(2 * e) & 31], b1 = s[c + (e >> 4)][(2 * e + 1) & 31];
-          float p0 = exp2_approx(fmaf(__uint_as_float(b0), scale2, -ref));
-          float p1 = exp2_approx(fmaf(__uint_as_float(b1), scale2, -ref));
-          if (scale2 <= 0.f) {  // -inf times a scale that is not positive is not a masked score
-            const uint32_t seen = mask[c + (e >> 4)] >> ((2 * e) & 31);
-            if (!(seen & 1)) p0 = 0.f;
-            if (!(seen & 2)) p1 = 0.f;
-          }
+          const float p0 = exp2_approx(fmaf(__uint_as_float(b0), scale2, -ref));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(b1), scale2, -ref));
           sum[e & 1] += p0;
           sum[2 + (e & 1)] += p1;
           p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
@@ -450,8 +450,9 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
         for (uint32_t x = tid - 64; x < (n0 + n1) * kVecs; x += kSoft) {
           const uint32_t z = x / kVecs, key = z < n0 ? z : z1 + (z - n0), v = x % kVecs;
           const uint32_t slot = (seq0 + key / C::kVKeys) % C::kSlots;
-          *reinterpret_cast<uint4 *>(sm + C::kOffRing + slot * kPiece + ((v >> 3) * C::kVKeys + key % C::kVKeys) * 128 +
-                                     (v & 7) * 16) = make_uint4(0, 0, 0, 0);
+          const uint32_t in = key % C::kVKeys;
+          *reinterpret_cast<uint4 *>(sm + C::kOffRing + slot * kPiece + in / vr * vr * 2 * D +
+                                     ((v >> 3) * vr + in % vr) * 128 + (v & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
       }
@@ -474,8 +475,7 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
           tc_wait_ld();
           if (gr < rows) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4 *>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 32; e += 8) st_global_32b(po + c + e, o + e);
           }
         }
       }
@@ -498,9 +498,9 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   __syncthreads();
 }
 
-// One layer's pool as a 4-D tensor: dim, token in the page, head, page; boxes of 64 dims of
-// `rows` tokens, 128-byte swizzle.
-cudaError_t pool_map(CUtensorMap *map, const void *pool, const PrefixArgs &a, uint32_t D, uint32_t rows) {
+// One layer's pool as a tensor of dim, token in the page, head and page (K: boxes of 64 dims
+// of `rows` tokens), for V with the dims in groups of 64 (boxes of all dims); 128-byte swizzle.
+cudaError_t pool_map(CUtensorMap *map, const void *pool, const PrefixArgs &a, uint32_t D, uint32_t rows, bool grouped) {
   static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -511,13 +511,14 @@ cudaError_t pool_map(CUtensorMap *map, const void *pool, const PrefixArgs &a, ui
   if (!encode) return cudaErrorNotSupported;
   // the stride of a dimension of one element is never used; torch may give any value there
   const cuuint64_t token = (cuuint64_t)a.token * 2;
-  const cuuint64_t dims[4] = {D, 1ull << a.shift, a.nkv, a.n_pages};
-  const cuuint64_t strides[3] = {token, a.nkv > 1 ? (cuuint64_t)a.head * 2 : token,
-                                 a.n_pages > 1 ? (cuuint64_t)a.page * 2 : token};
-  const cuuint32_t box[4] = {64, rows, 1, 1}, step[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(pool), dims, strides, box, step,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t head = a.nkv > 1 ? (cuuint64_t)a.head * 2 : token, page = a.n_pages > 1 ? (cuuint64_t)a.page * 2 : token;
+  const cuuint64_t dims4[4] = {D, 1ull << a.shift, a.nkv, a.n_pages}, strides4[3] = {token, head, page};
+  const cuuint64_t dims5[5] = {64, 1ull << a.shift, D / 64, a.nkv, a.n_pages}, strides5[4] = {token, 128, head, page};
+  const cuuint32_t box4[4] = {64, rows, 1, 1}, box5[5] = {64, rows, D / 64, 1, 1}, step[5] = {1, 1, 1, 1, 1};
+  const CUresult r =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, grouped ? 5 : 4, const_cast<void *>(pool), grouped ? dims5 : dims4,
+             grouped ? strides5 : strides4, grouped ? box5 : box4, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorNotSupported;
 }
 }  // namespace
