@@ -86,8 +86,8 @@ struct Work {       // in the caller's workspace
   float *o;    // [segments][group][D]; segment = run + pair, pair = stream * n_kv + head
   float2 *ml;  // [segments][group]: maximum, sum
 };
-// What a 128-key tile of the prefix and a unit's start and end cost, in 16-key tiles
-constexpr uint32_t kCostTile = 8, kCostUnit = 12;
+// What a 64-key tile of the prefix and a unit's start and end cost, in 16-key tiles
+constexpr uint32_t kCostTile = 4, kCostUnit = 12;
 
 CH_DEV Deal deal_work(unsigned long long own, uint32_t ptiles, uint32_t per_split, uint32_t max_splits, uint32_t ctas,
                       uint32_t warps) {

@@ -2,23 +2,22 @@
 // cores: every shared K and V row is read once for all streams.
 //
 // The query rows of one kv head -- `group` per stream, row b * group + g -- are the M = 128
-// rows of a tile (a batch of 64 streams with two q heads per kv head fills it); a CTA takes
-// one row tile and a run of the prefix's 128-key tiles, and per key tile
-//   S (128 x 128) = Q K^T,   P = 2^(scale log2(e) S - m),   O (128 x D) += P V.
-// Q stays in shared memory; K and V come by TMA from the pages (K: a box per page and 64
-// dims, V: a box per page; 128-byte swizzle) through one ring of 16 KB pieces in the order the products take
-// them: K_0, K_1, V_0, K_2, V_1, ...; S (two buffers), P (over its S, as the TMEM operand A)
-// and O live in tensor memory (256 + 2 x 128 columns).  A softmax thread owns a row: no
-// shuffles.  O is rescaled only when a row's maximum has grown by more than 2^8 since its
-// last scale (P then stays below 2^8, exact in either type up to its rounding); a row's sum
-// is kept in f32 before P is rounded.
+// rows of a tile (a batch of 64 streams with two q heads per kv head fills it); a unit is one
+// row tile and a run of the prefix's 64-key tiles, and per key tile
+//   S (128 x 64) = Q K^T,   P = 2^(scale log2(e) S - m),   O (128 x D) += P V.
+// Q, S (two buffers), P (over its S) and O live in tensor memory (128 + 2 x 64 + 256 columns
+// at D = 256; Q and P are the products' operand A), so that shared memory is one ring of K
+// and V alone: 16 KB pieces by TMA from the pages (K: a box per page and 64 dims, V: a box
+// per page; 128-byte swizzle) in the order the products take them: K_0, K_1, V_0, K_2, V_1,
+// ...  A softmax thread owns a row: no shuffles.  O is rescaled only when a row's maximum has
+// grown by more than 2^8 since its last scale (P then stays below 2^8, where either type
+// rounds as it does below 1); a row's sum is kept in f32 before P is rounded.
 //
-// Bound: HBM.  A key tile of D = 256 is 128 KB, about 5,700 cycles of one SM's share of the
-// bandwidth; its MMAs take 2,048 and its exponentials (16 per SM and cycle) 1,024, both
-// under the next tile's loads.
+// Bound: HBM.  A key tile of D = 256 is 64 KB, about 2,850 cycles of one SM's share of the
+// bandwidth; its products take 1,024 and its exponentials (16 per SM and cycle) 512, both
+// under the loads of the three tiles in the ring.
 //
-// Warps: 0 copies, 1 MMA issue (lane 0), 2-5 softmax and epilogue (TMEM lanes 32 * (warp %
-// 4)).  Every wait is bounded; one that gives up sets the status word and the abort flag,
+// Warps: 0, 6, 7 copies, 1 MMA issue, 2-5 softmax and epilogue (TMEM lanes 32 * (warp % 4)).  Every wait is bounded; one that gives up sets the status word and the abort flag,
 // the roles leave their loops, and the MMA warp's last commit is waited for before tensor
 // memory is released.
 #pragma once
@@ -90,20 +89,20 @@ struct PrefixParts {
   uint32_t max_splits;  // 0: the prefix is read stream by stream
 };
 namespace {
-constexpr uint32_t kKeys = 128, kRows = 128;
-constexpr uint32_t kPiece = 16384;
-constexpr int kTcThreads = 6 * 32, kSoft = 4 * 32;
-constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. D - 1; S: 256 and 384
+constexpr uint32_t kKeys = 64, kRows = 128;
+constexpr int kTcThreads = 8 * 32, kSoft = 4 * 32;
+constexpr uint32_t kTmemCols = 512, kQCol = 256, kSCol = 384;  // O: columns 0 .. D - 1; S: 384 and 448
 constexpr int kMasks = 8;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 
 template <int D>
 struct Tc {
-  static constexpr int kParts = D / 64;  // pieces of a K tile (64 dims each) and of a V tile
-  static constexpr uint32_t kVKeys = kPiece / (2 * D);  // keys of a V piece
-  static constexpr int kSlots = D == 256 ? 9 : D == 128 ? 11 : 12;
-  static constexpr uint32_t kOffRing = kRows * D * 2;
-  static constexpr uint32_t kBytes = kOffRing + kSlots * kPiece;
+  static constexpr uint32_t kPiece = D == 64 ? 8192 : 16384;
+  static constexpr int kParts = kKeys * D * 2 / kPiece;  // pieces of a K tile, and of a V tile
+  static constexpr int kDims = D / 64 / kParts;          // groups of 64 dims in a K piece
+  static constexpr uint32_t kVKeys = kPiece / (2 * D);   // keys of a V piece
+  static constexpr int kSlots = 13;
+  static constexpr uint32_t kBytes = kSlots * kPiece;
 };
 
 CH_DEV void tma_load_5d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int u, int w, uint64_t *bar) {
@@ -120,14 +119,7 @@ CH_DEV void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
-// A from shared memory / from tensor memory
-CH_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
+// A from tensor memory, B from shared memory
 CH_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -151,6 +143,12 @@ CH_DEV void tc_st32(uint32_t taddr, const uint32_t (&v)[32]) {
 }
 CH_DEV void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+CH_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r;
+}
+
 // instruction descriptor of kind::f16 with f32 sums: A K-major, B K-major or (mn) N-major
 CH_DEV uint32_t idesc_of(uint32_t n, bool bf16, bool mn) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) |
@@ -169,8 +167,8 @@ CH_DEV void st_global_32b(float *p, const uint32_t *v) {  // 32 bytes, 32-byte a
 }
 
 struct TcBars {
-  uint64_t full[12], empty[12], q_ready, s_full[2], p_ready[2], pv_done, done, mask_full[kMasks];
-  uint32_t masks[kMasks][4], tmem_slot, abort_flag;
+  uint64_t full[13], empty[13], q_ready, s_full[2], p_ready[2], pv_done, done, mask_full[kMasks];
+  uint32_t masks[kMasks][2], tmem_slot, abort_flag;
 };
 
 // One unit: kv head h, row tile rt, key tiles [i0, i0 + nt) of the prefix, whose positions
@@ -181,7 +179,8 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
                         uint8_t *sm, TcBars &bars, uint32_t h, uint32_t rt, uint32_t split, uint32_t i0, uint32_t nt,
                         uint32_t zlo) {
   using C = Tc<D>;
-  const uint32_t sbase = smem_u32(sm), ring = sbase + C::kOffRing;
+  constexpr uint32_t kPiece = C::kPiece;
+  const uint32_t ring = smem_u32(sm);
   uint64_t *full = bars.full, *empty = bars.empty, *s_full = bars.s_full, *p_ready = bars.p_ready,
            *mask_full = bars.mask_full;
   uint64_t &q_ready = bars.q_ready, &pv_done = bars.pv_done, &done = bars.done;
@@ -195,9 +194,9 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
 
   if (tid == 0) {
     for (int s = 0; s < C::kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 1), mbar_init(&p_ready[s], kSoft);
+    for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 1), mbar_init(&p_ready[s], 4);
     for (int s = 0; s < kMasks; s++) mbar_init(&mask_full[s], 1);
-    mbar_init(&q_ready, kSoft);
+    mbar_init(&q_ready, 4);
     mbar_init(&pv_done, 1);
     mbar_init(&done, 1);
     abort_flag = 0u;
@@ -214,151 +213,167 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   tc_fence_after();
   const uint32_t tmem = *(volatile uint32_t *)&bars.tmem_slot;
 
-  if (warp == 0) {
-    // ---- copies.  Lane l of a tile holds the page of its keys [l * kr, (l + 1) * kr) ----
+  // place in the ring's order of the first piece of K_i and of V_i
+  auto k_seq = [&](uint32_t i) { return i ? C::kParts * (2 * i - 1) : 0u; };
+  auto v_seq = [&](uint32_t i) { return C::kParts * (i + 1 < nt ? 2 * i + 2 : 2 * nt - 1); };
+
+  if (warp == 0 || warp == 6 || (warp == 7 && C::kParts == 2)) {
+    // ---- copies: warps 0 and 7 a half of each K tile, warp 6 V.  A box costs its warp about
+    // 60 cycles to issue and a piece 300 to claim; one warp for all of it took 3,750 cycles a
+    // tile of 16-token pages.  Lane l knows the page of keys [l * kr, (l + 1) * kr) ----
     const uint32_t ps = 1u << a.shift, kr = min(ps, kKeys), boxes = kKeys / kr;
-    auto look_up = [&](uint32_t i) {
-      const uint32_t j = i * kKeys + lane * kr;
-      if (lane >= (int)boxes || j >= a.prefix) return -1;
-      const int32_t page = a.prefix_table[j >> a.shift];
-      if (page >= 0 && (uint32_t)page < a.n_pages) return page;
-      if (a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
-      return -1;
+    const bool is_v = warp == 6;
+    auto look_up = [&](uint32_t i) {  // read a tile ahead, looked at when it is used
+      const uint32_t j = (i0 + i) * kKeys + lane * kr;
+      return i < nt && lane < (int)boxes && j < a.prefix ? a.prefix_table[j >> a.shift] : -1;
     };
-    uint32_t seq = 0;
+    int32_t next = look_up(0);
+    uint32_t last = 0;  // pieces up to here are on their way
     bool ok = true;
-    auto claim = [&]() {  // the next slot of the ring, its barrier armed
-      const uint32_t s = seq % C::kSlots;
-      if (seq >= (uint32_t)C::kSlots) ok = tc_wait(&empty[s], ((seq / C::kSlots) - 1) & 1, &abort_flag, a.status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && lane == 0) mbar_arrive_expect_tx(&full[s], kPiece);
-      __syncwarp();
-      if (ok) seq++;
-      return s;
-    };
-    // a page index past the pool reads as zeros
-    int32_t page = look_up(i0), next = -1, prev = -1;
-    for (uint32_t i = 0; i <= nt && ok; i++) {
-      if (i < nt) {
-        const uint32_t tile = i0 + i, j0 = tile * kKeys;
-        next = i + 1 < nt ? look_up(tile + 1) : -1;
-        // which keys are there: four per lane, put together to a word per eight lanes
-        const int32_t mine = __shfl_sync(0xffffffffu, page, lane * 4 / kr);
-        uint32_t bits = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) bits |= (mine >= 0 && j0 + lane * 4 + e < a.prefix ? 1u : 0u) << e;
-        bits <<= (lane & 7) * 4;
-        bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
-        bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
-        bits |= __shfl_xor_sync(0xffffffffu, bits, 4);
-        if ((lane & 7) == 0) masks[i % kMasks][lane >> 3] = bits;
+    for (uint32_t i = 0; i < nt && ok; i++) {
+      const uint32_t j0 = (i0 + i) * kKeys;
+      int32_t page = next;
+      next = look_up(i + 1);
+      const bool there = page >= 0 && (uint32_t)page < a.n_pages;
+      if (!there) {
+        if (a.status && lane < (int)boxes && j0 + lane * kr < a.prefix) atomicOr(a.status, DEV_ERR_BAD_LIST);
+        page = (int32_t)a.n_pages;  // reads as zeros
+      }
+      if (warp == 0) {  // which keys are there, a lane per key of each half
+        for (uint32_t half = 0; half < 2; half++) {
+          const uint32_t key = half * 32 + lane;
+          const bool in = __shfl_sync(0xffffffffu, there, key / kr);
+          const uint32_t bits = __ballot_sync(0xffffffffu, in && j0 + key < a.prefix);
+          if (lane == 0) masks[i % kMasks][half] = bits;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&mask_full[i % kMasks]);
-        for (int c = 0; c < C::kParts && ok; c++) {
-          const uint32_t s = claim();
-          if (ok && lane < (int)boxes)
-            tma_load_4d(ring + s * kPiece + lane * kr * 128, &kmap, c * 64, ps > kKeys ? (int)(j0 & (ps - 1)) : 0, (int)h,
-                        page >= 0 ? page : (int)a.n_pages, &full[s]);
-        }
       }
-      if (i > 0) {
-        const uint32_t j0 = (i0 + i - 1) * kKeys;
-        for (int c = 0; c < C::kParts && ok; c++) {
-          const uint32_t s = claim();
+      for (uint32_t c = is_v ? 0 : warp / 7; c < (is_v ? C::kParts : warp / 7 + 1u) && ok; c++) {
+        const uint32_t seq = (is_v ? v_seq(i) : k_seq(i)) + c, s = seq % C::kSlots;
+        if (seq >= (uint32_t)C::kSlots) ok = tc_wait(&empty[s], ((seq / C::kSlots) - 1) & 1, &abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], kPiece);
+        __syncwarp();
+        last = seq + 1;
+        if (is_v) {
           const uint32_t key = c * C::kVKeys + min((uint32_t)lane, C::kVKeys / vr - 1) * vr;
-          const int32_t pg = __shfl_sync(0xffffffffu, prev, key / kr);
-          if (ok && lane < (int)(C::kVKeys / vr))
-            tma_load_5d(ring + s * kPiece + lane * vr * 2 * D, &vmap, 0, (int)((j0 + key) & (ps - 1)), 0, (int)h,
-                        pg >= 0 ? pg : (int)a.n_pages, &full[s]);
+          const int32_t pg = __shfl_sync(0xffffffffu, page, key / kr);
+          if (lane < (int)(C::kVKeys / vr))
+            tma_load_5d(ring + s * kPiece + lane * vr * 2 * D, &vmap, 0, (int)((j0 + key) & (ps - 1)), 0, (int)h, pg,
+                        &full[s]);
+        } else {
+          const uint32_t b = lane % boxes, g = lane / boxes;  // box, and its group of dims
+          const int32_t pg = __shfl_sync(0xffffffffu, page, b);
+          if (g < C::kDims)
+            tma_load_4d(ring + s * kPiece + g * kKeys * 128 + b * kr * 128, &kmap, (c * C::kDims + g) * 64,
+                        ps > kKeys ? (int)(j0 & (ps - 1)) : 0, (int)h, pg, &full[s]);
         }
       }
-      prev = page;
-      page = next;
     }
     // the last copies land before the CTA may leave (normally long done)
-    if (lane == 0)
-      for (uint32_t j = seq > (uint32_t)C::kSlots ? seq - C::kSlots : 0; j < seq; j++)
-        tc_wait(&full[j % C::kSlots], (j / C::kSlots) & 1, nullptr, a.status);
+    const uint32_t total = 2 * C::kParts * nt, from = total > (uint32_t)C::kSlots ? total - C::kSlots : 0u;
+    for (uint32_t q = from; q < last; q++) tc_wait(&full[q % C::kSlots], (q / C::kSlots) & 1, &abort_flag, a.status);
   } else if (warp == 1) {
-    // ---- products ----
-    if (lane == 0) {
-      const uint32_t s_idesc = idesc_of(kKeys, std::is_same<T, __nv_bfloat16>::value, false);
-      const uint32_t o_idesc = idesc_of(D, std::is_same<T, __nv_bfloat16>::value, true);
-      uint32_t seq = 0;
-      bool ok = tc_wait(&q_ready, 0, &abort_flag, a.status);
-      auto take = [&]() {  // the next piece of the ring
-        const uint32_t s = seq % C::kSlots;
-        ok = ok && tc_wait(&full[s], (seq / C::kSlots) & 1, &abort_flag, a.status);
-        tc_fence_after();
-        seq++;
-        return s;
-      };
-      for (uint32_t i = 0; i <= nt && ok; i++) {
-        if (i < nt) {
-          // S_i lies where P_{i-2} lay
-          if (i >= 2) ok = tc_wait(&pv_done, (i - 2) & 1, &abort_flag, a.status);
-          for (int c = 0; c < C::kParts && ok; c++) {
-            const uint32_t s = take();
-            if (!ok) break;
-            const uint64_t qd = umma_desc_sw128(sbase + c * kRows * 128), kd = umma_desc_sw128(ring + s * kPiece);
+    // ---- products.  The warp walks the loop together and one elected lane issues: with the
+    // branch on lane 0 around everything and the descriptors built per instruction, issue
+    // (80 cycles an instruction) was slower than the products of N = 64 (49 cycles) ----
+    const uint32_t issuer = elect_one();
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    const uint32_t s_idesc = idesc_of(kKeys, kBf16, false), o_idesc = idesc_of(D, kBf16, true);
+    const uint32_t vs = vr == 8 ? 3 : vr == 16 ? 4 : vr == 32 ? 5 : 6;  // log2
+    const uint64_t v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 16u * D), k_hi = umma_desc_sw128(0);
+    uint32_t slot = 0, phase = 0;
+    bool ok = __all_sync(0xffffffffu, tc_wait(&q_ready, 0, &abort_flag, a.status));
+    tc_fence_after();
+    auto take = [&]() {  // waits for the next piece of the ring
+      ok = ok && tc_wait(&full[slot], phase, &abort_flag, a.status);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      return (ring + slot * kPiece) >> 4;
+    };
+    auto pass = [&]() {
+      if (++slot == (uint32_t)C::kSlots) slot = 0, phase ^= 1;
+    };
+    for (uint32_t i = 0; i <= nt && ok; i++) {
+      if (i < nt) {
+        // S_i lies where P_{i-2} lay
+        if (i >= 2) ok = __all_sync(0xffffffffu, tc_wait(&pv_done, (i - 2) & 1, &abort_flag, a.status));
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-              mma_ss(tmem + kSCol + (i & 1) * kKeys, qd + 2 * k, kd + 2 * k, s_idesc, (c | k) != 0);
-            commit(&empty[s]);
-          }
-          if (ok) commit(&s_full[i & 1]);
-        }
-        if (i > 0 && ok) {
-          const uint32_t j = i - 1;
-          ok = tc_wait(&p_ready[j & 1], (j >> 1) & 1, &abort_flag, a.status);
-          tc_fence_after();
-          for (int c = 0; c < C::kParts && ok; c++) {
-            const uint32_t s = take();
-            if (!ok) break;
+        for (int c = 0; c < C::kParts; c++) {
+          const uint32_t at = take();
+          if (!ok) break;
+          if (issuer) {
+            const uint32_t d = tmem + kSCol + (i & 1) * kKeys;
 #pragma unroll
-            for (uint32_t k = 0; k < C::kVKeys / 16; k++)
-              mma_ts(tmem, tmem + kSCol + (j & 1) * kKeys + (c * C::kVKeys + k * 16) / 2,
-                     v_desc(ring + s * kPiece + k * 16 / vr * vr * 2 * D + k * 16 % vr * 128, vr * 128,
-                            vr > 8 ? 1024u : 16u * D),
-                     o_idesc, (j | c | k) != 0);
-            commit(&empty[s]);
+            for (int k = 0; k < 4 * C::kDims; k++)
+              mma_ts(d, tmem + kQCol + (c * C::kDims * 4 + k) * 8, k_hi + (at + k / 4 * (kKeys * 8) + 2 * (k % 4)), s_idesc,
+                     (c | k) != 0);
+            commit(&empty[slot]);
+            if (c + 1 == C::kParts) commit(&s_full[i & 1]);
           }
-          if (ok) commit(&pv_done);
+          __syncwarp();
+          pass();
         }
       }
-      commit(&done);  // every MMA issued (all of them, or those before an abort) is complete
+      if (i > 0 && ok) {
+        const uint32_t j = i - 1;
+        ok = __all_sync(0xffffffffu, tc_wait(&p_ready[j & 1], (j >> 1) & 1, &abort_flag, a.status));
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < C::kParts; c++) {
+          const uint32_t at = take();
+          if (!ok) break;
+          if (issuer) {
+            const uint32_t p = tmem + kSCol + (j & 1) * kKeys + c * (C::kVKeys / 2);
+#pragma unroll
+            for (uint32_t k = 0; k < C::kVKeys / 16; k++) {
+              const uint32_t box = k * 16 >> vs, in = k * 16 & (vr - 1);
+              mma_ts(tmem, p + k * 8, v_hi + (at + box * (vr * D / 8) + in * 8), o_idesc, (j | c | k) != 0);
+            }
+            commit(&empty[slot]);
+            if (c + 1 == C::kParts) commit(&pv_done);
+          }
+          __syncwarp();
+          pass();
+        }
+      }
     }
-  } else if (warp < 6) {
+    if (issuer) commit(&done);  // every MMA issued (all of them, or those before an abort) is complete
+  } else if (warp >= 2 && warp < 6) {
     // ---- softmax: thread = query row ----
     const uint32_t quad = warp & 3, row = quad * 32 + lane, row0 = rt * kRows;
     const uint32_t lanes = (quad * 32u) << 16;
     constexpr uint32_t kVecs = D / 8;  // 16-byte pieces of a row
-    // the warp's 32 rows of Q, all copies in flight together; lane l knows row l's place
+    // this row of Q into tensor memory, 16 loads of 16 bytes in flight; a scale that is not
+    // positive goes into it: below it is |scale|
     const uint32_t gr = row0 + row;
-    const T *mine = gr < rows ? static_cast<const T *>(a.q) + (gr / a.group) * a.qs + (h * a.group + gr % a.group) * a.qh
-                              : nullptr;
-#pragma unroll 8
-    for (uint32_t u = 0; u < kVecs; u++) {
-      const uint32_t x = u * 32 + lane, v = x % kVecs, r = x / kVecs;
-      const T *src = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
-      uint8_t *dst = sm + (v >> 3) * kRows * 128 + (quad * 32 + r) * 128 + (((v & 7) ^ (r & 7)) << 4);
-      if (src)
-        cp_async16(dst, src + v * 8);
-      else
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
-    }
-    cp_async_wait_all();
-    if (!(a.scale > 0.f)) {  // a scale that is not positive goes into Q: below it is |scale|
-      __syncwarp();
-      for (uint32_t u = 0; u < kVecs; u++) {
-        const uint32_t x = u * 32 + lane, v = x % kVecs, r = x / kVecs;
-        uint4 *q = reinterpret_cast<uint4 *>(sm + (v >> 3) * kRows * 128 + (quad * 32 + r) * 128 + ((v & 7) << 4));
-        const uint32_t keep = a.scale < 0.f ? 0xFFFFFFFFu : 0u, flip = a.scale < 0.f ? 0x80008000u : 0u;
-        *q = make_uint4((q->x & keep) ^ flip, (q->y & keep) ^ flip, (q->z & keep) ^ flip, (q->w & keep) ^ flip);
+    const uint4 *q = gr < rows ? reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (gr / a.group) * a.qs +
+                                                                 (h * a.group + gr % a.group) * a.qh)
+                               : nullptr;
+    const uint32_t q_keep = a.scale == 0.f ? 0u : 0xFFFFFFFFu, q_flip = a.scale < 0.f ? 0x80008000u : 0u;
+    constexpr uint32_t kAt = kVecs < 16 ? kVecs : 16;
+#pragma unroll 1
+    for (uint32_t v0 = 0; v0 < kVecs; v0 += kAt) {
+      uint4 x[kAt];
+#pragma unroll
+      for (uint32_t v = 0; v < kAt; v++) x[v] = q ? q[v0 + v] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (uint32_t v = 0; v < kAt; v += 8) {
+        uint32_t r[32];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          r[4 * e] = (x[v + e].x & q_keep) ^ q_flip, r[4 * e + 1] = (x[v + e].y & q_keep) ^ q_flip;
+          r[4 * e + 2] = (x[v + e].z & q_keep) ^ q_flip, r[4 * e + 3] = (x[v + e].w & q_keep) ^ q_flip;
+        }
+        tc_st32(tmem + kQCol + lanes + (v0 + v) * 4, r);
       }
     }
-    fence_proxy_async();
-    mbar_arrive(&q_ready);
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_ready);
 
     uint32_t lo = 0;
     if (a.window && gr < rows) {
@@ -374,22 +389,19 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
            tc_wait(&mask_full[i % kMasks], (i / kMasks) & 1, &abort_flag, a.status);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; c++) tc_ld32(scol + c * 32, s[c]);
+      uint32_t s[2][32];
+      tc_ld32(scol, s[0]);
+      tc_ld32(scol + 32, s[1]);
       tc_wait_ld();
-      uint32_t mask[4];
-#pragma unroll
-      for (int c = 0; c < 4; c++) mask[c] = masks[i % kMasks][c];
+      uint32_t mask[2] = {masks[i % kMasks][0], masks[i % kMasks][1]};
       if (lo > j0) {  // hidden by the window
         const uint32_t hide = lo - j0;
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          if (hide >= 32u * c) mask[c] &= hide >= 32u * (c + 1) ? 0u : 0xFFFFFFFFu << (hide - 32u * c);
+        mask[0] &= hide >= 32 ? 0u : 0xFFFFFFFFu << hide;
+        if (hide >= 32) mask[1] &= hide >= 64 ? 0u : 0xFFFFFFFFu << (hide - 32);
       }
-      if (__any_sync(0xffffffffu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu)) {
+      if (__any_sync(0xffffffffu, (mask[0] & mask[1]) != 0xFFFFFFFFu)) {
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
           for (int e = 0; e < 32; e++)
             if (!((mask[c] >> e) & 1)) s[c][e] = 0xFF800000u;  // -inf
@@ -398,7 +410,7 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
 #pragma unroll
       for (int e = 0; e < 32; e++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
+        for (int c = 0; c < 2; c++) top[(2 * e + c) & 3] = fmaxf(top[(2 * e + c) & 3], __uint_as_float(s[c][e]));
       const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
       const bool grow = mx > m + kGrow || (m == -INFINITY && mx > -INFINITY);
       const float m1 = grow ? mx : m, ref = m1 == -INFINITY ? 0.f : m1;
@@ -422,27 +434,26 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
       }
       m = m1;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t p[32];
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        uint32_t p[32];
+      for (int c = 0; c < 2; c++) {
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const uint32_t b0 = s[c + (e >> 4)][(2 * e) & 31], b1 = s[c + (e >> 4)][(2 * e + 1) & 31];
-          const float p0 = exp2_approx(fmaf(__uint_as_float(b0), scale2, -ref));
-          const float p1 = exp2_approx(fmaf(__uint_as_float(b1), scale2, -ref));
+        for (int e = 0; e < 16; e++) {
+          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e]), scale2, -ref));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e + 1]), scale2, -ref));
           sum[e & 1] += p0;
           sum[2 + (e & 1)] += p1;
-          p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
+          p[c * 16 + e] = pack2(p0, p1, static_cast<const T *>(nullptr));
         }
-        tc_st32(scol + c * 16, p);
       }
+      tc_st32(scol, p);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tc_wait_st();
       // rows of V that no stream sees (past the prefix in its last page, before the first
       // visible position) are cleared: a weight of 0 must not meet stale bits
       const uint32_t z0 = zlo > j0 ? min(zlo - j0, kKeys) : 0u, z1 = a.prefix - j0 < kKeys ? a.prefix - j0 : kKeys;
       if (z0 > 0 || z1 < kKeys) {
-        const uint32_t seq0 = C::kParts * (i + 1 < nt ? 2 * i + 2 : 2 * nt - 1);
+        const uint32_t seq0 = v_seq(i);
         for (int c = 0; c < C::kParts; c++)
           ok = ok && tc_wait(&full[(seq0 + c) % C::kSlots], ((seq0 + c) / C::kSlots) & 1, &abort_flag, a.status);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -451,13 +462,14 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
           const uint32_t z = x / kVecs, key = z < n0 ? z : z1 + (z - n0), v = x % kVecs;
           const uint32_t slot = (seq0 + key / C::kVKeys) % C::kSlots;
           const uint32_t in = key % C::kVKeys;
-          *reinterpret_cast<uint4 *>(sm + C::kOffRing + slot * kPiece + in / vr * vr * 2 * D +
+          *reinterpret_cast<uint4 *>(sm + slot * kPiece + in / vr * vr * 2 * D +
                                      ((v >> 3) * vr + in % vr) * 128 + (v & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
       }
       tc_fence_before();
-      mbar_arrive(&p_ready[i & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[i & 1]);
     }
     // ---- this split's part ----
     ok = tc_wait(&done, 0, nullptr, a.status);
