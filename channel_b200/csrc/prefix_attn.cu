@@ -86,41 +86,45 @@ struct Work {       // in the caller's workspace
   float *o;    // [segments][group][D]; segment = run + pair, pair = stream * n_kv + head
   float2 *ml;  // [segments][group]: maximum, sum
 };
-// What a 64-key tile of the prefix and a unit's start and end cost, in 16-key tiles
-constexpr uint32_t kCostTile = 4, kCostUnit = 12;
+// What a 64-key tile of the prefix and a unit's start and end cost, in 16-key tiles.  By
+// bytes a tile costs 4; measured best is 3 (64 streams behind 4K / 32K tokens: 64 / 143 us,
+// with 4: 66 / 148, with 5: 67 / 157), because a unit's CTA has its SM's copies to itself.
+constexpr uint32_t kCostTile = 3, kCostUnit = 24;
 
-CH_DEV Deal deal_work(unsigned long long own, uint32_t ptiles, uint32_t per_split, uint32_t max_splits, uint32_t ctas,
+// own: 16-key tiles of all streams and kv heads (below 2^31).  The shares are estimates in
+// f32, the same in every CTA; y is then what exactly covers all tiles.
+CH_DEV Deal deal_work(uint32_t own, uint32_t ptiles, uint32_t per_split, uint32_t max_splits, uint32_t ctas,
                       uint32_t warps) {
   Deal d;
-  const unsigned long long prefix = (unsigned long long)ptiles * per_split * kCostTile;
+  const float prefix = (float)ptiles * per_split * kCostTile;
   d.splits = 0;
-  if (prefix) {
-    const unsigned long long all = own + prefix, step = all * per_split;
-    d.splits = (uint32_t)min((unsigned long long)min(max_splits, ptiles), (prefix * ctas + step - 1) / step);
-    d.splits = max(d.splits, 1u);
+  if (ptiles) {
+    const float want = ceilf(prefix * ctas / ((own + prefix) * per_split));
+    d.splits = max(1u, min(min(max_splits, ptiles), (uint32_t)want));
   }
   d.units = d.splits * per_split;
   d.unit_ctas = min(d.units, ctas);
-  const uint32_t rest = ctas - d.unit_ctas;
-  // a CTA's cost of its units, and the even share of everything
-  const unsigned long long used =
-      d.units ? (prefix + (unsigned long long)d.units * kCostUnit + d.unit_ctas - 1) / d.unit_ctas : 0ull;
-  const unsigned long long share = (own + used * d.unit_ctas + ctas - 1) / ctas;
+  const uint32_t rest = ctas - d.unit_ctas, x_runs = d.unit_ctas * warps;
   d.y_runs = rest * warps;
-  d.y = d.x = 0;
+  // a CTA's cost of its units, and the even share of everything
+  const float used = d.units ? (prefix + (float)d.units * kCostUnit) / d.unit_ctas : 0.f;
+  const float share = (own + used * d.unit_ctas) / ctas;
+  d.y = 0;
   if (rest == 0) {
-    d.x = (uint32_t)((own + (unsigned long long)ctas * warps - 1) / ((unsigned long long)ctas * warps));
-  } else if (used >= share) {
-    d.y = (uint32_t)((own + d.y_runs - 1) / d.y_runs);
+    d.x = (own + x_runs - 1) / x_runs;
   } else {
-    d.y = (uint32_t)((share + warps - 1) / warps);
-    d.x = (uint32_t)((share - used + warps - 1) / warps);
+    d.x = used < share ? (uint32_t)((share - used) / warps) : 0u;
+    if (own > d.x * x_runs) d.y = (own - d.x * x_runs + d.y_runs - 1) / d.y_runs;
   }
   return d;
 }
 
+// Registers: room for the join's CTAs beside it (they wait on the SM while this kernel runs),
+// but not where 16 query rows need them all.
+constexpr int attend_bound(int D, int NR) { return D == 256 && NR == 2 ? 256 : 320; }
+
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(Own<D>::kThreads, 1)
+__global__ void __launch_bounds__(attend_bound(D, NR), 1)
     attend_kernel(const PrefixArgs a, const Work w, const PrefixParts pp, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using O = Own<D>;
@@ -133,6 +137,7 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   __shared__ uint32_t masks[O::kWarps][O::kStages], sums[kThreads / 32], lo_min;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
 
+  grid_dep_wait();  // the kernel in front may still be running
   // ---- tiles per stream, summed over the streams; the first position any stream sees ----
   const uint32_t per_thread = (a.n + kThreads - 1) / kThreads, b0 = min(a.n, tid * per_thread), b1 = min(a.n, b0 + per_thread);
   uint32_t mine = 0, low = 0xFFFFFFFFu;
@@ -176,8 +181,7 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   const uint32_t zlo = min(lo_min, a.prefix), tile0 = zlo / kKeys;
   const uint32_t ptiles = pp.max_splits && zlo < a.prefix ? (a.prefix + kKeys - 1) / kKeys - tile0 : 0u;
   const uint32_t row_tiles = (a.n * a.group + kRows - 1) / kRows;
-  // 64-bit: n_kv times the tiles of all streams
-  const unsigned long long total = (unsigned long long)all * a.nkv;
+  const uint32_t total = all * a.nkv;
   const Deal d = deal_work(total, ptiles, a.nkv * row_tiles, pp.max_splits, gridDim.x, O::kWarps);
   if (blockIdx.x == gridDim.x - 1) {
     for (uint32_t b = tid; b <= a.n; b += kThreads) w.start[b] = start[b];
@@ -188,8 +192,8 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   // ---- the shared prefix ----
   for (uint32_t u = blockIdx.x; u < d.units; u += gridDim.x) {
     const uint32_t h = u % a.nkv, rt = (u / a.nkv) % row_tiles, split = u / (a.nkv * row_tiles);
-    const uint32_t i0 = (uint32_t)((unsigned long long)split * ptiles / d.splits);
-    const uint32_t i1 = (uint32_t)((unsigned long long)(split + 1) * ptiles / d.splits);
+    const uint32_t i0 = split * (ptiles / d.splits) + min(split, ptiles % d.splits);
+    const uint32_t i1 = i0 + ptiles / d.splits + (split < ptiles % d.splits);
     prefix_unit<T, D>(a, pp, kmap, vmap, smem, tc_bars, h, rt, split, tile0 + i0, i1 - i0, zlo);
   }
 
@@ -200,11 +204,9 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   const uint32_t run = with_unit ? d.y_runs + warp * d.unit_ctas + blockIdx.x
                                  : warp * (gridDim.x - d.unit_ctas) + blockIdx.x - d.unit_ctas;
   const uint32_t per = with_unit ? d.x : d.y;
-  const unsigned long long first =
-      with_unit ? (unsigned long long)d.y_runs * d.y + (unsigned long long)(run - d.y_runs) * d.x
-                : (unsigned long long)run * d.y;
+  const uint32_t first = with_unit ? d.y_runs * d.y + (run - d.y_runs) * d.x : run * d.y;
   if (per == 0 || first >= total) return;
-  uint32_t left = (uint32_t)min((unsigned long long)per, total - first);
+  uint32_t left = min(per, total - first);
 
   struct Cursor {
     uint32_t b, h, i, tiles, lo, hi;
@@ -220,12 +222,12 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
     uint32_t lo = 0, hi = a.n;
     while (lo + 1 < hi) {
       const uint32_t mid = (lo + hi) >> 1;
-      if ((unsigned long long)start[mid] * a.nkv <= first) lo = mid; else hi = mid;
+      if (start[mid] * a.nkv <= first) lo = mid; else hi = mid;
     }
     ld.b = lo;
     while (start[ld.b + 1] == start[ld.b]) ld.b++;
     enter(ld, true);
-    const uint32_t rem = (uint32_t)(first - (unsigned long long)start[ld.b] * a.nkv);
+    const uint32_t rem = first - start[ld.b] * a.nkv;
     ld.h = rem / ld.tiles;
     ld.i = rem % ld.tiles;
   }
@@ -239,6 +241,28 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
     if (c.b < a.n) enter(c, bounds);
   };
   Cursor cu = ld;
+  uint32_t qf[NR][kSteps][2];
+  float o[NR][kSteps][4], m[NR][2], l[NR][2];
+  const float scale2 = a.scale * 1.44269504088896341f;
+  const T *tag = nullptr;
+  auto begin_pair = [&]() {  // the pair's query rows and empty sums
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+      const uint32_t qr = r * 8 + g;
+      const T *q = static_cast<const T *>(a.q) + cu.b * a.qs + (cu.h * a.group + qr) * a.qh + 2 * t4;
+#pragma unroll
+      for (int k = 0; k < kSteps; k++) {
+        qf[r][k][0] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k) : 0u;
+        qf[r][k][1] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8) : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[r][k][e] = 0.f;
+      }
+      m[r][0] = m[r][1] = -INFINITY;
+      l[r][0] = l[r][1] = 0.f;
+    }
+  };
+  begin_pair();  // these reads and the first page reads are in flight together
+  bool fresh = false;
   uint8_t *ring = smem + warp * O::kStages * O::kStage;
   const T *pool = static_cast<const T *>(lane < 16 ? a.k : a.v);
   uint32_t to_load = left;
@@ -296,11 +320,6 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   };
   read_ahead();
 
-  uint32_t qf[NR][kSteps][2];
-  float o[NR][kSteps][4], m[NR][2], l[NR][2];
-  const float scale2 = a.scale * 1.44269504088896341f;
-  const T *tag = nullptr;
-  bool fresh = true;
   const uint32_t frag = smem_u32(ring);
   // fragment addresses of this lane: K rows by key, V columns by key
   const uint32_t k_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * O::kPitch + (lane >> 4) * 16;
@@ -308,22 +327,9 @@ __global__ void __launch_bounds__(Own<D>::kThreads, 1)
   int stage = 0;
   uint32_t parity = 0;
   for (; left; left--) {
-    if (fresh) {  // the pair's query rows and empty sums
+    if (fresh) {
       fresh = false;
-#pragma unroll
-      for (int r = 0; r < NR; r++) {
-        const uint32_t qr = r * 8 + g;
-        const T *q = static_cast<const T *>(a.q) + cu.b * a.qs + (cu.h * a.group + qr) * a.qh + 2 * t4;
-#pragma unroll
-        for (int k = 0; k < kSteps; k++) {
-          qf[r][k][0] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k) : 0u;
-          qf[r][k][1] = qr < a.group ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8) : 0u;
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[r][k][e] = 0.f;
-        }
-        m[r][0] = m[r][1] = -INFINITY;
-        l[r][0] = l[r][1] = 0.f;
-      }
+      begin_pair();
     }
     const bool ok = mbar_wait_bounded(&bars[warp][stage], parity, a.status);
     if (!__all_sync(0xffffffffu, ok)) {  // reported; the copies still in flight get a wait of their own
@@ -432,15 +438,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
   if (row >= a.n * a.nq) return;
   const uint32_t b = row / a.nq, hq = row % a.nq, h = hq / a.group, r = hq % a.group;
   grid_dep_wait();
+  grid_dep_launch();
   // the row's parts: one per split of the shared prefix, then one per warp whose run touched
   // the pair (b, h)
   const uint32_t s0 = w.start[b], tiles = w.start[b + 1] - s0;
   const Deal d = *w.deal;
-  const unsigned long long t0 = (unsigned long long)s0 * a.nkv + (unsigned long long)h * tiles;
-  const unsigned long long y_tiles = (unsigned long long)d.y_runs * d.y;
-  auto run_of = [&](unsigned long long t) {
-    return t < y_tiles ? (uint32_t)(t / d.y) : d.y_runs + (uint32_t)((t - y_tiles) / d.x);
-  };
+  const uint32_t t0 = s0 * a.nkv + h * tiles, y_tiles = d.y_runs * d.y;
+  auto run_of = [&](uint32_t t) { return t < y_tiles ? t / d.y : d.y_runs + (t - y_tiles) / d.x; };
   const uint32_t w0 = tiles ? run_of(t0) : 0u, own = tiles ? run_of(t0 + tiles - 1) - w0 + 1 : 0u;
   const size_t rows = (size_t)a.n * a.group, at_prefix = (size_t)h * rows + (size_t)b * a.group + r;
   const size_t at_own = ((size_t)w0 + (size_t)b * a.nkv + h) * a.group + r;
@@ -452,6 +456,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
     return (p < d.splits ? pp.o + (at_prefix + (size_t)p * a.nkv * rows) * D
                           : w.o + (at_own + (size_t)(p - d.splits) * a.group) * D) + lane * EPL;
   };
+  constexpr uint32_t kU = 4;  // parts whose loads are in flight together, the first before the maxima are known
+  float v[kU][EPL];
+  auto load = [&](uint32_t p0) {
+#pragma unroll
+    for (uint32_t u = 0; u < kU; u++) {
+      if (p0 + u >= parts) break;
+      const float *src = o_of(p0 + u);
+      if constexpr (EPL == 2) {
+        *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4 *>(&v[u][e]) = *reinterpret_cast<const float4 *>(src + e);
+      }
+    }
+  };
+  load(0);
   float top = -INFINITY;
   for (uint32_t p = lane; p < parts; p += 32) top = fmaxf(top, ml_of(p).x);
   top = warp_max(top);
@@ -460,35 +480,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Pref
 #pragma unroll
   for (int e = 0; e < EPL; e++) o[e] = 0.f;
   for (uint32_t p0 = 0; p0 < parts; p0 += 32) {
-    const uint32_t n = min(32u, parts - p0);
     float f = 0.f;
-    if ((uint32_t)lane < n) {
-      const float2 v = ml_of(p0 + lane);
-      f = exp2_approx(v.x - ref);
-      sum = fmaf(v.y, f, sum);
+    if (p0 + lane < parts) {
+      const float2 x = ml_of(p0 + lane);
+      f = exp2_approx(x.x - ref);
+      sum = fmaf(x.y, f, sum);
     }
-    constexpr uint32_t kU = 4;  // parts whose loads are in flight together
-    for (uint32_t k = 0; k < n; k += kU) {
-      float v[kU][EPL], fk[kU];
+    for (uint32_t k = 0; k < 32 && p0 + k < parts; k += kU) {
+      if (p0 + k) load(p0 + k);
 #pragma unroll
       for (uint32_t u = 0; u < kU; u++) {
-        fk[u] = __shfl_sync(0xffffffffu, f, (k + u) & 31);
-        if (k + u >= n) fk[u] = 0.f;
+        const float fk = __shfl_sync(0xffffffffu, f, k + u);  // 0 past the last part
+        if (fk == 0.f) continue;  // a part without a visible position has no O
 #pragma unroll
-        for (int e = 0; e < EPL; e++) v[u][e] = 0.f;
-        if (fk[u] == 0.f) continue;  // a part without a visible position has no O
-        const float *src = o_of(p0 + k + u);
-        if constexpr (EPL == 2) {
-          *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
-        } else {
-#pragma unroll
-          for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4 *>(&v[u][e]) = *reinterpret_cast<const float4 *>(src + e);
-        }
+        for (int e = 0; e < EPL; e++) o[e] = fmaf(v[u][e], fk, o[e]);
       }
-#pragma unroll
-      for (uint32_t u = 0; u < kU; u++)
-#pragma unroll
-        for (int e = 0; e < EPL; e++) o[e] = fmaf(v[u][e], fk[u], o[e]);
     }
   }
   sum = warp_sum(sum);
@@ -572,10 +578,10 @@ size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w, PrefixParts *
   return at;
 }
 
-// kernel<<<grid, block, smem, s>>>(args...); after: it may start before the kernel in front of
-// it ends
+// kernel<<<grid, block, smem, s>>>(args...), which may start before the kernel in front of it
+// ends: both kernels here wait for that one before they read or write anything
 template <typename K, typename... A>
-cudaError_t start_kernel(K kernel, uint32_t grid, uint32_t block, size_t smem, cudaStream_t s, bool after, const A &...args) {
+cudaError_t start_kernel(K kernel, uint32_t grid, uint32_t block, size_t smem, cudaStream_t s, const A &...args) {
   cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -587,7 +593,7 @@ cudaError_t start_kernel(K kernel, uint32_t grid, uint32_t block, size_t smem, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = after ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -606,10 +612,9 @@ cudaError_t launch_t(PrefixArgs a, const Work &w, PrefixParts pp, cudaStream_t s
   a.from = pp.max_splits ? a.prefix : 0;
   const size_t smem = 1024 + Own<D>::kOffStart + ((size_t)a.n + 1) * sizeof(uint32_t);
   const cudaError_t e = start_kernel(a.group <= 8 ? attend_kernel<T, D, 1> : attend_kernel<T, D, 2>, num_sms(),
-                                     Own<D>::kThreads, smem, s, false, a, w, pp, kmap, vmap);
+                                     Own<D>::kThreads, smem, s, a, w, pp, kmap, vmap);
   if (e != cudaSuccess) return e;
-  return start_kernel(attend_join_kernel<T, D>, (a.n * a.nq + kJoinWarps - 1) / kJoinWarps, kJoinWarps * 32, 0, s, true, a,
-                      w, pp);
+  return start_kernel(attend_join_kernel<T, D>, (a.n * a.nq + kJoinWarps - 1) / kJoinWarps, kJoinWarps * 32, 0, s, a, w, pp);
 }
 template <typename T>
 cudaError_t launch(const PrefixArgs &a, const Work &w, const PrefixParts &pp, uint32_t D, cudaStream_t s) {
@@ -628,8 +633,8 @@ const char *check(const ch_prefix_attn_args *p) {
   if (p->n_pages > 0x7FFFFFFFu || p->table_cols > 0x7FFFFFFFu || p->prefix_len > 0x7FFFFFFFu)
     return "a size is 2^31 or more";
   const unsigned long long reach = p->prefix_len + (unsigned long long)p->table_cols * p->page_size;
-  if (reach >= 1ull << 32 || (reach / 16 + 1) * p->n_streams >= 1ull << 32)
-    return "the positions of all streams exceed 2^36";
+  if (reach >= 1ull << 32 || (reach / 16 + 1) * p->n_streams >= (1ull << 31) / p->n_kv)
+    return "the positions of all streams and kv heads exceed 2^35";
   if (p->dtype != CH_F16 && p->dtype != CH_BF16) return "dtype must be CH_F16 or CH_BF16";
   return nullptr;
 }

@@ -57,7 +57,11 @@ CH_DEV float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-CH_DEV uint32_t pack2(float lo, float hi, const __half *) { return pack_half2(__float2half_rn(lo), __float2half_rn(hi)); }
+// two values in one conversion: single ones share the exponential's pipe (16 a cycle and SM)
+CH_DEV uint32_t pack2(float lo, float hi, const __half *) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
 CH_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16 *) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&v);
