@@ -191,11 +191,12 @@ SIGNATURES = {
     "ch_ring_dev_lists": (i32, [vp, u32, i32, sz, vp, vp, vp, vp, vp]),
     "ch_ring_dev_prefill_prev": (i32, [vp, u32, u32, vp, vp]),
     "ch_decode_run_ring": (i32, [vp, vp, vp, u32, u32, u32]),
-    "ch_page_plan": (i32, [P(ChPagePlanArgs), vp]),
-    "ch_paged_kv_write": (i32, [P(ChKvWriteArgs), vp]),
-    "ch_prefix_attention_workspace": (sz, [P(ChPrefixAttnArgs)]),
-    "ch_prefix_attention": (i32, [P(ChPrefixAttnArgs), vp, sz, vp]),
-    "ch_sample_rows": (i32, [P(ChSampleRowsArgs), vp]),
+    # argument records: byref(ChPagePlanArgs(...)) and so on, or their packed bytes
+    "ch_page_plan": (i32, [vp, vp]),
+    "ch_paged_kv_write": (i32, [vp, vp]),
+    "ch_prefix_attention_workspace": (sz, [vp]),
+    "ch_prefix_attention": (i32, [vp, vp, sz, vp]),
+    "ch_sample_rows": (i32, [vp, vp]),
 }
 
 _lib = None

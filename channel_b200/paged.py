@@ -16,7 +16,7 @@ ch_ctx_device_status that the kernels report; ``check_status`` raises on them.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -24,7 +24,20 @@ import torch
 from . import _lib as L
 
 _DTYPES = {torch.float32: L.CH_F32, torch.float16: L.CH_F16, torch.bfloat16: L.CH_BF16}
+_I32 = torch.int32
 _NO_PAGES, _BAD = 1 << 5, (1 << 1) | (1 << 2)
+
+# A step makes these calls once per layer, so their host time counts: the argument records
+# are packed in one go (the layouts of the ctypes structures of the same name in _lib).
+_PLAN = struct.Struct("@10Pq6IP")
+_WRITE = struct.Struct("@5P7q5I2iP")
+_ATTEND = struct.Struct("@7P8q9IfiP")
+
+try:  # torch's current stream of a device as a cudaStream_t, without building a Stream object
+    _stream_of = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _stream_of(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 class PagePlan(NamedTuple):
@@ -41,32 +54,46 @@ def _fail(msg: str):
     raise L.ChannelError(L.CH_EINVAL, msg)
 
 
-def _i32(t: torch.Tensor, dim: int, dev, name: str) -> int:
-    """Pointer of a dense int32 tensor (the last dimension; a table's rows may be strided)."""
-    if t.dtype is not torch.int32 or t.dim() != dim or t.device != dev or (t.stride(-1) != 1 and t.numel() > 1):
-        _fail(f"{name}: a {dim}-dimensional int32 tensor on {dev}, dense in its last dimension, is wanted")
+def _vec(t: torch.Tensor, n: int, at: int, name: str) -> int:
+    """Pointer of a dense int32 vector of n elements (n < 0: any) on device `at`."""
+    if t.dtype is not _I32 or t.dim() != 1 or t.get_device() != at or (n >= 0 and t.shape[0] != n) or \
+            not t.is_contiguous():
+        _fail(f"{name}: a dense int32 vector{f' of {n} elements' if n >= 0 else ''} on the other tensors' device is wanted")
     return t.data_ptr()
 
 
-def _status(status: Optional[torch.Tensor], dev) -> Optional[int]:
+def _table(t: torch.Tensor, n: int, at: int, name: str) -> int:
+    """Pointer of an int32 table of n rows, dense along a row, on device `at`."""
+    if t.dtype is not _I32 or t.dim() != 2 or t.get_device() != at or t.shape[0] != n or \
+            (t.stride(1) != 1 and t.shape[1] > 1):
+        _fail(f"{name}: an int32 table of {n} rows, dense along a row, on the other tensors' device is wanted")
+    return t.data_ptr()
+
+
+def _status(status: Optional[torch.Tensor], at: int) -> int:
     if status is None:
-        return None
-    if status.dtype is not torch.int32 or status.device != dev or status.numel() != 1:
+        return 0
+    if status.dtype is not _I32 or status.get_device() != at or status.numel() != 1:
         _fail("status: an int32 tensor of one element on the other tensors' device is wanted")
     return status.data_ptr()
 
 
-def _run(fn, dev, *args) -> None:
-    """fn(*args, stream) on dev's current torch stream."""
-    if dev.type != "cuda":
-        _fail("tensors on a CUDA device are wanted")
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _run(fn, at: int, *args) -> None:
+    """fn(*args, stream) on device `at` and its current torch stream."""
+    if at == torch.cuda.current_device():
+        rc = fn(*args, _stream_of(at))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    if rc != L.CH_OK:
+        with torch.cuda.device(at):
+            rc = fn(*args, _stream_of(at))
+    if rc:
         L.check(rc)
+
+
+def _device(t: torch.Tensor) -> int:
+    at = t.get_device()
+    if at < 0:
+        _fail("tensors on a CUDA device are wanted")
+    return at
 
 
 def check_status(status: torch.Tensor) -> None:
@@ -77,6 +104,8 @@ def check_status(status: torch.Tensor) -> None:
         raise L.ChannelError(L.CH_ENOMEM, "a page plan ran out of pages, table columns or token rows")
     if bits & _BAD:
         raise L.ChannelError(L.CH_EDEVICE, "a kernel saw a slot or page outside its pool")
+    if bits:
+        raise L.ChannelError(L.CH_ETIMEOUT, "a bounded device wait gave up")
 
 
 def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -85,43 +114,51 @@ def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor
     """Block tables (``table``, in place), slot map, positions and row map of a step that
     appends ``new_tokens`` to streams holding ``lens`` tokens; pages come from the front of
     ``free_pages`` (``counts[1]`` of them)."""
-    dev, n = lens.device, lens.shape[0]
-    pad = (max_tokens + 3) & ~3  # the token arrays start on 16 bytes
-    buf = torch.empty(3 * pad + 2 * n + 3, dtype=torch.int32, device=dev)
-    slots, positions, rows, lens_out, starts, counts = buf.split_with_sizes((pad, pad, pad, n, n + 1, 2))
-    a = L.ChPagePlanArgs(
-        _i32(lens, 1, dev, "lens"), _i32(new_tokens, 1, dev, "new_tokens"), _i32(free_pages, 1, dev, "free_pages"),
-        _i32(table, 2, dev, "table"), lens_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-        rows.data_ptr(), counts.data_ptr(), table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
-        max_tokens, prefix_len, _status(status, dev))
-    if new_tokens.shape[0] != n or table.shape[0] != n:
-        _fail("plan_pages: lens, new_tokens and table differ in their number of streams")
-    _run(L.load().ch_page_plan, dev, C.byref(a))
-    if pad != max_tokens:
-        slots, positions, rows = slots[:max_tokens], positions[:max_tokens], rows[:max_tokens]
+    at, n = _device(lens), lens.shape[0]
+    p_lens, p_new = _vec(lens, n, at, "lens"), _vec(new_tokens, n, at, "new_tokens")
+    p_free, p_table = _vec(free_pages, -1, at, "free_pages"), _table(table, n, at, "table")
+    if max_tokens < 0 or prefix_len < 0 or page_size < 0:
+        _fail("plan_pages: negative size")
+    pad = -max_tokens & 3  # the token arrays start on 16 bytes
+    buf = lens.new_empty(3 * (max_tokens + pad) + 2 * n + 3)
+    if pad:
+        slots, _, positions, _, rows, _, lens_out, starts, counts = buf.split_with_sizes(
+            (max_tokens, pad, max_tokens, pad, max_tokens, pad, n, n + 1, 2))
+    else:
+        slots, positions, rows, lens_out, starts, counts = buf.split_with_sizes(
+            (max_tokens, max_tokens, max_tokens, n, n + 1, 2))
+    p, step = buf.data_ptr(), 4 * (max_tokens + pad)
+    args = _PLAN.pack(p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step, p + 2 * step,
+                      p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
+                      max_tokens, prefix_len, _status(status, at))
+    _run(L.load().ch_page_plan, at, args)
     return PagePlan(table, lens_out, starts, slots, positions, rows, counts)
 
 
-def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor, dev):
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride() or \
-            k_pool.dtype is not v_pool.dtype or k_pool.device != dev or v_pool.device != dev or k_pool.stride(3) != 1:
+def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor, at: int):
+    shape, strides = k_pool.shape, k_pool.stride()
+    if len(shape) != 4 or shape != v_pool.shape or strides != v_pool.stride() or k_pool.dtype is not v_pool.dtype or \
+            k_pool.get_device() != at or v_pool.get_device() != at or strides[3] != 1:
         _fail("k_pool and v_pool: [n_pages, page_size, n_kv, head_dim] of one type, strides and device")
-    return k_pool.shape, k_pool.stride()
+    return shape, strides
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
              status: Optional[torch.Tensor] = None) -> None:
     """Rows k[t], v[t] (``[tokens, n_kv, head_dim]``, any token and head strides) into slot
     slots[t] of the pools; negative slots are skipped."""
-    dev = k.device
-    (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, dev)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (n_kv, dim) or k.dtype is not v.dtype or \
-            v.device != dev or k.stride(2) != 1 or v.stride(2) != 1 or slots.shape[0] != k.shape[0]:
-        _fail("kv_write: k and v are [tokens, n_kv, head_dim] of one type, with one slot per token")
-    a = L.ChKvWriteArgs(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _i32(slots, 1, dev, "slots"),
-                        k.stride(0), k.stride(1), v.stride(0), v.stride(1), ps, ts, hs, k.shape[0], n_kv, dim, page,
-                        pages, _DTYPES.get(k.dtype, -1), _DTYPES.get(k_pool.dtype, -1), _status(status, dev))
-    _run(L.load().ch_paged_kv_write, dev, C.byref(a))
+    at = k.get_device()
+    (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
+    shape, kind = k.shape, k.dtype
+    (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
+    if len(shape) != 3 or shape != v.shape or shape[1] != n_kv or shape[2] != dim or kind is not v.dtype or \
+            v.get_device() != at or k1 != 1 or v1 != 1:
+        _fail("kv_write: k and v are [tokens, n_kv, head_dim] of one type, dense in the last dimension")
+    _device(k)
+    args = _WRITE.pack(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _vec(slots, shape[0], at, "slots"),
+                       kt, kh, vt, vh, ps, ts, hs, shape[0], n_kv, dim, page, pages, _DTYPES.get(kind, -1),
+                       _DTYPES.get(k_pool.dtype, -1), _status(status, at))
+    _run(L.load().ch_paged_kv_write, at, args)
 
 
 def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
@@ -132,29 +169,32 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     prefix_len tokens in the pages of prefix_table and the stream's own lens[b] tokens in
     those of table[b]; window > 0 leaves the last ``window`` positions visible.  scale
     defaults to head_dim ** -0.5."""
-    dev = q.device
-    (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, dev)
-    if q.dim() != 3 or q.shape[2] != dim or q.dtype is not k_pool.dtype or q.stride(2) != 1 or \
-            lens.shape[0] != q.shape[0] or table.shape[0] != q.shape[0]:
-        _fail("prefix_attention: q is [streams, n_q, head_dim] of the pools' type, with lens and table rows per stream")
-    n, n_q, _ = q.shape
-    if out is None:
-        out = torch.empty((n, n_q, dim), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1:
-        _fail("prefix_attention: out is like q")
+    at = q.get_device()
+    (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
+    shape, kind = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != dim or kind is not k_pool.dtype or q.stride(2) != 1:
+        _fail("prefix_attention: q is [streams, n_q, head_dim] of the pools' type, dense in the last dimension")
+    n, n_q, _ = shape
+    if prefix_len < 0 or window < 0:
+        _fail("prefix_attention: negative size")
     if prefix_len and (prefix_table is None or prefix_table.shape[0] * page < prefix_len):
         _fail("prefix_attention: prefix_table is shorter than prefix_len")
-    a = L.ChPrefixAttnArgs(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
-        None if prefix_table is None else _i32(prefix_table, 1, dev, "prefix_table"), _i32(table, 2, dev, "table"),
-        _i32(lens, 1, dev, "lens"), q.stride(0), q.stride(1), out.stride(0), out.stride(1), ps, ts, hs,
-        table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1], prefix_len, window,
-        dim ** -0.5 if scale is None else scale, _DTYPES.get(q.dtype, -1), _status(status, dev))
-    lib, ref = L.load(), C.byref(a)
-    if dev.type != "cuda":
-        _fail("tensors on a CUDA device are wanted")
-    need = lib.ch_prefix_attention_workspace(ref)
-    # torch's caching allocator hands the workspace out in the stream's order
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _run(lib.ch_prefix_attention, dev, ref, work.data_ptr() if need else None, need)
+    p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
+    p_table, p_lens = _table(table, n, at, "table"), _vec(lens, n, at, "lens")
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not kind or out.get_device() != at or out.stride(2) != 1:
+        _fail("prefix_attention: out is like q")
+    _device(q)
+    (qs, qh, _), (os, oh, _) = q.stride(), out.stride()
+    args = _ATTEND.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_prefix, p_table, p_lens, qs,
+                        qh, os, oh, ps, ts, hs, table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1], prefix_len,
+                        window, dim ** -0.5 if scale is None else scale, _DTYPES.get(kind, -1), _status(status, at))
+    lib = L.load()
+    need = lib.ch_prefix_attention_workspace(args)
+    if need:  # torch's caching allocator hands the workspace out in the stream's order
+        work = q.new_empty(need, dtype=torch.uint8)
+        _run(lib.ch_prefix_attention, at, args, work.data_ptr(), need)
+    else:  # sizes the call refuses
+        _run(lib.ch_prefix_attention, at, args, None, 0)
     return out

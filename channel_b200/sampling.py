@@ -8,20 +8,23 @@ gives.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib as L
-from .paged import _DTYPES, _fail, _run
+from .paged import _DTYPES, _device, _fail, _run
+
+_ROWS = struct.Struct("@9Pq2Ifi")  # ChSampleRowsArgs of _lib
+_F32, _I32 = torch.float32, torch.int32
 
 
-def _per_row(t: Optional[torch.Tensor], kind, n: int, dev, name: str) -> Optional[int]:
+def _per_row(t: Optional[torch.Tensor], kind, n: int, at: int, name: str) -> int:
     if t is None:
-        return None
-    if t.dtype is not kind or t.dim() != 1 or t.shape[0] != n or t.device != dev or (n > 1 and t.stride(0) != 1):
-        _fail(f"sample_rows: {name} is a dense {kind} tensor of one value per row on {dev}")
+        return 0
+    if t.dtype is not kind or t.dim() != 1 or t.shape[0] != n or t.get_device() != at or not t.is_contiguous():
+        _fail(f"sample_rows: {name} is a dense {kind} tensor of one value per row on the logits' device")
     return t.data_ptr()
 
 
@@ -34,22 +37,25 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
     may be strided).  uniform: float32 in [0, 1) per row.  Settings are tensors of one value
     per row (top_k int32, the rest float32) or None; temperature <= 0 takes the largest
     logit."""
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        _fail("sample_rows: logits is [rows, vocab], dense in its last dimension")
-    n, vocab = logits.shape
-    dev, f32 = logits.device, torch.float32
-    out = torch.empty((3, n), dtype=torch.int32, device=dev)
-    tokens, kept, logprobs = out.unbind(0)
-    logprobs = logprobs.view(f32)
-    if n == 0:
-        return tokens, logprobs, kept
-    at = out.data_ptr()
+    shape = logits.shape
+    if len(shape) != 2:
+        _fail("sample_rows: logits is [rows, vocab]")
+    (n, vocab), (row, step) = shape, logits.stride()
+    if step != 1 and vocab > 1:
+        _fail("sample_rows: logits is dense in its last dimension")
     if uniform is None:
         _fail("sample_rows: uniform is needed")
-    a = L.ChSampleRowsArgs(
-        logits.data_ptr(), _per_row(uniform, f32, n, dev, "uniform"), _per_row(temperature, f32, n, dev, "temperature"),
-        _per_row(top_p, f32, n, dev, "top_p"), _per_row(min_p, f32, n, dev, "min_p"),
-        _per_row(top_k, torch.int32, n, dev, "top_k"), at, at + 4 * n, at + 8 * n, logits.stride(0), n, vocab, softcap,
-        _DTYPES.get(logits.dtype, -1))
-    _run(L.load().ch_sample_rows, dev, C.byref(a))
+    at = logits.get_device()
+    p_uniform, p_temp = _per_row(uniform, _F32, n, at, "uniform"), _per_row(temperature, _F32, n, at, "temperature")
+    p_top_p, p_min_p = _per_row(top_p, _F32, n, at, "top_p"), _per_row(min_p, _F32, n, at, "min_p")
+    p_top_k = _per_row(top_k, _I32, n, at, "top_k")
+    _device(logits)
+    out = logits.new_empty(3 * n, dtype=_I32)
+    tokens, kept, logprobs = out.split_with_sizes((n, n, n))
+    logprobs = logprobs.view(_F32)
+    if n:
+        p = out.data_ptr()
+        _run(L.load().ch_sample_rows, at,
+             _ROWS.pack(logits.data_ptr(), p_uniform, p_temp, p_top_p, p_min_p, p_top_k, p, p + 4 * n, p + 8 * n, row, n,
+                        vocab, softcap, _DTYPES.get(logits.dtype, -1)))
     return tokens, logprobs, kept

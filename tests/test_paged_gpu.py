@@ -489,3 +489,16 @@ def test_wrappers_refuse():
                  (lens, lens, table.long(), lens, 16, 4), (lens, lens, table, lens, 16, 4)]:
         with pytest.raises(L.ChannelError):
             paged.plan_pages(*args)
+
+
+def test_packed_arguments_match_the_structures():
+    """the wrappers' packed records have the field offsets of the ctypes structures"""
+    import ctypes as C
+
+    from channel_b200 import sampling
+    for fmt, kind in ((paged._PLAN, L.ChPagePlanArgs), (paged._WRITE, L.ChKvWriteArgs), (paged._ATTEND, L.ChPrefixAttnArgs),
+                      (sampling._ROWS, L.ChSampleRowsArgs)):
+        assert fmt.size == C.sizeof(kind)
+        values = [float(i + 1) if t is C.c_float else i + 1 for i, (_, t) in enumerate(kind._fields_)]
+        got = kind.from_buffer_copy(fmt.pack(*values))
+        assert [getattr(got, n) for n, _ in kind._fields_] == values
