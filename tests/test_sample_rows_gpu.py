@@ -214,6 +214,50 @@ def test_masked_rows():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("v", [600, 70000])
+def test_masks_stay_masked_under_the_cap(v, dtype):
+    """tokens masked with -inf or the type's lowest value are not drawn, however warm; a row
+    of nothing but masks of the lowest value is even"""
+    x = torch.randn(64, v)
+    x[:, 10:] = torch.finfo(dtype).min
+    x[:, 100:] = -torch.inf
+    x[1:3] = torch.finfo(dtype).min
+    for kw in (dict(), dict(top_p=0.99999), dict(top_k=300), dict(min_p=1e-6), dict(top_k=1)):
+        token, lp, kept = draw(x.to(dtype), (np.arange(64) + 0.5) / 64, 30.0, temperature=50.0, **kw)
+        assert (token[[0, *range(3, 64)]] < 10).all() and (kept[[0, *range(3, 64)]] <= 10).all()
+        if not kw:
+            assert kept[1] == kept[2] == v and token[1] == int(1.5 / 64 * v)
+
+
+@gpu
+def test_saturated_cap_ties():
+    """logits far past the cap are equal: cuts and greedy take the lowest indices"""
+    x = torch.full((4, 50000), 1.0)
+    x[:, 7::5000] = 400.0 + torch.arange(10.0)
+    x[2] = 400.0 + torch.rand(50000)
+    x[3] = 400.0 + torch.rand(50000)
+    token, _, kept = draw(x, 0.999, 30.0, temperature=[0.0, 1.0, 0.0, 1.0], top_k=[0, 4, 0, 100])
+    assert token.tolist() == [7, 15007, 0, 99] and kept.tolist() == [1, 4, 1, 100]
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-3, 0.37, 3.0, 1e4, 1e30])
+@pytest.mark.parametrize("scale", [1e-4, 1.0, 1e4])
+def test_scales(scale, temperature):
+    """logits of any scale, temperatures from near 0 to where all weights are equal"""
+    n = 9
+    x = lm_logits(n, 70001, 4) * scale
+    u = np.linspace(0, 0.999, n).astype(np.float32)
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.1), dict(top_k=900, top_p=0.99)):
+        full = dict(temperature=temperature, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(kw)
+        token, lp, kept = draw(x, u, **full)
+        rt, rl, rk = plain(x, torch.from_numpy(u).cuda(), 0.0, **settings(n, **full))
+        assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
+
+
+@gpu
 def test_greedy_takes_the_lowest_index():
     x = torch.randn(4, 262144)
     x[0, [200000, 5, 70000]] = 9.0
