@@ -16,19 +16,21 @@
 // after that touches shared memory only.
 //
 // Few candidates (the usual case).  min-p bounds the weights that can stay from below, and
-// top-k the logits: the k-th largest of the threads' own maxima (32 tokens each) is at most
-// the row's k-th largest logit.  The tokens above such a bound -- lowered by more than the
-// rounding of the soft cap, the division and the exponential can reorder -- are gathered
-// into one CTA, at most 2,048 of them, sorted there by (e, index) and cut.  With top-p alone
-// the 512 largest are gathered, and the sum of all weights says whether the cut lies among
-// them.
+// top-k the logits: if each of the C CTAs has ceil(k / C) tokens not below b, the k largest
+// logits are not below b, and the threads' own maxima (32 tokens each) give each CTA such a
+// b.  The tokens above such a bound -- lowered by more than the rounding of the soft cap, the
+// division and the exponential can reorder -- are gathered into one CTA in index order, at
+// most 2,048 of them, and weighed and cut there.
 //
-// Otherwise e_cut comes from a radix selection over the bits of e (non-negative floats
-// order like their bits; 2^-44 <= e <= 1 spans 1409 bins of 2^18 ulps, then 2048 of 2^7, then
-// 128), by counts for top-k and by sums of w for top-p, and
+// The cut.  By counts for top-k and by sums of w for top-p, a radix selection over the bits
+// of e (non-negative floats order like their bits; 2^-44 <= e <= 1 spans 1409 bins of 2^18
+// ulps, then 512 of 2^9, then 512) finds e_cut and i_cut with which
 //   { i : e_i > e_cut  or  (e_i = e_cut and i <= i_cut) }
-// is what stays.  The histograms of a round are added over distributed shared memory (CTA r
-// adds every CTA's bins of part r and gives the sums to all), two cluster barriers a round.
+// stays: over the gathered tokens in one CTA, or else over all CTAs' tokens, whose histograms
+// are added over distributed shared memory (CTA r adds every CTA's bins of part r and gives
+// the sums to all, two cluster barriers a round).  The tokens of a bin share the exponent of
+// e, so a bin's sum of w is exactly a count and a sum of low mantissa bits, both in 32 bits:
+// 64-bit shared-memory atomics were several times slower.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -48,9 +50,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr uint32_t kSlice = 16384, kMaxCluster = 16;
 constexpr uint32_t kMaxVocab = kSlice * kMaxCluster;
 constexpr uint32_t kKeyLow = 0x29800000u;  // bits of 2^-44: the least e of non-zero weight
-constexpr uint32_t kKeyOne = 0x3F800000u;  // bits of 1
-constexpr uint32_t kBins = 2048;
-constexpr float kOne = 17592186044416.0f;  // 2^44
+constexpr uint32_t kBins = 1409, kSub = 512;  // of the first round, of the others
 
 struct RowsArgs {
   const void *logits;
@@ -63,26 +63,23 @@ struct RowsArgs {
   float softcap;
 };
 
-constexpr uint32_t kList = 2048;    // candidates one CTA sorts
-constexpr uint32_t kMaxima = 1024;  // bins of the threads' maxima
+constexpr uint32_t kList = 2048;    // candidates one CTA takes
+constexpr uint32_t kMaxima = 1024;  // bins of a CTA's threads' maxima
 constexpr int32_t kMostK = 1024;    // largest top-k that goes by the maxima
-constexpr uint32_t kNucleus = 512;  // tokens gathered for top-p alone
 
 struct Shared {
   union {
-    struct {
-      unsigned long long hist[kBins], tot[kBins];
-    };
-    struct {
-      unsigned long long list[kList];  // candidates
-      uint32_t maxima[kMaxima], all_maxima[kMaxima];
-    };
+    unsigned long long tot[kBins];
+    uint32_t maxima[kMaxima];
   };
+  uint32_t cnt[kBins], low[kBins];  // tokens of a bin, and their sum above the bin's least
+  float list[kList];                // candidates: logits, then weights, by index
+  uint32_t list_id[kList];
   unsigned long long xch[2][kMaxCluster][2];  // what every CTA gives to all, two sets in turn
   unsigned long long warp_a[kWarps];
   uint32_t warp_b[kWarps];
   unsigned long long found[3];  // bin, sum above it, its sum
-  uint32_t cut_idx, n_list, again, pick;
+  uint32_t cut_at, pick;
   alignas(16) float e[kSlice + 8];
 };
 
@@ -108,41 +105,73 @@ CH_DEV void unpack16(const uint4 &r, float (&f)[8], const __nv_bfloat16 *) {
 #pragma unroll
   for (int i = 0; i < 4; i++) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
 }
-CH_DEV unsigned long long weight_of(float e) { return (unsigned long long)(e * kOne); }
+// floor(2^44 e) for 0 <= e <= 1: the mantissa shifted (a conversion to 64 bits is many times slower)
+CH_DEV unsigned long long weight_of(float e) {
+  const uint32_t bits = __float_as_uint(e), mant = (bits & 0x7FFFFFu) | 0x800000u;
+  return (unsigned long long)mant << 21 >> min(127u - (bits >> 23), 63u);
+}
 CH_DEV unsigned long long warp_sum64(unsigned long long v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-struct Cut {  // kept: key > key_, or key == key_ and idx <= idx_
-  uint32_t key, idx;
-  CH_DEV bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= idx); }
+struct Cut {  // kept: key > key_, or key == key_ and place <= at_
+  uint32_t key, at;
+  CH_DEV bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= at); }
 };
 
-// gives (a, b) of this CTA to every CTA of the cluster; after the barrier inside,
-// s->xch[set][rank] holds every CTA's pair
-CH_DEV void exchange(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, int set, unsigned long long a,
-                     unsigned long long b) {
-  if (threadIdx.x < C) {
-    unsigned long long *to = cl.map_shared_rank(&s->xch[set][rank][0], threadIdx.x);
-    to[0] = a;
-    to[1] = b;
+// The tokens a cut is taken over: those of all CTAs of the cluster, place = base + i, or
+// (CLUSTER false) the list of this CTA
+template <bool CLUSTER>
+struct Tokens {
+  Shared *s;
+  cg::cluster_group &cl;
+  uint32_t C, rank;  // 1, 0 for a list
+  const float *e;    // weights
+  uint32_t n, base;
+  int &set;
+
+  CH_DEV void sync() const {
+    if (CLUSTER) cl.sync(); else __syncthreads();
   }
-  cl.sync();
-}
+  // gives (a, b) of this CTA to every CTA; afterwards s->xch[set][c] holds CTA c's pair
+  CH_DEV void exchange(unsigned long long a, unsigned long long b) const {
+    if (threadIdx.x < C) {
+      unsigned long long *to = &s->xch[set][rank][0];
+      if (CLUSTER) to = cl.map_shared_rank(to, threadIdx.x);
+      to[0] = a;
+      to[1] = b;
+    }
+    sync();
+  }
+};
+
+// The bins of a round: tokens of one bin differ in the `shift` low bits of their keys only.
+// Below 2^-21 a weight loses mantissa bits: there the sum is of weights above the bin's least.
+struct Round {
+  uint32_t bins, shift;
+  CH_DEV uint32_t low_of(uint32_t key) const {
+    const uint32_t lost = 127 - (key >> 23) > 21 ? 106 - (key >> 23) : 0u, mant = (key & 0x7FFFFFu) | 0x800000u;
+    return (mant >> lost) - ((mant & ~((1u << shift) - 1)) >> lost);
+  }
+  CH_DEV unsigned long long sum_of(uint32_t count, uint32_t low, uint32_t key0) const {
+    const uint32_t ex = 127 - (key0 >> 23);
+    return count * weight_of(__uint_as_float(key0)) + ((unsigned long long)low << (ex > 21 ? 0 : 21 - ex));
+  }
+};
 
 // bin of s->tot[0, nb) (from the highest) with sum above < target <= sum above + its own;
 // s->found = {bin, sum above, its sum}; bin = nb when the bins hold less than target.
-// *all gets the sum of all bins.
 CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
-  constexpr int kPer = kBins / kThreads;
+  constexpr int kPer = (kBins + kThreads - 1) / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t per = (nb + kThreads - 1) / kThreads;
   unsigned long long v[kPer], mine = 0;
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
-    const uint32_t at = threadIdx.x * kPer + j;
-    v[j] = at < nb ? s->tot[nb - 1 - at] : 0;
+    const uint32_t at = threadIdx.x * per + j;
+    v[j] = j < (int)per && at < nb ? s->tot[nb - 1 - at] : 0;
     mine += v[j];
   }
   unsigned long long inc = mine;
@@ -159,7 +188,7 @@ CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     if (above < target && target <= above + v[j]) {
-      s->found[0] = nb - 1 - (threadIdx.x * kPer + j);
+      s->found[0] = nb - 1 - (threadIdx.x * per + j);
       s->found[1] = above;
       s->found[2] = v[j];
     }
@@ -168,46 +197,50 @@ CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
   __syncthreads();
 }
 
-// bins [b0, b1) of every CTA's `mine` added up into every CTA's `all`; C (a power of two)
-// neighbouring threads share a bin, so that the remote reads are in flight together
-template <typename V>
-CH_DEV void gather_bins(cg::cluster_group &cl, uint32_t C, V *mine, V *all, uint32_t b0, uint32_t b1) {
-  const uint32_t c = threadIdx.x & (C - 1);
-  for (uint32_t b = b0 + threadIdx.x / C; b < ((b1 - b0 + 31) & ~31u) + b0; b += kThreads / C) {
-    V sum = b < b1 ? *cl.map_shared_rank(&mine[b], c) : V(0);
-    for (uint32_t o = 1; o < C; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (b < b1) *cl.map_shared_rank(&all[b], c) = sum;
-  }
-}
-
-// Narrows `cut` to the first part of the order that holds `target` tokens (COUNT) or,
-// with target = 0, the weight ceil(p * sum).
-template <bool COUNT>
-CH_DEV Cut select(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, const float *e, uint32_t n,
-                  uint32_t base, Cut cut, unsigned long long target, double p, int &set) {
+// Narrows `cut` to the first part of the order that holds `target` tokens (COUNT) or the
+// weight ceil(p * sum of all kept so far).
+template <bool COUNT, bool CLUSTER>
+CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, double p) {
+  Shared *s = t.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float *e = t.e;
   uint32_t prefix = 0;
   for (int round = 0; round < 3; round++) {
-    const uint32_t nb = round == 0 ? ((kKeyOne - kKeyLow) >> 18) + 1 : round == 1 ? 2048 : 128;
-    const uint32_t shift = round == 0 ? 18 : round == 1 ? 7 : 0;
-    for (uint32_t i = threadIdx.x; i < nb; i += kThreads) s->hist[i] = 0;
+    const Round rd = {round == 0 ? kBins : kSub, round == 0 ? 18u : round == 1 ? 9u : 0u};
+    const uint32_t nb = rd.bins;
+    for (uint32_t i = threadIdx.x; i < nb; i += kThreads) s->cnt[i] = s->low[i] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < t.n; i += kThreads) {
       const uint32_t key = __float_as_uint(e[i]);
-      if (key == 0 || !cut.keeps(key, base + i)) continue;
-      uint32_t bin;
-      if (round == 0) {
-        bin = (key - kKeyLow) >> 18;
-      } else {
-        if ((key >> (round == 1 ? 18 : 7)) != prefix) continue;
-        bin = (key >> shift) & (nb - 1);
+      if (key == 0 || !cut.keeps(key, t.base + i)) continue;
+      uint32_t bin = (key - kKeyLow) >> 18;
+      if (round > 0) {
+        if (key >> (rd.shift + 9) != prefix) continue;
+        bin = (key >> rd.shift) & (kSub - 1);
       }
-      atomicAdd(&s->hist[bin], COUNT ? 1ull : weight_of(e[i]));
+      atomicAdd(&s->cnt[bin], 1u);
+      if (!COUNT && rd.shift > 0) atomicAdd(&s->low[bin], rd.low_of(key));
     }
-    cl.sync();  // every CTA's bins are complete
-    const uint32_t part = (nb + C - 1) / C, b0 = min(nb, rank * part), b1 = min(nb, b0 + part);
-    gather_bins(cl, C, s->hist, s->tot, b0, b1);
-    cl.sync();  // every CTA has every sum, and is done with every CTA's bins
+    t.sync();  // every CTA's bins are complete
+    const uint32_t key_base = round == 0 ? kKeyLow : prefix << (rd.shift + 9);
+    if (CLUSTER) {
+      // C (a power of two) neighbouring threads share a bin: remote reads in flight together
+      const uint32_t part = (nb + t.C - 1) / t.C, b0 = min(nb, t.rank * part), b1 = min(nb, b0 + part);
+      const uint32_t c = threadIdx.x & (t.C - 1);
+      for (uint32_t b = b0 + threadIdx.x / t.C; b < ((b1 - b0 + 31) & ~31u) + b0; b += kThreads / t.C) {
+        unsigned long long sum = 0;
+        if (b < b1) {
+          const uint32_t n = *t.cl.map_shared_rank(&s->cnt[b], c);
+          sum = COUNT ? n : rd.sum_of(n, *t.cl.map_shared_rank(&s->low[b], c), key_base + (b << rd.shift));
+        }
+        for (uint32_t o = 1; o < t.C; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (b < b1) *t.cl.map_shared_rank(&s->tot[b], c) = sum;
+      }
+    } else {
+      for (uint32_t b = threadIdx.x; b < nb; b += kThreads)
+        s->tot[b] = COUNT ? s->cnt[b] : rd.sum_of(s->cnt[b], s->low[b], key_base + (b << rd.shift));
+    }
+    t.sync();  // every CTA has every sum, and is done with every CTA's bins
     if (!COUNT && round == 0) {  // what top-p asks for, from the sum of all weights
       unsigned long long sum = 0;
       for (uint32_t i = threadIdx.x; i < nb; i += kThreads) sum += s->tot[i];
@@ -224,8 +257,8 @@ CH_DEV Cut select(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, c
     const uint32_t bin = (uint32_t)s->found[0];
     const unsigned long long above = s->found[1], in_bin = s->found[2];
     if (bin >= nb) return cut;  // fewer tokens than asked for: all stay
-    prefix = round == 0 ? bin + (kKeyLow >> 18) : (prefix << (round == 1 ? 11 : 7)) | bin;
-    const uint32_t low = prefix << shift;  // the bin's lowest key
+    const uint32_t low = key_base + (bin << rd.shift);  // the bin's lowest key
+    prefix = low >> rd.shift;
     target -= above;
     // the whole bin stays when all its tokens are asked for; by weight, when it holds one token
     const bool whole = COUNT ? target == in_bin : in_bin < 2 * weight_of(__uint_as_float(low));
@@ -233,7 +266,7 @@ CH_DEV Cut select(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, c
       if (low > cut.key) cut = Cut{low, 0xFFFFFFFFu};
       return cut;
     }
-    if (round == 2) {  // one key: the `take` lowest indices of it stay
+    if (round == 2) {  // one key: the `take` first places of it stay
       const unsigned long long w = COUNT ? 1 : weight_of(__uint_as_float(low));
       const unsigned long long take = (target + w - 1) / w;
       if (take == in_bin / w) {
@@ -241,11 +274,11 @@ CH_DEV Cut select(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, c
         return cut;
       }
       // tokens of this key per warp part (a warp owns a contiguous part of the slice)
-      const uint32_t seg = ((n + kThreads - 1) / kThreads) * 32, w0 = min(n, warp * seg), w1 = min(n, w0 + seg);
+      const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
       uint32_t cnt = 0;
       for (uint32_t i = w0 + lane; i < w1; i += 32) {
         const uint32_t key = __float_as_uint(e[i]);
-        cnt += key == low && cut.keeps(key, base + i);
+        cnt += key == low && cut.keeps(key, t.base + i);
       }
       cnt = __reduce_add_sync(0xffffffffu, cnt);
       if (lane == 0) s->warp_b[warp] = cnt;
@@ -255,70 +288,103 @@ CH_DEV Cut select(Shared *s, cg::cluster_group &cl, uint32_t C, uint32_t rank, c
         if (k < warp) before += s->warp_b[k];
         mine += s->warp_b[k];
       }
-      exchange(s, cl, C, rank, set, mine, 0);
-      for (uint32_t c = 0; c < rank; c++) before += (uint32_t)s->xch[set][c][0];
-      set ^= 1;
+      t.exchange(mine, 0);
+      for (uint32_t c = 0; c < t.rank; c++) before += (uint32_t)s->xch[t.set][c][0];
+      t.set ^= 1;
       if (before < take && take <= before + cnt) {  // this warp's part holds the last one that stays
         uint32_t left = (uint32_t)take - before;
         for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
           const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
-          const uint32_t hit = __ballot_sync(0xffffffffu, key == low && cut.keeps(key, base + i));
+          const uint32_t hit = __ballot_sync(0xffffffffu, key == low && cut.keeps(key, t.base + i));
           const uint32_t c = __popc(hit);
           if (left <= c) {
-            const int at = __fns(hit, 0, left);
-            if (lane < (int)C) *cl.map_shared_rank(&s->cut_idx, lane) = base + i0 + at;
+            const uint32_t at = t.base + i0 + __fns(hit, 0, left);
+            if (CLUSTER) {
+              if (lane < (int)t.C) *t.cl.map_shared_rank(&s->cut_at, lane) = at;
+            } else if (lane == 0) {
+              s->cut_at = at;
+            }
             break;
           }
           left -= c;
         }
       }
-      cl.sync();
-      return Cut{low, s->cut_idx};
+      t.sync();
+      return Cut{low, s->cut_at};
     }
   }
   return cut;
 }
 
-// Descending order of a[0, n), padded to a power of two with zeros (no key is 0).  Threads of
-// a warp own 64 neighbouring keys, so that short strides need no CTA barrier.
-CH_DEV void sort_down(unsigned long long *a, uint32_t n) {
-  uint32_t size = 64;
-  while (size < n) size <<= 1;
-  for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) a[i] = 0;
-  __syncthreads();
-  for (uint32_t k = 2; k <= size; k <<= 1) {
-    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-      for (uint32_t p = threadIdx.x; p < size / 2; p += kThreads) {
-        const uint32_t lo = 2 * p - (p & (j - 1)), hi = lo + j;
-        const unsigned long long x = a[lo], y = a[hi];
-        if ((x < y) == ((lo & k) == 0)) a[lo] = y, a[hi] = x;
-      }
-      if (j > 32) __syncthreads(); else __syncwarp();
-    }
-    __syncthreads();
-  }
-}
-
-// Inclusive sums over the CTA of v (4 neighbouring values per thread); s->warp_a is used.
-CH_DEV void scan4(Shared *s, const unsigned long long (&v)[4], unsigned long long (&inc)[4]) {
+// Top-k and top-p among the tokens (what min-p drops has weight 0), then the draw, in the
+// order of their places: warp w owns the part [w * seg, (w + 1) * seg).  id: a place's token,
+// or NULL for the place itself.
+template <bool CLUSTER>
+CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> &t, int32_t top_k, float top_p, float u,
+                         const uint32_t *id) {
+  Shared *s = t.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  inc[0] = v[0];
-#pragma unroll
-  for (int j = 1; j < 4; j++) inc[j] = inc[j - 1] + v[j];
-  unsigned long long run = inc[3];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long u = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += u;
+  const float *e = t.e;
+  Cut cut{kKeyLow, 0xFFFFFFFFu};
+  if (top_k > 0) cut = select<true>(t, cut, (unsigned long long)top_k, 0.0);
+  if (top_p < 1.0f) cut = select<false>(t, cut, 0, (double)top_p);
+  const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
+  unsigned long long mass = 0;
+  uint32_t cnt = 0;
+  for (uint32_t i = w0 + lane; i < w1; i += 32) {
+    const uint32_t key = __float_as_uint(e[i]);
+    if (key != 0 && cut.keeps(key, t.base + i)) {
+      mass += weight_of(e[i]);
+      cnt++;
+    }
   }
+  mass = warp_sum64(mass);
+  cnt = __reduce_add_sync(0xffffffffu, cnt);
   __syncthreads();
-  if (lane == 31) s->warp_a[warp] = run;
+  if (lane == 0) s->warp_a[warp] = mass, s->warp_b[warp] = cnt;
   __syncthreads();
-  unsigned long long before = run - inc[3];
-  for (int w = 0; w < warp; w++) before += s->warp_a[w];
+  unsigned long long mine = 0, before = 0;
+  uint32_t kept = 0;
+  for (int w = 0; w < kWarps; w++) {
+    if (w < warp) before += s->warp_a[w];
+    mine += s->warp_a[w];
+    kept += s->warp_b[w];
+  }
+  unsigned long long total = mine;
+  if (CLUSTER) {
+    t.exchange(mine, kept);
+    total = kept = 0;
+    for (uint32_t c = 0; c < t.C; c++) {
+      if (c < t.rank) before += s->xch[t.set][c][0];
+      total += s->xch[t.set][c][0];
+      kept += (uint32_t)s->xch[t.set][c][1];
+    }
+  }
+  unsigned long long goal = u > 0.f ? (unsigned long long)((double)u * (double)total) : 0ull;
+  goal = min(goal, total - 1);
+  if (before <= goal && goal < before + mass) {  // this warp's part holds the token
+    unsigned long long run = before;
+    for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
+      const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
+      const unsigned long long w = key != 0 && cut.keeps(key, t.base + i) ? weight_of(e[i]) : 0ull;
+      unsigned long long inc = w;
 #pragma unroll
-  for (int j = 0; j < 4; j++) inc[j] += before;
-  __syncthreads();
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, run + inc > goal);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          a.tokens[row] = (int32_t)(id ? id[i] : t.base + i);
+          if (a.logprobs) a.logprobs[row] = (float)log((double)w / (double)total);
+          if (a.kept) a.kept[row] = (int32_t)kept;
+        }
+        break;
+      }
+      run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
 }
 
 // What one row asks for
@@ -380,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
   int set = 0;
   for (uint32_t i = threadIdx.x; i < kMaxima; i += kThreads) s->maxima[i] = 0;
-  if (threadIdx.x == 0) s->n_list = 0;
+  if (threadIdx.x == 0) s->pick = kMaxima;
 
   // ---- the logits, once from global memory; 16-byte loads between a ragged head and tail.
   // Element i lies at e[i], with e shifted so that 16-byte loads meet 16-byte stores. ----
@@ -420,8 +486,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   r.quick = r.temp > 1e-15f && r.temp < 1e15f && (__float_as_uint(r.temp) & 0x7FFFFFu) != 0x7FFFFFu;
   if (r.top_k <= 0 || (uint32_t)r.top_k >= a.vocab) r.top_k = 0;
 
-  // ---- the largest logit m, and the least of the threads' maxima ----
-  float m = warp_max(own), least = own > -INFINITY ? own : INFINITY;
+  const Tokens<true> all{s, cl, C, rank, e, n, base, set};
+  // the CTA's maximum of v
+  auto cta_max = [&](float v) {
+    v = warp_max(v);
+    __syncthreads();
+    if (lane == 0) s->warp_b[warp] = __float_as_uint(v);
+    __syncthreads();
+    for (int w = 0; w < kWarps; w++) v = fmaxf(v, __uint_as_float(s->warp_b[w]));
+    return v;
+  };
+
+  // ---- the largest logit m.  Beside it, for top-k, a bound that at least top_k tokens of the
+  // row are not below: every CTA finds its threads' maxima's ceil(top_k / C)-th largest by a
+  // histogram over their range, and the least of these counts ----
+  const bool by_k = r.top_k > 0 && r.top_k <= kMostK, bounded = a.vocab > kList && by_k && r.temp > 0.f;
+  float m = warp_max(own), least = own > -INFINITY ? own : INFINITY, bound = -INFINITY;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
   if (lane == 0) s->warp_a[warp] = (unsigned long long)__float_as_uint(m) << 32 | __float_as_uint(least);
@@ -430,10 +510,35 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
     m = fmaxf(m, __uint_as_float((uint32_t)(s->warp_a[w] >> 32)));
     least = fminf(least, __uint_as_float((uint32_t)s->warp_a[w]));
   }
-  exchange(s, cl, C, rank, set, __float_as_uint(m), __float_as_uint(least));
+  if (bounded) {
+    const float per_bin = least < m && m < INFINITY ? (kMaxima - 1) / (m - least) : 0.f;
+    if (own > -INFINITY) atomicAdd(&s->maxima[min(kMaxima - 1, (uint32_t)((m - own) * per_bin))], 1u);
+    __syncthreads();
+    const uint32_t want = ((uint32_t)r.top_k + C - 1) / C;
+    const uint32_t v0 = s->maxima[2 * threadIdx.x], v1 = s->maxima[2 * threadIdx.x + 1];
+    static_assert(kMaxima == 2 * kThreads, "two bins per thread");
+    uint32_t run = v0 + v1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
+    }
+    if (lane == 31) s->warp_b[warp] = run;
+    __syncthreads();
+    uint32_t before = run - v0 - v1;
+    for (int w = 0; w < warp; w++) before += s->warp_b[w];
+    if (before < want && want <= before + v0) s->pick = 2 * threadIdx.x;
+    if (before + v0 < want && want <= before + v0 + v1) s->pick = 2 * threadIdx.x + 1;
+    __syncthreads();
+    if (s->pick < kMaxima - 1 && per_bin > 0.f) {
+      const float end = m - (s->pick + 1) / per_bin;  // the bin's lower end, lowered by its rounding
+      bound = end - (fabsf(end) + fabsf(m)) * 1e-6f;
+    }
+  }
+  all.exchange(__float_as_uint(m), __float_as_uint(bound));
   for (uint32_t c = 0; c < C; c++) {
     m = fmaxf(m, __uint_as_float((uint32_t)s->xch[set][c][0]));
-    least = fminf(least, __uint_as_float((uint32_t)s->xch[set][c][1]));
+    bound = fminf(bound, __uint_as_float((uint32_t)s->xch[set][c][1]));
   }
   set ^= 1;
 
@@ -461,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
     if (lane == 0) s->warp_a[warp] = best;
     __syncthreads();
     for (int w = 0; w < kWarps; w++) best = max(best, s->warp_a[w]);
-    exchange(s, cl, C, rank, set, best, 0);
+    all.exchange(best, 0);
     for (uint32_t c = 0; c < C; c++) best = max(best, s->xch[set][c][0]);
     if (rank == 0 && threadIdx.x == 0) {
       a.tokens[row] = (int32_t)~(uint32_t)best;
@@ -472,184 +577,90 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   }
 
   // ---- few candidates: a bound `low` on the logits that can stay ----
-  const bool by_k = r.top_k > 0 && r.top_k <= kMostK, by_p = !(r.min_p > 0.f) && r.top_k == 0 && r.top_p < 1.f;
-  if (m < INFINITY && (a.vocab <= kList || by_k || by_p || r.min_p > 0.f)) {
+  if (m < INFINITY && (a.vocab <= kList || by_k || r.min_p > 0.f)) {
     float low = -INFINITY;
     if (r.min_p > 0.f) low = r.below(mc + r.temp * (logf(fminf(r.min_p, 1.f)) - 1e-5f) - r.slack(mc));
-    // with top-p alone, as many as the threads' maxima can bound well
-    const uint32_t nucleus = min(kNucleus, C * kThreads / 4);
-    if (a.vocab > kList && (by_k || by_p)) {
-      const uint32_t want = by_k ? r.top_k : nucleus;
-      // the bin of the want-th largest of the threads' maxima
-      const float per_bin = least < m ? (kMaxima - 1) / (m - least) : 0.f;
-      if (own > -INFINITY) atomicAdd(&s->maxima[min(kMaxima - 1, (uint32_t)((m - own) * per_bin))], 1u);
-      cl.sync();
-      const uint32_t part = kMaxima / C;
-      gather_bins(cl, C, s->maxima, s->all_maxima, rank * part, (rank + 1) * part);
-      cl.sync();
-      uint32_t v[2] = {s->all_maxima[2 * threadIdx.x], s->all_maxima[2 * threadIdx.x + 1]}, run = v[0] + v[1];
-      static_assert(kMaxima == 2 * kThreads, "two bins per thread");
+    if (bound > -INFINITY) low = fmaxf(low, r.below(r.capped(bound) - r.slack(mc)));
+    // which of its tokens each lane gives: four neighbouring ones per 128 of the warp's part
+    constexpr uint32_t kPart = kSlice / kWarps, kSteps = kPart / 128 + 1;  // one more for the shift
+    static_assert(kSteps * 4 <= 64, "bits");
+    const uint32_t skip = off & 3u, ends = skip + n;  // token i lies at place skip + i of 16-byte groups
+    const uint32_t g0 = warp * kPart + (warp ? 8u : 0u), g1 = min(ends, (warp + 1) * kPart + 8u);
+    unsigned long long in = 0;
+    uint32_t cnt = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += u;
-      }
-      if (lane == 31) s->warp_b[warp] = run;
-      if (threadIdx.x == 0) s->pick = kMaxima;
-      __syncthreads();
-      uint32_t before = run - v[0] - v[1];
-      for (int w = 0; w < warp; w++) before += s->warp_b[w];
-      if (before < want && want <= before + v[0]) s->pick = 2 * threadIdx.x;
-      if (before + v[0] < want && want <= before + v[0] + v[1]) s->pick = 2 * threadIdx.x + 1;
-      __syncthreads();
-      // at least `want` tokens are not below the bin's lower end
-      if (s->pick < kMaxima - 1 && per_bin > 0.f) {
-        const float end = m - (s->pick + 1) / per_bin, t0 = end - (fabsf(end) + fabsf(m)) * 1e-6f;
-        low = fmaxf(low, r.below(r.capped(t0) - r.slack(mc)));
-      }
-    }
-    // candidates into the first CTA's list, in any order
-    Shared *to = cl.map_shared_rank(s, 0);
-    unsigned long long mass = 0;  // of all tokens, where top-p alone asks for it
-    const bool all_mass = by_p && a.vocab > kList;
-    // (with a cap the largest capped logit is only known up to its rounding: the sum of all
-    // weights needs it exactly)
-    float top = mc;
-    if (all_mass && r.cap > 0.f) {
-      const float near = r.below(mc - r.cap * 1e-6f);
-      for (uint32_t i = threadIdx.x; i < n; i += kThreads)
-        if (e[i] >= near) top = fmaxf(top, r.capped(e[i]));
-      top = warp_max(top);
-      __syncthreads();
-      if (lane == 0) s->warp_b[warp] = __float_as_uint(top);
-      __syncthreads();
-      for (int w = 0; w < kWarps; w++) top = fmaxf(top, __uint_as_float(s->warp_b[w]));
-      exchange(s, cl, C, rank, set, __float_as_uint(top), 0);
-      for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
-      set ^= 1;
-    }
-    for (uint32_t i0 = warp * 32; i0 < n; i0 += kThreads) {
-      const uint32_t i = i0 + lane;
-      const float v = i < n ? e[i] : -INFINITY;
-      if (all_mass) mass += weight_of(r.weigh(r.capped(v), top));
-      const bool in = v >= low && v > -INFINITY;
-      const uint32_t votes = __ballot_sync(0xffffffffu, in);
-      if (!votes) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&to->n_list, __popc(votes));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << lane) - 1));
-      if (in && at < kList) to->list[at] = (unsigned long long)__float_as_uint(v) << 32 | (base + i);
-    }
-    if (all_mass) {
-      mass = warp_sum64(mass);
-      __syncthreads();
-      if (lane == 0) s->warp_a[warp] = mass;
-      __syncthreads();
-      mass = 0;
-      for (int w = 0; w < kWarps; w++) mass += s->warp_a[w];
-    }
-    exchange(s, cl, C, rank, set, mass, 0);
-    mass = 0;
-    for (uint32_t c = 0; c < C; c++) mass += s->xch[set][c][0];
-    set ^= 1;
-    const uint32_t count = to->n_list;
-    bool found = count <= kList;
-    if (found && rank == 0) {
-      // capped, weighed, sorted by (e, lower index first)
-      float xs[4], best = -INFINITY;
-      uint32_t id[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint32_t i = threadIdx.x + j * kThreads;
-        const unsigned long long it = i < count ? s->list[i] : 0ull;
-        xs[j] = i < count ? r.capped(__uint_as_float((uint32_t)(it >> 32))) : -INFINITY;
-        id[j] = (uint32_t)it;
-        best = fmaxf(best, xs[j]);
-      }
-      best = warp_max(best);
-      if (lane == 0) s->warp_b[warp] = __float_as_uint(best);
-      __syncthreads();
-      for (int w = 0; w < kWarps; w++) best = fmaxf(best, __uint_as_float(s->warp_b[w]));
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint32_t i = threadIdx.x + j * kThreads;
-        if (i >= count) continue;
-        const float w = r.weigh(xs[j], best);
-        s->list[i] = w > 0.f ? (unsigned long long)__float_as_uint(w) << 32 | (uint32_t)~id[j] : 0ull;
-      }
-      __syncthreads();
-      sort_down(s->list, count);
-      auto w_of = [&](uint32_t i) { return weight_of(__uint_as_float((uint32_t)(s->list[i] >> 32))); };
-      // (for top-p alone only the first `nucleus` are sure to come before every other token)
-      const uint32_t limit = min(count, r.top_k > 0 ? (uint32_t)r.top_k : all_mass ? nucleus : count);
-      unsigned long long v[4], inc[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint32_t i = 4 * threadIdx.x + j;
-        v[j] = i < limit ? w_of(i) : 0ull;
-      }
-      scan4(s, v, inc);
-      if (threadIdx.x == kThreads - 1) s->found[0] = inc[3];
-      if (threadIdx.x == 0) s->pick = 0;
-      __syncthreads();
-      const unsigned long long here = s->found[0];
-      const unsigned long long whole = all_mass ? mass : here;
-      unsigned long long need = ~0ull;  // weight that the kept tokens reach
-      if (r.top_p < 1.0f) {
-        need = (unsigned long long)ceil((double)r.top_p * (double)whole);
-        need = need < 1 ? 1 : need;
-      }
-      found = !all_mass || need <= here;
-      uint32_t kept = 0;
-#pragma unroll
-      for (int j = 0; j < 4; j++) kept += v[j] > 0 && inc[j] - v[j] < need;
-      kept = __reduce_add_sync(0xffffffffu, kept);
-      if (lane == 0) atomicAdd(&s->pick, kept);
-      __syncthreads();
-      kept = s->pick;
-      if (found) {
-        // the same tokens by index, lowest first: key (index complement, weight's place)
-        unsigned long long total = 0, it[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t i = 4 * threadIdx.x + j;
-          it[j] = i < kept ? s->list[i] << 32 | s->list[i] >> 32 : 0ull;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; j++) s->list[4 * threadIdx.x + j] = it[j];
-        sort_down(s->list, kept);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t i = 4 * threadIdx.x + j;
-          v[j] = i < kept ? weight_of(__uint_as_float((uint32_t)s->list[i])) : 0ull;
-        }
-        scan4(s, v, inc);
-        if (threadIdx.x == kThreads - 1) s->found[0] = inc[3];
-        __syncthreads();
-        total = s->found[0];
-        unsigned long long goal = r.u > 0.f ? (unsigned long long)((double)r.u * (double)total) : 0ull;
-        goal = min(goal, total - 1);
+    for (uint32_t t = 0; t < kSteps; t++) {
+      const uint32_t g = g0 + t * 128 + lane * 4;
+      if (g0 + t * 128 >= g1) break;
+      uint32_t four = 0;
+      if (g < g1) {
+        const float4 q = *reinterpret_cast<const float4 *>(s->e + g);
+        const float v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (inc[j] - v[j] <= goal && goal < inc[j]) {
-            a.tokens[row] = (int32_t)~(uint32_t)(s->list[4 * threadIdx.x + j] >> 32);
-            if (a.logprobs) a.logprobs[row] = (float)log((double)v[j] / (double)total);
-            if (a.kept) a.kept[row] = (int32_t)kept;
+          four |= (v[j] >= low && v[j] > -INFINITY && g + j >= skip && g + j < g1 ? 1u : 0u) << j;
+      }
+      in |= (unsigned long long)four << (4 * t);
+      cnt += __popc(four);
+    }
+    const uint32_t warp_cnt = __reduce_add_sync(0xffffffffu, cnt);
+    __syncthreads();
+    if (lane == 0) s->warp_b[warp] = warp_cnt;
+    __syncthreads();
+    uint32_t at = 0, count = 0, mine = 0;
+    for (int w = 0; w < kWarps; w++) {
+      if (w < warp) at += s->warp_b[w];
+      mine += s->warp_b[w];
+    }
+    all.exchange(mine, 0);
+    for (uint32_t c = 0; c < C; c++) {
+      if (c < rank) at += (uint32_t)s->xch[set][c][0];
+      count += (uint32_t)s->xch[set][c][0];
+    }
+    set ^= 1;
+    if (count <= kList) {
+      if (warp_cnt) {  // into the first CTA's list, by index
+        float *list = cl.map_shared_rank(s->list, 0);
+        uint32_t *list_id = cl.map_shared_rank(s->list_id, 0);
+        for (uint32_t t = 0; t < kSteps; t++) {
+          const uint32_t four = (uint32_t)(in >> (4 * t)) & 15u;
+          if (!__any_sync(0xffffffffu, four)) continue;
+          uint32_t sum = __popc(four);
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
           }
+          uint32_t to = at + sum - __popc(four);
+          const uint32_t g = g0 + t * 128 + lane * 4;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if ((four >> j) & 1) {
+              list[to] = s->e[g + j];
+              list_id[to++] = base + g + j - skip;
+            }
+          at += __shfl_sync(0xffffffffu, sum, 31);
+        }
       }
-    }
-    if (!all_mass) {
-      if (found) {  // the first CTA stays until every other one has read its count
-        if (rank == 0) cl.sync();
-        return;
-      }
-    } else {  // the first CTA says whether the cut lay among its candidates
-      if (rank == 0 && threadIdx.x < C) *cl.map_shared_rank(&s->again, threadIdx.x) = found ? 0u : 1u;
       cl.sync();
-      if (!s->again) return;
+      if (rank != 0) return;
+      float x4[kList / kThreads], top = -INFINITY;
+#pragma unroll
+      for (uint32_t j = 0; j < kList / kThreads; j++) {
+        const uint32_t i = threadIdx.x + j * kThreads;
+        x4[j] = i < count ? r.capped(s->list[i]) : -INFINITY;
+        top = fmaxf(top, x4[j]);
+      }
+      top = cta_max(top);
+#pragma unroll
+      for (uint32_t j = 0; j < kList / kThreads; j++) {
+        const uint32_t i = threadIdx.x + j * kThreads;
+        if (i < count) s->list[i] = r.weigh(x4[j], top);
+      }
+      __syncthreads();
+      cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set}, r.top_k, r.top_p, r.u, s->list_id);
+      return;
     }
-    cl.sync();
   }
 
   // ---- many candidates: weights of all tokens; what min-p drops, and what rounds to weight
@@ -662,79 +673,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
       e[i] = v;
       top = fmaxf(top, v);
     }
-    top = warp_max(top);
-    __syncthreads();
-    if (lane == 0) s->warp_b[warp] = __float_as_uint(top);
-    __syncthreads();
-    for (int w = 0; w < kWarps; w++) top = fmaxf(top, __uint_as_float(s->warp_b[w]));
-    exchange(s, cl, C, rank, set, __float_as_uint(top), 0);
+    top = cta_max(top);
+    all.exchange(__float_as_uint(top), 0);
     for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
     set ^= 1;
   }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) e[i] = r.weigh(e[i], top);
   __syncthreads();
-
-  Cut cut{kKeyLow, 0xFFFFFFFFu};
-  if (r.top_k > 0) cut = select<true>(s, cl, C, rank, e, n, base, cut, (unsigned long long)r.top_k, 0.0, set);
-  if (r.top_p < 1.0f) cut = select<false>(s, cl, C, rank, e, n, base, cut, 0, (double)r.top_p, set);
-
-  // ---- the draw, in index order: warp w owns the part [w * seg, (w + 1) * seg) ----
-  const uint32_t seg = ((n + kThreads - 1) / kThreads) * 32, w0 = min(n, warp * seg), w1 = min(n, w0 + seg);
-  unsigned long long mass = 0;
-  uint32_t cnt = 0;
-  for (uint32_t i = w0 + lane; i < w1; i += 32) {
-    const uint32_t key = __float_as_uint(e[i]);
-    if (key != 0 && cut.keeps(key, base + i)) {
-      mass += weight_of(e[i]);
-      cnt++;
-    }
-  }
-  mass = warp_sum64(mass);
-  cnt = __reduce_add_sync(0xffffffffu, cnt);
-  __syncthreads();
-  if (lane == 0) s->warp_a[warp] = mass, s->warp_b[warp] = cnt;
-  __syncthreads();
-  unsigned long long mine = 0, before = 0;
-  uint32_t kept = 0;
-  for (int w = 0; w < kWarps; w++) {
-    if (w < warp) before += s->warp_a[w];
-    mine += s->warp_a[w];
-    kept += s->warp_b[w];
-  }
-  exchange(s, cl, C, rank, set, mine, kept);
-  unsigned long long total = 0;
-  kept = 0;
-  for (uint32_t c = 0; c < C; c++) {
-    if (c < rank) before += s->xch[set][c][0];
-    total += s->xch[set][c][0];
-    kept += (uint32_t)s->xch[set][c][1];
-  }
-  unsigned long long goal = r.u > 0.f ? (unsigned long long)((double)r.u * (double)total) : 0ull;
-  goal = min(goal, total - 1);
-  if (before <= goal && goal < before + mass) {  // this warp's part holds the token
-    unsigned long long run = before;
-    for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-      const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
-      const unsigned long long w = key != 0 && cut.keeps(key, base + i) ? weight_of(e[i]) : 0ull;
-      unsigned long long inc = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, run + inc > goal);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          a.tokens[row] = (int32_t)(base + i);
-          if (a.logprobs) a.logprobs[row] = (float)log((double)w / (double)total);
-          if (a.kept) a.kept[row] = (int32_t)kept;
-        }
-        break;
-      }
-      run += __shfl_sync(0xffffffffu, inc, 31);
-    }
-  }
+  cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr);
 }
 
 template <typename T>
