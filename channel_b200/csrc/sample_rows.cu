@@ -26,7 +26,7 @@
 // of e (non-negative floats order like their bits; 2^-44 <= e <= 1 spans 1409 bins of 2^18
 // ulps, then 512 of 2^9, then 512) finds e_cut and i_cut with which
 //   { i : e_i > e_cut  or  (e_i = e_cut and i <= i_cut) }
-// stays: over the gathered tokens in one CTA, or else over all CTAs' tokens, whose histograms
+// stays: over the gathered tokens in one CTA (up to 128 are ranked by comparing all with all), or else over all CTAs' tokens, whose histograms
 // are added over distributed shared memory (CTA r adds every CTA's bins of part r and gives
 // the sums to all, two cluster barriers a round).  The tokens of a bin share the exponent of
 // e, so a bin's sum of w is exactly a count and a sum of low mantissa bits, both in 32 bits:
@@ -51,6 +51,7 @@ constexpr uint32_t kSlice = 16384, kMaxCluster = 16;
 constexpr uint32_t kMaxVocab = kSlice * kMaxCluster;
 constexpr uint32_t kKeyLow = 0x29800000u;  // bits of 2^-44: the least e of non-zero weight
 constexpr uint32_t kBins = 1409, kSub = 512;  // of the first round, of the others
+constexpr uint32_t kFew = 128;     // candidates that are ranked by comparing all with all
 
 struct RowsArgs {
   const void *logits;
@@ -148,6 +149,7 @@ struct Tokens {
 };
 
 // The bins of a round: tokens of one bin differ in the `shift` low bits of their keys only.
+// (16,384 tokens of a CTA sum to less than 2^32 of low bits.)
 // Below 2^-21 a weight loses mantissa bits: there the sum is of weights above the bin's least.
 struct Round {
   uint32_t bins, shift;
@@ -210,16 +212,33 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
     const uint32_t nb = rd.bins;
     for (uint32_t i = threadIdx.x; i < nb; i += kThreads) s->cnt[i] = s->low[i] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < t.n; i += kThreads) {
-      const uint32_t key = __float_as_uint(e[i]);
-      if (key == 0 || !cut.keeps(key, t.base + i)) continue;
-      uint32_t bin = (key - kKeyLow) >> 18;
-      if (round > 0) {
-        if (key >> (rd.shift + 9) != prefix) continue;
-        bin = (key >> rd.shift) & (kSub - 1);
+    if (round == 0) {
+      for (uint32_t i = threadIdx.x; i < t.n; i += kThreads) {
+        const uint32_t key = __float_as_uint(e[i]), bin = (key - kKeyLow) >> 18;
+        if (key == 0 || !cut.keeps(key, t.base + i)) continue;
+        atomicAdd(&s->cnt[bin], 1u);
+        if (!COUNT) atomicAdd(&s->low[bin], rd.low_of(key));
       }
-      atomicAdd(&s->cnt[bin], 1u);
-      if (!COUNT && rd.shift > 0) atomicAdd(&s->low[bin], rd.low_of(key));
+    } else {
+      // few bins hold many tokens here (16-bit logits have few distinct values), and additions
+      // to one address go one by one: a warp adds each of its bins once
+      for (uint32_t i0 = warp * 32; i0 < t.n; i0 += kThreads) {
+        const uint32_t i = i0 + lane, key = i < t.n ? __float_as_uint(e[i]) : 0u, bin = (key >> rd.shift) & (kSub - 1);
+        const bool in = key != 0 && key >> (rd.shift + 9) == prefix && cut.keeps(key, t.base + i);
+        uint32_t left = __ballot_sync(0xffffffffu, in);
+        while (left) {
+          const int first = __ffs(left) - 1;
+          const uint32_t its = __shfl_sync(0xffffffffu, bin, first);  // by every lane
+          const bool mine = in && bin == its;
+          const uint32_t same = __ballot_sync(0xffffffffu, mine);
+          if (lane == first) atomicAdd(&s->cnt[bin], __popc(same));
+          if (!COUNT && rd.shift > 0) {
+            const uint32_t sum = __reduce_add_sync(0xffffffffu, mine ? rd.low_of(key) : 0u);
+            if (lane == first) atomicAdd(&s->low[bin], sum);
+          }
+          left &= ~same;
+        }
+      }
     }
     t.sync();  // every CTA's bins are complete
     const uint32_t key_base = round == 0 ? kKeyLow : prefix << (rd.shift + 9);
@@ -423,6 +442,7 @@ struct Row {
     const float y = __fdiv_rn(c, cap);
     if (!(y > -0.9999f)) return -INFINITY;
     float v = cap * atanhf(fminf(y, 0.9999998f)), step = (fabsf(v) + cap) * 1e-6f;
+    v -= 3.f * step;
     for (int i = 0; i < 40; i++) {
       if (capped(v) <= c - cap * 5e-7f) return v;
       v -= step;
@@ -434,6 +454,67 @@ struct Row {
   // roundings of the cap (3 ulp), the difference, the division (31 2^-23) and exp (2 ulp)
   CH_DEV float slack(float m) const { return temp * 1.6e-5f + (cap > 0.f ? cap : fabsf(m)) * 1e-6f; }
 };
+
+// cut_and_draw for at most kFew listed tokens: four threads compare one with all others.
+CH_DEV void rank_and_draw(const RowsArgs &a, uint32_t row, Shared *s, uint32_t n, int32_t top_k, float top_p, float u) {
+  static_assert(kFew * 4 == kThreads && 3 * kFew <= kBins, "threads and room");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long *key = s->tot, *w = key + kFew, *stay = w + kFew;
+  const uint32_t i = threadIdx.x >> 2, part = threadIdx.x & 3;
+  __syncthreads();
+  if (threadIdx.x < n) {
+    const float e = s->list[threadIdx.x];
+    key[threadIdx.x] = (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)~threadIdx.x;
+    w[threadIdx.x] = weight_of(e);
+  }
+  __syncthreads();
+  const unsigned long long k = i < n ? key[i] : ~0ull, wi = i < n ? w[i] : 0ull;
+  uint32_t rank = 0;
+  unsigned long long above = 0;
+#pragma unroll 4
+  for (uint32_t j = part; j < n; j += 4)
+    if (key[j] > k) rank++, above += w[j];
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    above += __shfl_xor_sync(0xffffffffu, above, o);
+  }
+  bool keep = wi > 0 && (top_k <= 0 || rank < (uint32_t)top_k);
+  if (top_p < 1.0f) {
+    unsigned long long sum = warp_sum64(keep && part == 0 ? wi : 0ull);
+    if (lane == 0) s->warp_a[warp] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int x = 0; x < kWarps; x++) sum += s->warp_a[x];
+    const unsigned long long need = (unsigned long long)ceil((double)top_p * (double)sum);
+    keep = keep && above < (need < 1 ? 1 : need);
+  }
+  if (part == 0) stay[i] = keep ? wi : 0ull;
+  const int kept = __syncthreads_count(keep && part == 0);
+  if (warp > 0) return;
+  unsigned long long v[4], run = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = stay[4 * lane + j], run += v[j];
+  const unsigned long long mine = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long x = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += x;
+  }
+  const unsigned long long total = __shfl_sync(0xffffffffu, run, 31);
+  unsigned long long goal = u > 0.f ? (unsigned long long)((double)u * (double)total) : 0ull;
+  goal = min(goal, total - 1);
+  run -= mine;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (run <= goal && goal < run + v[j]) {
+      a.tokens[row] = (int32_t)s->list_id[4 * lane + j];
+      if (a.logprobs) a.logprobs[row] = (float)log((double)v[j] / (double)total);
+      if (a.kept) a.kept[row] = kept;
+    }
+    run += v[j];
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs a) {
@@ -579,8 +660,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   // ---- few candidates: a bound `low` on the logits that can stay ----
   if (m < INFINITY && (a.vocab <= kList || by_k || r.min_p > 0.f)) {
     float low = -INFINITY;
-    if (r.min_p > 0.f) low = r.below(mc + r.temp * (logf(fminf(r.min_p, 1.f)) - 1e-5f) - r.slack(mc));
-    if (bound > -INFINITY) low = fmaxf(low, r.below(r.capped(bound) - r.slack(mc)));
+    if (r.min_p > 0.f) low = mc + r.temp * (logf(fminf(r.min_p, 1.f)) - 1e-5f) - r.slack(mc);
+    if (bound > -INFINITY) low = fmaxf(low, r.capped(bound) - r.slack(mc));
+    if (low > -INFINITY) low = r.below(low);
     // which of its tokens each lane gives: four neighbouring ones per 128 of the warp's part
     constexpr uint32_t kPart = kSlice / kWarps, kSteps = kPart / 128 + 1;  // one more for the shift
     static_assert(kSteps * 4 <= 64, "bits");
@@ -656,6 +738,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
       for (uint32_t j = 0; j < kList / kThreads; j++) {
         const uint32_t i = threadIdx.x + j * kThreads;
         if (i < count) s->list[i] = r.weigh(x4[j], top);
+      }
+      if (count <= kFew) {
+        rank_and_draw(a, row, s, count, r.top_k, r.top_p, r.u);
+        return;
       }
       __syncthreads();
       cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set}, r.top_k, r.top_p, r.u, s->list_id);
