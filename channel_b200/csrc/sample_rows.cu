@@ -165,7 +165,8 @@ struct Round {
 
 // bin of s->tot[0, nb) (from the highest) with sum above < target <= sum above + its own;
 // s->found = {bin, sum above, its sum}; bin = nb when the bins hold less than target.
-CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
+// target 0: ceil(p * the sum of all bins), at least 1.  Returns the target.
+CH_DEV unsigned long long find_bin(Shared *s, uint32_t nb, unsigned long long target, double p) {
   constexpr int kPer = (kBins + kThreads - 1) / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t per = (nb + kThreads - 1) / kThreads;
@@ -185,8 +186,17 @@ CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
   if (lane == 31) s->warp_a[warp] = inc;
   if (threadIdx.x == 0) s->found[0] = nb;
   __syncthreads();
-  unsigned long long above = inc - mine;
-  for (int w = 0; w < warp; w++) above += s->warp_a[w];
+  unsigned long long above = inc - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    const unsigned long long x = s->warp_a[w];
+    if (w < warp) above += x;
+    all += x;
+  }
+  if (target == 0) {
+    const unsigned long long need = (unsigned long long)ceil(p * (double)all);
+    target = need < 1 ? 1 : need;
+  }
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     if (above < target && target <= above + v[j]) {
@@ -197,12 +207,22 @@ CH_DEV void find_bin(Shared *s, uint32_t nb, unsigned long long target) {
     above += v[j];
   }
   __syncthreads();
+  return target;
+}
+
+// The bin of a token in the first round, added to the CTA's bins
+template <bool COUNT>
+CH_DEV void add_first(Shared *s, uint32_t key) {
+  const Round rd = {kBins, 18};
+  const uint32_t bin = (key - kKeyLow) >> 18;
+  atomicAdd(&s->cnt[bin], 1u);
+  if (!COUNT) atomicAdd(&s->low[bin], rd.low_of(key));
 }
 
 // Narrows `cut` to the first part of the order that holds `target` tokens (COUNT) or the
-// weight ceil(p * sum of all kept so far).
+// weight ceil(p * sum of all kept so far).  binned: the first round's bins are filled already.
 template <bool COUNT, bool CLUSTER>
-CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, double p) {
+CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, double p, bool binned) {
   Shared *s = t.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float *e = t.e;
@@ -210,14 +230,14 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
   for (int round = 0; round < 3; round++) {
     const Round rd = {round == 0 ? kBins : kSub, round == 0 ? 18u : round == 1 ? 9u : 0u};
     const uint32_t nb = rd.bins;
-    for (uint32_t i = threadIdx.x; i < nb; i += kThreads) s->cnt[i] = s->low[i] = 0;
-    __syncthreads();
+    if (round > 0 || !binned) {
+      for (uint32_t i = threadIdx.x; i < nb; i += kThreads) s->cnt[i] = s->low[i] = 0;
+      __syncthreads();
+    }
     if (round == 0) {
-      for (uint32_t i = threadIdx.x; i < t.n; i += kThreads) {
-        const uint32_t key = __float_as_uint(e[i]), bin = (key - kKeyLow) >> 18;
-        if (key == 0 || !cut.keeps(key, t.base + i)) continue;
-        atomicAdd(&s->cnt[bin], 1u);
-        if (!COUNT) atomicAdd(&s->low[bin], rd.low_of(key));
+      for (uint32_t i = threadIdx.x; i < t.n && !binned; i += kThreads) {
+        const uint32_t key = __float_as_uint(e[i]);
+        if (key != 0 && cut.keeps(key, t.base + i)) add_first<COUNT>(s, key);
       }
     } else {
       // few bins hold many tokens here (16-bit logits have few distinct values), and additions
@@ -243,36 +263,36 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
     t.sync();  // every CTA's bins are complete
     const uint32_t key_base = round == 0 ? kKeyLow : prefix << (rd.shift + 9);
     if (CLUSTER) {
-      // C (a power of two) neighbouring threads share a bin: remote reads in flight together
-      const uint32_t part = (nb + t.C - 1) / t.C, b0 = min(nb, t.rank * part), b1 = min(nb, b0 + part);
-      const uint32_t c = threadIdx.x & (t.C - 1);
-      for (uint32_t b = b0 + threadIdx.x / t.C; b < ((b1 - b0 + 31) & ~31u) + b0; b += kThreads / t.C) {
-        unsigned long long sum = 0;
-        if (b < b1) {
-          const uint32_t n = *t.cl.map_shared_rank(&s->cnt[b], c);
-          sum = COUNT ? n : rd.sum_of(n, *t.cl.map_shared_rank(&s->low[b], c), key_base + (b << rd.shift));
+      // this CTA's part of the bins: warp w reads CTA w's (neighbouring words), the sums go
+      // through the list's memory, and warp w gives them to CTA w
+      const uint32_t part = (nb + t.C - 1) / t.C, b0 = min(nb, t.rank * part), mine = min(nb, b0 + part) - b0;
+      unsigned long long *sums = reinterpret_cast<unsigned long long *>(s->list);  // [C][part]
+      static_assert((kBins + kMaxCluster) * sizeof(unsigned long long) <= sizeof(s->list) + sizeof(s->list_id), "room");
+      for (uint32_t c = warp; c < t.C; c += kWarps) {
+        const uint32_t *cnt = t.cl.map_shared_rank(s->cnt, c) + b0, *lows = t.cl.map_shared_rank(s->low, c) + b0;
+#pragma unroll 4
+        for (uint32_t b = lane; b < mine; b += 32) {
+          const uint32_t n = cnt[b];
+          sums[c * part + b] = COUNT ? n : rd.sum_of(n, lows[b], key_base + ((b0 + b) << rd.shift));
         }
-        for (uint32_t o = 1; o < t.C; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (b < b1) *t.cl.map_shared_rank(&s->tot[b], c) = sum;
+      }
+      __syncthreads();
+      for (uint32_t b = threadIdx.x; b < mine; b += kThreads) {
+        unsigned long long sum = 0;
+        for (uint32_t c = 0; c < t.C; c++) sum += sums[c * part + b];
+        sums[b] = sum;  // read by this thread alone
+      }
+      __syncthreads();
+      for (uint32_t c = warp; c < t.C; c += kWarps) {
+        unsigned long long *tot = t.cl.map_shared_rank(s->tot, c) + b0;
+        for (uint32_t b = lane; b < mine; b += 32) tot[b] = sums[b];
       }
     } else {
       for (uint32_t b = threadIdx.x; b < nb; b += kThreads)
         s->tot[b] = COUNT ? s->cnt[b] : rd.sum_of(s->cnt[b], s->low[b], key_base + (b << rd.shift));
     }
     t.sync();  // every CTA has every sum, and is done with every CTA's bins
-    if (!COUNT && round == 0) {  // what top-p asks for, from the sum of all weights
-      unsigned long long sum = 0;
-      for (uint32_t i = threadIdx.x; i < nb; i += kThreads) sum += s->tot[i];
-      sum = warp_sum64(sum);
-      if (lane == 0) s->warp_a[warp] = sum;
-      __syncthreads();
-      sum = 0;
-      for (int w = 0; w < kWarps; w++) sum += s->warp_a[w];
-      __syncthreads();
-      const unsigned long long need = (unsigned long long)ceil(p * (double)sum);
-      target = need < 1 ? 1 : need;
-    }
-    find_bin(s, nb, target);
+    target = find_bin(s, nb, target, p);
     const uint32_t bin = (uint32_t)s->found[0];
     const unsigned long long above = s->found[1], in_bin = s->found[2];
     if (bin >= nb) return cut;  // fewer tokens than asked for: all stay
@@ -340,13 +360,13 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
 // or NULL for the place itself.
 template <bool CLUSTER>
 CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> &t, int32_t top_k, float top_p, float u,
-                         const uint32_t *id) {
+                         const uint32_t *id, bool binned) {
   Shared *s = t.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float *e = t.e;
   Cut cut{kKeyLow, 0xFFFFFFFFu};
-  if (top_k > 0) cut = select<true>(t, cut, (unsigned long long)top_k, 0.0);
-  if (top_p < 1.0f) cut = select<false>(t, cut, 0, (double)top_p);
+  if (top_k > 0) cut = select<true>(t, cut, (unsigned long long)top_k, 0.0, binned);
+  if (top_p < 1.0f) cut = select<false>(t, cut, 0, (double)top_p, binned && top_k <= 0);
   const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
   unsigned long long mass = 0;
   uint32_t cnt = 0;
@@ -744,7 +764,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
         return;
       }
       __syncthreads();
-      cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set}, r.top_k, r.top_p, r.u, s->list_id);
+      cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set}, r.top_k, r.top_p, r.u, s->list_id,
+                   false);
       return;
     }
   }
@@ -764,10 +785,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
     for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
     set ^= 1;
   }
+  // (the first round's bins are filled on the way)
+  for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) s->cnt[i] = s->low[i] = 0;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) e[i] = r.weigh(e[i], top);
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    const float w = r.weigh(e[i], top);
+    e[i] = w;
+    if (w > 0.f) {
+      if (r.top_k > 0)
+        add_first<true>(s, __float_as_uint(w));
+      else if (r.top_p < 1.0f)
+        add_first<false>(s, __float_as_uint(w));
+    }
+  }
   __syncthreads();
-  cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr);
+  cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
 
 template <typename T>
