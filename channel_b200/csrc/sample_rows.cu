@@ -242,21 +242,33 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
     } else {
       // few bins hold many tokens here (16-bit logits have few distinct values), and additions
       // to one address go one by one: a warp adds each of its bins once
-      for (uint32_t i0 = warp * 32; i0 < t.n; i0 += kThreads) {
-        const uint32_t i = i0 + lane, key = i < t.n ? __float_as_uint(e[i]) : 0u, bin = (key >> rd.shift) & (kSub - 1);
-        const bool in = key != 0 && key >> (rd.shift + 9) == prefix && cut.keeps(key, t.base + i);
-        uint32_t left = __ballot_sync(0xffffffffu, in);
-        while (left) {
-          const int first = __ffs(left) - 1;
-          const uint32_t its = __shfl_sync(0xffffffffu, bin, first);  // by every lane
-          const bool mine = in && bin == its;
-          const uint32_t same = __ballot_sync(0xffffffffu, mine);
-          if (lane == first) atomicAdd(&s->cnt[bin], __popc(same));
-          if (!COUNT && rd.shift > 0) {
-            const uint32_t sum = __reduce_add_sync(0xffffffffu, mine ? rd.low_of(key) : 0u);
-            if (lane == first) atomicAdd(&s->low[bin], sum);
+      for (uint32_t i0 = warp * 32; i0 < t.n; i0 += 4 * kThreads) {
+        uint32_t keys[4];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t i = i0 + j * kThreads + lane;
+          keys[j] = i < t.n ? __float_as_uint(e[i]) : 0u;
+          if (keys[j] >> (rd.shift + 9) != prefix || !cut.keeps(keys[j], t.base + i)) keys[j] = 0;
+          any |= keys[j] != 0;
+        }
+        if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t key = keys[j], bin = (key >> rd.shift) & (kSub - 1);
+          uint32_t left = __ballot_sync(0xffffffffu, key != 0);
+          while (left) {
+            const int first = __ffs(left) - 1;
+            const uint32_t its = __shfl_sync(0xffffffffu, bin, first);  // by every lane
+            const bool mine = key != 0 && bin == its;
+            const uint32_t same = __ballot_sync(0xffffffffu, mine);
+            if (lane == first) atomicAdd(&s->cnt[bin], __popc(same));
+            if (!COUNT && rd.shift > 0) {
+              const uint32_t sum = __reduce_add_sync(0xffffffffu, mine ? rd.low_of(key) : 0u);
+              if (lane == first) atomicAdd(&s->low[bin], sum);
+            }
+            left &= ~same;
           }
-          left &= ~same;
         }
       }
     }
@@ -356,7 +368,7 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
 }
 
 // Top-k and top-p among the tokens (what min-p drops has weight 0), then the draw, in the
-// order of their places: warp w owns the part [w * seg, (w + 1) * seg).  id: a place's token,
+// order of their places.  id: a place's token,
 // or NULL for the place itself.
 template <bool CLUSTER>
 CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> &t, int32_t top_k, float top_p, float u,
@@ -367,16 +379,24 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
   Cut cut{kKeyLow, 0xFFFFFFFFu};
   if (top_k > 0) cut = select<true>(t, cut, (unsigned long long)top_k, 0.0, binned);
   if (top_p < 1.0f) cut = select<false>(t, cut, 0, (double)top_p, binned && top_k <= 0);
-  const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
-  unsigned long long mass = 0;
+  // thread t owns the `run` places from t * run on, starting at one of them that spreads the
+  // lanes over the banks
+  const uint32_t run = (t.n + kThreads - 1) / kThreads, p0 = threadIdx.x * run;
+  unsigned long long own = 0;
   uint32_t cnt = 0;
-  for (uint32_t i = w0 + lane; i < w1; i += 32) {
-    const uint32_t key = __float_as_uint(e[i]);
-    if (key != 0 && cut.keeps(key, t.base + i)) {
-      mass += weight_of(e[i]);
-      cnt++;
-    }
+  auto kept_weight = [&](uint32_t i) {
+    const uint32_t key = i < t.n ? __float_as_uint(e[i]) : 0u;
+    return key != 0 && cut.keeps(key, t.base + i) ? weight_of(__uint_as_float(key)) : 0ull;
+  };
+  uint32_t place = run ? lane % run : 0u;
+#pragma unroll 4
+  for (uint32_t j = 0; j < run; j++) {
+    const unsigned long long w = kept_weight(p0 + place);
+    own += w;
+    cnt += w > 0;
+    place = place + 1 == run ? 0 : place + 1;
   }
+  unsigned long long mass = own;
   mass = warp_sum64(mass);
   cnt = __reduce_add_sync(0xffffffffu, cnt);
   __syncthreads();
@@ -402,17 +422,25 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
   unsigned long long goal = u > 0.f ? (unsigned long long)((double)u * (double)total) : 0ull;
   goal = min(goal, total - 1);
   if (before <= goal && goal < before + mass) {  // this warp's part holds the token
-    unsigned long long run = before;
-    for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-      const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
-      const unsigned long long w = key != 0 && cut.keeps(key, t.base + i) ? weight_of(e[i]) : 0ull;
-      unsigned long long inc = w;
+    unsigned long long inc = own;  // the lane that does, then the place in its run
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const int owner = __ffs(__ballot_sync(0xffffffffu, before + inc > goal)) - 1;
+    unsigned long long sum = before + __shfl_sync(0xffffffffu, inc - own, owner);
+    const uint32_t q0 = (warp * 32 + owner) * run;
+    for (uint32_t j0 = 0; j0 < run; j0 += 32) {
+      const uint32_t i = q0 + j0 + lane;
+      const unsigned long long w = j0 + lane < run ? kept_weight(i) : 0ull;
+      inc = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
-      const uint32_t hit = __ballot_sync(0xffffffffu, run + inc > goal);
+      const uint32_t hit = __ballot_sync(0xffffffffu, sum + inc > goal);
       if (hit) {
         if (lane == __ffs(hit) - 1) {
           a.tokens[row] = (int32_t)(id ? id[i] : t.base + i);
@@ -421,28 +449,37 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
         }
         break;
       }
-      run += __shfl_sync(0xffffffffu, inc, 31);
+      sum += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
 }
 
 // What one row asks for
 struct Row {
-  float temp, inv, top_p, min_p, cap, lowest, u;
+  float temp, inv, top_p, min_p, cap, cap_inv, lowest, u;
   int32_t top_k;
-  bool quick;  // q_of may divide by multiplication
+  bool quick, cap_quick;  // divisions by temp, by cap may go by multiplication
+
+  // x / y correctly rounded, from r = 1 / y correctly rounded: with q = x r the quotient is
+  // q + (x - q y) r, each step one FMA (P. Markstein, IBM J. Res. Dev. 34, 1990), for y far from
+  // the ends of the range and with a mantissa that is not all ones
+  static CH_DEV bool divides(float y) {
+    return y > 1e-15f && y < 1e15f && (__float_as_uint(y) & 0x7FFFFFu) != 0x7FFFFFu;
+  }
+  static CH_DEV float divide(float x, float y, float r) {
+    const float q = x * r;
+    return __fmaf_rn(__fmaf_rn(-y, q, x), r, q);
+  }
 
   // (a logit of -inf or the type's lowest value masks its token and stays as it is)
-  CH_DEV float capped(float v) const { return cap > 0.f && v > lowest ? tanhf(__fdiv_rn(v, cap)) * cap : v; }
-  // (x - m) / T, correctly rounded.  quick: with r = 1 / T correctly rounded and q = d r, the
-  // quotient is q + (d - q T) r, each step one FMA (P. Markstein, IBM J. Res. Dev. 34, 1990);
-  // d and T are far from the ends of the range there, and where d / T is below -64 only the
-  // sign of the answer matters.
+  CH_DEV float capped(float v) const {
+    if (!(cap > 0.f && v > lowest)) return v;
+    return tanhf(cap_quick && fabsf(v) < 1e30f ? divide(v, cap, cap_inv) : __fdiv_rn(v, cap)) * cap;
+  }
+  // (x - m) / T, correctly rounded (where it is below -64 only the sign matters)
   CH_DEV float q_of(float x, float m) const {
     const float d = x - m;
-    if (!quick) return __fdiv_rn(d, temp);
-    const float q = d * inv;
-    return __fmaf_rn(__fmaf_rn(-temp, q, d), inv, q);
+    return quick ? divide(d, temp, inv) : __fdiv_rn(d, temp);
   }
   // e, or 0 where the weight is 0 or min-p drops the token
   CH_DEV float weigh(float x, float m) const {
@@ -584,7 +621,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   r.cap = a.softcap;
   r.lowest = lowest_of(x);
   r.inv = __frcp_rn(r.temp);
-  r.quick = r.temp > 1e-15f && r.temp < 1e15f && (__float_as_uint(r.temp) & 0x7FFFFFu) != 0x7FFFFFu;
+  r.quick = Row::divides(r.temp);
+  r.cap_inv = __frcp_rn(r.cap);
+  r.cap_quick = Row::divides(r.cap);
   if (r.top_k <= 0 || (uint32_t)r.top_k >= a.vocab) r.top_k = 0;
 
   const Tokens<true> all{s, cl, C, rank, e, n, base, set};
