@@ -51,7 +51,8 @@ constexpr uint32_t kSlice = 16384, kMaxCluster = 16;
 constexpr uint32_t kMaxVocab = kSlice * kMaxCluster;
 constexpr uint32_t kKeyLow = 0x29800000u;  // bits of 2^-44: the least e of non-zero weight
 constexpr uint32_t kBins = 1409, kSub = 512;  // of the first round, of the others
-constexpr uint32_t kFew = 128;     // candidates that are ranked by comparing all with all
+constexpr uint32_t kFew = 256;     // candidates that are ranked by comparing all with all
+constexpr int32_t kLeft = -2;      // the token of a row that the second kernel takes
 
 struct RowsArgs {
   const void *logits;
@@ -62,6 +63,7 @@ struct RowsArgs {
   float *logprobs;
   uint32_t vocab, per;  // tokens per CTA
   float softcap;
+  bool left_only;  // rows whose token is kLeft
 };
 
 constexpr uint32_t kList = 2048;    // candidates one CTA takes
@@ -105,6 +107,11 @@ CH_DEV void unpack16(const uint4 &r, float (&f)[8], const __nv_bfloat16 *) {
   const uint32_t u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; i++) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+}
+CH_DEV void answer(const RowsArgs &a, uint32_t row, int32_t token, float logprob, int32_t kept) {
+  a.tokens[row] = token;
+  if (a.logprobs) a.logprobs[row] = logprob;
+  if (a.kept) a.kept[row] = kept;
 }
 // floor(2^44 e) for 0 <= e <= 1: the mantissa shifted (a conversion to 64 bits is many times slower)
 CH_DEV unsigned long long weight_of(float e) {
@@ -443,9 +450,7 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
       const uint32_t hit = __ballot_sync(0xffffffffu, sum + inc > goal);
       if (hit) {
         if (lane == __ffs(hit) - 1) {
-          a.tokens[row] = (int32_t)(id ? id[i] : t.base + i);
-          if (a.logprobs) a.logprobs[row] = (float)log((double)w / (double)total);
-          if (a.kept) a.kept[row] = (int32_t)kept;
+          answer(a, row, (int32_t)(id ? id[i] : t.base + i), (float)log((double)w / (double)total), (int32_t)kept);
         }
         break;
       }
@@ -507,69 +512,134 @@ struct Row {
     }
     return -INFINITY;
   }
+  // A bound on the logits that can stay, from the largest capped logit and a logit that top_k
+  // tokens are not below (or -inf)
+  CH_DEV float least_logit(float mc, float bound) const {
+    float c = -INFINITY;
+    if (min_p > 0.f) c = mc + temp * (logf(fminf(min_p, 1.f)) - 1e-5f) - slack(mc);
+    if (bound > -INFINITY) c = fmaxf(c, capped(bound) - slack(mc));
+    return c > -INFINITY ? below(c) : c;
+  }
   // by how much a capped logit has to be lower for its e to be lower too, whatever the
   // roundings of the cap (3 ulp), the difference, the division (31 2^-23) and exp (2 ulp)
   CH_DEV float slack(float m) const { return temp * 1.6e-5f + (cap > 0.f ? cap : fabsf(m)) * 1e-6f; }
 };
 
-// cut_and_draw for at most kFew listed tokens: four threads compare one with all others.
-CH_DEV void rank_and_draw(const RowsArgs &a, uint32_t row, Shared *s, uint32_t n, int32_t top_k, float top_p, float u) {
-  static_assert(kFew * 4 == kThreads && 3 * kFew <= kBins, "threads and room");
+// The CTA's largest logit m from its threads' (own) and, for want > 0, a bound that `want` of
+// them are not below (or -inf), by a histogram over the range of the threads' maxima.
+// maxima[kMaxima] is 0 and *pick kMaxima before.
+CH_DEV void cta_bound(float own, uint32_t want, uint32_t *maxima, unsigned long long *warp_a, uint32_t *warp_b,
+                      uint32_t *pick, float &m, float &bound) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long *key = s->tot, *w = key + kFew, *stay = w + kFew;
-  const uint32_t i = threadIdx.x >> 2, part = threadIdx.x & 3;
-  __syncthreads();
-  if (threadIdx.x < n) {
-    const float e = s->list[threadIdx.x];
-    key[threadIdx.x] = (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)~threadIdx.x;
-    w[threadIdx.x] = weight_of(e);
-  }
-  __syncthreads();
-  const unsigned long long k = i < n ? key[i] : ~0ull, wi = i < n ? w[i] : 0ull;
-  uint32_t rank = 0;
-  unsigned long long above = 0;
-#pragma unroll 4
-  for (uint32_t j = part; j < n; j += 4)
-    if (key[j] > k) rank++, above += w[j];
+  float least = own > -INFINITY ? own : INFINITY;
+  m = warp_max(own);
+  bound = -INFINITY;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    above += __shfl_xor_sync(0xffffffffu, above, o);
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  if (lane == 0) warp_a[warp] = (unsigned long long)__float_as_uint(m) << 32 | __float_as_uint(least);
+  __syncthreads();
+  for (int w = 0; w < kWarps; w++) {
+    m = fmaxf(m, __uint_as_float((uint32_t)(warp_a[w] >> 32)));
+    least = fminf(least, __uint_as_float((uint32_t)warp_a[w]));
   }
-  bool keep = wi > 0 && (top_k <= 0 || rank < (uint32_t)top_k);
-  if (top_p < 1.0f) {
-    unsigned long long sum = warp_sum64(keep && part == 0 ? wi : 0ull);
-    if (lane == 0) s->warp_a[warp] = sum;
-    __syncthreads();
-    sum = 0;
-    for (int x = 0; x < kWarps; x++) sum += s->warp_a[x];
-    const unsigned long long need = (unsigned long long)ceil((double)top_p * (double)sum);
-    keep = keep && above < (need < 1 ? 1 : need);
-  }
-  if (part == 0) stay[i] = keep ? wi : 0ull;
-  const int kept = __syncthreads_count(keep && part == 0);
-  if (warp > 0) return;
-  unsigned long long v[4], run = 0;
-#pragma unroll
-  for (int j = 0; j < 4; j++) v[j] = stay[4 * lane + j], run += v[j];
-  const unsigned long long mine = run;
+  if (want == 0) return;
+  const float per_bin = least < m && m < INFINITY ? (kMaxima - 1) / (m - least) : 0.f;
+  if (own > -INFINITY) atomicAdd(&maxima[min(kMaxima - 1, (uint32_t)((m - own) * per_bin))], 1u);
+  __syncthreads();
+  const uint32_t v0 = maxima[2 * threadIdx.x], v1 = maxima[2 * threadIdx.x + 1];
+  static_assert(kMaxima == 2 * kThreads, "two bins per thread");
+  uint32_t run = v0 + v1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long x = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += x;
+    const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += u;
   }
-  const unsigned long long total = __shfl_sync(0xffffffffu, run, 31);
-  unsigned long long goal = u > 0.f ? (unsigned long long)((double)u * (double)total) : 0ull;
-  goal = min(goal, total - 1);
-  run -= mine;
+  if (lane == 31) warp_b[warp] = run;
+  __syncthreads();
+  uint32_t before = run - v0 - v1;
+  for (int w = 0; w < warp; w++) before += warp_b[w];
+  if (before < want && want <= before + v0) *pick = 2 * threadIdx.x;
+  if (before + v0 < want && want <= before + v0 + v1) *pick = 2 * threadIdx.x + 1;
+  __syncthreads();
+  if (*pick < kMaxima - 1 && per_bin > 0.f) {
+    const float end = m - (*pick + 1) / per_bin;  // the bin's lower end, lowered by its rounding
+    bound = end - (fabsf(end) + fabsf(m)) * 1e-6f;
+  }
+}
+
+CH_DEV Row row_of(const RowsArgs &a, uint32_t row, float lowest) {
+  Row r;
+  r.temp = a.temperature ? a.temperature[row] : 1.0f;
+  r.top_p = a.top_p ? a.top_p[row] : 1.0f;
+  r.min_p = a.min_p ? a.min_p[row] : 0.f;
+  r.top_k = a.top_k ? a.top_k[row] : 0;
+  r.u = a.uniform[row];
+  r.cap = a.softcap;
+  r.lowest = lowest;
+  r.inv = __frcp_rn(r.temp);
+  r.quick = Row::divides(r.temp);
+  r.cap_inv = __frcp_rn(r.cap);
+  r.cap_quick = Row::divides(r.cap);
+  if (r.top_k <= 0 || (uint32_t)r.top_k >= a.vocab) r.top_k = 0;
+  return r;
+}
+
+struct Few {
+  unsigned long long key[kFew], w[kFew], warp_a[kWarps];
+};
+// cut_and_draw for n <= kFew tokens with weights e and indices id, in any order: two threads
+// compare one with all others.
+CH_DEV void rank_and_draw(const RowsArgs &a, uint32_t row, Few *s, const float *e, const uint32_t *id, uint32_t n,
+                          int32_t top_k, float top_p, float u) {
+  static_assert(kFew * 2 == kThreads, "threads");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t i = threadIdx.x >> 1, part = threadIdx.x & 1;
+  __syncthreads();
+  if (threadIdx.x < n) {
+    s->key[threadIdx.x] = (unsigned long long)__float_as_uint(e[threadIdx.x]) << 32 | (uint32_t)~id[threadIdx.x];
+    s->w[threadIdx.x] = weight_of(e[threadIdx.x]);
+  }
+  __syncthreads();
+  const unsigned long long k = i < n ? s->key[i] : ~0ull, wi = i < n ? s->w[i] : 0ull;
+  uint32_t rank = 0;
+  unsigned long long above = 0;
+  if (warp * 16u < n) {
+#pragma unroll 4
+    for (uint32_t j = part; j < n; j += 2)
+      if (s->key[j] > k) rank++, above += s->w[j];
+  }
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  above += __shfl_xor_sync(0xffffffffu, above, 1);
+  bool keep = wi > 0 && (top_k <= 0 || rank < (uint32_t)top_k);
+  auto sum_of = [&](unsigned long long v) {
+    v = warp_sum64(v);
+    __syncthreads();
+    if (lane == 0) s->warp_a[warp] = v;
+    __syncthreads();
+    v = 0;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    if (run <= goal && goal < run + v[j]) {
-      a.tokens[row] = (int32_t)s->list_id[4 * lane + j];
-      if (a.logprobs) a.logprobs[row] = (float)log((double)v[j] / (double)total);
-      if (a.kept) a.kept[row] = kept;
-    }
-    run += v[j];
+    for (int x = 0; x < kWarps; x++) v += s->warp_a[x];
+    return v;
+  };
+  if (top_p < 1.0f) {
+    const unsigned long long need = (unsigned long long)ceil((double)top_p * (double)sum_of(keep && part == 0 ? wi : 0ull));
+    keep = keep && above < (need < 1 ? 1 : need);
+  }
+  __syncthreads();  // every thread has compared
+  if (part == 0 && i < n) s->w[i] = keep ? wi : 0ull;  // read after the barriers of the sum
+  const unsigned long long total = sum_of(keep && part == 0 ? wi : 0ull);
+  const int kept = __syncthreads_count(keep && part == 0);
+  unsigned long long goal = u > 0.f ? (unsigned long long)((double)u * (double)total) : 0ull, before = 0;
+  goal = min(goal, total - 1);
+  const uint32_t mine = ~(uint32_t)k;
+  if (warp * 16u < n) {
+#pragma unroll 4
+    for (uint32_t j = part; j < n; j += 2)
+      if (~(uint32_t)s->key[j] < mine) before += s->w[j];
+  }
+  before += __shfl_xor_sync(0xffffffffu, before, 1);
+  if (keep && part == 0 && before <= goal && goal < before + wi) {
+    answer(a, row, (int32_t)mine, (float)log((double)wi / (double)total), kept);
   }
 }
 
@@ -579,6 +649,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   Shared *s = reinterpret_cast<Shared *>(smem_raw);
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
+  grid_dep_wait();
+  if (a.left_only && a.tokens[row] != kLeft) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
@@ -612,20 +684,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
       *reinterpret_cast<float4 *>(e + head + j * E + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
   }
   for (uint32_t i = head + vecs * E + threadIdx.x; i < n; i += kThreads) e[i] = put(load1(x + i));
-  Row r;
-  r.temp = a.temperature ? a.temperature[row] : 1.0f;
-  r.top_p = a.top_p ? a.top_p[row] : 1.0f;
-  r.min_p = a.min_p ? a.min_p[row] : 0.f;
-  r.top_k = a.top_k ? a.top_k[row] : 0;
-  r.u = a.uniform[row];
-  r.cap = a.softcap;
-  r.lowest = lowest_of(x);
-  r.inv = __frcp_rn(r.temp);
-  r.quick = Row::divides(r.temp);
-  r.cap_inv = __frcp_rn(r.cap);
-  r.cap_quick = Row::divides(r.cap);
-  if (r.top_k <= 0 || (uint32_t)r.top_k >= a.vocab) r.top_k = 0;
-
+  const Row r = row_of(a, row, lowest_of(x));
   const Tokens<true> all{s, cl, C, rank, e, n, base, set};
   // the CTA's maximum of v
   auto cta_max = [&](float v) {
@@ -637,44 +696,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
     return v;
   };
 
-  // ---- the largest logit m.  Beside it, for top-k, a bound that at least top_k tokens of the
-  // row are not below: every CTA finds its threads' maxima's ceil(top_k / C)-th largest by a
-  // histogram over their range, and the least of these counts ----
+  // ---- the largest logit m; beside it, for top-k, a bound that at least top_k tokens of the
+  // row are not below: what every CTA's share of them is not below, the least of these ----
   const bool by_k = r.top_k > 0 && r.top_k <= kMostK, bounded = a.vocab > kList && by_k && r.temp > 0.f;
-  float m = warp_max(own), least = own > -INFINITY ? own : INFINITY, bound = -INFINITY;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-  if (lane == 0) s->warp_a[warp] = (unsigned long long)__float_as_uint(m) << 32 | __float_as_uint(least);
-  __syncthreads();
-  for (int w = 0; w < kWarps; w++) {
-    m = fmaxf(m, __uint_as_float((uint32_t)(s->warp_a[w] >> 32)));
-    least = fminf(least, __uint_as_float((uint32_t)s->warp_a[w]));
-  }
-  if (bounded) {
-    const float per_bin = least < m && m < INFINITY ? (kMaxima - 1) / (m - least) : 0.f;
-    if (own > -INFINITY) atomicAdd(&s->maxima[min(kMaxima - 1, (uint32_t)((m - own) * per_bin))], 1u);
-    __syncthreads();
-    const uint32_t want = ((uint32_t)r.top_k + C - 1) / C;
-    const uint32_t v0 = s->maxima[2 * threadIdx.x], v1 = s->maxima[2 * threadIdx.x + 1];
-    static_assert(kMaxima == 2 * kThreads, "two bins per thread");
-    uint32_t run = v0 + v1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += u;
-    }
-    if (lane == 31) s->warp_b[warp] = run;
-    __syncthreads();
-    uint32_t before = run - v0 - v1;
-    for (int w = 0; w < warp; w++) before += s->warp_b[w];
-    if (before < want && want <= before + v0) s->pick = 2 * threadIdx.x;
-    if (before + v0 < want && want <= before + v0 + v1) s->pick = 2 * threadIdx.x + 1;
-    __syncthreads();
-    if (s->pick < kMaxima - 1 && per_bin > 0.f) {
-      const float end = m - (s->pick + 1) / per_bin;  // the bin's lower end, lowered by its rounding
-      bound = end - (fabsf(end) + fabsf(m)) * 1e-6f;
-    }
-  }
+  float m, bound;
+  cta_bound(own, bounded ? ((uint32_t)r.top_k + C - 1) / C : 0u, s->maxima, s->warp_a, s->warp_b, &s->pick, m, bound);
   all.exchange(__float_as_uint(m), __float_as_uint(bound));
   for (uint32_t c = 0; c < C; c++) {
     m = fmaxf(m, __uint_as_float((uint32_t)s->xch[set][c][0]));
@@ -683,11 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   set ^= 1;
 
   if (m == -INFINITY) {  // nothing to choose from
-    if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[row] = -1;
-      if (a.logprobs) a.logprobs[row] = -INFINITY;
-      if (a.kept) a.kept[row] = 0;
-    }
+    if (rank == 0 && threadIdx.x == 0) answer(a, row, -1, -INFINITY, 0);
     return;
   }
   const float mc = r.capped(m);  // the largest capped logit, up to the cap's rounding
@@ -708,20 +730,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
     for (int w = 0; w < kWarps; w++) best = max(best, s->warp_a[w]);
     all.exchange(best, 0);
     for (uint32_t c = 0; c < C; c++) best = max(best, s->xch[set][c][0]);
-    if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[row] = (int32_t)~(uint32_t)best;
-      if (a.logprobs) a.logprobs[row] = 0.f;
-      if (a.kept) a.kept[row] = 1;
-    }
+    if (rank == 0 && threadIdx.x == 0) answer(a, row, (int32_t)~(uint32_t)best, 0.f, 1);
     return;
   }
 
   // ---- few candidates: a bound `low` on the logits that can stay ----
   if (m < INFINITY && (a.vocab <= kList || by_k || r.min_p > 0.f)) {
-    float low = -INFINITY;
-    if (r.min_p > 0.f) low = mc + r.temp * (logf(fminf(r.min_p, 1.f)) - 1e-5f) - r.slack(mc);
-    if (bound > -INFINITY) low = fmaxf(low, r.capped(bound) - r.slack(mc));
-    if (low > -INFINITY) low = r.below(low);
+    const float low = r.least_logit(mc, bound);
     // which of its tokens each lane gives: four neighbouring ones per 128 of the warp's part
     constexpr uint32_t kPart = kSlice / kWarps, kSteps = kPart / 128 + 1;  // one more for the shift
     static_assert(kSteps * 4 <= 64, "bits");
@@ -799,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
         if (i < count) s->list[i] = r.weigh(x4[j], top);
       }
       if (count <= kFew) {
-        rank_and_draw(a, row, s, count, r.top_k, r.top_p, r.u);
+        rank_and_draw(a, row, reinterpret_cast<Few *>(s->tot), s->list, s->list_id, count, r.top_k, r.top_p, r.u);
         return;
       }
       __syncthreads();
@@ -841,28 +856,156 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
 
+// Many rows: first those with few candidates, without keeping logits in shared memory, so that
+// all rows are on the SMs at once (the kernel above holds 16 to 18 rows of 262,144 logits; 64
+// rows took it 70 us).  A cluster reads its row once for the threads' maxima; only the threads
+// whose maximum is not below the bound read theirs again, from L2.  Rows without min-p and
+// top-k, and rows with more than 256 candidates, are left for the other kernel.
 template <typename T>
-cudaError_t launch_rows(const RowsArgs &a, uint32_t rows, uint32_t C, cudaStream_t stream) {
-  const size_t smem = sizeof(Shared);
-  cudaError_t e = ensure_smem_attr((const void *)sample_rows_kernel<T>, smem);
-  if (e != cudaSuccess) return e;
-  if (C > 8) {
-    e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+__global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs a) {
+  struct Mem {
+    uint32_t maxima[kMaxima];
+    float list[kFew];
+    uint32_t list_id[kFew];
+    Few few;
+    unsigned long long xch[2][kMaxCluster], warp_a[kWarps];
+    uint32_t warp_b[kWarps], pick, n_list;
+  };
+  __shared__ Mem mem;
+  cg::cluster_group cl = cg::this_cluster();
+  const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
+  const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
+  grid_dep_wait();
+  grid_dep_launch();
+  const Row r = row_of(a, row, lowest_of(x));
+  const bool greedy = !(r.temp > 0.f), by_k = r.top_k > 0 && r.top_k <= (int32_t)kFew;
+  if (!(greedy || by_k || r.min_p > 0.f)) {
+    if (rank == 0 && threadIdx.x == 0) a.tokens[row] = kLeft;
+    return;
   }
+  for (uint32_t i = threadIdx.x; i < kMaxima; i += kThreads) mem.maxima[i] = 0;
+  if (threadIdx.x == 0) mem.pick = kMaxima, mem.n_list = 0;
+
+  // f(place, logit) for this thread's tokens: 16-byte pieces, and single ones at the ragged ends
+  constexpr uint32_t E = 16 / sizeof(T);
+  const uint32_t head = min(n, (E - (uint32_t)(((uintptr_t)x / sizeof(T)) % E)) % E), vecs = (n - head) / E;
+  const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+  auto each = [&](auto f) {
+#pragma unroll 4
+    for (uint32_t j = threadIdx.x; j < vecs; j += kThreads) {
+      float v[E];
+      unpack16(xv[j], v, x);
+#pragma unroll
+      for (uint32_t k = 0; k < E; k++) f(head + j * E + k, v[k]);
+    }
+    if (threadIdx.x < head) f(threadIdx.x, load1(x + threadIdx.x));
+    const uint32_t tail = head + vecs * E + threadIdx.x;
+    if (tail < n) f(tail, load1(x + tail));
+  };
+  float own = -INFINITY;  // NaN counts as masked: fmaxf drops it
+  each([&](uint32_t, float v) { own = fmaxf(own, v); });
+  float m, bound;
+  cta_bound(own, by_k && !greedy ? ((uint32_t)r.top_k + C - 1) / C : 0u, mem.maxima, mem.warp_a, mem.warp_b, &mem.pick, m,
+            bound);
+  if (threadIdx.x < C)
+    cl.map_shared_rank(&mem, threadIdx.x)->xch[0][rank] = (unsigned long long)__float_as_uint(m) << 32 | __float_as_uint(bound);
+  cl.sync();
+  for (uint32_t c = 0; c < C; c++) {
+    m = fmaxf(m, __uint_as_float((uint32_t)(mem.xch[0][c] >> 32)));
+    bound = fminf(bound, __uint_as_float((uint32_t)mem.xch[0][c]));
+  }
+  if (m == -INFINITY || m == INFINITY) {  // nothing to choose from; infinite ones go the other way
+    if (rank == 0 && threadIdx.x == 0) answer(a, row, m > 0.f ? kLeft : -1, -INFINITY, 0);
+    return;
+  }
+  const float mc = r.capped(m);
+  if (greedy) {  // the lowest index of the largest capped logit
+    const float low = r.cap > 0.f ? r.below(mc - r.cap * 1e-6f) : m;
+    unsigned long long best = 0;
+    if (own >= low)
+      each([&](uint32_t i, float v) {
+        if (!(v >= low)) return;
+        const uint32_t bits = __float_as_uint(r.capped(v)), key = bits >> 31 ? ~bits : bits | 0x80000000u;
+        best = max(best, (unsigned long long)key << 32 | (uint32_t)~(base + i));
+      });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();
+    if (lane == 0) mem.warp_a[warp] = best;
+    __syncthreads();
+    for (int w = 0; w < kWarps; w++) best = max(best, mem.warp_a[w]);
+    if (threadIdx.x == 0) cl.map_shared_rank(&mem, 0)->xch[1][rank] = best;
+    cl.sync();
+    if (rank == 0 && threadIdx.x == 0) {
+      for (uint32_t c = 0; c < C; c++) best = max(best, mem.xch[1][c]);
+      answer(a, row, (int32_t)~(uint32_t)best, 0.f, 1);
+    }
+    return;
+  }
+  const float low = r.least_logit(mc, bound);
+  if (own >= low && own > -INFINITY) {
+    Mem *to = cl.map_shared_rank(&mem, 0);
+    each([&](uint32_t i, float v) {
+      if (!(v >= low) || v == -INFINITY) return;
+      const uint32_t at = atomicAdd(&to->n_list, 1u);
+      if (at < kFew) to->list[at] = v, to->list_id[at] = base + i;
+    });
+  }
+  cl.sync();
+  if (rank != 0) return;
+  const uint32_t count = mem.n_list;
+  if (count > kFew) {
+    if (threadIdx.x == 0) a.tokens[row] = kLeft;
+    return;
+  }
+  float v = threadIdx.x < count ? r.capped(mem.list[threadIdx.x]) : -INFINITY, top = warp_max(v);
+  if (lane == 0) mem.warp_b[warp] = __float_as_uint(top);
+  __syncthreads();
+  for (int w = 0; w < kWarps; w++) top = fmaxf(top, __uint_as_float(mem.warp_b[w]));
+  if (threadIdx.x < count) mem.list[threadIdx.x] = r.weigh(v, top);
+  rank_and_draw(a, row, &mem.few, mem.list, mem.list_id, count, r.top_k, r.top_p, r.u);
+}
+
+template <typename K>
+cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t rows, uint32_t C, size_t smem, cudaStream_t stream) {
+  cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
+  if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * C);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, a);
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <typename T>
+cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
+  uint32_t C = 1;
+  while (C * kSlice < a.vocab) C *= 2;
+  // When the rows need more than one wave of the kernel that keeps them (two CTAs per SM, and
+  // the SMs of a cluster are neighbours: about 14 per 16 SMs' worth), the rows with few
+  // candidates go first; a setting that no row can have them by leaves that kernel out
+  a.left_only = rows * C > (uint32_t)num_sms() * 7 / 4 && (a.temperature || a.top_k || a.min_p);
+  if (a.left_only) {
+    const uint32_t few = C > 8 ? 8 : C;
+    a.per = (a.vocab + few - 1) / few;
+    const cudaError_t e = start_clusters(sample_few_kernel<T>, a, rows, few, 0, stream);
+    if (e != cudaSuccess) return e;
+  }
+  a.per = (a.vocab + C - 1) / C;
+  return start_clusters(sample_rows_kernel<T>, a, rows, C, sizeof(Shared), stream);
 }
 
 int sample_rows(const ch_sample_rows_args *p, void *stream) {
@@ -892,13 +1035,10 @@ int sample_rows(const ch_sample_rows_args *p, void *stream) {
   a.logprobs = p->logprobs;
   a.vocab = p->vocab;
   a.softcap = p->softcap;
-  uint32_t C = 1;
-  while (C * kSlice < p->vocab) C *= 2;
-  a.per = (p->vocab + C - 1) / C;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = p->dtype == CH_F32   ? launch_rows<float>(a, p->n_rows, C, s)
-                        : p->dtype == CH_F16 ? launch_rows<__half>(a, p->n_rows, C, s)
-                                             : launch_rows<__nv_bfloat16>(a, p->n_rows, C, s);
+  const cudaError_t e = p->dtype == CH_F32   ? launch_rows<float>(a, p->n_rows, s)
+                        : p->dtype == CH_F16 ? launch_rows<__half>(a, p->n_rows, s)
+                                             : launch_rows<__nv_bfloat16>(a, p->n_rows, s);
   if (e != cudaSuccess) return set_last_error(CH_ECUDA, std::string("sample_rows: ") + cudaGetErrorString(e));
   return CH_OK;
 }

@@ -154,6 +154,32 @@ def test_equals_the_integer_arithmetic(v, pad, dtype, softcap):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v,pad", [(40, 262144, 0), (67, 100003, 2), (300, 9001, 1), (600, 300, 3)])
+def test_many_rows(n, v, pad, dtype):
+    """batches of more rows than are taken at once, of every kind: greedy, few candidates, many,
+    ties at the cuts, rows of masks, of +inf"""
+    for seed, softcap in ((1, 0.0), (2, 30.0)):
+        rng = np.random.default_rng(seed)
+        x = lm_logits(n, v + pad, seed, dtype)[:, :v]
+        x[3], x[4, 5:], x[5, v // 2] = -torch.inf, -torch.inf, torch.inf
+        x[6], x[7] = 1.5, torch.finfo(dtype).min
+        x[8:12] = (x[8:12] * 2).round() / 2
+        kw, u = random_settings(n, rng), rng.random(n).astype(np.float32)
+        for k in ("temperature", "top_k", "top_p", "min_p"):  # a setting left out, too
+            given = {i: j for i, j in kw.items() if i != k}
+            token, lp, kept = draw(x, u, softcap, **given)
+            s = settings(n, **{**kw, k: np.full(n, dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)[k])})
+            seen = torch.arange(n, device="cuda") != 3
+            if softcap:
+                seen &= (torch.arange(n, device="cuda") != 4) & (torch.arange(n, device="cuda") != 7)
+            rt, rl, rk = plain(x[seen], torch.from_numpy(u).cuda()[seen], softcap, **{i: j[seen] for i, j in s.items()})
+            at = seen.cpu().numpy()
+            assert np.array_equal(token[at], rt.cpu().numpy()) and np.array_equal(kept[at], rk.cpu().numpy())
+            assert token[3] == -1 and kept[3] == 0 and token[4] < 5
+
+
+@gpu
 def test_wide_nucleus():
     """flat rows: the kept part is most of the vocabulary, cut inside runs of near-equal weights"""
     n, v = 6, 262144
