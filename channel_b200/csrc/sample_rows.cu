@@ -54,6 +54,9 @@ constexpr uint32_t kBins = 1409, kSub = 512;  // of the first round, of the othe
 constexpr uint32_t kFew = 256;     // candidates that are ranked by comparing all with all
 constexpr int32_t kLeft = -2;      // the token of a row that the second kernel takes
 
+// Which rows a launch takes: all; those whose settings leave many candidates; those of the rest
+// whose token is kLeft
+enum class Rows { kAll, kMany, kLeftOver };
 struct RowsArgs {
   const void *logits;
   long long row_stride;
@@ -63,7 +66,7 @@ struct RowsArgs {
   float *logprobs;
   uint32_t vocab, per;  // tokens per CTA
   float softcap;
-  bool left_only;  // rows whose token is kLeft
+  Rows which;
 };
 
 constexpr uint32_t kList = 2048;    // candidates one CTA takes
@@ -465,6 +468,8 @@ struct Row {
   int32_t top_k;
   bool quick, cap_quick;  // divisions by temp, by cap may go by multiplication
 
+  // whether the settings leave few tokens: the largest one, up to kFew, or those min-p keeps
+  CH_DEV bool few() const { return !(temp > 0.f) || (top_k > 0 && top_k <= (int32_t)kFew) || min_p > 0.f; }
   // x / y correctly rounded, from r = 1 / y correctly rounded: with q = x r the quotient is
   // q + (x - q y) r, each step one FMA (P. Markstein, IBM J. Res. Dev. 34, 1990), for y far from
   // the ends of the range and with a mantissa that is not all ones
@@ -486,16 +491,12 @@ struct Row {
     const float d = x - m;
     return quick ? divide(d, temp, inv) : __fdiv_rn(d, temp);
   }
-  // e, or 0 where the weight is 0 or min-p drops the token
+  // e, or 0 where the weight is 0 or min-p drops the token.  No branches: x = m gives exp(0),
+  // and what over- or underflows on the way (x far below m, or masked) gives 0 or NaN, which the
+  // comparison drops
   CH_DEV float weigh(float x, float m) const {
-    float w = 1.0f;
-    if (x != m) {
-      const float d = x - m;
-      if (!(d >= -64.f * temp)) return 0.f;  // far below 2^-44
-      w = expf(q_of(x, m));
-    }
-    if (!(w >= __uint_as_float(kKeyLow)) || (min_p > 0.f && w < min_p && w != 1.0f)) w = 0.f;
-    return w;
+    const float w = x == m ? 1.0f : expf(q_of(x, m));
+    return w >= __uint_as_float(kKeyLow) && (!(min_p > 0.f) || w >= min_p || w == 1.0f) ? w : 0.f;
   }
   // A logit below which no capped one exceeds c: the cap's inverse, lowered until the cap
   // itself says so
@@ -650,7 +651,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
   grid_dep_wait();
-  if (a.left_only && a.tokens[row] != kLeft) return;
+  grid_dep_launch();
+  const Row r = row_of(a, row, lowest_of(static_cast<const T *>(a.logits)));
+  if (a.which != Rows::kAll && r.few() != (a.which == Rows::kLeftOver)) return;
+  if (a.which == Rows::kLeftOver && a.tokens[row] != kLeft) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
@@ -684,7 +688,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
       *reinterpret_cast<float4 *>(e + head + j * E + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
   }
   for (uint32_t i = head + vecs * E + threadIdx.x; i < n; i += kThreads) e[i] = put(load1(x + i));
-  const Row r = row_of(a, row, lowest_of(x));
   const Tokens<true> all{s, cl, C, rank, e, n, base, set};
   // the CTA's maximum of v
   auto cta_max = [&](float v) {
@@ -827,13 +830,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   // ---- many candidates: weights of all tokens; what min-p drops, and what rounds to weight
   // 0, becomes 0 ----
   float top = m;
-  if (r.cap > 0.f) {
-    top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-      const float v = r.capped(e[i]);
-      e[i] = v;
-      top = fmaxf(top, v);
-    }
+  if (r.cap > 0.f) {  // the largest capped logit is that of the largest one up to the cap's rounding
+    top = mc;
+    const float near = r.below(mc - r.cap * 1e-6f);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+      if (e[i] >= near) top = fmaxf(top, r.capped(e[i]));
     top = cta_max(top);
     all.exchange(__float_as_uint(top), 0);
     for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
@@ -842,49 +844,54 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   // (the first round's bins are filled on the way)
   for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) s->cnt[i] = s->low[i] = 0;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-    const float w = r.weigh(e[i], top);
-    e[i] = w;
-    if (w > 0.f) {
-      if (r.top_k > 0)
-        add_first<true>(s, __float_as_uint(w));
-      else if (r.top_p < 1.0f)
-        add_first<false>(s, __float_as_uint(w));
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
+    if (r.cap > 0.f) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = r.capped(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = r.weigh(v[j], top);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
+      if (v[j] > 0.f) {
+        if (r.top_k > 0)
+          add_first<true>(s, __float_as_uint(v[j]));
+        else if (r.top_p < 1.0f)
+          add_first<false>(s, __float_as_uint(v[j]));
+      }
     }
   }
   __syncthreads();
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
 
-// Many rows: first those with few candidates, without keeping logits in shared memory, so that
-// all rows are on the SMs at once (the kernel above holds 16 to 18 rows of 262,144 logits; 64
-// rows took it 70 us).  A cluster reads its row once for the threads' maxima; only the threads
-// whose maximum is not below the bound read theirs again, from L2.  Rows without min-p and
-// top-k, and rows with more than 256 candidates, are left for the other kernel.
+// Many rows: those with few candidates by a kernel that keeps no logits in shared memory, so
+// that all rows are on the SMs at once (the kernel above holds 16 to 18 rows of 262,144
+// logits).  A cluster reads its row once for the threads' maxima; only the threads whose maximum
+// is not below the bound read theirs again, from L2.  Rows with more than 256 candidates are
+// left for the other kernel.
+struct FewMem {
+  uint32_t maxima[kMaxima];
+  float list[kFew];
+  uint32_t list_id[kFew];
+  Few few;
+  unsigned long long xch[2][kMaxCluster], warp_a[kWarps];
+  uint32_t warp_b[kWarps], pick, n_list;
+};
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs a) {
-  struct Mem {
-    uint32_t maxima[kMaxima];
-    float list[kFew];
-    uint32_t list_id[kFew];
-    Few few;
-    unsigned long long xch[2][kMaxCluster], warp_a[kWarps];
-    uint32_t warp_b[kWarps], pick, n_list;
-  };
-  __shared__ Mem mem;
+CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
-  grid_dep_wait();
-  grid_dep_launch();
   const Row r = row_of(a, row, lowest_of(x));
+  if (!r.few()) return;
   const bool greedy = !(r.temp > 0.f), by_k = r.top_k > 0 && r.top_k <= (int32_t)kFew;
-  if (!(greedy || by_k || r.min_p > 0.f)) {
-    if (rank == 0 && threadIdx.x == 0) a.tokens[row] = kLeft;
-    return;
-  }
   for (uint32_t i = threadIdx.x; i < kMaxima; i += kThreads) mem.maxima[i] = 0;
   if (threadIdx.x == 0) mem.pick = kMaxima, mem.n_list = 0;
 
@@ -946,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs 
   }
   const float low = r.least_logit(mc, bound);
   if (own >= low && own > -INFINITY) {
-    Mem *to = cl.map_shared_rank(&mem, 0);
+    FewMem *to = cl.map_shared_rank(&mem, 0);
     each([&](uint32_t i, float v) {
       if (!(v >= low) || v == -INFINITY) return;
       const uint32_t at = atomicAdd(&to->n_list, 1u);
@@ -967,10 +974,22 @@ __global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs 
   if (threadIdx.x < count) mem.list[threadIdx.x] = r.weigh(v, top);
   rank_and_draw(a, row, &mem.few, mem.list, mem.list_id, count, r.top_k, r.top_p, r.u);
 }
+// Runs beside the launch in front of it, which takes the rows with many candidates (and has
+// waited for the work before), and ends after it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs a) {
+  __shared__ FewMem mem;
+  grid_dep_launch();
+  few_row<T>(a, mem);
+  grid_dep_wait();
+}
 
 template <typename K>
 cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t rows, uint32_t C, size_t smem, cudaStream_t stream) {
   cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
+  // the same split of L1 for both kernels: an SM changes it only when it is empty
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -994,18 +1013,24 @@ template <typename T>
 cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   uint32_t C = 1;
   while (C * kSlice < a.vocab) C *= 2;
-  // When the rows need more than one wave of the kernel that keeps them (two CTAs per SM, and
-  // the SMs of a cluster are neighbours: about 14 per 16 SMs' worth), the rows with few
-  // candidates go first; a setting that no row can have them by leaves that kernel out
-  a.left_only = rows * C > (uint32_t)num_sms() * 7 / 4 && (a.temperature || a.top_k || a.min_p);
-  if (a.left_only) {
-    const uint32_t few = C > 8 ? 8 : C;
-    a.per = (a.vocab + few - 1) / few;
-    const cudaError_t e = start_clusters(sample_few_kernel<T>, a, rows, few, 0, stream);
-    if (e != cudaSuccess) return e;
-  }
-  a.per = (a.vocab + C - 1) / C;
-  return start_clusters(sample_rows_kernel<T>, a, rows, C, sizeof(Shared), stream);
+  const uint32_t few = C > 8 ? 8 : C, per = (a.vocab + C - 1) / C, few_per = (a.vocab + few - 1) / few;
+  auto launch = [&](Rows which) {
+    a.which = which;
+    a.per = per;
+    return start_clusters(sample_rows_kernel<T>, a, rows, C, sizeof(Shared), stream);
+  };
+  // One wave of the kernel that keeps the rows (two CTAs per SM, and the SMs of a cluster are
+  // neighbours: about 14 per 16 SMs' worth) takes them all.  More rows: first those with many
+  // candidates (40 us each, of 262,144 logits, whatever their number up to a wave), beside them
+  // those with few, then what those left.  64 rows took one launch after the other 72 us, the
+  // first kernel alone 70 us.
+  if (rows * C <= (uint32_t)num_sms() * 7 / 4) return launch(Rows::kAll);
+  cudaError_t e = launch(Rows::kMany);
+  if (e != cudaSuccess) return e;
+  a.per = few_per;
+  e = start_clusters(sample_few_kernel<T>, a, rows, few, 0, stream);
+  if (e != cudaSuccess) return e;
+  return launch(Rows::kLeftOver);
 }
 
 int sample_rows(const ch_sample_rows_args *p, void *stream) {
