@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <numeric>
 #include <string>
 
 #include "../../include/channel_cuda.h"
@@ -277,26 +278,45 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
   const S *x = static_cast<const S *>(blockIdx.y ? a.v : a.k);
   T *pool = static_cast<T *>(blockIdx.y ? a.v_pool : a.k_pool);
   const long long ts = blockIdx.y ? a.vs : a.ks, hs = blockIdx.y ? a.vh : a.kh;
-  const unsigned long long total = (unsigned long long)a.n_tokens * row;
-  for (unsigned long long i = (unsigned long long)blockIdx.x * kThreads + threadIdx.x; i < total;
-       i += (unsigned long long)gridDim.x * kThreads) {
-    const uint32_t t = (uint32_t)(i / row), r = (uint32_t)(i % row), h = r / a.d8, c = r % a.d8;
-    const int32_t slot = a.slots[t];
-    const uint4 val = to_pool(x + t * ts + h * hs + c * 8, static_cast<const T *>(nullptr));
-    if (slot < 0) continue;  // padding
-    if (slot >= a.n_slots) {
-      if (a.status) atomicOr(a.status, DEV_ERR_BAD_SLOT);
-      continue;
+  // the grid is a whole number of rows wide, so a thread keeps its place in the row
+  const uint32_t me = blockIdx.x * kThreads + threadIdx.x, dt = gridDim.x * kThreads / row;
+  const uint32_t r = me % row, h = r / a.d8, c = r % a.d8;
+  x += h * hs + c * 8;
+  pool += h * a.head + c * 8;
+  constexpr uint32_t kU = 4;  // rows whose loads are in flight together
+  for (unsigned long long t0 = me / row; t0 < a.n_tokens; t0 += kU * dt) {
+    int32_t slot[kU];
+    uint4 val[kU];
+#pragma unroll
+    for (uint32_t u = 0; u < kU; u++) {
+      const unsigned long long t = t0 + u * dt;
+      slot[u] = -1;
+      if (t >= a.n_tokens) continue;
+      slot[u] = a.slots[t];
+      val[u] = to_pool(x + (long long)t * ts, static_cast<const T *>(nullptr));
     }
-    const long long page = slot >> a.shift, at = slot & ((1 << a.shift) - 1);
-    *reinterpret_cast<uint4 *>(pool + page * a.page + at * a.token + h * a.head + c * 8) = val;
+#pragma unroll
+    for (uint32_t u = 0; u < kU; u++) {
+      if (slot[u] < 0) continue;  // padding
+      if (slot[u] >= a.n_slots) {
+        if (a.status) atomicOr(a.status, DEV_ERR_BAD_SLOT);
+        continue;
+      }
+      const long long page = slot[u] >> a.shift, at = slot[u] & ((1 << a.shift) - 1);
+      *reinterpret_cast<uint4 *>(pool + page * a.page + at * a.token) = val[u];
+    }
   }
 }
 
 template <typename S, typename T>
 cudaError_t launch_write(const WriteArgs &a, cudaStream_t s) {
-  const unsigned long long pieces = (unsigned long long)a.n_tokens * a.n_kv * a.d8;
-  const uint32_t grid = (uint32_t)std::min<unsigned long long>((pieces + kThreads - 1) / kThreads, num_sms() * 16ull);
+  const uint32_t row = a.n_kv * a.d8;
+  const unsigned long long pieces = (unsigned long long)a.n_tokens * row;
+  // whole rows: a multiple of row / gcd(row, threads) CTAs; eight CTAs per SM at most for K and
+  // for V, or what the rows need
+  const uint32_t unit = row / std::gcd(row, (uint32_t)kThreads);
+  const unsigned long long want = std::min<unsigned long long>((pieces + kThreads - 1) / kThreads, num_sms() * 8ull);
+  const uint32_t grid = (uint32_t)((want + unit - 1) / unit) * unit;
   kv_write_kernel<S, T><<<dim3(grid, 2), kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
@@ -306,8 +326,8 @@ int kv_write(const ch_kv_write_args *p, void *stream) {
   if (p->n_tokens == 0) return CH_OK;
   if (!p->k || !p->v || !p->slots || !p->k_pool || !p->v_pool)
     return set_last_error(CH_EINVAL, "paged_kv_write: NULL argument");
-  if (p->n_kv == 0 || p->head_dim == 0 || p->head_dim % 8 || p->head_dim > 1024 || p->n_kv > 65535)
-    return set_last_error(CH_EINVAL, "paged_kv_write: head_dim must be a multiple of 8 up to 1024");
+  if (p->n_kv == 0 || p->head_dim == 0 || p->head_dim % 8 || p->head_dim > 1024 || p->n_kv > 1024)
+    return set_last_error(CH_EINVAL, "paged_kv_write: head_dim must be a multiple of 8 up to 1024, n_kv at most 1024");
   if (p->page_size == 0 || (p->page_size & (p->page_size - 1)) || p->page_size > 65536)
     return set_last_error(CH_EINVAL, "paged_kv_write: page_size must be a power of two up to 65536");
   if ((p->k_token_stride | p->k_head_stride | p->v_token_stride | p->v_head_stride | p->page_stride | p->token_stride |
