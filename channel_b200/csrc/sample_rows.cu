@@ -34,7 +34,10 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <mutex>
+#include <set>
 #include <string>
+#include <utility>
 
 #include "../../include/channel_cuda.h"
 #include "common.cuh"
@@ -984,13 +987,27 @@ __global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs 
   grid_dep_wait();
 }
 
-template <typename K>
-cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t rows, uint32_t C, size_t smem, cudaStream_t stream) {
-  cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
-  // the same split of L1 for both kernels: an SM changes it only when it is empty
+// The kernel's attributes, once per device: its shared memory, clusters of 16, and the same split
+// of L1 for both kernels (an SM changes it only when it is empty)
+cudaError_t allow(const void *kernel, size_t smem) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void *>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({dev, kernel})) return cudaSuccess;
+  e = ensure_smem_attr(kernel, smem);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.insert({dev, kernel});
+  return e;
+}
+
+template <typename K>
+cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t rows, uint32_t C, size_t smem, cudaStream_t stream) {
+  const cudaError_t e = allow((const void *)kernel, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * C);

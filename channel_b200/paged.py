@@ -125,8 +125,8 @@ def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor
         slots, _, positions, _, rows, _, lens_out, starts, counts = buf.split_with_sizes(
             (max_tokens, pad, max_tokens, pad, max_tokens, pad, n, n + 1, 2))
     else:
-        slots, positions, rows, lens_out, starts, counts = buf.split_with_sizes(
-            (max_tokens, max_tokens, max_tokens, n, n + 1, 2))
+        slots, positions, rows, lens_out, starts, counts = torch.unsafe_split_with_sizes(
+            buf, (max_tokens, max_tokens, max_tokens, n, n + 1, 2))
     p, step = buf.data_ptr(), 4 * (max_tokens + pad)
     args = _PLAN.pack(p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step, p + 2 * step,
                       p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
@@ -182,7 +182,7 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
     p_table, p_lens = _table(table, n, at, "table"), _vec(lens, n, at, "lens")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q)
     elif out.shape != shape or out.dtype is not kind or out.get_device() != at or out.stride(2) != 1:
         _fail("prefix_attention: out is like q")
     _device(q)

@@ -51,7 +51,7 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
     p_top_k = _per_row(top_k, _I32, n, at, "top_k")
     _device(logits)
     out = logits.new_empty(3 * n, dtype=_I32)
-    tokens, kept, logprobs = out.split_with_sizes((n, n, n))
+    tokens, kept, logprobs = torch.unsafe_split_with_sizes(out, (n, n, n))
     logprobs = logprobs.view(_F32)
     if n:
         p = out.data_ptr()
