@@ -1057,8 +1057,6 @@ int sample_rows(const ch_sample_rows_args *p, void *stream) {
   if (p->vocab == 0 || p->vocab > kMaxVocab)
     return set_last_error(CH_EINVAL, "sample_rows: vocab must be 1.." + std::to_string(kMaxVocab));
   if (p->n_rows > 1u << 20) return set_last_error(CH_EINVAL, "sample_rows: at most 2^20 rows");
-  if (p->row_stride < (int64_t)p->vocab && p->n_rows > 1)
-    return set_last_error(CH_EINVAL, "sample_rows: row_stride is below vocab");
   if (!(p->softcap >= 0.f) || p->softcap > 3e38f)
     return set_last_error(CH_EINVAL, "sample_rows: softcap must be 0 (none) or positive and finite");
   const size_t es = p->dtype == CH_F32 ? 4 : p->dtype == CH_F16 || p->dtype == CH_BF16 ? 2 : 0;

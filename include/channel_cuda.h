@@ -475,7 +475,7 @@ size_t ch_prefix_attention_workspace(const ch_prefix_attn_args *args);
 int ch_prefix_attention(const ch_prefix_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* One token per row of logits (n_rows x vocab, vocab <= 262144, row stride row_stride
- * elements).  With x = softcap * tanh(logit / softcap) (softcap 0: the logit; NaN counts
+ * elements, 0 for one row of logits for all).  With x = softcap * tanh(logit / softcap) (softcap 0: the logit; NaN counts
  * as -inf; -inf and the type's lowest value mask a token and are not capped), m = max x, T = temperature[row], token i weighs e_i = exp((x_i - m) / T),
  * held as floor(2^44 e_i); tokens of weight 0 are never drawn.  Kept are, in the order of
  * falling e (equal ones by index):  e_i >= min_p (and every e_i = 1);  of those the first

@@ -332,6 +332,15 @@ def test_on_another_stream_and_in_a_graph():
 
 
 @gpu
+def test_one_row_for_all():
+    """logits broadcast over the rows (stride 0): as many draws from one row"""
+    x = lm_logits(1, 30000, 9)
+    u = torch.linspace(0, 0.999, 50, device="cuda")
+    many = sampling.sample_rows(x.expand(50, -1), u)
+    assert all(torch.equal(a, b) for a, b in zip(many, sampling.sample_rows(x.repeat(50, 1), u)))
+
+
+@gpu
 def test_no_rows():
     t, lp, k = sampling.sample_rows(torch.zeros(0, 100, device="cuda"), torch.zeros(0, device="cuda"))
     assert t.shape == lp.shape == k.shape == (0,)
@@ -351,7 +360,7 @@ def test_row_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("bad,why", [
-    (dict(vocab=0), "vocab"), (dict(vocab=262145, row_stride=300000), "vocab"), (dict(row_stride=99), "row_stride"),
+    (dict(vocab=0), "vocab"), (dict(vocab=262145, row_stride=300000), "vocab"),
     (dict(logits=None), "NULL"), (dict(uniform=None), "NULL"), (dict(tokens=None), "NULL"), (dict(dtype=7), "dtype"),
     (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(softcap=float("inf")), "softcap"),
     (dict(logits=4098), "aligned"), (dict(n_rows=(1 << 20) + 1), "rows")])
