@@ -37,6 +37,7 @@
 #include <mutex>
 #include <set>
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "../../include/channel_cuda.h"
@@ -487,20 +488,24 @@ struct Row {
   // (a logit of -inf or the type's lowest value masks its token and stays as it is)
   CH_DEV float capped(float v) const {
     if (!(cap > 0.f && v > lowest)) return v;
-    return tanhf(cap_quick && fabsf(v) < 1e30f ? divide(v, cap, cap_inv) : __fdiv_rn(v, cap)) * cap;
+    return tanhf(__fdiv_rn(v, cap)) * cap;
   }
-  // (x - m) / T, correctly rounded (where it is below -64 only the sign matters)
-  CH_DEV float q_of(float x, float m) const {
-    const float d = x - m;
-    return quick ? divide(d, temp, inv) : __fdiv_rn(d, temp);
+  // the same for a cap that divides(); past 1e30 the quotient's rounding is lost in tanh = 1
+  CH_DEV float capped_quick(float v) const {
+    const float c = tanhf(divide(fminf(fmaxf(v, -1e30f), 1e30f), cap, cap_inv)) * cap;
+    return v > lowest ? c : v;
   }
-  // e, or 0 where the weight is 0 or min-p drops the token.  No branches: x = m gives exp(0),
-  // and what over- or underflows on the way (x far below m, or masked) gives 0 or NaN, which the
-  // comparison drops
-  CH_DEV float weigh(float x, float m) const {
-    const float w = x == m ? 1.0f : expf(q_of(x, m));
+  // e, or 0 where the weight is 0 or min-p drops the token, for the quotient (x - m) / T,
+  // correctly rounded (where it is below -64 only the sign matters).  No branches in the common
+  // form (QUICK: quick is true): x = m gives exp(0), and what over- or underflows on the way (x
+  // far below m, or masked) gives 0 or NaN, which the comparison drops.
+  template <bool QUICK>
+  CH_DEV float weigh_as(float x, float m) const {
+    const float d = x - m, q = QUICK ? divide(d, temp, inv) : __fdiv_rn(d, temp);
+    const float w = x == m ? 1.0f : expf(q);
     return w >= __uint_as_float(kKeyLow) && (!(min_p > 0.f) || w >= min_p || w == 1.0f) ? w : 0.f;
   }
+  CH_DEV float weigh(float x, float m) const { return quick ? weigh_as<true>(x, m) : weigh_as<false>(x, m); }
   // A logit below which no capped one exceeds c: the cap's inverse, lowered until the cap
   // itself says so
   CH_DEV float below(float c) const {
@@ -836,9 +841,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   if (r.cap > 0.f) {  // the largest capped logit is that of the largest one up to the cap's rounding
     top = mc;
     const float near = r.below(mc - r.cap * 1e-6f);
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads)
-      if (e[i] >= near) top = fmaxf(top, r.capped(e[i]));
+    if (own >= near) {  // this thread read such a one
+      auto look = [&](float v) { top = v >= near ? fmaxf(top, r.capped(v)) : top; };
+      if (threadIdx.x < head) look(e[threadIdx.x]);
+      for (uint32_t j = threadIdx.x; j < vecs; j += kThreads)
+        for (uint32_t k = 0; k < E; k++) look(e[head + j * E + k]);
+      if (head + vecs * E + threadIdx.x < n) look(e[head + vecs * E + threadIdx.x]);
+    }
     top = cta_max(top);
     all.exchange(__float_as_uint(top), 0);
     for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
@@ -847,27 +856,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   // (the first round's bins are filled on the way)
   for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) s->cnt[i] = s->low[i] = 0;
   __syncthreads();
-  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
-    float v[4];
+  // four tokens at a time; the kind of row is decided outside the loop, whose body then has no
+  // calls and no branches but tanh's (with them inside it the loop took twice as long)
+  auto weigh_all = [&](auto with_cap, auto quick, auto bin) {
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
+      float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
-    if (r.cap > 0.f) {
+      for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
+      if constexpr (decltype(with_cap)::value) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = r.capped(v[j]);
-    }
+        for (int j = 0; j < 4; j++) v[j] = decltype(quick)::value ? r.capped_quick(v[j]) : r.capped(v[j]);
+      }
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = r.weigh(v[j], top);
+      for (int j = 0; j < 4; j++) v[j] = r.template weigh_as<decltype(quick)::value>(v[j], top);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
-      if (v[j] > 0.f) {
-        if (r.top_k > 0)
-          add_first<true>(s, __float_as_uint(v[j]));
-        else if (r.top_p < 1.0f)
-          add_first<false>(s, __float_as_uint(v[j]));
+      for (int j = 0; j < 4; j++)
+        if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
+      if constexpr (decltype(bin)::value > 0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (v[j] > 0.f && i0 + j * kThreads < n) add_first<decltype(bin)::value == 1>(s, __float_as_uint(v[j]));
       }
     }
-  }
+  };
+  using std::integral_constant;
+  auto weigh_binned = [&](auto with_cap, auto quick) {
+    if (r.top_k > 0)
+      weigh_all(with_cap, quick, integral_constant<int, 1>());
+    else if (r.top_p < 1.0f)
+      weigh_all(with_cap, quick, integral_constant<int, 2>());
+    else
+      weigh_all(with_cap, quick, integral_constant<int, 0>());
+  };
+  if (r.quick && !(r.cap > 0.f))
+    weigh_binned(integral_constant<bool, false>(), integral_constant<bool, true>());
+  else if (r.quick && r.cap_quick)
+    weigh_binned(integral_constant<bool, true>(), integral_constant<bool, true>());
+  else
+    weigh_binned(integral_constant<bool, true>(), integral_constant<bool, false>());
   __syncthreads();
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
