@@ -34,6 +34,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <mutex>
 #include <set>
 #include <string>
@@ -68,7 +69,7 @@ struct RowsArgs {
   const int32_t *top_k;
   int32_t *tokens, *kept;
   float *logprobs;
-  uint32_t vocab, per;  // tokens per CTA
+  uint32_t rows, vocab, per;  // per: tokens per CTA
   float softcap;
   Rows which;
 };
@@ -652,17 +653,10 @@ CH_DEV void rank_and_draw(const RowsArgs &a, uint32_t row, Few *s, const float *
   }
 }
 
+// One row by a cluster that keeps it in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  Shared *s = reinterpret_cast<Shared *>(smem_raw);
-  cg::cluster_group cl = cg::this_cluster();
-  const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
-  grid_dep_wait();
-  grid_dep_launch();
-  const Row r = row_of(a, row, lowest_of(static_cast<const T *>(a.logits)));
-  if (a.which != Rows::kAll && r.few() != (a.which == Rows::kLeftOver)) return;
-  if (a.which == Rows::kLeftOver && a.tokens[row] != kLeft) return;
+CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, cg::cluster_group &cl) {
+  const uint32_t C = cl.num_blocks(), rank = cl.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
@@ -898,6 +892,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  cg::cluster_group cl = cg::this_cluster();
+  const uint32_t step = gridDim.x / cl.num_blocks();
+  grid_dep_wait();
+  grid_dep_launch();
+  for (uint32_t row = blockIdx.x / cl.num_blocks(); row < a.rows; row += step) {
+    if (a.which == Rows::kLeftOver && a.tokens[row] != kLeft) continue;
+    const Row r = row_of(a, row, lowest_of(static_cast<const T *>(a.logits)));
+    if (a.which != Rows::kAll && r.few() != (a.which == Rows::kLeftOver)) continue;
+    keep_row<T>(a, row, r, reinterpret_cast<Shared *>(smem_raw), cl);
+    if (row + step < a.rows) cl.sync();  // every CTA is done with the row
+  }
+}
+
 // Many rows: those with few candidates by a kernel that keeps no logits in shared memory, so
 // that all rows are on the SMs at once (the kernel above holds 16 to 18 rows of 262,144
 // logits).  A cluster reads its row once for the threads' maxima; only the threads whose maximum
@@ -1056,18 +1066,21 @@ template <typename T>
 cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   uint32_t C = 1;
   while (C * kSlice < a.vocab) C *= 2;
-  const uint32_t few = C > 8 ? 8 : C, per = (a.vocab + C - 1) / C, few_per = (a.vocab + few - 1) / few;
+  const uint32_t wave = (uint32_t)num_sms() * 7 / 4, few = C > 8 ? 8 : C, per = (a.vocab + C - 1) / C, few_per = (a.vocab + few - 1) / few;
   auto launch = [&](Rows which) {
     a.which = which;
+    a.rows = rows;
     a.per = per;
-    return start_clusters(sample_rows_kernel<T>, a, rows, C, sizeof(Shared), stream);
+    // the rows left over are few if any: one wave of clusters looks through them
+    const uint32_t clusters = which == Rows::kLeftOver ? std::min(rows, wave / C) : rows;
+    return start_clusters(sample_rows_kernel<T>, a, clusters, C, sizeof(Shared), stream);
   };
   // One wave of the kernel that keeps the rows (two CTAs per SM, and the SMs of a cluster are
   // neighbours: about 14 per 16 SMs' worth) takes them all.  More rows: first those with many
   // candidates (40 us each, of 262,144 logits, whatever their number up to a wave), beside them
   // those with few, then what those left.  64 rows took one launch after the other 72 us, the
   // first kernel alone 70 us.
-  if (rows * C <= (uint32_t)num_sms() * 7 / 4) return launch(Rows::kAll);
+  if (rows * C <= wave) return launch(Rows::kAll);
   cudaError_t e = launch(Rows::kMany);
   if (e != cudaSuccess) return e;
   a.per = few_per;
