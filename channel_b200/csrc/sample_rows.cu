@@ -255,35 +255,49 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
         if (key != 0 && cut.keeps(key, t.base + i)) add_first<COUNT>(s, key);
       }
     } else {
-      // few bins hold many tokens here (16-bit logits have few distinct values), and additions
-      // to one address go one by one: a warp adds each of its bins once
-      for (uint32_t i0 = warp * 32; i0 < t.n; i0 += 4 * kThreads) {
-        uint32_t keys[4];
-        bool any = false;
+      // the tokens of the bin found last, collected in the first of these rounds where they fit
+      auto matches = [&](uint32_t key, uint32_t i) { return key >> (rd.shift + 9) == prefix && cut.keeps(key, t.base + i); };
+      if (CLUSTER && round == 1) {
+        if (threadIdx.x == 0) s->pick = 0;
+        __syncthreads();
+        for (uint32_t i0 = threadIdx.x; i0 < t.n; i0 += 4 * kThreads) {
+          uint32_t keys[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t i = i0 + j * kThreads + lane;
-          keys[j] = i < t.n ? __float_as_uint(e[i]) : 0u;
-          if (keys[j] >> (rd.shift + 9) != prefix || !cut.keeps(keys[j], t.base + i)) keys[j] = 0;
-          any |= keys[j] != 0;
-        }
-        if (!__any_sync(0xffffffffu, any)) continue;
+          for (int j = 0; j < 4; j++) keys[j] = i0 + j * kThreads < t.n ? __float_as_uint(e[i0 + j * kThreads]) : 0u;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t key = keys[j], bin = (key >> rd.shift) & (kSub - 1);
-          uint32_t left = __ballot_sync(0xffffffffu, key != 0);
-          while (left) {
-            const int first = __ffs(left) - 1;
-            const uint32_t its = __shfl_sync(0xffffffffu, bin, first);  // by every lane
-            const bool mine = key != 0 && bin == its;
-            const uint32_t same = __ballot_sync(0xffffffffu, mine);
-            if (lane == first) atomicAdd(&s->cnt[bin], __popc(same));
-            if (!COUNT && rd.shift > 0) {
-              const uint32_t sum = __reduce_add_sync(0xffffffffu, mine ? rd.low_of(key) : 0u);
-              if (lane == first) atomicAdd(&s->low[bin], sum);
+          for (int j = 0; j < 4; j++)
+            if (matches(keys[j], i0 + j * kThreads)) {
+              const uint32_t at = atomicAdd(&s->pick, 1u);
+              if (at < kList) s->list_id[at] = keys[j];
             }
-            left &= ~same;
+        }
+        __syncthreads();
+      }
+      const bool listed = CLUSTER && s->pick <= kList;
+      const uint32_t many = listed ? s->pick : t.n;
+      // few bins hold many tokens here (16-bit logits have few distinct values), and additions
+      // to one address go one by one: a warp adds its first bins once each
+      for (uint32_t i0 = warp * 32; i0 < many; i0 += kThreads) {
+        const uint32_t i = i0 + lane;
+        uint32_t key = i < many ? listed ? s->list_id[i] : __float_as_uint(e[i]) : 0u;
+        if (listed ? key >> (rd.shift + 9) != prefix : !matches(key, i)) key = 0;
+        const uint32_t bin = (key >> rd.shift) & (kSub - 1);
+        uint32_t left = __ballot_sync(0xffffffffu, key != 0);
+        for (int k = 0; k < 4 && left; k++) {
+          const int first = __ffs(left) - 1;
+          const uint32_t its = __shfl_sync(0xffffffffu, bin, first);  // by every lane
+          const bool mine = key != 0 && bin == its;
+          const uint32_t same = __ballot_sync(0xffffffffu, mine);
+          if (lane == first) atomicAdd(&s->cnt[bin], __popc(same));
+          if (!COUNT && rd.shift > 0) {
+            const uint32_t sum = __reduce_add_sync(0xffffffffu, mine ? rd.low_of(key) : 0u);
+            if (lane == first) atomicAdd(&s->low[bin], sum);
           }
+          left &= ~same;
+        }
+        if ((left >> lane) & 1u) {
+          atomicAdd(&s->cnt[bin], 1u);
+          if (!COUNT && rd.shift > 0) atomicAdd(&s->low[bin], rd.low_of(key));
         }
       }
     }
@@ -295,6 +309,7 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       const uint32_t part = (nb + t.C - 1) / t.C, b0 = min(nb, t.rank * part), mine = min(nb, b0 + part) - b0;
       unsigned long long *sums = reinterpret_cast<unsigned long long *>(s->list);  // [C][part]
       static_assert((kBins + kMaxCluster) * sizeof(unsigned long long) <= sizeof(s->list) + sizeof(s->list_id), "room");
+      static_assert((kSub + kMaxCluster) * sizeof(unsigned long long) <= sizeof(s->list), "beside the collected tokens");
       for (uint32_t c = warp; c < t.C; c += kWarps) {
         const uint32_t *cnt = t.cl.map_shared_rank(s->cnt, c) + b0, *lows = t.cl.map_shared_rank(s->low, c) + b0;
 #pragma unroll 4
@@ -394,22 +409,20 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
   Cut cut{kKeyLow, 0xFFFFFFFFu};
   if (top_k > 0) cut = select<true>(t, cut, (unsigned long long)top_k, 0.0, binned);
   if (top_p < 1.0f) cut = select<false>(t, cut, 0, (double)top_p, binned && top_k <= 0);
-  // thread t owns the `run` places from t * run on, starting at one of them that spreads the
-  // lanes over the banks
-  const uint32_t run = (t.n + kThreads - 1) / kThreads, p0 = threadIdx.x * run;
+  // thread t owns the `run` places from t * run on, an odd number, which spreads the lanes over
+  // the banks
+  const uint32_t run = ((t.n + kThreads - 1) / kThreads) | 1u, p0 = threadIdx.x * run;
   unsigned long long own = 0;
   uint32_t cnt = 0;
   auto kept_weight = [&](uint32_t i) {
     const uint32_t key = i < t.n ? __float_as_uint(e[i]) : 0u;
     return key != 0 && cut.keeps(key, t.base + i) ? weight_of(__uint_as_float(key)) : 0ull;
   };
-  uint32_t place = run ? lane % run : 0u;
 #pragma unroll 4
   for (uint32_t j = 0; j < run; j++) {
-    const unsigned long long w = kept_weight(p0 + place);
+    const unsigned long long w = kept_weight(p0 + j);
     own += w;
     cnt += w > 0;
-    place = place + 1 == run ? 0 : place + 1;
   }
   unsigned long long mass = own;
   mass = warp_sum64(mass);
@@ -832,16 +845,23 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   // ---- many candidates: weights of all tokens; what min-p drops, and what rounds to weight
   // 0, becomes 0 ----
   float top = m;
-  if (r.cap > 0.f) {  // the largest capped logit is that of the largest one up to the cap's rounding
-    top = mc;
-    const float near = r.below(mc - r.cap * 1e-6f);
-    if (own >= near) {  // this thread read such a one
-      auto look = [&](float v) { top = v >= near ? fmaxf(top, r.capped(v)) : top; };
-      if (threadIdx.x < head) look(e[threadIdx.x]);
-      for (uint32_t j = threadIdx.x; j < vecs; j += kThreads)
-        for (uint32_t k = 0; k < E; k++) look(e[head + j * E + k]);
-      if (head + vecs * E + threadIdx.x < n) look(e[head + vecs * E + threadIdx.x]);
-    }
+  if (r.cap > 0.f) {  // in a pass of its own, which finds the largest capped logit
+    auto cap_all = [&](auto quick) {
+      top = -INFINITY;
+      for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = decltype(quick)::value ? r.capped_quick(v[j]) : r.capped(v[j]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
+          top = i0 + j * kThreads < n ? fmaxf(top, v[j]) : top;
+        }
+      }
+    };
+    if (r.cap_quick) cap_all(std::true_type()); else cap_all(std::false_type());
     top = cta_max(top);
     all.exchange(__float_as_uint(top), 0);
     for (uint32_t c = 0; c < C; c++) top = fmaxf(top, __uint_as_float((uint32_t)s->xch[set][c][0]));
@@ -851,16 +871,12 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) s->cnt[i] = s->low[i] = 0;
   __syncthreads();
   // four tokens at a time; the kind of row is decided outside the loop, whose body then has no
-  // calls and no branches but tanh's (with them inside it the loop took twice as long)
-  auto weigh_all = [&](auto with_cap, auto quick, auto bin) {
+  // calls and no branches (with them inside it the loop took twice as long)
+  auto weigh_all = [&](auto quick, auto bin) {
     for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
-      if constexpr (decltype(with_cap)::value) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = decltype(quick)::value ? r.capped_quick(v[j]) : r.capped(v[j]);
-      }
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = r.template weigh_as<decltype(quick)::value>(v[j], top);
 #pragma unroll
@@ -874,20 +890,15 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
     }
   };
   using std::integral_constant;
-  auto weigh_binned = [&](auto with_cap, auto quick) {
+  auto weigh_binned = [&](auto quick) {
     if (r.top_k > 0)
-      weigh_all(with_cap, quick, integral_constant<int, 1>());
+      weigh_all(quick, integral_constant<int, 1>());
     else if (r.top_p < 1.0f)
-      weigh_all(with_cap, quick, integral_constant<int, 2>());
+      weigh_all(quick, integral_constant<int, 2>());
     else
-      weigh_all(with_cap, quick, integral_constant<int, 0>());
+      weigh_all(quick, integral_constant<int, 0>());
   };
-  if (r.quick && !(r.cap > 0.f))
-    weigh_binned(integral_constant<bool, false>(), integral_constant<bool, true>());
-  else if (r.quick && r.cap_quick)
-    weigh_binned(integral_constant<bool, true>(), integral_constant<bool, true>());
-  else
-    weigh_binned(integral_constant<bool, true>(), integral_constant<bool, false>());
+  if (r.quick) weigh_binned(std::true_type()); else weigh_binned(std::false_type());
   __syncthreads();
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
