@@ -260,13 +260,18 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       if (CLUSTER && round == 1) {
         if (threadIdx.x == 0) s->pick = 0;
         __syncthreads();
-        for (uint32_t i0 = threadIdx.x; i0 < t.n; i0 += 4 * kThreads) {
-          uint32_t keys[4];
+        // 16-byte groups around the tokens; the places that fill them up have weight 0
+        const uint32_t shift = (uint32_t)(e - s->e);
+        for (uint32_t g = threadIdx.x; g < (shift + t.n + 3) / 4; g += kThreads) {
+          const uint4 four = reinterpret_cast<const uint4 *>(s->e)[g];
+          const uint32_t keys[4] = {four.x, four.y, four.z, four.w};
+          bool any = false;
 #pragma unroll
-          for (int j = 0; j < 4; j++) keys[j] = i0 + j * kThreads < t.n ? __float_as_uint(e[i0 + j * kThreads]) : 0u;
+          for (int j = 0; j < 4; j++) any |= keys[j] >> 18 == prefix;
+          if (!any) continue;
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            if (matches(keys[j], i0 + j * kThreads)) {
+            if (matches(keys[j], 4 * g + j - shift)) {
               const uint32_t at = atomicAdd(&s->pick, 1u);
               if (at < kList) s->list_id[at] = keys[j];
             }
@@ -412,18 +417,23 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
   // thread t owns the `run` places from t * run on, an odd number, which spreads the lanes over
   // the banks
   const uint32_t run = ((t.n + kThreads - 1) / kThreads) | 1u, p0 = threadIdx.x * run;
-  unsigned long long own = 0;
   uint32_t cnt = 0;
   auto kept_weight = [&](uint32_t i) {
     const uint32_t key = i < t.n ? __float_as_uint(e[i]) : 0u;
     return key != 0 && cut.keeps(key, t.base + i) ? weight_of(__uint_as_float(key)) : 0ull;
   };
+  // The thread's sum of floor(2^44 e), below 2^52 (run <= 33), as a double from 2^52 on, where one
+  // step is 1: an addition that rounds towards zero takes the floor.  2^44 e is e's bits moved.
+  double sum = 4503599627370496.0;
+  const uint32_t p1 = min(t.n, p0 + run);
 #pragma unroll 4
-  for (uint32_t j = 0; j < run; j++) {
-    const unsigned long long w = kept_weight(p0 + j);
-    own += w;
-    cnt += w > 0;
+  for (uint32_t i = p0; i < p1; i++) {
+    uint32_t key = __float_as_uint(e[i]);
+    if (!cut.keeps(key, t.base + i)) key = 0;
+    sum = __dadd_rz(sum, __hiloint2double((int)((key >> 3) + ((1023u - 127u + 44u) << 20)), (int)(key << 29)));
+    cnt += key != 0;
   }
+  const unsigned long long own = (unsigned long long)(sum - 4503599627370496.0);
   unsigned long long mass = own;
   mass = warp_sum64(mass);
   cnt = __reduce_add_sync(0xffffffffu, cnt);
@@ -482,7 +492,7 @@ CH_DEV void cut_and_draw(const RowsArgs &a, uint32_t row, const Tokens<CLUSTER> 
 
 // What one row asks for
 struct Row {
-  float temp, inv, top_p, min_p, cap, cap_inv, lowest, u;
+  float temp, inv, top_p, min_p, least, cap, cap_inv, lowest, u;  // least: e that stays at least
   int32_t top_k;
   bool quick, cap_quick;  // divisions by temp, by cap may go by multiplication
 
@@ -517,7 +527,7 @@ struct Row {
   CH_DEV float weigh_as(float x, float m) const {
     const float d = x - m, q = QUICK ? divide(d, temp, inv) : __fdiv_rn(d, temp);
     const float w = x == m ? 1.0f : expf(q);
-    return w >= __uint_as_float(kKeyLow) && (!(min_p > 0.f) || w >= min_p || w == 1.0f) ? w : 0.f;
+    return w >= least ? w : 0.f;
   }
   CH_DEV float weigh(float x, float m) const { return quick ? weigh_as<true>(x, m) : weigh_as<false>(x, m); }
   // A logit below which no capped one exceeds c: the cap's inverse, lowered until the cap
@@ -597,6 +607,7 @@ CH_DEV Row row_of(const RowsArgs &a, uint32_t row, float lowest) {
   r.min_p = a.min_p ? a.min_p[row] : 0.f;
   r.top_k = a.top_k ? a.top_k[row] : 0;
   r.u = a.uniform[row];
+  r.least = fmaxf(__uint_as_float(kKeyLow), r.min_p > 0.f ? fminf(r.min_p, 1.f) : 0.f);  // e = 1 always stays
   r.cap = a.softcap;
   r.lowest = lowest;
   r.inv = __frcp_rn(r.temp);
@@ -703,6 +714,11 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
       *reinterpret_cast<float4 *>(e + head + j * E + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
   }
   for (uint32_t i = head + vecs * E + threadIdx.x; i < n; i += kThreads) e[i] = put(load1(x + i));
+  // as 16-byte groups, filled up with masked places
+  const uint32_t shift = off & 3u, groups = (shift + n + 3) / 4;
+  float4 *e4 = reinterpret_cast<float4 *>(s->e);
+  if (threadIdx.x < shift) s->e[threadIdx.x] = -INFINITY;
+  if (threadIdx.x < 4 * groups - shift - n) e[n + threadIdx.x] = -INFINITY;
   const Tokens<true> all{s, cl, C, rank, e, n, base, set};
   // the CTA's maximum of v
   auto cta_max = [&](float v) {
@@ -848,17 +864,15 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   if (r.cap > 0.f) {  // in a pass of its own, which finds the largest capped logit
     auto cap_all = [&](auto quick) {
       top = -INFINITY;
-      for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = decltype(quick)::value ? r.capped_quick(v[j]) : r.capped(v[j]);
+      for (uint32_t g = threadIdx.x; g < groups; g += kThreads) {
+        const float4 x4 = e4[g];
+        float v[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
-          top = i0 + j * kThreads < n ? fmaxf(top, v[j]) : top;
+          v[j] = decltype(quick)::value ? r.capped_quick(v[j]) : r.capped(v[j]);
+          top = fmaxf(top, v[j]);
         }
+        e4[g] = make_float4(v[0], v[1], v[2], v[3]);
       }
     };
     if (r.cap_quick) cap_all(std::true_type()); else cap_all(std::false_type());
@@ -873,19 +887,16 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   // four tokens at a time; the kind of row is decided outside the loop, whose body then has no
   // calls and no branches (with them inside it the loop took twice as long)
   auto weigh_all = [&](auto quick, auto bin) {
-    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
-      float v[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = i0 + j * kThreads < n ? e[i0 + j * kThreads] : -INFINITY;
+    for (uint32_t g = threadIdx.x; g < groups; g += kThreads) {
+      const float4 x4 = e4[g];
+      float v[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = r.template weigh_as<decltype(quick)::value>(v[j], top);
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (i0 + j * kThreads < n) e[i0 + j * kThreads] = v[j];
+      e4[g] = make_float4(v[0], v[1], v[2], v[3]);
       if constexpr (decltype(bin)::value > 0) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (v[j] > 0.f && i0 + j * kThreads < n) add_first<decltype(bin)::value == 1>(s, __float_as_uint(v[j]));
+          if (v[j] > 0.f) add_first<decltype(bin)::value == 1>(s, __float_as_uint(v[j]));
       }
     }
   };
