@@ -35,11 +35,11 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <map>
 #include <mutex>
-#include <set>
 #include <string>
+#include <tuple>
 #include <type_traits>
-#include <utility>
 
 #include "../../include/channel_cuda.h"
 #include "common.cuh"
@@ -914,24 +914,61 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   cut_and_draw(a, row, all, r.top_k, r.top_p, r.u, nullptr, true);
 }
 
+// Number `want`, from 0, of the rows from, from + step, ... below `rows` that `takes`; `rows`
+// when there are fewer.  The same for every thread of the cluster.
+template <typename F>
+CH_DEV uint32_t nth_row(Shared *s, uint32_t rows, uint32_t from, uint32_t step, uint32_t want, F takes) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (; from < rows; from += step * kThreads) {
+    const uint32_t row = from + step * threadIdx.x;
+    const bool it = row < rows && takes(row);
+    const uint32_t its = __ballot_sync(0xffffffffu, it);
+    __syncthreads();
+    if (lane == 0) s->warp_b[warp] = __popc(its);
+    __syncthreads();
+    uint32_t before = __popc(its & ((1u << lane) - 1)), total = 0;
+    for (int w = 0; w < kWarps; w++) {
+      if (w < warp) before += s->warp_b[w];
+      total += s->warp_b[w];
+    }
+    if (want < total) {
+      if (it && before == want) s->cut_at = row;
+      __syncthreads();
+      return s->cut_at;
+    }
+    want -= total;
+  }
+  return rows;
+}
+
+// As many clusters as rows (kAll), or as run at once.  The rows with many candidates are dealt
+// to them in turn, each cluster counting them for itself.  Of the rows left over a cluster takes
+// those whose number is its own modulo the number of clusters, so that nobody else changes the
+// tokens it looks at.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
+  Shared *s = reinterpret_cast<Shared *>(smem_raw);
   cg::cluster_group cl = cg::this_cluster();
-  const uint32_t step = gridDim.x / cl.num_blocks();
+  const uint32_t N = gridDim.x / cl.num_blocks(), number = blockIdx.x / cl.num_blocks();
+  const float lowest = lowest_of(static_cast<const T *>(a.logits));
   grid_dep_wait();
   grid_dep_launch();
-  for (uint32_t row = blockIdx.x / cl.num_blocks(); row < a.rows; row += step) {
-    if (a.which == Rows::kLeftOver && a.tokens[row] != kLeft) continue;
-    const Row r = row_of(a, row, lowest_of(static_cast<const T *>(a.logits)));
-    if (a.which != Rows::kAll && r.few() != (a.which == Rows::kLeftOver)) continue;
-    keep_row<T>(a, row, r, reinterpret_cast<Shared *>(smem_raw), cl);
-    if (row + step < a.rows) cl.sync();  // every CTA is done with the row
+  auto many = [&](uint32_t row) { return !row_of(a, row, lowest).few(); };
+  auto left = [&](uint32_t row) { return a.tokens[row] == kLeft; };
+  uint32_t row = number;
+  if (a.which == Rows::kMany) row = nth_row(s, a.rows, 0, 1, number, many);
+  if (a.which == Rows::kLeftOver) row = nth_row(s, a.rows, number, N, 0, left);
+  while (row < a.rows) {
+    keep_row<T>(a, row, row_of(a, row, lowest), s, cl);
+    if (a.which == Rows::kAll) return;
+    cl.sync();  // every CTA is done with the row
+    row = a.which == Rows::kMany ? nth_row(s, a.rows, row + 1, 1, N - 1, many) : nth_row(s, a.rows, row + N, N, 0, left);
   }
 }
 
 // Many rows: those with few candidates by a kernel that keeps no logits in shared memory, so
-// that all rows are on the SMs at once (the kernel above holds 16 to 18 rows of 262,144
+// that all rows are on the SMs at once (the kernel above holds 14 rows of 262,144
 // logits).  A cluster reads its row once for the threads' maxima; only the threads whose maximum
 // is not below the bound read theirs again, from L2.  Rows with more than 256 candidates are
 // left for the other kernel.
@@ -1045,30 +1082,47 @@ __global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs 
   grid_dep_wait();
 }
 
-// The kernel's attributes, once per device: its shared memory, clusters of 16, and the same split
-// of L1 for both kernels (an SM changes it only when it is empty)
-cudaError_t allow(const void *kernel, size_t smem) {
+// The kernel's attributes, once per device and cluster size: its shared memory, clusters of 16, and
+// the same split of L1 for both kernels (an SM changes it only when it is empty).  running (if
+// not NULL): how many clusters of C CTAs run at once
+cudaError_t allow(const void *kernel, size_t smem, uint32_t C, uint32_t *running) {
   static std::mutex mu;
-  static std::set<std::pair<int, const void *>> done;
+  static std::map<std::tuple<int, const void *, uint32_t>, int> done;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(mu);
-  if (done.count({dev, kernel})) return cudaSuccess;
-  e = ensure_smem_attr(kernel, smem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) done.insert({dev, kernel});
-  return e;
+  const auto key = std::make_tuple(dev, kernel, C);
+  auto at = done.find(key);
+  if (at == done.end()) {
+    e = ensure_smem_attr(kernel, smem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    at = done.emplace(key, std::max(n, 1)).first;
+  }
+  if (running) *running = (uint32_t)at->second;
+  return cudaSuccess;
 }
 
 template <typename K>
-cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t rows, uint32_t C, size_t smem, cudaStream_t stream) {
-  const cudaError_t e = allow((const void *)kernel, smem);
-  if (e != cudaSuccess) return e;
+cudaError_t start_clusters(K kernel, const RowsArgs &a, uint32_t clusters, uint32_t C, size_t smem, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows * C);
+  cfg.gridDim = dim3(clusters * C);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1088,24 +1142,27 @@ template <typename T>
 cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   uint32_t C = 1;
   while (C * kSlice < a.vocab) C *= 2;
-  const uint32_t wave = (uint32_t)num_sms() * 7 / 4, few = C > 8 ? 8 : C, per = (a.vocab + C - 1) / C, few_per = (a.vocab + few - 1) / few;
+  uint32_t few = C > 8 ? 8 : C;
+  a.rows = rows;
+  uint32_t running = 0;
+  cudaError_t e = allow((const void *)sample_rows_kernel<T>, sizeof(Shared), C, &running);
+  for (uint32_t at_once = 0; e == cudaSuccess; few /= 2) {
+    e = allow((const void *)sample_few_kernel<T>, 0, few, &at_once);
+    if (rows <= at_once / 2 || few <= 4) break;
+  }
+  if (e != cudaSuccess) return e;
   auto launch = [&](Rows which) {
     a.which = which;
-    a.rows = rows;
-    a.per = per;
-    // the rows left over are few if any: one wave of clusters looks through them
-    const uint32_t clusters = which == Rows::kLeftOver ? std::min(rows, wave / C) : rows;
-    return start_clusters(sample_rows_kernel<T>, a, clusters, C, sizeof(Shared), stream);
+    a.per = (a.vocab + C - 1) / C;
+    return start_clusters(sample_rows_kernel<T>, a, std::min(rows, running), C, sizeof(Shared), stream);
   };
-  // One wave of the kernel that keeps the rows (two CTAs per SM, and the SMs of a cluster are
-  // neighbours: about 14 per 16 SMs' worth) takes them all.  More rows: first those with many
-  // candidates (40 us each, of 262,144 logits, whatever their number up to a wave), beside them
-  // those with few, then what those left.  64 rows took one launch after the other 72 us, the
-  // first kernel alone 70 us.
-  if (rows * C <= wave) return launch(Rows::kAll);
-  cudaError_t e = launch(Rows::kMany);
+  // Rows that run at once in the kernel that keeps them (14 of 262,144 logits) all go there.
+  // More rows: first those with many candidates, beside them those with few, then what those
+  // left.
+  if (rows <= running) return launch(Rows::kAll);
+  e = launch(Rows::kMany);
   if (e != cudaSuccess) return e;
-  a.per = few_per;
+  a.per = (a.vocab + few - 1) / few;
   e = start_clusters(sample_few_kernel<T>, a, rows, few, 0, stream);
   if (e != cudaSuccess) return e;
   return launch(Rows::kLeftOver);
