@@ -1011,6 +1011,39 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   };
   float own = -INFINITY;  // NaN counts as masked: fmaxf drops it
   each([&](uint32_t, float v) { own = fmaxf(own, v); });
+  // The same for the tokens of the warp's threads in `owners`, by the whole warp: one thread alone
+  // would wait for its pieces several times (10 us for 128 tokens), the warp waits once per two
+  // threads.
+  auto each_of = [&](uint32_t owners, auto f) {
+    constexpr uint32_t kNone = 1u << 30;
+    while (owners) {
+      const uint32_t t0 = warp * 32 + __ffs(owners) - 1;
+      owners &= owners - 1;
+      const uint32_t t1 = owners ? warp * 32 + __ffs(owners) - 1 : kNone;
+      owners &= owners - 1;
+      for (uint32_t j = lane * kThreads; j < vecs; j += 32 * kThreads) {
+        uint4 r0, r1;
+        float v[E];
+        if (j + t0 < vecs) r0 = xv[j + t0];
+        if (j + t1 < vecs && t1 != kNone) r1 = xv[j + t1];
+        if (j + t0 < vecs) {
+          unpack16(r0, v, x);
+#pragma unroll
+          for (uint32_t k = 0; k < E; k++) f(head + (j + t0) * E + k, v[k]);
+        }
+        if (j + t1 < vecs && t1 != kNone) {
+          unpack16(r1, v, x);
+#pragma unroll
+          for (uint32_t k = 0; k < E; k++) f(head + (j + t1) * E + k, v[k]);
+        }
+      }
+      if (lane < 2 && (lane ? t1 : t0) != kNone) {
+        const uint32_t t = lane ? t1 : t0, tail = head + vecs * E + t;
+        if (t < head) f(t, load1(x + t));
+        if (tail < n) f(tail, load1(x + tail));
+      }
+    }
+  };
   float m, bound;
   cta_bound(own, by_k && !greedy ? ((uint32_t)r.top_k + C - 1) / C : 0u, mem.maxima, mem.warp_a, mem.warp_b, &mem.pick, m,
             bound);
@@ -1029,12 +1062,11 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   if (greedy) {  // the lowest index of the largest capped logit
     const float low = r.cap > 0.f ? r.below(mc - r.cap * 1e-6f) : m;
     unsigned long long best = 0;
-    if (own >= low)
-      each([&](uint32_t i, float v) {
-        if (!(v >= low)) return;
-        const uint32_t bits = __float_as_uint(r.capped(v)), key = bits >> 31 ? ~bits : bits | 0x80000000u;
-        best = max(best, (unsigned long long)key << 32 | (uint32_t)~(base + i));
-      });
+    each_of(__ballot_sync(0xffffffffu, own >= low), [&](uint32_t i, float v) {
+      if (!(v >= low)) return;
+      const uint32_t bits = __float_as_uint(r.capped(v)), key = bits >> 31 ? ~bits : bits | 0x80000000u;
+      best = max(best, (unsigned long long)key << 32 | (uint32_t)~(base + i));
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     __syncthreads();
@@ -1050,14 +1082,12 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
     return;
   }
   const float low = r.least_logit(mc, bound);
-  if (own >= low && own > -INFINITY) {
-    FewMem *to = cl.map_shared_rank(&mem, 0);
-    each([&](uint32_t i, float v) {
-      if (!(v >= low) || v == -INFINITY) return;
-      const uint32_t at = atomicAdd(&to->n_list, 1u);
-      if (at < kFew) to->list[at] = v, to->list_id[at] = base + i;
-    });
-  }
+  FewMem *to = cl.map_shared_rank(&mem, 0);
+  each_of(__ballot_sync(0xffffffffu, own >= low && own > -INFINITY), [&](uint32_t i, float v) {
+    if (!(v >= low) || v == -INFINITY) return;
+    const uint32_t at = atomicAdd(&to->n_list, 1u);
+    if (at < kFew) to->list[at] = v, to->list_id[at] = base + i;
+  });
   cl.sync();
   if (rank != 0) return;
   const uint32_t count = mem.n_list;
