@@ -90,7 +90,7 @@ struct Shared {
   unsigned long long warp_a[kWarps];
   uint32_t warp_b[kWarps];
   unsigned long long found[3];  // bin, sum above it, its sum
-  uint32_t cut_at, pick;
+  uint32_t cut_at, pick, least, most;
   alignas(16) float e[kSlice + 8];
 };
 
@@ -242,6 +242,54 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float *e = t.e;
   uint32_t prefix = 0;
+  unsigned long long in_bin = 0;
+  // one key holds what is left, `in_bin` in all: its first places stay
+  auto of_one_key = [&](uint32_t low) {
+    const unsigned long long w = COUNT ? 1 : weight_of(__uint_as_float(low));
+    const unsigned long long take = (target + w - 1) / w;
+    if (take == in_bin / w) {
+      if (low > cut.key) cut = Cut{low, 0xFFFFFFFFu};
+      return cut;
+    }
+    // tokens of this key per warp part (a warp owns a contiguous part of the slice)
+    const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
+    uint32_t cnt = 0;
+    for (uint32_t i = w0 + lane; i < w1; i += 32) {
+      const uint32_t key = __float_as_uint(e[i]);
+      cnt += key == low && cut.keeps(key, t.base + i);
+    }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) s->warp_b[warp] = cnt;
+    __syncthreads();
+    uint32_t mine = 0, before = 0;
+    for (int k = 0; k < kWarps; k++) {
+      if (k < warp) before += s->warp_b[k];
+      mine += s->warp_b[k];
+    }
+    t.exchange(mine, 0);
+    for (uint32_t c = 0; c < t.rank; c++) before += (uint32_t)s->xch[t.set][c][0];
+    t.set ^= 1;
+    if (before < take && take <= before + cnt) {  // this warp's part holds the last one that stays
+      uint32_t left = (uint32_t)take - before;
+      for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
+        const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
+        const uint32_t hit = __ballot_sync(0xffffffffu, key == low && cut.keeps(key, t.base + i));
+        const uint32_t c = __popc(hit);
+        if (left <= c) {
+          const uint32_t at = t.base + i0 + __fns(hit, 0, left);
+          if (CLUSTER) {
+            if (lane < (int)t.C) *t.cl.map_shared_rank(&s->cut_at, lane) = at;
+          } else if (lane == 0) {
+            s->cut_at = at;
+          }
+          break;
+        }
+        left -= c;
+      }
+    }
+    t.sync();
+    return Cut{low, s->cut_at};
+  };
   for (int round = 0; round < 3; round++) {
     const Round rd = {round == 0 ? kBins : kSub, round == 0 ? 18u : round == 1 ? 9u : 0u};
     const uint32_t nb = rd.bins;
@@ -258,8 +306,9 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       // the tokens of the bin found last, collected in the first of these rounds where they fit
       auto matches = [&](uint32_t key, uint32_t i) { return key >> (rd.shift + 9) == prefix && cut.keeps(key, t.base + i); };
       if (CLUSTER && round == 1) {
-        if (threadIdx.x == 0) s->pick = 0;
+        if (threadIdx.x == 0) s->pick = 0, s->least = 0xFFFFFFFFu, s->most = 0;
         __syncthreads();
+        uint32_t least = 0xFFFFFFFFu, most = 0;
         // 16-byte groups around the tokens; the places that fill them up have weight 0
         const uint32_t shift = (uint32_t)(e - s->e);
         for (uint32_t g = threadIdx.x; g < (shift + t.n + 3) / 4; g += kThreads) {
@@ -274,9 +323,19 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
             if (matches(keys[j], 4 * g + j - shift)) {
               const uint32_t at = atomicAdd(&s->pick, 1u);
               if (at < kList) s->list_id[at] = keys[j];
+              least = min(least, keys[j]);
+              most = max(most, keys[j]);
             }
         }
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && most) atomicMin(&s->least, least), atomicMax(&s->most, most);
         __syncthreads();
+        if (threadIdx.x < t.C) {  // read after the next barrier of the cluster
+          unsigned long long *to = t.cl.map_shared_rank(&s->xch[t.set][t.rank][0], threadIdx.x);
+          to[0] = s->least;
+          to[1] = s->most;
+        }
       }
       const bool listed = CLUSTER && s->pick <= kList;
       const uint32_t many = listed ? s->pick : t.n;
@@ -307,6 +366,12 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       }
     }
     t.sync();  // every CTA's bins are complete
+    if (CLUSTER && round == 1) {  // one key, as often with 16-bit logits: nothing is left to find
+      unsigned long long least = ~0ull, most = 0;
+      for (uint32_t c = 0; c < t.C; c++) least = min(least, s->xch[t.set][c][0]), most = max(most, s->xch[t.set][c][1]);
+      t.set ^= 1;
+      if (least == most) return of_one_key((uint32_t)most);
+    }
     const uint32_t key_base = round == 0 ? kKeyLow : prefix << (rd.shift + 9);
     if (CLUSTER) {
       // this CTA's part of the bins: warp w reads CTA w's (neighbouring words), the sums go
@@ -341,7 +406,8 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
     t.sync();  // every CTA has every sum, and is done with every CTA's bins
     target = find_bin(s, nb, target, p);
     const uint32_t bin = (uint32_t)s->found[0];
-    const unsigned long long above = s->found[1], in_bin = s->found[2];
+    const unsigned long long above = s->found[1];
+    in_bin = s->found[2];
     if (bin >= nb) return cut;  // fewer tokens than asked for: all stay
     const uint32_t low = key_base + (bin << rd.shift);  // the bin's lowest key
     prefix = low >> rd.shift;
@@ -352,52 +418,7 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       if (low > cut.key) cut = Cut{low, 0xFFFFFFFFu};
       return cut;
     }
-    if (round == 2) {  // one key: the `take` first places of it stay
-      const unsigned long long w = COUNT ? 1 : weight_of(__uint_as_float(low));
-      const unsigned long long take = (target + w - 1) / w;
-      if (take == in_bin / w) {
-        if (low > cut.key) cut = Cut{low, 0xFFFFFFFFu};
-        return cut;
-      }
-      // tokens of this key per warp part (a warp owns a contiguous part of the slice)
-      const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
-      uint32_t cnt = 0;
-      for (uint32_t i = w0 + lane; i < w1; i += 32) {
-        const uint32_t key = __float_as_uint(e[i]);
-        cnt += key == low && cut.keeps(key, t.base + i);
-      }
-      cnt = __reduce_add_sync(0xffffffffu, cnt);
-      if (lane == 0) s->warp_b[warp] = cnt;
-      __syncthreads();
-      uint32_t mine = 0, before = 0;
-      for (int k = 0; k < kWarps; k++) {
-        if (k < warp) before += s->warp_b[k];
-        mine += s->warp_b[k];
-      }
-      t.exchange(mine, 0);
-      for (uint32_t c = 0; c < t.rank; c++) before += (uint32_t)s->xch[t.set][c][0];
-      t.set ^= 1;
-      if (before < take && take <= before + cnt) {  // this warp's part holds the last one that stays
-        uint32_t left = (uint32_t)take - before;
-        for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-          const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
-          const uint32_t hit = __ballot_sync(0xffffffffu, key == low && cut.keeps(key, t.base + i));
-          const uint32_t c = __popc(hit);
-          if (left <= c) {
-            const uint32_t at = t.base + i0 + __fns(hit, 0, left);
-            if (CLUSTER) {
-              if (lane < (int)t.C) *t.cl.map_shared_rank(&s->cut_at, lane) = at;
-            } else if (lane == 0) {
-              s->cut_at = at;
-            }
-            break;
-          }
-          left -= c;
-        }
-      }
-      t.sync();
-      return Cut{low, s->cut_at};
-    }
+    if (round == 2) return of_one_key(low);
   }
   return cut;
 }
