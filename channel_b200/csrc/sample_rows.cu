@@ -147,6 +147,7 @@ struct Tokens {
   const float *e;    // weights
   uint32_t n, base;
   int &set;
+  bool coarse;  // logits of 16 bits: a bin often holds one key only
 
   CH_DEV void sync() const {
     if (CLUSTER) cl.sync(); else __syncthreads();
@@ -251,15 +252,14 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       if (low > cut.key) cut = Cut{low, 0xFFFFFFFFu};
       return cut;
     }
-    // tokens of this key per warp part (a warp owns a contiguous part of the slice)
-    const uint32_t seg = ((t.n + kThreads - 1) / kThreads) * 32, w0 = min(t.n, warp * seg), w1 = min(t.n, w0 + seg);
+    // thread t counts those of the places from t * run on (an odd run spreads the lanes over the banks)
+    const uint32_t run = ((t.n + kThreads - 1) / kThreads) | 1u, p0 = threadIdx.x * run, p1 = min(t.n, p0 + run);
+    auto is = [&](uint32_t i) { return __float_as_uint(e[i]) == low && cut.keeps(low, t.base + i); };
     uint32_t cnt = 0;
-    for (uint32_t i = w0 + lane; i < w1; i += 32) {
-      const uint32_t key = __float_as_uint(e[i]);
-      cnt += key == low && cut.keeps(key, t.base + i);
-    }
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
-    if (lane == 0) s->warp_b[warp] = cnt;
+#pragma unroll 4
+    for (uint32_t i = p0; i < p1; i++) cnt += is(i);
+    const uint32_t all = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) s->warp_b[warp] = all;
     __syncthreads();
     uint32_t mine = 0, before = 0;
     for (int k = 0; k < kWarps; k++) {
@@ -269,18 +269,23 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
     t.exchange(mine, 0);
     for (uint32_t c = 0; c < t.rank; c++) before += (uint32_t)s->xch[t.set][c][0];
     t.set ^= 1;
-    if (before < take && take <= before + cnt) {  // this warp's part holds the last one that stays
-      uint32_t left = (uint32_t)take - before;
-      for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-        const uint32_t i = i0 + lane, key = i < w1 ? __float_as_uint(e[i]) : 0u;
-        const uint32_t hit = __ballot_sync(0xffffffffu, key == low && cut.keeps(key, t.base + i));
-        const uint32_t c = __popc(hit);
+    if (before < take && take <= before + all) {  // this warp's part holds the last one that stays
+      uint32_t inc = cnt;  // the lane that does, then the place in its run
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      const int owner = __ffs(__ballot_sync(0xffffffffu, before + inc >= take)) - 1;
+      uint32_t left = (uint32_t)take - before - __shfl_sync(0xffffffffu, inc - cnt, owner);
+      const uint32_t q0 = (warp * 32 + owner) * run, q1 = min(t.n, q0 + run);
+      for (uint32_t i0 = q0; i0 < q1; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        const bool hit = i < q1 && is(i);
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit), c = __popc(hits);
         if (left <= c) {
-          const uint32_t at = t.base + i0 + __fns(hit, 0, left);
-          if (CLUSTER) {
-            if (lane < (int)t.C) *t.cl.map_shared_rank(&s->cut_at, lane) = at;
-          } else if (lane == 0) {
-            s->cut_at = at;
+          if (hit && __popc(hits & ((1u << lane) - 1)) == (int)left - 1) {
+            for (uint32_t c = 0; c < t.C; c++) (CLUSTER ? *t.cl.map_shared_rank(&s->cut_at, c) : s->cut_at) = t.base + i;
           }
           break;
         }
@@ -327,11 +332,13 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
               most = max(most, keys[j]);
             }
         }
-        least = __reduce_min_sync(0xffffffffu, least);
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 0 && most) atomicMin(&s->least, least), atomicMax(&s->most, most);
+        if (t.coarse) {
+          least = __reduce_min_sync(0xffffffffu, least);
+          most = __reduce_max_sync(0xffffffffu, most);
+          if (lane == 0 && most) atomicMin(&s->least, least), atomicMax(&s->most, most);
+        }
         __syncthreads();
-        if (threadIdx.x < t.C) {  // read after the next barrier of the cluster
+        if (t.coarse && threadIdx.x < t.C) {  // read after the next barrier of the cluster
           unsigned long long *to = t.cl.map_shared_rank(&s->xch[t.set][t.rank][0], threadIdx.x);
           to[0] = s->least;
           to[1] = s->most;
@@ -366,7 +373,7 @@ CH_DEV Cut select(const Tokens<CLUSTER> &t, Cut cut, unsigned long long target, 
       }
     }
     t.sync();  // every CTA's bins are complete
-    if (CLUSTER && round == 1) {  // one key, as often with 16-bit logits: nothing is left to find
+    if (CLUSTER && t.coarse && round == 1) {  // one key: nothing is left to find
       unsigned long long least = ~0ull, most = 0;
       for (uint32_t c = 0; c < t.C; c++) least = min(least, s->xch[t.set][c][0]), most = max(most, s->xch[t.set][c][1]);
       t.set ^= 1;
@@ -723,7 +730,7 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   };
   for (uint32_t i = threadIdx.x; i < head; i += kThreads) e[i] = put(load1(x + i));
   const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t j = threadIdx.x; j < vecs; j += kThreads) {
     const uint4 r = xv[j];
     float f[E];
@@ -740,7 +747,7 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   float4 *e4 = reinterpret_cast<float4 *>(s->e);
   if (threadIdx.x < shift) s->e[threadIdx.x] = -INFINITY;
   if (threadIdx.x < 4 * groups - shift - n) e[n + threadIdx.x] = -INFINITY;
-  const Tokens<true> all{s, cl, C, rank, e, n, base, set};
+  const Tokens<true> all{s, cl, C, rank, e, n, base, set, sizeof(T) == 2};
   // the CTA's maximum of v
   auto cta_max = [&](float v) {
     v = warp_max(v);
@@ -873,7 +880,7 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
         return;
       }
       __syncthreads();
-      cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set}, r.top_k, r.top_p, r.u, s->list_id,
+      cut_and_draw(a, row, Tokens<false>{s, cl, 1, 0, s->list, count, 0, set, false}, r.top_k, r.top_p, r.u, s->list_id,
                    false);
       return;
     }
