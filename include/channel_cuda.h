@@ -453,8 +453,9 @@ int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
  * positions [max(0, T - window), T) (window 0 = all), q head h to kv head
  * h / (n_q / n_kv):  out = softmax(scale q.k) v, zeros when no position is visible.
  * q / out element (b, head, d) at b * stream_stride + head * head_stride + d.
- * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096; page_size a power of two from 8 to 256;
- * dtype (of q, out and both pools) CH_F16 or CH_BF16, sums in f32.  Strides are multiples
+ * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096;
+ * page_size a power of two from 8 to 256; dtype (of q, out and both pools) CH_F16 or CH_BF16,
+ * sums in f32.  Strides are multiples
  * of 8 elements, q, out and the pools 16-byte aligned.  Positions whose page index is not
  * in [0, n_pages) are left out (status bit 2), as are own positions past table_cols pages.
  * The shared pages are read once for the whole batch.  workspace: at least
@@ -475,8 +476,9 @@ size_t ch_prefix_attention_workspace(const ch_prefix_attn_args *args);
 int ch_prefix_attention(const ch_prefix_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* One token per row of logits (n_rows x vocab, vocab <= 262144, row stride row_stride
- * elements, 0 for one row of logits for all).  With x = softcap * tanh(logit / softcap) (softcap 0: the logit; NaN counts
- * as -inf; -inf and the type's lowest value mask a token and are not capped), m = max x, T = temperature[row], token i weighs e_i = exp((x_i - m) / T),
+ * elements, 0 for one row of logits for all).  With x = softcap * tanh(logit / softcap)
+ * (softcap 0: the logit; NaN counts as -inf; -inf and the type's lowest value mask a token and
+ * are not capped), m = max x, T = temperature[row], token i weighs e_i = exp((x_i - m) / T),
  * held as floor(2^44 e_i); tokens of weight 0 are never drawn.  Kept are, in the order of
  * falling e (equal ones by index):  e_i >= min_p (and every e_i = 1);  of those the first
  * top_k (0 = all);  of those the first whose weights before them sum to less than top_p of
