@@ -1034,7 +1034,7 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   const uint32_t head = min(n, (E - (uint32_t)(((uintptr_t)x / sizeof(T)) % E)) % E), vecs = (n - head) / E;
   const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
   auto each = [&](auto f) {
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t j = threadIdx.x; j < vecs; j += kThreads) {
       float v[E];
       unpack16(xv[j], v, x);
@@ -1212,12 +1212,12 @@ cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   a.rows = rows;
   uint32_t running = 0;
   cudaError_t e = allow((const void *)sample_rows_kernel<T>, sizeof(Shared), C, &running);
-  // Rows with few candidates in clusters of 8, or of 4 where the rows then fill more than half
-  // of the SMs (64 rows: 46 us in clusters of 4, a second wave of clusters of 8 took 57; for 24
-  // rows and fewer 8 read faster).
+  // Rows with few candidates in clusters of 8, which read faster (48 such rows 28 us, in clusters
+  // of 4 37), or of 4 where 8 leave less than a quarter of the SMs for the rows with many: 64
+  // rows, 7 of them with many, take 47 us in clusters of 4, 54 in clusters of 8.
   for (uint32_t at_once = 0; e == cudaSuccess; few /= 2) {
     e = allow((const void *)sample_few_kernel<T>, 0, few, &at_once);
-    if (rows <= at_once / 2 || few <= 4) break;
+    if (rows <= at_once * 3 / 4 || few <= 4) break;
   }
   if (e != cudaSuccess) return e;
   auto launch = [&](Rows which) {
