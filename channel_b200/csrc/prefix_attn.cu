@@ -60,8 +60,8 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
 //
 // Measured (8 kv heads of 256, two q heads each, with the shared prefix of prefix_tc.cuh beside
 // it in the same launch, and the join): 64 streams of 1 to 1,023 own tokens behind 4,096 shared
-// ones 59 us (303 MB, 5.1 TB/s; a kernel per row 1,648 us), behind 32,768 with 1 to 2,047 own
-// ones 136 to 141 us (5.8 TB/s), a window of 1,024 71 us; 37 streams of 32 q on 8 kv heads of 128 25 us,
+// ones 60 us (303 MB, 5.0 TB/s; a kernel per row 1,648 us), behind 32,768 with 1 to 2,047 own
+// ones 136 to 141 us (5.8 TB/s), a window of 1,024 68 us; 37 streams of 32 q on 8 kv heads of 128 25 us,
 // 4 streams behind 192 tokens 12 us.  The small ones are the latency of one launch with a join.
 constexpr uint32_t kTile = 16;  // keys
 template <int D>

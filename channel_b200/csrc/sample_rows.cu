@@ -37,7 +37,7 @@
 // Bound.  For one row the chain of passes, scans and cluster barriers, not HBM.  One row of
 // 262,144 capped f32 logits takes 12 us with top-k 64 and 31 us by top-p alone (58,000 cycles:
 // the cap 7,400, weights and first bins 9,400, a round of the cut 7,000 to 8,000, collecting a
-// bin's tokens 5,000, the kept sum 3,300).  64 such rows of mixed settings take 43 us, where
+// bin's tokens 5,000, the kept sum 3,300).  64 such rows of mixed settings take 45 us, where
 // reading them takes 10.4; 48 rows of 100,003 bf16 logits by top-p and min-p 35 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -268,6 +268,36 @@ def test_saturated_cap_ties():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(min_p=1e-5, top_p=0.95), dict(top_k=5000, top_p=0.8)])
+def test_more_rows_with_many_candidates_than_run_at_once(kw, dtype):
+    n = 150
+    x = lm_logits(n, 50001, 11, dtype)
+    u = np.linspace(0, 0.999, n).astype(np.float32)
+    full = dict(temperature=1.2, top_k=0, top_p=1.0, min_p=0.0)
+    full.update(kw)
+    token, _, kept = draw(x, u, **full)
+    rt, _, rk = plain(x, torch.from_numpy(u).cuda(), 0.0, **settings(n, **full))
+    assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("step", [0.0, 1e-6, 2e-3, 0.7])
+def test_cuts_among_thousands_of_near_weights(step, dtype):
+    """six values, so that thousands of tokens share a weight or differ in its last bits"""
+    v, p = 100003, [0.05, 0.37, 0.8, 0.999]
+    g = torch.Generator("cuda").manual_seed(3)
+    x = (step * torch.randint(0, 6, (8, v), generator=g, device="cuda")).to(dtype)
+    x[:, 77] += 0.5
+    u = np.linspace(0, 0.99, 8).astype(np.float32)
+    full = dict(temperature=0.9, top_k=[0] * 4 + [1, 3000, 50000, 99999], top_p=p + p[::-1], min_p=0.0)
+    token, _, kept = draw(x, u, **full)
+    rt, _, rk = plain(x, torch.from_numpy(u).cuda(), 0.0, **settings(8, **full))
+    assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
+
+
+@gpu
 @pytest.mark.parametrize("temperature", [1e-3, 0.37, 3.0, 1e4, 1e30])
 @pytest.mark.parametrize("scale", [1e-4, 1.0, 1e4])
 def test_scales(scale, temperature):
