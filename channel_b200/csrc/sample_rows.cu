@@ -1208,17 +1208,9 @@ template <typename T>
 cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   uint32_t C = 1;
   while (C * kSlice < a.vocab) C *= 2;
-  uint32_t few = C > 8 ? 8 : C;
   a.rows = rows;
-  uint32_t running = 0;
+  uint32_t running = 0, few = std::min(C, 8u), few_running = 0;
   cudaError_t e = allow((const void *)sample_rows_kernel<T>, sizeof(Shared), C, &running);
-  // Rows with few candidates in clusters of 8, which read faster (48 such rows 28 us, in clusters
-  // of 4 37), or of 4 where 8 leave less than a quarter of the SMs for the rows with many: 64
-  // rows, 7 of them with many, take 47 us in clusters of 4, 54 in clusters of 8.
-  for (uint32_t at_once = 0; e == cudaSuccess; few /= 2) {
-    e = allow((const void *)sample_few_kernel<T>, 0, few, &at_once);
-    if (rows <= at_once * 3 / 4 || few <= 4) break;
-  }
   if (e != cudaSuccess) return e;
   auto launch = [&](Rows which) {
     a.which = which;
@@ -1230,7 +1222,15 @@ cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
   // many candidates, dealt to the clusters that run at once, beside them those with few, then
   // what those left (64 rows: all of them through the first kernel 70 us, so 46).
   if (rows <= running) return launch(Rows::kAll);
-  e = launch(Rows::kMany);
+  // Rows with few candidates in clusters of 8, which read faster (48 such rows 28 us, in clusters
+  // of 4 37), or of 4 where 8 leave less than a quarter of the SMs for the rows with many: 64
+  // rows, 7 of them with many, take 47 us in clusters of 4, 54 in clusters of 8.
+  e = allow((const void *)sample_few_kernel<T>, 0, few, &few_running);
+  if (e == cudaSuccess && few == 8 && rows > few_running * 3 / 4) {
+    few = 4;
+    e = allow((const void *)sample_few_kernel<T>, 0, few, nullptr);
+  }
+  if (e == cudaSuccess) e = launch(Rows::kMany);
   if (e != cudaSuccess) return e;
   a.per = (a.vocab + few - 1) / few;
   e = start_clusters(sample_few_kernel<T>, a, rows, few, 0, stream);
