@@ -561,9 +561,11 @@ uint32_t max_splits(const ch_prefix_attn_args *p) {
   return (uint32_t)std::max(1ull, std::min<unsigned long long>((unsigned)num_sms() / per_split,
                                                                (p->prefix_len + kKeys - 1) / kKeys));
 }
-// workspace: w.start | w.deal | w.ml | w.o | the prefix's ml | o
+// workspace: w.start | w.deal | w.ml | w.o | the prefix's ml | o, each on 256 bytes (the parts of O
+// are stored 32 bytes at a time); the caller's base is on 16 only, so there is room to align it
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w, PrefixParts *pp) {
+  base = reinterpret_cast<uint8_t *>(aligned(reinterpret_cast<uintptr_t>(base)));
   const uint32_t runs = (uint32_t)num_sms() * (p->head_dim == 256 ? Own<256>::kWarps : Own<128>::kWarps);
   static_assert(Own<64>::kWarps == Own<128>::kWarps, "runs");
   const size_t rows = ((size_t)runs + (size_t)p->n_streams * p->n_kv) * (p->n_q / p->n_kv);
@@ -581,7 +583,7 @@ size_t carve(const ch_prefix_attn_args *p, uint8_t *base, Work *w, PrefixParts *
   const size_t shared = (size_t)pp->max_splits * p->n_streams * p->n_q;
   pp->ml = reinterpret_cast<float2 *>(take(shared * sizeof(float2)));
   pp->o = reinterpret_cast<float *>(take(shared * p->head_dim * sizeof(float)));
-  return at;
+  return at + 256 - 16;
 }
 
 // kernel<<<grid, block, smem, s>>>(args...), which may start before the kernel in front of it
