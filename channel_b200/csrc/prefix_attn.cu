@@ -196,17 +196,19 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
   grid_dep_launch();
 
   // ---- the shared prefix ----
+  const bool with_unit = blockIdx.x < d.unit_ctas;
+  if (with_unit && warp == 1) tmem_take(tc_bars);
   for (uint32_t u = blockIdx.x; u < d.units; u += gridDim.x) {
     const uint32_t h = u % a.nkv, rt = (u / a.nkv) % row_tiles, split = u / (a.nkv * row_tiles);
     const uint32_t i0 = split * (ptiles / d.splits) + min(split, ptiles % d.splits);
     const uint32_t i1 = i0 + ptiles / d.splits + (split < ptiles % d.splits);
     prefix_unit<T, D>(a, pp, kmap, vmap, smem, tc_bars, h, rt, split, tile0 + i0, i1 - i0, zlo);
   }
+  if (with_unit && warp == 1) tmem_give(tc_bars);
 
   // ---- this warp's run of the streams' own tiles; consecutive runs lie on different SMs, so
   // that few tiles spread over all of them ----
   if (warp >= O::kWarps) return;
-  const bool with_unit = blockIdx.x < d.unit_ctas;
   const uint32_t run = with_unit ? d.y_runs + warp * d.unit_ctas + blockIdx.x
                                  : warp * (gridDim.x - d.unit_ctas) + blockIdx.x - d.unit_ctas;
   const uint32_t per = with_unit ? d.x : d.y;

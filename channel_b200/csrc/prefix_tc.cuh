@@ -181,9 +181,22 @@ struct TcBars {
   uint32_t masks[kMasks][2], tmem_slot, abort_flag;
 };
 
+// Tensor memory for all units of a CTA, by one whole warp: taken before the first (a CTA that has
+// given up the permit may not allocate again), given back after the last.
+CH_DEV void tmem_take(TcBars &bars) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_slot)),
+               "r"(kTmemCols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+CH_DEV void tmem_give(TcBars &bars) {
+  tc_fence_after();
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars.tmem_slot), "r"(kTmemCols) : "memory");
+}
+
 // One unit: kv head h, row tile rt, key tiles [i0, i0 + nt) of the prefix, whose positions
 // below zlo no stream sees.  Leaves the rows' parts at split `split`.  All threads of the CTA
-// call it; sm (1024-byte aligned) is free before and after.
+// call it, after tmem_take by warp 1; sm (1024-byte aligned) is free before and after.
 template <typename T, int D>
 CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtensorMap &kmap, const CUtensorMap &vmap,
                         uint8_t *sm, TcBars &bars, uint32_t h, uint32_t rt, uint32_t split, uint32_t i0, uint32_t nt,
@@ -211,12 +224,6 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     mbar_init(&done, 1);
     abort_flag = 0u;
     fence_mbar_init();
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_slot)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -506,10 +513,6 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   __syncwarp();
   tc_fence_before();
   __syncthreads();  // every role done with tensor memory and the barriers
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-  }
   if (tid == 0) {  // the barriers' memory may be initialised again
     auto drop = [](uint64_t *bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
     for (int s = 0; s < C::kSlots; s++) drop(&full[s]), drop(&empty[s]);

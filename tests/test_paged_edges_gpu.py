@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from channel_b200 import _lib as L
-from tests.test_paged_gpu import attend, attn_args, make
+from tests.test_paged_gpu import attend, attn_args, check, make
 
 gpu = pytest.mark.gpu
 
@@ -30,3 +30,14 @@ def test_attention_with_a_workspace_on_16_bytes(d):
         L.check(lib.ch_prefix_attention(ctypes.byref(a), buf.data_ptr() + at, need, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(out, ref)
         assert int(buf[:at].max()) == 0 and int(buf[at + need:].max()) == 0
+
+
+@gpu
+@pytest.mark.parametrize("n,nq,nkv,d,prefix", [
+    (17, 1024, 64, 64, 150),    # 192 pairs of kv head and 128 query rows, two for some of the SMs
+    (1153, 16, 8, 256, 70),     # 152 of them
+    (300, 64, 8, 128, 65),      # 152, and more streams than threads
+    (4096, 2, 1, 128, 100)])    # as many streams as a call takes
+def test_attention_of_more_prefix_work_than_sms(n, nq, nkv, d, prefix):
+    lens = [(5 * i) % 11 for i in range(n)]
+    check(*make(n, prefix, lens, nq, nkv, d, 8, torch.float16, seed=n), prefix)
