@@ -102,7 +102,7 @@ namespace {
 constexpr uint32_t kKeys = 64, kRows = 128;
 constexpr int kTcThreads = 8 * 32, kSoft = 4 * 32;
 constexpr uint32_t kTmemCols = 512, kQCol = 256, kSCol = 384;  // O: columns 0 .. D - 1; S: 384 and 448
-constexpr int kMasks = 8;
+constexpr int kMasks = 16;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 
 template <int D>
@@ -113,6 +113,11 @@ struct Tc {
   static constexpr uint32_t kVKeys = kPiece / (2 * D);   // keys of a V piece
   static constexpr int kSlots = 13;
   static constexpr uint32_t kBytes = kSlots * kPiece;
+  // The mask of tile i is written when K_{i-1}, first piece P (2i - 3) of the ring's order (P =
+  // kParts), is on its way, for which piece P (2i - 3) - kSlots had to be taken.  The last V piece
+  // up to there, place P (2j + 3) - 1, is of tile j = i - 3 - ceil((kSlots - 1) / 2P), so softmax is
+  // done with tile j and may still be at the mask of tile j + 1: tiles j + 1 .. i need one each.
+  static_assert(kMasks >= 3 + (kSlots + 2 * kParts - 2) / (2 * kParts), "masks in use at a time");
 };
 
 CH_DEV void tma_load_5d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int u, int w, uint64_t *bar) {

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from channel_b200 import _lib as L
-from tests.test_paged_gpu import attend, attn_args, check, make
+from tests.test_paged_gpu import U, attend, attn_args, check, make
 
 gpu = pytest.mark.gpu
 
@@ -41,3 +41,40 @@ def test_attention_with_a_workspace_on_16_bytes(d):
 def test_attention_of_more_prefix_work_than_sms(n, nq, nkv, d, prefix):
     lens = [(5 * i) % 11 for i in range(n)]
     check(*make(n, prefix, lens, nq, nkv, d, 8, torch.float16, seed=n), prefix)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,nq,nkv,d,prefix,page", [
+    (3, 4, 2, 64, 9001, 16), (3, 4, 2, 128, 9001, 16), (16, 64, 64, 128, 8000, 32), (16, 64, 64, 64, 7990, 64),
+    (64, 16, 8, 128, 32767, 64)])
+def test_attention_long_prefix_of_narrow_heads(n, nq, nkv, d, prefix, page, dtype):
+    """many key tiles per unit, and a ragged last one; among them pages that are not in the pool,
+    whose tiles have masks of their own"""
+    lens = [(37 * i) % 50 for i in range(n)]
+    args = make(n, prefix, lens, nq, nkv, d, page, dtype, seed=d + n)
+    if n < 64:
+        check(*args, prefix)
+    q, k, v, pt, table, lens = args
+    gone = torch.arange(0, len(pt) - 1, 11)  # every 11th page
+    bad = pt.clone()
+    bad[gone] = -1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attend(q, k, v, bad, table, lens, prefix, status=status)
+    assert int(status.item()) == 1 << 2
+    # the definition over the rest: the positions of those pages are left out
+    seen = torch.ones(prefix, dtype=torch.bool)
+    for i in gone.tolist():
+        seen[i * page:(i + 1) * page] = False
+    rows = (pt.long().repeat_interleave(page)[:prefix] * page + torch.arange(prefix) % page)[seen]
+    kr, vr, u = k.flatten(0, 1).cuda(), v.flatten(0, 1).cuda(), U[dtype]
+    group = nq // nkv
+    for b in range(n):
+        own = torch.tensor([int(table[b, i // page]) * page + i % page for i in range(lens[b])], dtype=torch.long)
+        at = torch.cat([rows, own]).cuda()
+        for h in range(nkv):
+            p = torch.softmax(q[b, h * group:(h + 1) * group].cuda().double() @ kr[at, h].double().T * d ** -0.5, 1)
+            values = vr[at, h].double()
+            ref, mag = p @ values, p @ values.abs()
+            far = (out[b, h * group:(h + 1) * group].double() - ref).abs() - (u * ref.abs() + (u + 2.0 ** -14) * mag)
+            assert float(far.max()) <= 1e-7, (b, h)
