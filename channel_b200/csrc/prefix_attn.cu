@@ -197,18 +197,21 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
 
   // ---- the shared prefix ----
   const bool with_unit = blockIdx.x < d.unit_ctas;
+  bool dead = false;  // a wait gave up
   if (with_unit && warp == 1) tmem_take(tc_bars);
   for (uint32_t u = blockIdx.x; u < d.units; u += gridDim.x) {
     const uint32_t h = u % a.nkv, rt = (u / a.nkv) % row_tiles, split = u / (a.nkv * row_tiles);
     const uint32_t i0 = split * (ptiles / d.splits) + min(split, ptiles % d.splits);
     const uint32_t i1 = i0 + ptiles / d.splits + (split < ptiles % d.splits);
-    prefix_unit<T, D>(a, pp, kmap, vmap, smem, tc_bars, h, rt, split, tile0 + i0, i1 - i0, zlo);
+    dead = dead || !prefix_unit<T, D>(a, pp, kmap, vmap, smem, tc_bars, h, rt, split, tile0 + i0, i1 - i0, zlo);
+    const uint32_t rows = a.n * a.group, gr = rt * kRows + tid;
+    if (dead && tid < (int)kRows && gr < rows) pp.ml[((size_t)split * a.nkv + h) * rows + gr] = make_float2(0.f, NAN);
   }
   if (with_unit && warp == 1) tmem_give(tc_bars);
 
   // ---- this warp's run of the streams' own tiles; consecutive runs lie on different SMs, so
   // that few tiles spread over all of them ----
-  if (warp >= O::kWarps) return;
+  if (warp >= O::kWarps) return;  // (no barrier of the CTA from here on)
   const uint32_t run = with_unit ? d.y_runs + warp * d.unit_ctas + blockIdx.x
                                  : warp * (gridDim.x - d.unit_ctas) + blockIdx.x - d.unit_ctas;
   const uint32_t per = with_unit ? d.x : d.y;
@@ -249,6 +252,14 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
     if (c.b < a.n) enter(c, bounds);
   };
   Cursor cu = ld;
+  auto give_up = [&]() {  // the rest of the run: sums of NaN, as for a prefix unit
+    for (; left; left--) {
+      const unsigned long long seg = (unsigned long long)run + cu.b * a.nkv + cu.h;
+      if ((cu.i + 1 == cu.tiles || left == 1) && lane < (int)a.group) w.ml[seg * a.group + lane] = make_float2(0.f, NAN);
+      advance(cu, false);
+    }
+  };
+  if (dead) return give_up();
   uint32_t qf[NR][kSteps][2];
   float o[NR][kSteps][4], m[NR][2], l[NR][2];
   const float scale2 = a.scale * 1.44269504088896341f;
@@ -341,11 +352,11 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
     }
     const bool ok = mbar_wait_bounded(&bars[warp][stage], parity, a.status);
     if (!__all_sync(0xffffffffu, ok)) {  // reported; the copies still in flight get a wait of their own
-      for (int k = 1; k < O::kStages && (uint32_t)k < left; k++) {
-        if (++stage == O::kStages) stage = 0, parity ^= 1;
+      for (int k = 0; k < O::kStages && (uint32_t)k < left; k++) {
         mbar_wait_bounded(&bars[warp][stage], parity, a.status);
+        if (++stage == O::kStages) stage = 0, parity ^= 1;
       }
-      return;
+      return give_up();
     }
     const uint32_t base = frag + stage * O::kStage, mask = masks[warp][stage];
     float s[NR][2][4];

@@ -24,8 +24,9 @@
 //
 // Warps: 0, 6, 7 copies, 1 MMA issue, 2-5 softmax and epilogue (TMEM lanes 32 * (warp % 4)).
 // Every wait is bounded; one that gives up sets the status word and the abort flag, the roles
-// leave their loops, and the MMA warp's last commit is waited for before tensor memory is
-// released.
+// leave their loops, and the copies and products in flight are waited for (again with a limit)
+// before the CTA goes on.  The rows of that unit get a sum of NaN, for which the join computes a
+// row again on its own.
 #pragma once
 #include <cuda_bf16.h>
 #include <cudaTypedefs.h>
@@ -184,6 +185,7 @@ CH_DEV void st_global_32b(float *p, const uint32_t *v) {  // 32 bytes, 32-byte a
 struct TcBars {
   uint64_t full[13], empty[13], q_ready, s_full[2], p_ready[2], pv_done, done, mask_full[kMasks];
   uint32_t masks[kMasks][2], tmem_slot, abort_flag;
+  uint32_t issued[13];  // 1 + the last piece on its way to a slot of the ring
 };
 
 // Tensor memory for all units of a CTA, by one whole warp: taken before the first (a CTA that has
@@ -200,10 +202,10 @@ CH_DEV void tmem_give(TcBars &bars) {
 }
 
 // One unit: kv head h, row tile rt, key tiles [i0, i0 + nt) of the prefix, whose positions
-// below zlo no stream sees.  Leaves the rows' parts at split `split`.  All threads of the CTA
-// call it, after tmem_take by warp 1; sm (1024-byte aligned) is free before and after.
+// below zlo no stream sees.  Leaves the rows' parts at split `split`; false if it gave up, and
+// then shared memory is not to be used again.  All threads of the CTA call it, after tmem_take by warp 1; sm (1024-byte aligned) is free before and after.
 template <typename T, int D>
-CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtensorMap &kmap, const CUtensorMap &vmap,
+CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtensorMap &kmap, const CUtensorMap &vmap,
                         uint8_t *sm, TcBars &bars, uint32_t h, uint32_t rt, uint32_t split, uint32_t i0, uint32_t nt,
                         uint32_t zlo) {
   using C = Tc<D>;
@@ -228,6 +230,7 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     mbar_init(&pv_done, 1);
     mbar_init(&done, 1);
     abort_flag = 0u;
+    for (int s = 0; s < C::kSlots; s++) bars.issued[s] = 0u;
     fence_mbar_init();
   }
   tc_fence_before();
@@ -250,7 +253,6 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
       return i < nt && lane < (int)boxes && j < a.prefix ? a.prefix_table[j >> a.shift] : -1;
     };
     int32_t next = look_up(0);
-    uint32_t last = 0;  // pieces up to here are on their way
     bool ok = true;
     for (uint32_t i = 0; i < nt && ok; i++) {
       const uint32_t j0 = (i0 + i) * kKeys;
@@ -276,9 +278,8 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
         if (seq >= (uint32_t)C::kSlots) ok = tc_wait(&empty[s], ((seq / C::kSlots) - 1) & 1, &abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], kPiece);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], kPiece), bars.issued[s] = seq + 1;
         __syncwarp();
-        last = seq + 1;
         if (is_v) {
           const uint32_t key = c * C::kVKeys + min((uint32_t)lane, C::kVKeys / vr - 1) * vr;
           const int32_t pg = __shfl_sync(0xffffffffu, page, key / kr);
@@ -294,9 +295,6 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
         }
       }
     }
-    // the last copies land before the CTA may leave (normally long done)
-    const uint32_t total = 2 * C::kParts * nt, from = total > (uint32_t)C::kSlots ? total - C::kSlots : 0u;
-    for (uint32_t q = from; q < last; q++) tc_wait(&full[q % C::kSlots], (q / C::kSlots) & 1, &abort_flag, a.status);
   } else if (warp == 1) {
     // ---- products.  The warp walks the loop together and one elected lane issues: with the
     // branch on lane 0 around everything and the descriptors built per instruction, issue
@@ -518,6 +516,17 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   __syncwarp();
   tc_fence_before();
   __syncthreads();  // every role done with tensor memory and the barriers
+  // what is still on its way to shared memory or the barriers lands (normally long done): the
+  // last copy into each slot and, unless a role gave up, the arrivals of the last products
+  if (tid < C::kSlots && bars.issued[tid]) {
+    const uint32_t parity = ((bars.issued[tid] - 1) / C::kSlots) & 1;
+    if (!tc_wait(&full[tid], parity, nullptr, a.status) || (!abort_flag && !tc_wait(&empty[tid], parity, nullptr, a.status)))
+      abort_flag = 1u;
+  } else if (tid == 32 && !abort_flag && !tc_wait(&pv_done, (nt - 1) & 1, nullptr, a.status)) {
+    abort_flag = 1u;
+  }
+  __syncthreads();
+  if (abort_flag) return false;
   if (tid == 0) {  // the barriers' memory may be initialised again
     auto drop = [](uint64_t *bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); };
     for (int s = 0; s < C::kSlots; s++) drop(&full[s]), drop(&empty[s]);
@@ -526,6 +535,7 @@ CH_DEV void prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     drop(&q_ready), drop(&pv_done), drop(&done);
   }
   __syncthreads();
+  return true;
 }
 
 // One layer's pool as a tensor of dim, token in the page, head and page (K: boxes of 64 dims
