@@ -713,9 +713,11 @@ CH_DEV void rank_and_draw(const RowsArgs &a, uint32_t row, Few *s, const float *
   }
 }
 
-// One row by a cluster that keeps it in shared memory.
+// One row by a cluster that keeps it in shared memory.  first: the cluster's first row, before
+// which every CTA has arrived at the cluster's barrier; it is waited for ahead of the first store
+// to another CTA, which must have started by then (the barrier costs nothing behind the row's read).
 template <typename T>
-CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, cg::cluster_group &cl) {
+CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, cg::cluster_group &cl, bool first) {
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
@@ -771,6 +773,7 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
   const bool by_k = r.top_k > 0 && r.top_k <= kMostK, bounded = a.vocab > kList && by_k && r.temp > 0.f;
   float m, bound;
   cta_bound(own, bounded ? ((uint32_t)r.top_k + C - 1) / C : 0u, s->maxima, s->warp_a, s->warp_b, &s->pick, m, bound);
+  if (first) cl.barrier_wait();
   all.exchange(__float_as_uint(m), __float_as_uint(bound));
   for (uint32_t c = 0; c < C; c++) {
     m = fmaxf(m, __uint_as_float((uint32_t)s->xch[set][c][0]));
@@ -986,6 +989,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared *s = reinterpret_cast<Shared *>(smem_raw);
   cg::cluster_group cl = cg::this_cluster();
+  cl.barrier_arrive();
   const uint32_t N = gridDim.x / cl.num_blocks(), number = blockIdx.x / cl.num_blocks();
   const float lowest = lowest_of(static_cast<const T *>(a.logits));
   grid_dep_wait();
@@ -995,8 +999,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   uint32_t row = number;
   if (a.which == Rows::kMany) row = nth_row(s, a.rows, 0, 1, number, many);
   if (a.which == Rows::kLeftOver) row = nth_row(s, a.rows, number, N, 0, left);
-  while (row < a.rows) {
-    keep_row<T>(a, row, row_of(a, row, lowest), s, cl);
+  if (row >= a.rows) cl.barrier_wait();  // no row; an arrival is not left without its wait
+  for (bool first = true; row < a.rows; first = false) {
+    keep_row<T>(a, row, row_of(a, row, lowest), s, cl, first);
     if (a.which == Rows::kAll) return;
     cl.sync();  // every CTA is done with the row
     row = a.which == Rows::kMany ? nth_row(s, a.rows, row + 1, 1, N - 1, many) : nth_row(s, a.rows, row + N, N, 0, left);
@@ -1019,12 +1024,13 @@ struct FewMem {
 template <typename T>
 CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   cg::cluster_group cl = cg::this_cluster();
+  cl.barrier_arrive();  // waited for ahead of the first store to another CTA
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = min(a.vocab, rank * a.per), n = min(a.vocab - base, a.per);
   const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride + base;
   const Row r = row_of(a, row, lowest_of(x));
-  if (!r.few()) return;
+  if (!r.few()) return cl.barrier_wait();
   const bool greedy = !(r.temp > 0.f), by_k = r.top_k > 0 && r.top_k <= (int32_t)kFew;
   for (uint32_t i = threadIdx.x; i < kMaxima; i += kThreads) mem.maxima[i] = 0;
   if (threadIdx.x == 0) mem.pick = kMaxima, mem.n_list = 0;
@@ -1083,6 +1089,7 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   float m, bound;
   cta_bound(own, by_k && !greedy ? ((uint32_t)r.top_k + C - 1) / C : 0u, mem.maxima, mem.warp_a, mem.warp_b, &mem.pick, m,
             bound);
+  cl.barrier_wait();
   if (threadIdx.x < C)
     cl.map_shared_rank(&mem, threadIdx.x)->xch[0][rank] = (unsigned long long)__float_as_uint(m) << 32 | __float_as_uint(bound);
   cl.sync();

@@ -1,0 +1,36 @@
+"""ch_sample_rows: batches, launches and values at the ends of what it takes."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_sample_rows_gpu import draw, lm_logits, plain, random_settings, settings
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("n,v", [(310, 16391), (310, 32768), (160, 40001), (310, 500)])
+def test_batches_of_small_clusters(n, v, dtype):
+    """more rows than run at once where a row takes two CTAs, four, or one"""
+    for seed, softcap in ((3, 0.0), (4, 30.0)):
+        rng = np.random.default_rng(seed)
+        x = lm_logits(n, v, seed, dtype)
+        kw, u = random_settings(n, rng), rng.random(n).astype(np.float32)
+        token, _, kept = draw(x, u, softcap, **kw)
+        rt, _, rk = plain(x, torch.from_numpy(u).cuda(), softcap, **settings(n, **kw))
+        assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
+
+
+@gpu
+@pytest.mark.parametrize("n", [200, 400])
+def test_clusters_without_a_row(n):
+    """batches in which no row has many candidates, or every one has"""
+    x = lm_logits(n, 20000, 5)
+    u = np.linspace(0, 0.999, n).astype(np.float32)
+    for kw in (dict(top_k=20), dict(temperature=0.0), dict(top_p=0.9)):
+        full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(kw)
+        token, _, kept = draw(x, u, **full)
+        rt, _, rk = plain(x, torch.from_numpy(u).cuda(), 0.0, **settings(n, **full))
+        assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
