@@ -980,6 +980,10 @@ CH_DEV uint32_t nth_row(Shared *s, uint32_t rows, uint32_t from, uint32_t step, 
   return rows;
 }
 
+// Counts the CTAs of launches of kMany that have seen the end of the work in front of them (it wraps,
+// and is shared by all streams: only the order of its additions matters, never its value)
+__device__ uint32_t seen_before;
+
 // As many clusters as rows (kAll), or as run at once.  The rows with many candidates are dealt
 // to them in turn, each cluster counting them for itself.  Of the rows left over a cluster takes
 // those whose number is its own modulo the number of clusters, so that nobody else changes the
@@ -993,6 +997,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const RowsArgs
   const uint32_t N = gridDim.x / cl.num_blocks(), number = blockIdx.x / cl.num_blocks();
   const float lowest = lowest_of(static_cast<const T *>(a.logits));
   grid_dep_wait();
+  if (a.which == Rows::kMany && threadIdx.x == 0)
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(&seen_before) : "memory");
   grid_dep_launch();
   auto many = [&](uint32_t row) { return !row_of(a, row, lowest).few(); };
   auto left = [&](uint32_t row) { return a.tokens[row] == kLeft; };
@@ -1145,11 +1151,16 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
   if (threadIdx.x < count) mem.list[threadIdx.x] = r.weigh(v, top);
   rank_and_draw(a, row, &mem.few, mem.list, mem.list_id, count, r.top_k, r.top_p, r.u);
 }
-// Runs beside the launch in front of it, which takes the rows with many candidates (and has
-// waited for the work before), and ends after it.
+// Runs beside the launch in front of it, which takes the rows with many candidates, and ends
+// after it.  Its own griddepcontrol.wait comes last, so what orders its reads after the work before
+// both is this: it starts when every CTA of that launch has waited for that work, added to
+// seen_before with release and only then let dependents start; its load of seen_before with
+// acquire therefore takes one of those additions or a later one (additions carry a release on).
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) sample_few_kernel(const RowsArgs a) {
   __shared__ FewMem mem;
+  uint32_t seen;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(&seen_before) : "memory");
   grid_dep_launch();
   few_row<T>(a, mem);
   grid_dep_wait();

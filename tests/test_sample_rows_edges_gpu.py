@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+from channel_b200 import sampling
 from tests.test_sample_rows_gpu import draw, lm_logits, plain, random_settings, settings
 
 gpu = pytest.mark.gpu
@@ -34,3 +35,37 @@ def test_clusters_without_a_row(n):
         token, _, kept = draw(x, u, **full)
         rt, _, rk = plain(x, torch.from_numpy(u).cuda(), 0.0, **settings(n, **full))
         assert np.array_equal(token, rt.cpu().numpy()) and np.array_equal(kept, rk.cpu().numpy())
+
+
+@gpu
+def test_many_rows_in_a_graph():
+    """the launches of a batch of many rows, replayed with other logits and settings that the work
+    just in front of them writes"""
+    n, v = 64, 262144
+    rng = np.random.default_rng(9)
+    kw = random_settings(n, rng)
+    kw["temperature"][:] = np.where(kw["temperature"] == 0, 0, 1.0)
+    s = settings(n, **kw)
+    source = [lm_logits(n, v, seed) for seed in (1, 2, 3)]
+    heat = [s["temperature"] * f for f in (0.7, 1.0, 1.3)]
+    x, u = torch.empty_like(source[0]), torch.rand(n, device="cuda")
+    x.copy_(source[0])
+    sampling.sample_rows(x, u, **s)
+    torch.cuda.synchronize()
+    graph, new_x, new_t = torch.cuda.CUDAGraph(), source[0].clone(), heat[0].clone()
+    with torch.cuda.graph(graph):
+        x.copy_(new_x)
+        s["temperature"].copy_(new_t)
+        got = sampling.sample_rows(x, u, **s)
+    for i in (0, 1, 2, 1):
+        new_x.copy_(source[i])
+        new_t.copy_(heat[i])
+        graph.replay()
+        rt, _, rk = plain(source[i], u, 0.0, **{**s, "temperature": heat[i]})
+        assert torch.equal(got[0].long(), rt) and torch.equal(got[2].long(), rk)
+        # and without the graph, right behind the copies
+        x.copy_(source[(i + 1) % 3])
+        s["temperature"].copy_(heat[i])
+        now = sampling.sample_rows(x, u, **s)
+        rt, _, rk = plain(source[(i + 1) % 3], u, 0.0, **{**s, "temperature": heat[i]})
+        assert torch.equal(now[0].long(), rt) and torch.equal(now[2].long(), rk)
