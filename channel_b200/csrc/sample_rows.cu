@@ -129,6 +129,12 @@ CH_DEV void answer(const RowsArgs &a, uint32_t row, int32_t token, float logprob
   if (a.logprobs) a.logprobs[row] = logprob;
   if (a.kept) a.kept[row] = kept;
 }
+// A token's place in the order of greedy rows: by its (capped) logit, equal ones by index from the
+// lowest on.  + 0.0f: zeros of either sign are equal, and their bits are not.
+CH_DEV unsigned long long greedy_key(float x, uint32_t token) {
+  const uint32_t bits = __float_as_uint(x + 0.0f), key = bits >> 31 ? ~bits : bits | 0x80000000u;
+  return (unsigned long long)key << 32 | (uint32_t)~token;
+}
 // floor(2^44 e) for 0 <= e <= 1: the mantissa shifted (a conversion to 64 bits is many times slower)
 CH_DEV unsigned long long weight_of(float e) {
   const uint32_t bits = __float_as_uint(e), mant = (bits & 0x7FFFFFu) | 0x800000u;
@@ -792,8 +798,7 @@ CH_DEV void keep_row(const RowsArgs &a, uint32_t row, const Row &r, Shared *s, c
     unsigned long long best = 0;
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
       if (!(e[i] >= low)) continue;
-      const uint32_t bits = __float_as_uint(r.capped(e[i])), key = bits >> 31 ? ~bits : bits | 0x80000000u;
-      best = max(best, (unsigned long long)key << 32 | (uint32_t)~(base + i));
+      best = max(best, greedy_key(r.capped(e[i]), base + i));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -1113,8 +1118,7 @@ CH_DEV void few_row(const RowsArgs &a, FewMem &mem) {
     unsigned long long best = 0;
     each_of(__ballot_sync(0xffffffffu, own >= low), [&](uint32_t i, float v) {
       if (!(v >= low)) return;
-      const uint32_t bits = __float_as_uint(r.capped(v)), key = bits >> 31 ? ~bits : bits | 0x80000000u;
-      best = max(best, (unsigned long long)key << 32 | (uint32_t)~(base + i));
+      best = max(best, greedy_key(r.capped(v), base + i));
     });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));

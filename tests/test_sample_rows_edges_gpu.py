@@ -69,3 +69,21 @@ def test_many_rows_in_a_graph():
         now = sampling.sample_rows(x, u, **s)
         rt, _, rk = plain(source[(i + 1) % 3], u, 0.0, **{**s, "temperature": heat[i]})
         assert torch.equal(now[0].long(), rt) and torch.equal(now[2].long(), rk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("n", [4, 400])
+def test_zeros_of_either_sign_are_equal(n, softcap, dtype):
+    """-0.0 at a lower index than +0.0 as a row's largest logit, greedy and with one kept"""
+    v = 20000
+    x = torch.full((n, v), -1.0)
+    x[:, 17], x[:, 16000] = -0.0, 0.0
+    x[1::2, 17], x[1::2, 16000] = 0.0, -0.0
+    x[2::4, 3:9000] = -0.0
+    want = np.full(n, 17)
+    want[2::4] = 3
+    for kw in (dict(temperature=0.0), dict(top_k=1)):
+        token, _, kept = draw(x.to(dtype), 0.5, softcap, **kw)
+        assert np.array_equal(token, want) and (kept == 1).all()
