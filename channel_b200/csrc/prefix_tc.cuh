@@ -53,12 +53,6 @@ struct PrefixArgs {
 
 CH_DEV float to_f32(__half v) { return __half2float(v); }
 CH_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-// own tokens of stream b, limited to what its table can hold
-CH_DEV uint32_t own_len(const PrefixArgs &a, uint32_t b) {
-  const long long len = a.lens[b];
-  return (uint32_t)min(max(len, 0ll), (long long)a.cols << a.shift);
-}
-
 CH_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -74,10 +68,12 @@ CH_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16 *) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// positions stream b attends to: [lo, hi)
+// positions stream b attends to: [lo, hi).  A length past what the table can hold is cut, but the
+// window still ends where the stream does.  (prefix + table is below 2^32, as is prefix + length.)
 CH_DEV void visible(const PrefixArgs &a, uint32_t b, uint32_t &lo, uint32_t &hi) {
-  hi = a.prefix + own_len(a, b);  // both below 2^31
-  lo = a.window && hi > a.window ? hi - a.window : 0u;
+  const uint32_t len = (uint32_t)max(a.lens[b], 0), end = a.prefix + len;
+  hi = a.prefix + (uint32_t)min((unsigned long long)len, (unsigned long long)a.cols << a.shift);
+  lo = a.window && end > a.window ? min(end - a.window, hi) : 0u;
 }
 // page and row inside it of position j of stream b; -1 when the page is not in the pool
 CH_DEV int32_t page_of(const PrefixArgs &a, uint32_t b, uint32_t j, uint32_t &row) {

@@ -457,7 +457,8 @@ int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
  * page_size a power of two from 8 to 256; dtype (of q, out and both pools) CH_F16 or CH_BF16,
  * sums in f32.  Strides are multiples
  * of 8 elements, q, out and the pools 16-byte aligned.  Positions whose page index is not
- * in [0, n_pages) are left out (status bit 2), as are own positions past table_cols pages.
+ * in [0, n_pages) are left out (status bit 2); own positions past table_cols pages are left
+ * out too (the window still ends at T), a negative length counts as 0.
  * The shared pages are read once for the whole batch.  workspace: at least
  * ch_prefix_attention_workspace(args) bytes (0 when a size is invalid), 16-byte aligned,
  * contents irrelevant; calls that may overlap need one each. */

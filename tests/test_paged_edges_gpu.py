@@ -78,3 +78,29 @@ def test_attention_long_prefix_of_narrow_heads(n, nq, nkv, d, prefix, page, dtyp
             ref, mag = p @ values, p @ values.abs()
             far = (out[b, h * group:(h + 1) * group].double() - ref).abs() - (u * ref.abs() + (u + 2.0 ** -14) * mag)
             assert float(far.max()) <= 1e-7, (b, h)
+
+
+@gpu
+@pytest.mark.parametrize("window", [0, 60, 120, 300])
+@pytest.mark.parametrize("d,prefix", [(128, 200), (256, 200), (64, 0)])
+def test_attention_window_of_a_stream_past_its_table(d, prefix, window):
+    """T counts the tokens that the table cannot hold: the window ends there, and only what the
+    table holds of it is seen"""
+    page, held = 16, 48
+    lens = [100, 48, 1000, 49, 20, 2**31 - 1]
+    q, k, v, pt, table, _ = make(6, prefix, [held] * 6, 4, 2, d, page, torch.float16, seed=window)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attend(q, k, v, pt, table, lens, prefix, window, status=status).cpu().double()
+    u, none = U[torch.float16], 0
+    for b, n in enumerate(lens):
+        lo, hi = max(0, prefix + n - window) if window else 0, prefix + min(n, held)
+        at = [int(pt[i // page]) * page + i % page if i < prefix else
+              int(table[b, (i - prefix) // page]) * page + (i - prefix) % page for i in range(lo, hi)]
+        none += not at
+        for h in range(4):
+            p = torch.softmax(k.flatten(0, 1)[at, h // 2].double() @ q[b, h].double() * d ** -0.5, 0)
+            values = v.flatten(0, 1)[at, h // 2].double()
+            ref, mag = p @ values, p @ values.abs()
+            assert bool(((out[b, h] - ref).abs() <= u * ref.abs() + (u + 2.0 ** -14) * mag + 1e-7).all()), (b, h)
+    assert none == (2 if window else 0)
+    assert int(status.item()) == 0
