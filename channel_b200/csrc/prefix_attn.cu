@@ -54,8 +54,9 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
 //   S^T (16 keys x 8 rows) = K (16 x D) Q^T,   O^T (D x 8 rows) += V^T (D x 16 keys) P^T,
 // with K and V as the 16-row A operand of mma.m16n8k16 (the query rows, at most 8 or 16, are
 // its narrow side) and P^T from S^T by two 8 x 8 register transposes.  P is rounded to the
-// type of V (what the tensor core takes); its sum is kept in f32 before rounding.  The
-// running maximum, in units of log2, is per warp; each cut pair leaves (O, m, l) in the
+// type of V (what the tensor core takes), in f16 times 2^15 (at most 32,768 then), so that
+// weights far below the run's largest one do not fall under the type's least; its sum is kept in
+// f32 before rounding.  The running maximum, in units of log2, is per warp; each cut pair leaves (O, m, l) in the
 // workspace and attend_join_kernel adds the parts.
 //
 // Measured (8 kv heads of 256, two q heads each, with the shared prefix of prefix_tc.cuh beside
@@ -64,6 +65,8 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
 // ones 136 to 141 us (5.8 TB/s), a window of 1,024 68 us; 37 streams of 32 q on 8 kv heads of 128 25 us,
 // 4 streams behind 192 tokens 12 us.  The small ones are the latency of one launch with a join.
 constexpr uint32_t kTile = 16;  // keys
+template <typename T>
+constexpr float kOwnBias = std::is_same<T, __half>::value ? 15.f : 0.f;  // log2 of the factor on P
 template <int D>
 struct Own {
   static constexpr int kWarps = D == 256 ? 6 : 8;
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
         const float m1 = fmaxf(m[r][c], top), ref = m1 == -INFINITY ? 0.f : m1;
         const float keep = exp2_approx(m[r][c] - ref);
         m[r][c] = m1;
-        const float p0 = exp2_approx(s0 - ref), p1 = exp2_approx(s1 - ref);
+        const float below = ref - kOwnBias<T>, p0 = exp2_approx(s0 - below), p1 = exp2_approx(s1 - below);
         l[r][c] = l[r][c] * keep + (p0 + p1);
         s[r][0][c] = p0;
         s[r][0][c + 2] = p1;
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
           for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
           const uint32_t qr = r * 8 + 2 * t4 + c;
           if (qr >= a.group) continue;
-          if (g == 0) pm[qr] = make_float2(m[r][c], sum);
+          if (g == 0) pm[qr] = make_float2(m[r][c] - kOwnBias<T>, sum);
 #pragma unroll
           for (int k = 0; k < kSteps; k++) {
             po[qr * D + 16 * k + g] = o[r][k][c];

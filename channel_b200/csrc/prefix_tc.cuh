@@ -10,8 +10,11 @@
 // and V alone: 16 KB pieces by TMA from the pages (K: a box per page and 64 dims, V: a box
 // per page; 128-byte swizzle) in the order the products take them: K_0, K_1, V_0, K_2, V_1,
 // ...  A softmax thread owns a row: no shuffles.  O is rescaled only when a row's maximum has
-// grown by more than 2^8 since its last scale (P then stays below 2^8, where either type
-// rounds as it does below 1); a row's sum is kept in f32 before P is rounded.
+// grown by more than 2^8 since its last scale; a row's sum is kept in f32 before P is rounded
+// to the type of V, which is what the tensor cores take.  In f16 that loses weights below the
+// type's least, so there m is taken 7 lower (P then reaches 2^15 at most): a weight is
+// off by 2^-11 of itself or 2^-32 of the row's largest, and 32,768 small ones beside one large
+// key by 2^-17 of the whole (unbiased, 2^-10).
 //
 // Bound: HBM.  A key tile of D = 256 is 64 KB, about 2,850 cycles of one SM's share of the
 // bandwidth; its products take 1,024 and its exponentials (16 per SM and cycle) 512, both
@@ -100,6 +103,8 @@ constexpr uint32_t kKeys = 64, kRows = 128;
 constexpr int kTcThreads = 8 * 32, kSoft = 4 * 32;
 constexpr uint32_t kTmemCols = 512, kQCol = 256, kSCol = 384;  // O: columns 0 .. D - 1; S: 384 and 448
 constexpr int kMasks = 16;
+template <typename T>
+constexpr float kPrefixBias = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 
 template <int D>
@@ -449,14 +454,15 @@ CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
         }
       }
       m = m1;
+      const float low = ref - kPrefixBias<T>;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t p[32];
 #pragma unroll
       for (int c = 0; c < 2; c++) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e]), scale2, -ref));
-          const float p1 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e + 1]), scale2, -ref));
+          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e]), scale2, -low));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(s[c][2 * e + 1]), scale2, -low));
           sum[e & 1] += p0;
           sum[2 + (e & 1)] += p1;
           p[c * 16 + e] = pack2(p0, p1, static_cast<const T *>(nullptr));
@@ -493,7 +499,7 @@ CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     ok = __all_sync(0xffffffffu, ok && !abort_flag);
     if (ok) {
       const size_t at = ((size_t)split * a.nkv + h) * rows + gr;
-      if (gr < rows) w.ml[at] = make_float2(m, l);
+      if (gr < rows) w.ml[at] = make_float2(m - kPrefixBias<T>, l);
       {
         float *po = w.o + at * D;
 #pragma unroll 1

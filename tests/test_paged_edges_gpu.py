@@ -1,10 +1,12 @@
 """Page plans, page writes and shared-prefix attention at the ends of their documented ranges."""
 import ctypes
+import math
 
 import pytest
 import torch
 
 from channel_b200 import _lib as L
+from channel_b200 import paged
 from tests.test_paged_gpu import U, attend, attn_args, check, make
 
 gpu = pytest.mark.gpu
@@ -104,3 +106,31 @@ def test_attention_window_of_a_stream_past_its_table(d, prefix, window):
             assert bool(((out[b, h] - ref).abs() <= u * ref.abs() + (u + 2.0 ** -14) * mag + 1e-7).all()), (b, h)
     assert none == (2 if window else 0)
     assert int(status.item()) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sink", [15.0, 16.0, 17.0, 17.5, 19.0])
+@pytest.mark.parametrize("n,heads,d,prefix,own", [(2, 64, 64, 32768, 0), (64, 8, 128, 0, 2000), (33, 8, 256, 5000, 900)])
+def test_attention_flat_keys_beside_a_large_one(n, heads, d, prefix, own, sink, dtype):
+    """One key takes nearly all the weight and has V = 0, so the output is the small weights' part,
+    which f16 holds only with its exponent moved.  Weights are off by u of themselves or, under
+    the least normal f16 (P moved by 7 or more places, rounded to 2^-24), by 2^-32 of the largest:
+    |out - ref| <= u |ref| + (u + 2^-14) sum p|v| / sum p + 2^-32 sum |v| / sum p."""
+    page, u = 64, U[dtype]
+    shared, mine = -(-prefix // page), -(-own // page)
+    k = torch.zeros(shared + n * mine, page, heads, d, dtype=dtype, device="cuda")
+    v = torch.full_like(k, 16.0)
+    first = [0] if prefix else [b * mine for b in range(n)]
+    k[first, 3, :, 0] = sink
+    v[first, 3] = 0.0
+    q = torch.zeros(n, heads, d, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    table = (shared + torch.arange(n * mine, dtype=torch.int32, device="cuda")).view(n, mine)
+    pt, lens = torch.arange(shared, dtype=torch.int32, device="cuda"), torch.full((n,), own, dtype=torch.int32, device="cuda")
+    out = paged.prefix_attention(q, k, v, table, lens, pt, prefix, scale=1.0).double()
+    count, p = prefix + own - 1, math.exp(-sink)
+    whole = 1 + count * p
+    ref = 16.0 * count * p / whole
+    bound = u * ref + (u + 2.0 ** -14) * ref + 2.0 ** -32 * 16 * count / whole
+    assert float((out - ref).abs().max()) <= bound
