@@ -334,8 +334,10 @@ int kv_write(const ch_kv_write_args *p, void *stream) {
     return set_last_error(CH_EINVAL, "paged_kv_write: head_dim must be a multiple of 8 up to 1024, n_kv at most 1024");
   if (p->page_size == 0 || (p->page_size & (p->page_size - 1)) || p->page_size > 65536)
     return set_last_error(CH_EINVAL, "paged_kv_write: page_size must be a power of two up to 65536");
-  if ((p->k_token_stride | p->k_head_stride | p->v_token_stride | p->v_head_stride | p->page_stride | p->token_stride |
-       p->head_stride) & 7)
+  // (the stride of a dimension of one element is never used, and may be any number)
+  const int64_t tokens = p->n_tokens > 1 ? p->k_token_stride | p->v_token_stride : 0;
+  const int64_t heads = p->n_kv > 1 ? p->k_head_stride | p->v_head_stride | p->head_stride : 0;
+  if ((tokens | heads | (p->n_pages > 1 ? p->page_stride : 0) | (p->page_size > 1 ? p->token_stride : 0)) & 7)
     return set_last_error(CH_EINVAL, "paged_kv_write: strides must be multiples of 8 elements");
   if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->k_pool | (uintptr_t)p->v_pool) & 15)
     return set_last_error(CH_EINVAL, "paged_kv_write: k, v and the pools must be 16-byte aligned");

@@ -669,8 +669,10 @@ int prefix_attention(const ch_prefix_attn_args *p, void *workspace, size_t bytes
   if (!p->q || !p->out || !p->k_pool || !p->v_pool || !p->lens || (p->prefix_len && !p->prefix_table) ||
       (p->table_cols && !p->table))
     return set_last_error(CH_EINVAL, "prefix_attention: NULL argument");
-  if ((p->q_stream_stride | p->q_head_stride | p->out_stream_stride | p->out_head_stride | p->page_stride |
-       p->token_stride | p->head_stride) & 7)
+  // (the stride of a dimension of one element is never used, and may be any number)
+  const int64_t streams = p->n_streams > 1 ? p->q_stream_stride | p->out_stream_stride : 0;
+  const int64_t heads = (p->n_q > 1 ? p->q_head_stride | p->out_head_stride : 0) | (p->n_kv > 1 ? p->head_stride : 0);
+  if ((streams | heads | (p->n_pages > 1 ? p->page_stride : 0) | p->token_stride) & 7)
     return set_last_error(CH_EINVAL, "prefix_attention: strides must be multiples of 8 elements");
   if (((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->k_pool | (uintptr_t)p->v_pool) & 15)
     return set_last_error(CH_EINVAL, "prefix_attention: q, out and the pools must be 16-byte aligned");

@@ -65,7 +65,7 @@ def _vec(t: torch.Tensor, n: int, at: int, name: str) -> int:
 def _table(t: torch.Tensor, n: int, at: int, name: str) -> int:
     """Pointer of an int32 table of n rows, dense along a row, on device `at`."""
     if t.dtype is not _I32 or t.dim() != 2 or t.get_device() != at or t.shape[0] != n or \
-            (t.stride(1) != 1 and t.numel() > 1):
+            (t.stride(1) != 1 and t.shape[1] > 1 and n > 0):
         _fail(f"{name}: an int32 table of {n} rows, dense along a row, on the other tensors' device is wanted")
     return t.data_ptr()
 

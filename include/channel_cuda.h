@@ -435,7 +435,7 @@ int ch_page_plan(const ch_page_plan_args *args, void *stream);
  * its tensor) into the pages: row t goes to slots[t]; a negative slot is skipped, one past
  * n_pages * page_size too (status bit 1).  Slots of one call are distinct.  src_dtype
  * CH_F32 (rounded to nearest) or dst_dtype; dst_dtype CH_F16 or CH_BF16.  Strides are
- * multiples of 8 elements, k, v and the pools 16-byte aligned, head_dim % 8 == 0. */
+ * multiples of 8 elements (any number where the dimension is 1), k, v and the pools 16-byte aligned, head_dim % 8 == 0. */
 typedef struct {
   const void *k, *v;
   void *k_pool, *v_pool;
@@ -455,8 +455,8 @@ int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
  * q / out element (b, head, d) at b * stream_stride + head * head_stride + d.
  * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096;
  * page_size a power of two from 8 to 256; dtype (of q, out and both pools) CH_F16 or CH_BF16,
- * sums in f32.  Strides are multiples
- * of 8 elements, q, out and the pools 16-byte aligned.  Positions whose page index is not
+ * sums in f32.  Strides are multiples of 8
+ * elements (any number where the dimension is 1), q, out and the pools 16-byte aligned.  Positions whose page index is not
  * in [0, n_pages) are left out (status bit 2); own positions past table_cols pages are left
  * out too (the window still ends at T), a negative length counts as 0.
  * The shared pages are read once for the whole batch.  workspace: at least

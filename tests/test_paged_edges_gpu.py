@@ -134,3 +134,40 @@ def test_attention_flat_keys_beside_a_large_one(n, heads, d, prefix, own, sink, 
     ref = 16.0 * count * p / whole
     bound = u * ref + (u + 2.0 ** -14) * ref + 2.0 ** -32 * 16 * count / whole
     assert float((out - ref).abs().max()) <= bound
+
+
+def odd_strides(t):
+    """t with an odd stride wherever a dimension is 1 (never used; torch may give any number there)"""
+    return t.as_strided(t.shape, [2 * i + 3 if n == 1 else s for i, (n, s) in enumerate(zip(t.shape, t.stride()))])
+
+
+@gpu
+@pytest.mark.parametrize("n,nq,nkv,pages_of_one", [(1, 1, 1, True), (1, 4, 2, False), (3, 1, 1, False), (5, 4, 1, True)])
+def test_strides_of_dimensions_of_one(n, nq, nkv, pages_of_one):
+    d, page, lens = 64, 64, [7] + [0] * (n - 1)
+    q, k, v, pt, table, lens = make(n, 0, lens, nq, nkv, d, page, torch.float16)
+    if pages_of_one:  # a pool of one page
+        k, v, table = k[table[0, :1].long()], v[table[0, :1].long()], torch.zeros_like(table)
+    dev = [t.cuda() for t in (q, k, v, table)]
+    own = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = paged.prefix_attention(*dev, own)
+    out = paged.prefix_attention(*map(odd_strides, dev), own, out=odd_strides(torch.zeros_like(dev[0])))
+    assert torch.equal(out, ref) and float(out[0].abs().max()) > 0
+    new = torch.randn(n, nkv, d, device="cuda")
+    slots = torch.arange(10, 10 + n, dtype=torch.int32, device="cuda")
+    for pools in (dev[1:3], [t.flatten(0, 1)[:, None] for t in dev[1:3]]):  # pages of 64, of one token
+        one = [t.clone() for t in pools]
+        two = [t.clone() for t in pools]
+        paged.kv_write(new, new, slots, *one)
+        paged.kv_write(odd_strides(new), odd_strides(new), slots, *map(odd_strides, two))
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(one, two))
+        assert torch.equal(one[0].flatten(0, 1)[10:10 + n], new.half())
+
+
+@gpu
+def test_plan_of_a_table_of_one_column():
+    lens, new = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3, 16], [1, 1, 0]))
+    table = torch.full((3, 1), 9, dtype=torch.int32, device="cuda")
+    free = torch.tensor([5, 6], dtype=torch.int32, device="cuda")
+    plan = paged.plan_pages(lens, new, odd_strides(table), free, 16, 2)
+    assert table[:, 0].tolist() == [5, 9, 9] and plan.slots.tolist() == [80, 147]
