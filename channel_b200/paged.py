@@ -25,6 +25,7 @@ from . import _lib as L
 
 _DTYPES = {torch.float32: L.CH_F32, torch.float16: L.CH_F16, torch.bfloat16: L.CH_BF16}
 _I32 = torch.int32
+_F32_MAX = torch.finfo(torch.float32).max
 _NO_PAGES, _BAD = 1 << 5, (1 << 1) | (1 << 2)
 
 # A step makes these calls once per layer, so their host time counts: the argument records
@@ -52,6 +53,14 @@ class PagePlan(NamedTuple):
 
 def _fail(msg: str):
     raise L.ChannelError(L.CH_EINVAL, msg)
+
+
+def _pack(record: struct.Struct, what: str, *values) -> bytes:
+    """The packed record; ChannelError for a value that its field does not hold."""
+    try:
+        return record.pack(*values)
+    except struct.error as e:
+        _fail(f"{what}: an argument is out of range ({e})")
 
 
 def _vec(t: torch.Tensor, n: int, at: int, name: str) -> int:
@@ -114,11 +123,11 @@ def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor
     """Block tables (``table``, in place), slot map, positions and row map of a step that
     appends ``new_tokens`` to streams holding ``lens`` tokens; pages come from the front of
     ``free_pages`` (``counts[1]`` of them)."""
-    at, n = _device(lens), lens.shape[0]
+    at, n = _device(lens), lens.numel()
     p_lens, p_new = _vec(lens, n, at, "lens"), _vec(new_tokens, n, at, "new_tokens")
     p_free, p_table = _vec(free_pages, -1, at, "free_pages"), _table(table, n, at, "table")
-    if max_tokens < 0 or prefix_len < 0 or page_size < 0:
-        _fail("plan_pages: negative size")
+    if not 0 <= max_tokens < 1 << 31 or prefix_len < 0 or page_size < 0:
+        _fail("plan_pages: a size is negative or 2^31 or more")
     pad = -max_tokens & 3  # the token arrays start on 16 bytes
     buf = lens.new_empty(3 * (max_tokens + pad) + 2 * n + 3)
     if pad:
@@ -128,9 +137,9 @@ def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor
         slots, positions, rows, lens_out, starts, counts = torch.unsafe_split_with_sizes(
             buf, (max_tokens, max_tokens, max_tokens, n, n + 1, 2))
     p, step = buf.data_ptr(), 4 * (max_tokens + pad)
-    args = _PLAN.pack(p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step, p + 2 * step,
-                      p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
-                      max_tokens, prefix_len, _status(status, at))
+    args = _pack(_PLAN, "plan_pages", p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step,
+                 p + 2 * step, p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
+                 max_tokens, prefix_len, _status(status, at))
     _run(L.load().ch_page_plan, at, args)
     return PagePlan(table, lens_out, starts, slots, positions, rows, counts)
 
@@ -149,15 +158,14 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pool: torc
     slots[t] of the pools; negative slots are skipped."""
     at = k.get_device()
     (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
-    shape, kind = k.shape, k.dtype
-    (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
+    shape, kind, k_strides, v_strides = k.shape, k.dtype, k.stride(), v.stride()
     if len(shape) != 3 or shape != v.shape or shape[1] != n_kv or shape[2] != dim or kind is not v.dtype or \
-            v.get_device() != at or k1 != 1 or v1 != 1:
+            v.get_device() != at or k_strides[2] != 1 or v_strides[2] != 1:
         _fail("kv_write: k and v are [tokens, n_kv, head_dim] of one type, dense in the last dimension")
     _device(k)
-    args = _WRITE.pack(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _vec(slots, shape[0], at, "slots"),
-                       kt, kh, vt, vh, ps, ts, hs, shape[0], n_kv, dim, page, pages, _DTYPES.get(kind, -1),
-                       _DTYPES.get(k_pool.dtype, -1), _status(status, at))
+    args = _pack(_WRITE, "kv_write", k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                 _vec(slots, shape[0], at, "slots"), k_strides[0], k_strides[1], v_strides[0], v_strides[1], ps, ts, hs,
+                 shape[0], n_kv, dim, page, pages, _DTYPES.get(kind, -1), _DTYPES.get(k_pool.dtype, -1), _status(status, at))
     _run(L.load().ch_paged_kv_write, at, args)
 
 
@@ -177,9 +185,9 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     n, n_q, _ = shape
     if prefix_len < 0 or window < 0:
         _fail("prefix_attention: negative size")
+    p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
     if prefix_len and (prefix_table is None or prefix_table.shape[0] * page < prefix_len):
         _fail("prefix_attention: prefix_table is shorter than prefix_len")
-    p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
     p_table, p_lens = _table(table, n, at, "table"), _vec(lens, n, at, "lens")
     if out is None:
         out = torch.empty_like(q)
@@ -187,9 +195,13 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
         _fail("prefix_attention: out is like q")
     _device(q)
     (qs, qh, _), (os, oh, _) = q.stride(), out.stride()
-    args = _ATTEND.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_prefix, p_table, p_lens, qs,
-                        qh, os, oh, ps, ts, hs, table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1], prefix_len,
-                        window, dim ** -0.5 if scale is None else scale, _DTYPES.get(kind, -1), _status(status, at))
+    if scale is None:
+        scale = dim ** -0.5
+    elif not abs(scale) <= _F32_MAX:  # packing would make it infinite
+        _fail("prefix_attention: scale is out of range")
+    args = _pack(_ATTEND, "prefix_attention", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_prefix,
+                 p_table, p_lens, qs, qh, os, oh, ps, ts, hs, table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1],
+                 prefix_len, window, scale, _DTYPES.get(kind, -1), _status(status, at))
     lib = L.load()
     need = lib.ch_prefix_attention_workspace(args)
     if need:  # torch's caching allocator hands the workspace out in the stream's order

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from channel_b200 import _lib as L
-from channel_b200 import paged
+from channel_b200 import paged, sampling
 from tests.test_paged_gpu import U, attend, attn_args, check, make
 
 gpu = pytest.mark.gpu
@@ -171,3 +171,42 @@ def test_plan_of_a_table_of_one_column():
     free = torch.tensor([5, 6], dtype=torch.int32, device="cuda")
     plan = paged.plan_pages(lens, new, odd_strides(table), free, 16, 2)
     assert table[:, 0].tolist() == [5, 9, 9] and plan.slots.tolist() == [80, 147]
+
+
+# ---- what the wrappers refuse, always as a ChannelError -----------------------------------------
+
+
+def test_wrappers_refuse_other_dimensions():
+    z, i = torch.zeros, torch.int32
+    pool, k, slots = z(4, 16, 2, 64, dtype=torch.float16), z(5, 2, 64, dtype=torch.float16), z(5, dtype=i)
+    for args in [(k[0], k[0], slots, pool, pool), (k, k[0], slots, pool, pool), (k[None], k[None], slots, pool, pool),
+                 (k, k, slots, pool[0], pool[0]), (k, k, z((), dtype=i), pool, pool)]:
+        with pytest.raises(L.ChannelError):
+            paged.kv_write(*args)
+    q, table, lens = z(3, 4, 64, dtype=torch.float16), z(3, 2, dtype=i), z(3, dtype=i)
+    for args, kw in [((q[0], pool, pool, table, lens), {}), ((q, pool, pool, table[0], lens), {}),
+                     ((q, pool, pool, table, z((), dtype=i)), {}),
+                     ((q, pool, pool, table, lens), dict(prefix_table=z((), dtype=i), prefix_len=5))]:
+        with pytest.raises(L.ChannelError):
+            paged.prefix_attention(*args, **kw)
+    for args in [(z((), dtype=i), lens, table, lens, 16, 4), (lens, lens, table, z((), dtype=i), 16, 4)]:
+        with pytest.raises(L.ChannelError):
+            paged.plan_pages(*args)
+
+
+@gpu
+def test_wrappers_refuse_sizes_that_no_field_holds():
+    def z(*shape, dtype=torch.int32):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+    pool, q = z(4, 16, 2, 64, dtype=torch.float16), z(3, 4, 64, dtype=torch.float16)
+    table, lens = z(3, 2), z(3)
+    for kw in (dict(window=1 << 32), dict(window=0.5), dict(scale=1e300)):
+        with pytest.raises(L.ChannelError, match="out of range"):
+            paged.prefix_attention(q, pool, pool, table, lens, **kw)
+    for args in [(lens, lens, table, lens, 1 << 32, 4), (lens, lens, table, lens, 16, 4, 1 << 32),
+                 (lens, lens, table, lens, 16, 1 << 40), (z(()), lens, table, lens, 16, 4), (z(()), z(()), table, lens, 16, 4),
+                 (z(3, 1), z(3, 1), table, lens, 16, 4)]:
+        with pytest.raises(L.ChannelError):
+            paged.plan_pages(*args)
+    with pytest.raises(L.ChannelError, match="out of range"):
+        sampling.sample_rows(z(2, 9, dtype=torch.float32), z(2, dtype=torch.float32), softcap=1e300)
