@@ -11,7 +11,8 @@ second one with the same strides.  A decode step of many streams is
     tokens, _, _ = sampling.sample_rows(logits, uniform, ...)                     # once per step
 
 Every call runs on torch's current stream of the tensors' device and returns without
-waiting for it.  ``status`` (int32 tensor of one element, optional) collects the bits of
+waiting for it; none has a backward pass, and a tensor that requires a gradient is refused
+unless gradients are off.  ``status`` (int32 tensor of one element, optional) collects the bits of
 ch_ctx_device_status that the kernels report; ``check_status`` raises on them.
 """
 from __future__ import annotations
@@ -61,6 +62,12 @@ def _pack(record: struct.Struct, what: str, *values) -> bytes:
         return record.pack(*values)
     except struct.error as e:
         _fail(f"{what}: an argument is out of range ({e})")
+
+
+def _no_graph(*tensors: torch.Tensor) -> None:
+    """The operators have no backward pass: no tensor may ask for one."""
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+        _fail("a tensor requires a gradient, and the call has none: detach it or use torch.no_grad()")
 
 
 def _vec(t: torch.Tensor, n: int, at: int, name: str) -> int:
@@ -158,6 +165,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pool: torc
     slots[t] of the pools; negative slots are skipped."""
     at = k.get_device()
     (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
+    _no_graph(k, v, k_pool, v_pool)
     shape, kind, k_strides, v_strides = k.shape, k.dtype, k.stride(), v.stride()
     if len(shape) != 3 or shape != v.shape or shape[1] != n_kv or shape[2] != dim or kind is not v.dtype or \
             v.get_device() != at or k_strides[2] != 1 or v_strides[2] != 1:
@@ -179,6 +187,7 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     defaults to head_dim ** -0.5."""
     at = q.get_device()
     (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
+    _no_graph(q, k_pool, v_pool)
     shape, kind = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != dim or kind is not k_pool.dtype or q.stride(2) != 1:
         _fail("prefix_attention: q is [streams, n_q, head_dim] of the pools' type, dense in the last dimension")

@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .paged import _DTYPES, _F32_MAX, _device, _fail, _pack, _run
+from .paged import _DTYPES, _F32_MAX, _device, _fail, _no_graph, _pack, _run
 
 _ROWS = struct.Struct("@9Pq2Ifi")  # ChSampleRowsArgs of _lib
 _F32, _I32 = torch.float32, torch.int32
@@ -36,7 +36,7 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
     were kept (int32), one each per row of logits ``[rows, vocab]`` (f32, f16 or bf16; rows
     may be strided).  uniform: float32 in [0, 1) per row.  Settings are tensors of one value
     per row (top_k int32, the rest float32) or None; temperature <= 0 takes the largest
-    logit."""
+    logit.  There is no backward pass."""
     shape = logits.shape
     if len(shape) != 2:
         _fail("sample_rows: logits is [rows, vocab]")
@@ -47,6 +47,7 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
         _fail("sample_rows: uniform is needed")
     if not abs(softcap) <= _F32_MAX:  # packing would make it infinite
         _fail("sample_rows: softcap is out of range")
+    _no_graph(logits)
     at = logits.get_device()
     p_uniform, p_temp = _per_row(uniform, _F32, n, at, "uniform"), _per_row(temperature, _F32, n, at, "temperature")
     p_top_p, p_min_p = _per_row(top_p, _F32, n, at, "top_p"), _per_row(min_p, _F32, n, at, "min_p")

@@ -210,3 +210,22 @@ def test_wrappers_refuse_sizes_that_no_field_holds():
             paged.plan_pages(*args)
     with pytest.raises(L.ChannelError, match="out of range"):
         sampling.sample_rows(z(2, 9, dtype=torch.float32), z(2, dtype=torch.float32), softcap=1e300)
+
+
+def test_wrappers_refuse_tensors_that_require_gradients():
+    z, i = torch.zeros, torch.int32
+    pool, k, q = (z(*s, dtype=torch.float16) for s in ((4, 16, 2, 64), (5, 2, 64), (3, 4, 64)))
+    slots, table, lens = z(5, dtype=i), z(3, 2, dtype=i), z(3, dtype=i)
+    x, u = z(2, 9), z(2)
+
+    def g(t):
+        return t.clone().requires_grad_()
+    for call in (lambda: paged.kv_write(g(k), k, slots, pool, pool), lambda: paged.kv_write(k, g(k), slots, pool, pool),
+                 lambda: paged.kv_write(k, k, slots, pool, g(pool)), lambda: sampling.sample_rows(g(x), u),
+                 lambda: paged.prefix_attention(g(q), pool, pool, table, lens),
+                 lambda: paged.prefix_attention(q, g(pool), pool, table, lens),
+                 lambda: paged.prefix_attention(q, pool, g(pool), table, lens)):
+        with pytest.raises(L.ChannelError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(L.ChannelError, match="device"):  # these are on the CPU
+            call()
