@@ -20,7 +20,7 @@ enum DevError : uint32_t {
   DEV_ERR_BAD_LIST = 1u << 2,
   DEV_ERR_PEER_TIMEOUT = 1u << 3,
   DEV_ERR_SCALE_RANGE = 1u << 4,  // a Q4 block scale outside the tensor-core GEMM's exact range
-  DEV_ERR_NO_PAGES = 1u << 5,     // a page plan ran out of free pages, table columns or token rows
+  DEV_ERR_NO_PAGES = 1u << 5,     // a page plan ran out of free pages, table columns, token rows or numbers
 };
 
 

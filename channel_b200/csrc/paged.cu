@@ -67,7 +67,8 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const PlanArgs a) {
     len = max(len, 0ll), add = max(add, 0ll);
     const uint32_t have = pages_for(len, a.shift), after = min(pages_for(len + add, a.shift), a.cols);
     take = after > have ? after - have : 0u;
-    return neg || pages_for(len + add, a.shift) > a.cols;
+    // (the new length, and the last position one below prefix + length, have to fit 31 bits)
+    return neg || pages_for(len + add, a.shift) > a.cols || len + add + max(a.prefix_len, 1u) > 1ll << 31;
   };
   unsigned long long tok = 0, pg = 0;
   bool odd = false;
@@ -167,7 +168,13 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const PlanArgs a) {
           page = r < a.n_free ? a.free_pages[r] : -1;
         }
       }
-      if (page >= 0) slot[j] = to_i32(((long long)page << a.shift) + (i & mask));
+      if (page >= 0) {
+        const long long at = ((long long)page << a.shift) + (i & mask);
+        if (at <= 0x7FFFFFFFll)
+          slot[j] = (int32_t)at;
+        else if (a.status)  // no slot number for it
+          atomicOr(a.status, DEV_ERR_NO_PAGES);
+      }
       pos[j] = to_i32(i + a.prefix_len);
       row[j] = (int32_t)b;
     }

@@ -117,7 +117,7 @@ def check_status(status: torch.Tensor) -> None:
     bits = int(status.item())
     status.zero_()
     if bits & _NO_PAGES:
-        raise L.ChannelError(L.CH_ENOMEM, "a page plan ran out of pages, table columns or token rows")
+        raise L.ChannelError(L.CH_ENOMEM, "a page plan ran out of pages, table columns, token rows or slot numbers")
     if bits & _BAD:
         raise L.ChannelError(L.CH_EDEVICE, "a kernel saw a slot or page outside its pool")
     if bits:

@@ -58,7 +58,7 @@ void *ch_ctx_stream(ch_ctx *ctx); /* cudaStream_t */
 /* Reads and clears the device status word (bit 0 bulk-copy wait timeout,
  * bit 1 bad slot, bit 2 bad slot-list entry, bit 3 peer wait timeout, bit 4 a Q4
  * block scale with |d| >= 16, outside the tensor-core GEMM's exact range, bit 5 a page
- * plan that ran out of pages, table columns or token rows). */
+ * plan that ran out of pages, table columns, token rows or slot numbers). */
 int ch_ctx_device_status(ch_ctx *ctx, uint32_t *flags);
 
 /* ------------------------------------------------------------------------
@@ -419,9 +419,10 @@ typedef enum { CH_F32 = 0, CH_F16 = 1, CH_BF16 = 2 } ch_dtype;
  *   slots, positions, rows [max_tokens]  per packed token: page * page_size + offset,
  *              prefix_len + index in the stream, stream; -1 past the total
  *   counts     [2]             packed tokens, pages taken
- * Status bit 5: the pages, the table's columns or max_tokens did not suffice, or a length
- * was negative (taken as 0).  A missing page is -1 in the table and its tokens' slots are
- * -1, which ch_paged_kv_write skips; counts[1] still says how many pages were needed. */
+ * Status bit 5: the pages, the table's columns or max_tokens did not suffice, a length
+ * was negative (taken as 0), or a slot or position is 2^31 or more.  A missing page is -1 in
+ * the table, and its tokens' slots are -1, which ch_paged_kv_write skips; so are slots of 2^31
+ * and more, and positions end at 2^31 - 1.  counts[1] still says how many pages were needed. */
 typedef struct {
   const int32_t *lens, *new_tokens, *free_pages;
   int32_t *table, *lens_out, *starts, *slots, *positions, *rows, *counts;

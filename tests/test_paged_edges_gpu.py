@@ -229,3 +229,31 @@ def test_wrappers_refuse_tensors_that_require_gradients():
             call()
         with torch.no_grad(), pytest.raises(L.ChannelError, match="device"):  # these are on the CPU
             call()
+
+
+# ---- page plan ----------------------------------------------------------------------------------
+
+
+@gpu
+def test_plan_of_slots_past_31_bits():
+    """a page whose tokens have no slot number below 2^31: not written, and reported"""
+    def ints(*x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+    top = (1 << 27) - 1  # the last page of 16 with slots below 2^31
+    for first, new, slots, bad in (([3, top], 18, [*range(48, 64), 2**31 - 16, 2**31 - 15], False),
+                                   ([top, top + 1], 18, [*range(2**31 - 16, 2**31), -1, -1], True),
+                                   ([2**31 - 1, 0], 17, [-1] * 16 + [0], True)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        table = torch.full((1, 2), -1, dtype=torch.int32, device="cuda")
+        plan = paged.plan_pages(ints(0), ints(new), table, ints(*first), 16, new, status=status)
+        assert plan.slots.tolist() == slots and table.tolist() == [first]
+        assert int(status.item()) == (1 << 5 if bad else 0)
+        # the same page already in the table
+        status.zero_()
+        plan = paged.plan_pages(ints(16), ints(new - 16), ints(5, first[1])[None], ints(first[1]), 16, new - 16, status=status)
+        assert plan.slots.tolist() == slots[16:] and int(status.item()) == (1 << 5 if slots[16] < 0 else 0)
+    for prefix, bad in ((2**31 - 3, False), (2**31 - 2, True)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        plan = paged.plan_pages(ints(0), ints(3), ints(-1)[None], ints(0), 16, 3, prefix, status=status)
+        assert plan.positions.tolist() == [min(prefix + i, 2**31 - 1) for i in range(3)]
+        assert int(status.item()) == (1 << 5 if bad else 0)
