@@ -21,7 +21,7 @@ import torch
 
 from . import _lib as L
 from .engine import GpuContext
-from .paged import PagePlan, check_status, kv_write, plan_pages, prefix_attention
+from .paged import PagePlan, _fail, check_status, kv_write, plan_pages, prefix_attention
 from .sampling import sample_rows
 
 
@@ -134,6 +134,11 @@ class SharedPromptDecoder:
         """n_tokens tokens for each of `streams` continuations of one prompt (a list of token
         ids), ``[streams, n_tokens]``.  share: the prompt is decoded once and its pages are
         shared; otherwise every stream holds a copy of its own."""
+        prompt = [int(t) for t in prompt]
+        if streams < 1 or n_tokens < 1 or not prompt:
+            _fail("decode: a stream, a token of the prompt and a token to decode are wanted at least")
+        if min(prompt) < 0 or max(prompt) >= self.shape.vocab:  # an index past the table is a fault on the device
+            _fail(f"decode: token ids are 0..{self.shape.vocab - 1}")
         with torch.cuda.stream(self.stream), torch.no_grad():
             g = torch.Generator(self.device).manual_seed(seed)
             self.free = torch.arange(self.max_pages, dtype=torch.int32, device=self.device)
