@@ -6,7 +6,8 @@ layer order (input norm, q|k|v, per-head RoPE at the token's position, attention
 residual, pre-FFN norm, GELU gate * up, down, residual; src/model/forward.zig:49-230) whose
 K/V caches are pages.  The prompt is decoded once, into the pages of a first stream; those
 pages then become the shared prefix of a batch of streams, each of which owns only the pages
-of its own tokens.  All work runs on the context's stream.
+of its own tokens.  All work runs on the context's stream; a step called from another torch
+stream is ordered after that stream's work, and what follows there after the step.
 
     python -m channel_b200.shared_prompt [--streams N] [--prompt N] [--tokens N]
 """
@@ -110,6 +111,17 @@ class SharedPromptDecoder:
     def step(self, tokens: torch.Tensor, plan: PagePlan, prefix_table=None, prefix_len: int = 0) -> torch.Tensor:
         """Logits ``[streams, vocab]`` of one token per stream, placed by plan (made for one
         new token per stream)."""
+        caller = torch.cuda.current_stream(self.device)
+        if caller == self.stream:
+            return self._step(tokens, plan, prefix_table, prefix_len)
+        self.stream.wait_stream(caller)
+        with torch.cuda.stream(self.stream):
+            logits = self._step(tokens, plan, prefix_table, prefix_len)
+        caller.wait_stream(self.stream)
+        logits.record_stream(caller)
+        return logits
+
+    def _step(self, tokens: torch.Tensor, plan: PagePlan, prefix_table, prefix_len: int) -> torch.Tensor:
         s, n = self.shape, tokens.shape[0]
         x = self.embed[tokens.long()] * math.sqrt(s.hidden)
         for layer, w in enumerate(self.layers):

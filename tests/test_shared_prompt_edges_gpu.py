@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from channel_b200 import _lib as L
+from channel_b200.paged import plan_pages
 from channel_b200.shared_prompt import DecoderShape, SharedPromptDecoder
 
 
@@ -13,3 +14,41 @@ def test_decode_refuses(prompt, streams, n):
     decoder.shape = DecoderShape()
     with pytest.raises(L.ChannelError):
         decoder.decode(prompt, streams, n)
+
+
+@pytest.fixture(scope="module")
+def decoder(ctx):
+    return SharedPromptDecoder(ctx, DecoderShape(), 64)
+
+
+def start(streams, columns=2):
+    """no tokens yet, and free pages"""
+    return (torch.zeros(streams, dtype=torch.int32, device="cuda"),
+            torch.full((streams, columns), -1, dtype=torch.int32, device="cuda"),
+            torch.arange(20, 60, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_a_step_from_another_stream(decoder):
+    """tokens and plan come from work on the caller's stream that takes a while, and the logits are
+    read there"""
+    lens, table, free = start(5)
+    ids = torch.tensor([3, 9, 27, 81, 243], device="cuda")
+    big = torch.randn(8192, 8192, device="cuda")
+
+    def one():
+        late = (big @ big @ big).abs().sum().clamp(max=0).long()  # 0
+        plan = plan_pages(lens, torch.ones_like(lens) + late.int(), table, free, 16, 5)
+        logits = decoder.step(ids + late, plan)
+        return logits.clone()
+    with torch.cuda.stream(decoder.stream):
+        ref = one()
+    decoder.stream.synchronize()
+    for stream in (torch.cuda.default_stream(), torch.cuda.Stream()):
+        decoder.k_pool.zero_(), decoder.v_pool.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            got = one()
+        stream.synchronize()
+        assert torch.equal(got, ref)
+    assert torch.isfinite(ref).all() and int(decoder.status.item()) == 0
