@@ -183,6 +183,8 @@ class SharedPromptDecoder:
                 lens = plan.lens
             result = torch.stack(out, 1)
             check_status(self.status)
+            if int(result.min()) < 0:  # and what followed took another token's embedding
+                raise L.ChannelError(L.CH_EDEVICE, "decode: a row of logits had nothing to choose from (NaN or -inf throughout)")
         self.stream.synchronize()
         return result
 

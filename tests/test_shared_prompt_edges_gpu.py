@@ -52,3 +52,19 @@ def test_a_step_from_another_stream(decoder):
         stream.synchronize()
         assert torch.equal(got, ref)
     assert torch.isfinite(ref).all() and int(decoder.status.item()) == 0
+
+
+@pytest.mark.gpu
+def test_rows_of_nan_are_not_tokens(decoder):
+    """an activation that is not a number ends in an error, not in token -1"""
+    with torch.cuda.stream(decoder.stream):
+        row = decoder.embed[7].clone()
+        decoder.embed[7] = float("nan")
+    try:
+        for share in (True, False):
+            with pytest.raises(L.ChannelError, match="nothing to choose"):
+                decoder.decode([1, 7], 3, 2, share=share)
+    finally:
+        with torch.cuda.stream(decoder.stream):
+            decoder.embed[7] = row
+    assert int(decoder.decode([1, 8], 3, 2).min()) >= 0
