@@ -47,6 +47,16 @@ def test_attention_of_more_prefix_work_than_sms(n, nq, nkv, d, prefix):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nq,nkv,d", [(9, 1, 256), (16, 1, 256), (32, 2, 256), (22, 2, 64), (16, 1, 64), (13, 1, 128)])
+def test_attention_of_many_query_heads_per_kv_head(nq, nkv, d, dtype):
+    """more than 8, with and without a shared prefix, windowed, and one stream alone"""
+    lens = [0, 1, 17, 64, 130, 333, 16]
+    for prefix, window in ((201, 0), (0, 0), (201, 100)):
+        check(*make(7, prefix, lens, nq, nkv, d, 16, dtype, seed=nq), prefix, window)
+    check(*make(1, 100, [700], nq, nkv, d, 32, dtype, seed=nq), 100)
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("n,nq,nkv,d,prefix,page", [
     (3, 4, 2, 64, 9001, 16), (3, 4, 2, 128, 9001, 16), (16, 64, 64, 128, 8000, 32), (16, 64, 64, 64, 7990, 64),
     (64, 16, 8, 128, 32767, 64)])
