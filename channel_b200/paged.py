@@ -56,17 +56,13 @@ def _fail(msg: str):
     raise L.ChannelError(L.CH_EINVAL, msg)
 
 
-def _pack(record: struct.Struct, what: str, *values) -> bytes:
-    """The packed record; ChannelError for a value that its field does not hold."""
-    try:
-        return record.pack(*values)
-    except struct.error as e:
-        _fail(f"{what}: an argument is out of range ({e})")
+def _out_of_range(what: str, why: struct.error):
+    _fail(f"{what}: an argument is out of range ({why})")
 
 
-def _no_graph(*tensors: torch.Tensor) -> None:
-    """The operators have no backward pass: no tensor may ask for one."""
-    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+def _no_graph() -> None:
+    """For a tensor that requires a gradient: the operators have no backward pass."""
+    if torch.is_grad_enabled():
         _fail("a tensor requires a gradient, and the call has none: detach it or use torch.no_grad()")
 
 
@@ -144,9 +140,12 @@ def plan_pages(lens: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor
         slots, positions, rows, lens_out, starts, counts = torch.unsafe_split_with_sizes(
             buf, (max_tokens, max_tokens, max_tokens, n, n + 1, 2))
     p, step = buf.data_ptr(), 4 * (max_tokens + pad)
-    args = _pack(_PLAN, "plan_pages", p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step,
-                 p + 2 * step, p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
-                 max_tokens, prefix_len, _status(status, at))
+    try:
+        args = _PLAN.pack(p_lens, p_new, p_free, p_table, p + 3 * step, p + 3 * step + 4 * n, p, p + step, p + 2 * step,
+                          p + 3 * step + 8 * n + 4, table.stride(0), n, table.shape[1], free_pages.shape[0], page_size,
+                          max_tokens, prefix_len, _status(status, at))
+    except struct.error as e:
+        _out_of_range("plan_pages", e)
     _run(L.load().ch_page_plan, at, args)
     return PagePlan(table, lens_out, starts, slots, positions, rows, counts)
 
@@ -165,15 +164,20 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pool: torc
     slots[t] of the pools; negative slots are skipped."""
     at = k.get_device()
     (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
-    _no_graph(k, v, k_pool, v_pool)
+    if k.requires_grad or v.requires_grad or k_pool.requires_grad or v_pool.requires_grad:
+        _no_graph()
     shape, kind, k_strides, v_strides = k.shape, k.dtype, k.stride(), v.stride()
     if len(shape) != 3 or shape != v.shape or shape[1] != n_kv or shape[2] != dim or kind is not v.dtype or \
             v.get_device() != at or k_strides[2] != 1 or v_strides[2] != 1:
         _fail("kv_write: k and v are [tokens, n_kv, head_dim] of one type, dense in the last dimension")
     _device(k)
-    args = _pack(_WRITE, "kv_write", k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                 _vec(slots, shape[0], at, "slots"), k_strides[0], k_strides[1], v_strides[0], v_strides[1], ps, ts, hs,
-                 shape[0], n_kv, dim, page, pages, _DTYPES.get(kind, -1), _DTYPES.get(k_pool.dtype, -1), _status(status, at))
+    try:
+        args = _WRITE.pack(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                           _vec(slots, shape[0], at, "slots"), k_strides[0], k_strides[1], v_strides[0], v_strides[1], ps,
+                           ts, hs, shape[0], n_kv, dim, page, pages, _DTYPES.get(kind, -1), _DTYPES.get(k_pool.dtype, -1),
+                           _status(status, at))
+    except struct.error as e:
+        _out_of_range("kv_write", e)
     _run(L.load().ch_paged_kv_write, at, args)
 
 
@@ -187,7 +191,8 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     defaults to head_dim ** -0.5."""
     at = q.get_device()
     (pages, page, n_kv, dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
-    _no_graph(q, k_pool, v_pool)
+    if q.requires_grad or k_pool.requires_grad or v_pool.requires_grad:
+        _no_graph()
     shape, kind = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != dim or kind is not k_pool.dtype or q.stride(2) != 1:
         _fail("prefix_attention: q is [streams, n_q, head_dim] of the pools' type, dense in the last dimension")
@@ -208,9 +213,12 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
         scale = dim ** -0.5
     elif not abs(scale) <= _F32_MAX:  # packing would make it infinite
         _fail("prefix_attention: scale is out of range")
-    args = _pack(_ATTEND, "prefix_attention", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_prefix,
-                 p_table, p_lens, qs, qh, os, oh, ps, ts, hs, table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1],
-                 prefix_len, window, scale, _DTYPES.get(kind, -1), _status(status, at))
+    try:
+        args = _ATTEND.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_prefix, p_table, p_lens, qs,
+                            qh, os, oh, ps, ts, hs, table.stride(0), n, n_q, n_kv, dim, page, pages, table.shape[1],
+                            prefix_len, window, scale, _DTYPES.get(kind, -1), _status(status, at))
+    except struct.error as e:
+        _out_of_range("prefix_attention", e)
     lib = L.load()
     need = lib.ch_prefix_attention_workspace(args)
     if need:  # torch's caching allocator hands the workspace out in the stream's order

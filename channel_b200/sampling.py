@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .paged import _DTYPES, _F32_MAX, _device, _fail, _no_graph, _pack, _run
+from .paged import _DTYPES, _F32_MAX, _device, _fail, _no_graph, _out_of_range, _run
 
 _ROWS = struct.Struct("@9Pq2Ifi")  # ChSampleRowsArgs of _lib
 _F32, _I32 = torch.float32, torch.int32
@@ -47,7 +47,8 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
         _fail("sample_rows: uniform is needed")
     if not abs(softcap) <= _F32_MAX:  # packing would make it infinite
         _fail("sample_rows: softcap is out of range")
-    _no_graph(logits)
+    if logits.requires_grad:
+        _no_graph()
     at = logits.get_device()
     p_uniform, p_temp = _per_row(uniform, _F32, n, at, "uniform"), _per_row(temperature, _F32, n, at, "temperature")
     p_top_p, p_min_p = _per_row(top_p, _F32, n, at, "top_p"), _per_row(min_p, _F32, n, at, "min_p")
@@ -58,7 +59,10 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: Option
     logprobs = logprobs.view(_F32)
     if n:
         p = out.data_ptr()
-        _run(L.load().ch_sample_rows, at,
-             _pack(_ROWS, "sample_rows", logits.data_ptr(), p_uniform, p_temp, p_top_p, p_min_p, p_top_k, p, p + 4 * n,
-                   p + 8 * n, row, n, vocab, softcap, _DTYPES.get(logits.dtype, -1)))
+        try:
+            args = _ROWS.pack(logits.data_ptr(), p_uniform, p_temp, p_top_p, p_min_p, p_top_k, p, p + 4 * n, p + 8 * n, row, n,
+                              vocab, softcap, _DTYPES.get(logits.dtype, -1))
+        except struct.error as e:
+            _out_of_range("sample_rows", e)
+        _run(L.load().ch_sample_rows, at, args)
     return tokens, logprobs, kept
