@@ -199,9 +199,7 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
   grid_dep_launch();
 
   // ---- the shared prefix ----
-  const bool with_unit = blockIdx.x < d.unit_ctas;
   bool dead = false;  // a wait gave up
-  if (with_unit && warp == 1) tmem_take(tc_bars);
   for (uint32_t u = blockIdx.x; u < d.units; u += gridDim.x) {
     const uint32_t h = u % a.nkv, rt = (u / a.nkv) % row_tiles, split = u / (a.nkv * row_tiles);
     const uint32_t i0 = split * (ptiles / d.splits) + min(split, ptiles % d.splits);
@@ -210,11 +208,11 @@ __global__ void __launch_bounds__(attend_bound(D, NR), 1)
     const uint32_t rows = a.n * a.group, gr = rt * kRows + tid;
     if (dead && tid < (int)kRows && gr < rows) pp.ml[((size_t)split * a.nkv + h) * rows + gr] = make_float2(0.f, NAN);
   }
-  if (with_unit && warp == 1) tmem_give(tc_bars);
 
   // ---- this warp's run of the streams' own tiles; consecutive runs lie on different SMs, so
   // that few tiles spread over all of them ----
   if (warp >= O::kWarps) return;  // (no barrier of the CTA from here on)
+  const bool with_unit = blockIdx.x < d.unit_ctas;
   const uint32_t run = with_unit ? d.y_runs + warp * d.unit_ctas + blockIdx.x
                                  : warp * (gridDim.x - d.unit_ctas) + blockIdx.x - d.unit_ctas;
   const uint32_t per = with_unit ? d.x : d.y;

@@ -189,22 +189,12 @@ struct TcBars {
   uint32_t issued[13];  // 1 + the last piece on its way to a slot of the ring
 };
 
-// Tensor memory for all units of a CTA, by one whole warp: taken before the first (a CTA that has
-// given up the permit may not allocate again), given back after the last.
-CH_DEV void tmem_take(TcBars &bars) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_slot)),
-               "r"(kTmemCols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-CH_DEV void tmem_give(TcBars &bars) {
-  tc_fence_after();
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars.tmem_slot), "r"(kTmemCols) : "memory");
-}
-
 // One unit: kv head h, row tile rt, key tiles [i0, i0 + nt) of the prefix, whose positions
 // below zlo no stream sees.  Leaves the rows' parts at split `split`; false if it gave up, and
-// then shared memory is not to be used again.  All threads of the CTA call it, after tmem_take by warp 1; sm (1024-byte aligned) is free before and after.
+// then shared memory is not to be used again.  All threads of the CTA call it; sm
+// (1024-byte aligned) is free before and after.  Each unit takes its tensor memory and gives it
+// back, so the CTA keeps the permit to allocate: after giving that up it could not take any for
+// its next unit.  (Taken once around all units, 32,768 shared tokens took 143 us instead of 138.)
 template <typename T, int D>
 CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtensorMap &kmap, const CUtensorMap &vmap,
                         uint8_t *sm, TcBars &bars, uint32_t h, uint32_t rt, uint32_t split, uint32_t i0, uint32_t nt,
@@ -234,6 +224,10 @@ CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
     for (int s = 0; s < C::kSlots; s++) bars.issued[s] = 0u;
     fence_mbar_init();
   }
+  if (warp == 1)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -518,6 +512,10 @@ CH_DEV bool prefix_unit(const PrefixArgs &a, const PrefixParts &w, const CUtenso
   __syncwarp();
   tc_fence_before();
   __syncthreads();  // every role done with tensor memory and the barriers
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
   // what is still on its way to shared memory or the barriers lands (normally long done): the
   // last copy into each slot and, unless a role gave up, the arrivals of the last products
   if (tid < C::kSlots && bars.issued[tid]) {
