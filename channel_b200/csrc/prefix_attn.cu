@@ -61,9 +61,9 @@ CH_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
 //
 // Measured (8 kv heads of 256, two q heads each, with the shared prefix of prefix_tc.cuh beside
 // it in the same launch, and the join): 64 streams of 1 to 1,023 own tokens behind 4,096 shared
-// ones 60 us (303 MB, 5.0 TB/s; a kernel per row 1,648 us), behind 32,768 with 1 to 2,047 own
-// ones 136 to 141 us (5.8 TB/s), a window of 1,024 68 us; 37 streams of 32 q on 8 kv heads of 128 25 us,
-// 4 streams behind 192 tokens 12 us.  The small ones are the latency of one launch with a join.
+// ones 61 to 62 us (303 MB, 4.9 TB/s; a kernel per row 1,648 us), behind 32,768 with 1 to 2,047 own
+// ones 138 to 141 us (5.8 TB/s), a window of 1,024 67 to 70 us; 37 streams of 32 q on 8 kv heads of 128
+// 26 us, 4 streams behind 192 tokens 12 us.  The small ones are the latency of one launch with a join.
 constexpr uint32_t kTile = 16;  // keys
 template <typename T>
 constexpr float kOwnBias = std::is_same<T, __half>::value ? 15.f : 0.f;  // log2 of the factor on P

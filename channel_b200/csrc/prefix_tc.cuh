@@ -20,7 +20,7 @@
 // bandwidth; its products take 1,024 and its exponentials (16 per SM and cycle) 512, both
 // under the loads of the three tiles in the ring.
 //
-// Measured with 64 streams: 4,096 shared tokens 60 us for the whole call, 32,768 136 to 141 us
+// Measured with 64 streams: 4,096 shared tokens 61 to 62 us for the whole call, 32,768 138 to 141 us
 // (805 MB with the streams' own, 5.8 TB/s).  128-key tiles with Q in shared memory, which left no room
 // for a third tile in the ring, took 76 us where this split first took 66; one copy warp needed
 // 3,750 cycles a tile.

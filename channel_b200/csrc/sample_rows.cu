@@ -37,8 +37,8 @@
 // Bound.  For one row the chain of passes, scans and cluster barriers, not HBM.  One row of
 // 262,144 capped f32 logits takes 12 us with top-k 64 and 31 us by top-p alone (58,000 cycles:
 // the cap 7,400, weights and first bins 9,400, a round of the cut 7,000 to 8,000, collecting a
-// bin's tokens 5,000, the kept sum 3,300).  64 such rows of mixed settings take 45 us, where
-// reading them takes 10.4; 48 rows of 100,003 bf16 logits by top-p and min-p 35 us.
+// bin's tokens 5,000, the kept sum 3,300).  64 such rows of mixed settings take 46 to 47 us, where
+// reading them takes 10.4; 48 rows of 100,003 bf16 logits by top-p and min-p 35 to 37 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -1240,11 +1240,11 @@ cudaError_t launch_rows(RowsArgs a, uint32_t rows, cudaStream_t stream) {
     return start_clusters(sample_rows_kernel<T>, a, std::min(rows, running), C, sizeof(Shared), stream);
   };
   // Rows that run at once in the kernel that keeps them (14 of 262,144 logits) all go there: one
-  // launch (8 rows of mixed settings 17.1 us, by the other way 19.3).  More rows: first those with
+  // launch (8 rows of mixed settings 18 us, 2 less than by the other way).  More rows: first those with
   // many candidates, dealt to the clusters that run at once, beside them those with few, then
   // what those left (64 rows: all of them through the first kernel 70 us, so 46).
   if (rows <= running) return launch(Rows::kAll);
-  // Rows with few candidates in clusters of 8, which read faster (48 such rows 28 us, in clusters
+  // Rows with few candidates in clusters of 8, which read faster (48 such rows 28 to 29 us, in clusters
   // of 4 37), or of 4 where 8 leave less than a quarter of the SMs for the rows with many: 64
   // rows, 7 of them with many, take 47 us in clusters of 4, 54 in clusters of 8.
   e = allow((const void *)sample_few_kernel<T>, 0, few, &few_running);
