@@ -101,6 +101,28 @@ class ChSampleRowsArgs(C.Structure):
                [("row_stride", i64), ("n_rows", u32), ("vocab", u32), ("softcap", f32), ("dtype", C.c_int32)]
 
 
+class ChChunkAttnArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "out", "starts", "parents", "k_pool", "v_pool", "prefix_table", "table",
+                                  "lens")] + \
+               [(n, i64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride", "v_token_stride",
+                                   "v_head_stride", "out_token_stride", "out_head_stride", "page_stride", "token_stride",
+                                   "head_stride", "table_stride")] + \
+               [(n, u32) for n in ("n_tokens", "n_streams", "n_q", "n_kv", "head_dim", "page_size", "n_pages", "table_cols",
+                                   "prefix_len", "window")] + \
+               [("scale", f32), ("dtype", C.c_int32), ("status", vp)]
+
+
+class ChAcceptArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("drafted", "parents", "starts", "sampled", "counts", "next", "kept")] + \
+               [("n_tokens", u32), ("n_streams", u32), ("status", vp)]
+
+
+class ChScoreArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "targets", "logprobs", "entropy", "ranks", "top_ids", "top_logprobs")] + \
+               [("row_stride", i64), ("n_rows", u32), ("vocab", u32), ("top", u32), ("softcap", f32), ("dtype", C.c_int32),
+                ("status", vp)]
+
+
 PROGRESS_FN = C.CFUNCTYPE(None, sz, sz, vp)
 
 # name -> (restype, argtypes); every symbol declared in include/channel_cuda.h
@@ -197,6 +219,10 @@ SIGNATURES = {
     "ch_prefix_attention_workspace": (sz, [vp]),
     "ch_prefix_attention": (i32, [vp, vp, sz, vp]),
     "ch_sample_rows": (i32, [vp, vp]),
+    "ch_chunk_attention_workspace": (sz, [vp]),
+    "ch_chunk_attention": (i32, [vp, vp, sz, vp]),
+    "ch_accept_drafts": (i32, [vp, vp]),
+    "ch_score_rows": (i32, [vp, vp]),
 }
 
 _lib = None

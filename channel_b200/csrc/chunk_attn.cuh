@@ -1,0 +1,140 @@
+// chunk_attn.cuh -- what the kernels of ch_chunk_attention share: the arguments, which keys a
+// query row sees, and one row computed on its own by a warp.
+#pragma once
+#include "common.cuh"
+#include "kernels.cuh"
+#include "tcgen05.cuh"
+
+namespace ch {
+
+struct ChunkArgs {
+  const void *q, *k, *v, *k_pool, *v_pool;
+  void *out;
+  const int32_t *starts, *parents, *prefix_table, *table, *lens;
+  long long qs, qh, ks, kh, vs, vh, os, oh;  // token and head strides
+  long long page, token, head, ts;           // pool and table strides
+  uint32_t n_tokens, n, nq, nkv, group, shift, n_pages, cols, prefix, window;
+  float scale;
+  uint32_t *status;
+};
+
+// A stream's new tokens [first, first + count) of the packed rows and its cached ones: `cached` of
+// them can be read (those in the table's columns), `before` positions lie ahead of the new ones.
+struct ChunkStream {
+  uint32_t first, count, cached;
+  long long before;
+};
+CH_DEV ChunkStream chunk_stream(const ChunkArgs &a, uint32_t b) {
+  ChunkStream s;
+  const long long lo = a.starts[b], hi = a.starts[b + 1], top = a.n_tokens;
+  s.first = (uint32_t)min(max(lo, 0ll), top);
+  const uint32_t end = (uint32_t)min(max(hi, 0ll), top);
+  s.count = end > s.first ? end - s.first : 0u;
+  const long long len = a.lens ? max(a.lens[b], 0) : 0;
+  s.cached = (uint32_t)min(len, (long long)a.cols << a.shift);
+  s.before = a.prefix + len;
+  return s;
+}
+// The first visible index of the prefix's, the cached and the new tokens for a row at position
+// `at`; at or past a run's end: none of it.
+struct ChunkLow {
+  uint32_t prefix, cached, fresh;
+};
+CH_DEV ChunkLow chunk_low(const ChunkArgs &a, const ChunkStream &s, long long at) {
+  const long long lo = a.window ? max(at + 1 - (long long)a.window, 0ll) : 0ll;
+  ChunkLow l;
+  l.prefix = (uint32_t)min(lo, (long long)a.prefix);
+  l.cached = (uint32_t)min(max(lo - a.prefix, 0ll), (long long)s.cached);
+  l.fresh = (uint32_t)max(lo - s.before, 0ll);
+  return l;
+}
+// node above node i of the stream whose rows start at `first`, -1 at a root (or where the parent
+// is not an earlier node)
+CH_DEV int32_t chunk_parent(const ChunkArgs &a, uint32_t first, uint32_t i) {
+  const int32_t p = a.parents[first + i];
+  return p >= 0 && (uint32_t)p < i ? p : -1;
+}
+// what the calling CTA's threads see of starts and parents that break the rules, into the status word
+CH_DEV void chunk_report(const ChunkArgs &a) {
+  if (!a.status) return;
+  bool bad = false;
+  for (uint32_t b = threadIdx.x; b < a.n; b += blockDim.x) {
+    const long long lo = a.starts[b], hi = a.starts[b + 1];
+    bad |= lo < 0 || hi < lo || hi > (long long)a.n_tokens;
+    const ChunkStream s = chunk_stream(a, b);
+    for (uint32_t i = 0; a.parents && i < s.count; i++) {
+      const int32_t p = a.parents[s.first + i];
+      bad |= p < -1 || p >= (int32_t)i;
+    }
+  }
+  if (bad) atomicOr(a.status, DEV_ERR_BAD_LIST);
+}
+CH_DEV uint32_t chunk_depth(const ChunkArgs &a, uint32_t first, uint32_t i) {
+  uint32_t d = 0;
+  for (int32_t j = chunk_parent(a, first, i); j >= 0; j = chunk_parent(a, first, (uint32_t)j)) d++;
+  return d;
+}
+
+// out row of new token i of stream s and q head hq, by one warp, key after key from the visible
+// ones only: EPL dims per lane.
+template <typename T, int D>
+__device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s, uint32_t b, uint32_t i, uint32_t hq) {
+  constexpr int EPL = D / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t h = hq / a.group, row = s.first + i;
+  const T *q = static_cast<const T *>(a.q) + row * a.qs + hq * a.qh + lane * EPL;
+  float qr[EPL], o[EPL], m = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[e]), o[e] = 0.f;
+  auto key = [&](const T *k, const T *v) {
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x = fmaf(qr[e], to_f32(k[lane * EPL + e]), x);
+    x = warp_sum(x) * a.scale;
+    if (x == -INFINITY) return;
+    const float m1 = fmaxf(m, x), c = m1 == m ? 1.f : expf(m - m1), p = expf(x - m1);
+    sum = sum * c + p;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = fmaf(p, to_f32(v[lane * EPL + e]), o[e] * c);
+    m = m1;
+  };
+  auto paged = [&](const int32_t *table, uint32_t j) {
+    const int32_t page = table[j >> a.shift];
+    if (page < 0 || (uint32_t)page >= a.n_pages) {
+      if (a.status && lane == 0) atomicOr(a.status, DEV_ERR_BAD_LIST);
+      return;
+    }
+    const long long at = page * a.page + (long long)(j & ((1u << a.shift) - 1)) * a.token + h * a.head;
+    key(static_cast<const T *>(a.k_pool) + at, static_cast<const T *>(a.v_pool) + at);
+  };
+  auto fresh = [&](uint32_t j) {
+    const long long at = (long long)s.first + j;
+    key(static_cast<const T *>(a.k) + at * a.ks + h * a.kh, static_cast<const T *>(a.v) + at * a.vs + h * a.vh);
+  };
+  const uint32_t depth = a.parents && a.window ? chunk_depth(a, s.first, i) : 0u;
+  const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? depth : i));
+  for (uint32_t j = lo.prefix; j < a.prefix; j++) paged(a.prefix_table, j);
+  for (uint32_t j = lo.cached; j < s.cached; j++) paged(a.table + b * a.ts, j);
+  if (a.parents) {  // the path to the root, down to the first depth in the window
+    int32_t j = (int32_t)i;
+    for (uint32_t d = depth; j >= 0 && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, s.first, (uint32_t)j))
+      fresh((uint32_t)j);
+  } else {
+    for (uint32_t j = lo.fresh; j <= i; j++) fresh(j);
+  }
+  T *out = static_cast<T *>(a.out) + row * a.os + hq * a.oh + lane * EPL;
+  uint32_t packed[EPL / 2];
+#pragma unroll
+  for (int e = 0; e < EPL / 2; e++) {
+    const float x = sum == 0.f ? 0.f : o[2 * e] / sum, y = sum == 0.f ? 0.f : o[2 * e + 1] / sum;
+    packed[e] = pack2(x, y, static_cast<const T *>(nullptr));
+  }
+  if constexpr (EPL == 8)
+    *reinterpret_cast<uint4 *>(out) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  else if constexpr (EPL == 4)
+    *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
+  else
+    *reinterpret_cast<uint32_t *>(out) = packed[0];
+}
+
+}  // namespace ch

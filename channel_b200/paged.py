@@ -1,6 +1,6 @@
 """Streams that share a prompt, on torch tensors: page plans, page writes and attention
-over the shared prefix (ch_page_plan, ch_paged_kv_write, ch_prefix_attention of
-include/channel_cuda.h, where the semantics are stated).
+over the shared prefix (ch_page_plan, ch_paged_kv_write, ch_prefix_attention and
+ch_chunk_attention of include/channel_cuda.h, where the semantics are stated).
 
 A layer's K rows lie in a pool ``[n_pages, page_size, n_kv, head_dim]`` and its V rows in a
 second one with the same strides.  A decode step of many streams is
@@ -9,6 +9,14 @@ second one with the same strides.  A decode step of many streams is
     kv_write(k, v, plan.slots, k_pool, v_pool)                                    # per layer
     out = prefix_attention(q, k_pool, v_pool, plan.table, plan.lens, prefix_table, prefix_len)
     tokens, _, _ = sampling.sample_rows(logits, uniform, ...)                     # once per step
+
+A step with several tokens per stream (a prompt, a chunk of one, drafted tokens) attends with
+
+    out = prompt_attention(q, k, v, plan.starts, k_pool, v_pool, table, lens, prefix_table, prefix_len)
+    out = tree_attention(q, k, v, starts, parents, k_pool, v_pool, table, lens, ...)
+
+where table and lens are the cache as it was before the step: the new tokens' keys and values
+are taken from k and v.
 
 Every call runs on torch's current stream of the tensors' device and returns without
 waiting for it; none has a backward pass, and a tensor that requires a gradient is refused
@@ -34,6 +42,7 @@ _NO_PAGES, _BAD = 1 << 5, (1 << 1) | (1 << 2)
 _PLAN = struct.Struct("@10Pq6IP")
 _WRITE = struct.Struct("@5P7q5I2iP")
 _ATTEND = struct.Struct("@7P8q9IfiP")
+_CHUNK = struct.Struct("@11P12q10IfiP")
 
 try:  # torch's current stream of a device as a cudaStream_t, without building a Stream object
     _stream_of = torch._C._cuda_getCurrentRawStream
@@ -227,3 +236,102 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     else:  # sizes the call refuses
         _run(lib.ch_prefix_attention, at, args, None, 0)
     return out
+
+
+def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table, lens, prefix_table, prefix_len, window,
+                     scale, out, status) -> torch.Tensor:
+    at, shape, kind = q.get_device(), q.shape, q.dtype
+    if len(shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or k.shape[0] != shape[0] or k.shape[2] != shape[2] or \
+            k.dtype is not kind or v.dtype is not kind or k.get_device() != at or v.get_device() != at or \
+            q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+        _fail(f"{name}: q is [tokens, n_q, head_dim], k and v are [tokens, n_kv, head_dim], of one type and device and dense "
+              "in the last dimension")
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_graph()
+    rows, n_q, dim = shape
+    n_kv = k.shape[1]
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        _fail(f"{name}: starts has one number more than there are streams")
+    n = starts.shape[0] - 1
+    p_starts = _vec(starts, n + 1, at, "starts")
+    p_parents = 0 if parents is None else _vec(parents, rows, at, "parents")
+    if prefix_len < 0 or window < 0:
+        _fail(f"{name}: negative size")
+    p_k = p_v = p_table = p_lens = p_prefix = 0
+    pages = page = cols = ps = ts = hs = row = 0
+    if k_pool is not None or v_pool is not None:
+        if k_pool is None or v_pool is None:
+            _fail(f"{name}: k_pool and v_pool go together")
+        (pages, page, pool_kv, pool_dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
+        if k_pool.dtype is not kind or pool_kv != n_kv or pool_dim != dim:
+            _fail(f"{name}: the pools have the type, kv heads and head_dim of k and v")
+        if k_pool.requires_grad or v_pool.requires_grad:
+            _no_graph()
+        p_k, p_v = k_pool.data_ptr(), v_pool.data_ptr()
+        if (table is None) != (lens is None):
+            _fail(f"{name}: table and lens go together")
+        if table is not None:
+            p_table, p_lens = _table(table, n, at, "table"), _vec(lens, n, at, "lens")
+            cols, row = table.shape[1], table.stride(0)
+        p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
+        if prefix_len and (prefix_table is None or prefix_table.shape[0] * page < prefix_len):
+            _fail(f"{name}: prefix_table is shorter than prefix_len")
+    elif table is not None or lens is not None or prefix_table is not None or prefix_len:
+        _fail(f"{name}: a cache needs k_pool and v_pool")
+    if out is None:
+        out = torch.empty(shape, dtype=kind, device=q.device)
+    elif out.shape != shape or out.dtype is not kind or out.get_device() != at or out.stride(2) != 1:
+        _fail(f"{name}: out is like q")
+    elif out.requires_grad:
+        _no_graph()
+    _device(q)
+    (qs, qh, _), (os, oh, _), (ks, kh, _), (vs, vh, _) = q.stride(), out.stride(), k.stride(), v.stride()
+    if scale is None:
+        scale = dim ** -0.5
+    elif not abs(scale) <= _F32_MAX:  # packing would make it infinite
+        _fail(f"{name}: scale is out of range")
+    try:
+        args = _CHUNK.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p_starts, p_parents, p_k, p_v, p_prefix,
+                           p_table, p_lens, qs, qh, ks, kh, vs, vh, os, oh, ps, ts, hs, row, rows, n, n_q, n_kv, dim, page,
+                           pages, cols, prefix_len, window, scale, _DTYPES.get(kind, -1), _status(status, at))
+    except struct.error as e:
+        _out_of_range(name, e)
+    lib = L.load()
+    need = lib.ch_chunk_attention_workspace(args)
+    if need:  # torch's caching allocator hands the workspace out in the stream's order
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _run(lib.ch_chunk_attention, at, args, work.data_ptr(), need)
+    else:  # nothing to do, or sizes the call refuses
+        _run(lib.ch_chunk_attention, at, args, None, 0)
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                     k_pool: Optional[torch.Tensor] = None, v_pool: Optional[torch.Tensor] = None,
+                     table: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                     prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, window: int = 0,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of packed new tokens (q ``[tokens, n_q, head_dim]``, k and v ``[tokens,
+    n_kv, head_dim]``; stream b's rows are starts[b] .. starts[b + 1] - 1) over the prefix_len
+    tokens in the pages of prefix_table, the stream's lens[b] cached tokens in those of table[b]
+    and its new tokens up to its own; window > 0 leaves the last ``window`` positions visible.
+    scale defaults to head_dim ** -0.5.  Rows of ``out`` that belong to no stream are not written."""
+    return _chunk_attention("prompt_attention", q, k, v, starts, None, k_pool, v_pool, table, lens, prefix_table, prefix_len,
+                            window, scale, out, status)
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, parents: torch.Tensor,
+                   k_pool: Optional[torch.Tensor] = None, v_pool: Optional[torch.Tensor] = None,
+                   table: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                   prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, window: int = 0,
+                   scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``prompt_attention`` where a stream's new tokens are nodes of a tree: parents[row] is the
+    node of the stream (an earlier one) that the row's token follows, -1 at a root.  A node sees
+    the prefix, the stream's cached tokens and the nodes on its path, itself among them; it is as
+    many positions behind the cached tokens as there are nodes above it."""
+    if parents is None:
+        _fail("tree_attention: parents are needed")
+    return _chunk_attention("tree_attention", q, k, v, starts, parents, k_pool, v_pool, table, lens, prefix_table, prefix_len,
+                            window, scale, out, status)

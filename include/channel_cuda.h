@@ -504,6 +504,95 @@ typedef struct {
 } ch_sample_rows_args;
 int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Steps with several tokens per stream (no reference counterpart), by the rules of the calls
+ * above: device pointers, no context, the current device, asynchronous on `stream`, nothing
+ * allocated, fit for a graph, arguments read before the call returns.
+ * The new tokens of all streams are packed: stream b has rows starts[b] .. starts[b + 1] - 1
+ * (n_streams + 1 numbers that do not fall, ch_page_plan's `starts`; a stream that ends ahead of its
+ * start has none, rows past n_tokens are left out, both status bit 2).
+ * ---------------------------------------------------------------------- */
+
+/* Attention of the new tokens.  Stream b's positions are the prefix_len tokens in the pages of
+ * prefix_table (shared), then its lens[b] cached tokens in those of its row of table, then its new
+ * tokens, whose keys and values are rows of k and v (they need not be in the pages yet):
+ *   parents NULL: new token i, at position t = prefix_len + lens[b] + i, attends to positions
+ *     [max(0, t + 1 - window), t] (window 0 = all): a packed prompt, or the next chunk of one;
+ *   parents [n_tokens]: the new tokens are nodes of a tree, parents[row] the node (counted in the
+ *     stream, before its own) that a node follows, -1 at a root (status bit 2 for others).  A
+ *     node at depth d (0 at a root) is at position t = prefix_len + lens[b] + d and attends to the
+ *     prefix, the cached tokens and the nodes on its path, itself among them, in the window.
+ * out = softmax(scale q.k) v over these, q head h on kv head h / (n_q / n_kv); zeros when no
+ * position is visible.  A position whose score is -inf counts as one that is not.  Rows of no stream are
+ * neither read as keys nor written.  out must not overlap q, k or v.
+ * q, k, v, out: element (row, head, d) at row * token_stride + head * head_stride + d.  Without
+ * a cache prefix_len and table_cols are 0, and the pools, the tables, lens and the page fields are not looked at.
+ * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096;
+ * page_size a power of two from 8 to 256; dtype (of all tensors) CH_F16 or CH_BF16, sums in f32.
+ * Strides are multiples of 8 elements (any number where the dimension is 1), q, k, v, out and the
+ * pools 16-byte aligned.  Positions whose page index is not in [0, n_pages) are left out (status
+ * bit 2); cached positions past table_cols pages too (the new tokens' positions stay), and a
+ * negative length counts as 0.
+ * workspace: at least ch_chunk_attention_workspace(args) bytes (0 when a size is invalid),
+ * 16-byte aligned, contents irrelevant; calls that may overlap need one each. */
+typedef struct {
+  const void *q, *k, *v;
+  void *out;
+  const int32_t *starts, *parents;
+  const void *k_pool, *v_pool;
+  const int32_t *prefix_table, *table, *lens;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t page_stride, token_stride, head_stride, table_stride;
+  uint32_t n_tokens, n_streams, n_q, n_kv, head_dim, page_size, n_pages, table_cols, prefix_len, window;
+  float scale;
+  int32_t dtype;
+  uint32_t *status;
+} ch_chunk_attn_args;
+size_t ch_chunk_attention_workspace(const ch_chunk_attn_args *args);
+int ch_chunk_attention(const ch_chunk_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Which drafted tokens the sampled ones confirm (n_streams <= 8192).  Per packed row: the node's
+ * token, its parent (as above) and the token sampled from the logits at it.  A stream's node 0 is
+ * its newest token and always accepted; after a node its first child (lowest row) whose token is
+ * the node's sampled one is accepted too, until there is none (a negative sampled token confirms
+ * nothing).
+ *   counts [n_streams]  accepted nodes (0 for a stream without nodes): new_tokens of ch_page_plan
+ *   next   [n_streams]  the token sampled at the last accepted node, -1 without nodes
+ *   kept   [n_tokens]   the node's place among the accepted ones of all streams, packed in the
+ *                       order of the streams (its place in that plan's slots), or -1 */
+typedef struct {
+  const int32_t *drafted, *parents, *starts, *sampled;
+  int32_t *counts, *next, *kept;
+  uint32_t n_tokens, n_streams;
+  uint32_t *status;
+} ch_accept_args;
+int ch_accept_drafts(const ch_accept_args *args, void *stream);
+
+/* Log-probabilities of given tokens.  Per row of logits (as for ch_sample_rows: f32, f16 or
+ * bf16, vocab <= 262144, x = softcap * tanh(logit / softcap), softcap >= 0 with 0 for the logit;
+ * NaN, -inf and the type's lowest value mask a token) and p = softmax(x):
+ *   logprobs [n_rows]  log p of targets[row]; -inf when it is masked; 0 for a target that is
+ *                      negative (nothing asked) or not below vocab (status bit 1)
+ *   entropy  [n_rows]  -sum p log p; 0 for a row whose tokens are all masked
+ *   ranks    [n_rows]  1 + how many tokens come before the target in the order of falling logits
+ *                      (equal ones, and masked ones, by index); 0 where logprobs is 0 for its target
+ *   top_ids, top_logprobs [n_rows x top]  the first `top` tokens of that order and their log p
+ * top is at most 64 and vocab.  Logits of +inf share the whole weight when softcap is 0. */
+typedef struct {
+  const void *logits;
+  const int32_t *targets;
+  float *logprobs, *entropy;
+  int32_t *ranks, *top_ids;
+  float *top_logprobs;
+  int64_t row_stride;
+  uint32_t n_rows, vocab, top;
+  float softcap;
+  int32_t dtype;
+  uint32_t *status;
+} ch_score_args;
+int ch_score_rows(const ch_score_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
