@@ -4,10 +4,13 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - m),
 // over the visible positions j; m is the running maximum, and sums are f32.
+#include <algorithm>
+#include <atomic>
+#include <cstring>
 #include <string>
 
 #include "../../include/channel_cuda.h"
-#include "chunk_attn.cuh"
+#include "chunk_tc.cuh"
 
 namespace ch {
 int set_last_error(int code, const std::string &msg);
@@ -16,10 +19,10 @@ namespace {
 constexpr uint32_t kMaxStreams = 4096;
 
 // ---------------------------------------------------------------------------
-// A warp per (new token, q head).
+// A warp per (new token, q head): tensors that no tensor map can describe.
 constexpr int kRowWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const __grid_constant__ ChunkArgs a) {
   const unsigned long long rows = (unsigned long long)a.n_tokens * a.nq;
   const uint32_t step = gridDim.x * kRowWarps;
   if (blockIdx.x == 0) chunk_report(a);
@@ -32,20 +35,125 @@ __global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const ChunkA
     }
     const ChunkStream s = chunk_stream(a, lo);
     if (t < s.first || t >= s.first + s.count) continue;  // behind the last stream
+    if (a.parents) chunk_report_parent(a, s.first, t - s.first);
     chunk_row<T, D>(a, s, lo, t - s.first, hq);
   }
 }
 
+template <int D>
+constexpr size_t tc_smem() {
+  return 1024 + Tc<D>::kMisc + sizeof(TcShared);
+}
+static_assert(tc_smem<64>() <= 232448 && tc_smem<128>() <= 232448 && tc_smem<256>() <= 232448, "shared memory per CTA");
+
+// pairs of CTAs that run at once on the current device; 0: the device does not say
+uint32_t tc_pairs() {
+  constexpr int kMaxDev = 64;
+  static std::atomic<int> cache[kMaxDev];  // 0: not asked yet, -1: unavailable
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 0;
+  int c = cache[dev].load(std::memory_order_relaxed);
+  if (c == 0) {
+    c = -1;
+    const void *kernel = (const void *)chunk_tc_kernel<__half, 256>;
+    if (ensure_smem_attr(kernel, tc_smem<256>()) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * (unsigned)(num_sms() / 2));
+      cfg.blockDim = dim3(kTcThreads);
+      cfg.dynamicSmemBytes = tc_smem<256>();
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0)
+        c = std::min(n, num_sms() / 2);
+      else
+        (void)cudaGetLastError();
+    }
+    cache[dev].store(c, std::memory_order_relaxed);
+  }
+  return c > 0 ? (uint32_t)c : 0u;
+}
+
+// workspace: w.cut | w.ml | w.o, each on 256 bytes (parts of O are stored 32 bytes at a time); the
+// caller's base is on 16 only, so there is room to align it
+size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+size_t carve(const ch_chunk_attn_args *p, uint8_t *base, ChunkWork *w) {
+  base = reinterpret_cast<uint8_t *>(aligned(reinterpret_cast<uintptr_t>(base)));
+  w->pairs = tc_pairs();
+  const size_t rows = (size_t)w->pairs * 2 * 2 * kRows;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t *r = base + at;
+    at += aligned(bytes);
+    return r;
+  };
+  w->cut = reinterpret_cast<Cut *>(take(w->pairs * sizeof(Cut)));
+  w->ml = reinterpret_cast<float2 *>(take(rows * sizeof(float2)));
+  w->o = reinterpret_cast<float *>(take(rows * p->head_dim * sizeof(float)));
+  return at + 256 - 16;
+}
+
+// kernel<<<grid, block, smem, s>>>(args...), which may start before the kernel in front of it
+// ends: both kernels wait for that one before they read or write anything
+template <typename K, typename... A>
+cudaError_t start_kernel(K kernel, dim3 grid, uint32_t block, size_t smem, cudaStream_t s, const A &...args) {
+  cudaError_t e = ensure_smem_attr((const void *)kernel, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// the tensors as the copies see them; false where a tensor map cannot describe one
+template <int D>
+bool encode_maps(const ChunkArgs &a, CUtensorMap (&maps)[5]) {
+  using C = Tc<D>;
+  std::memset(maps, 0, sizeof(maps));
+  const uint32_t tpt = kRows / a.group, ps = 1u << a.shift;
+  {  // Q: dim, q head, token; boxes of 64 dims of a kv head's q heads and a CTA's tokens
+    const cuuint64_t head = stride_or(a.nq, a.qh, 2 * D);
+    const MapDims d{3, {D, a.nq, a.n_tokens}, {head, stride_or(a.n_tokens, a.qs, head)}, {64, a.group, tpt}};
+    if (encode_map(&maps[0], a.q, d) != cudaSuccess) return false;
+  }
+  for (int v = 0; v < 2; v++) {  // new K and V: 64 dims, token, group of dims, head
+    const cuuint64_t token = stride_or(a.n_tokens, v ? a.vs : a.ks, 2 * D), head = stride_or(a.nkv, v ? a.vh : a.kh, 2 * D);
+    const MapDims d{4, {64, a.n_tokens, D / 64, a.nkv}, {token, 128, head},
+                    {64, v ? kKeys : kKeys / 2, (cuuint32_t)(v ? C::kVGroups : C::kGroups), 1}};
+    if (encode_map(&maps[1 + v], v ? a.v : a.k, d) != cudaSuccess) return false;
+  }
+  for (int v = 0; v < 2 && (a.prefix || a.cols); v++) {  // pools: 64 dims, token in the page, group of dims, head, page
+    const cuuint64_t token = (cuuint64_t)a.token * 2, head = stride_or(a.nkv, a.head, token), page = stride_or(a.n_pages, a.page, token);
+    const cuuint32_t rows = std::min(ps, v ? kKeys : kKeys / 2);
+    const cuuint32_t groups = v ? C::kVGroups : rows == kKeys / 2 ? C::kGroups : 1;
+    const MapDims d{5, {64, ps, D / 64, a.nkv, a.n_pages}, {token, 128, head, page}, {64, rows, groups, 1, 1}};
+    if (a.n_pages == 0 || encode_map(&maps[3 + v], v ? a.v_pool : a.k_pool, d) != cudaSuccess) return false;
+  }
+  return true;
+}
+
 template <typename T, int D>
-cudaError_t launch_t(const ChunkArgs &a, cudaStream_t s) {
+cudaError_t launch_t(const ChunkArgs &a, const ChunkWork &w, cudaStream_t s) {
+  alignas(64) CUtensorMap maps[5];
+  if (w.pairs && encode_maps<D>(a, maps)) {
+    const cudaError_t e = start_kernel(chunk_tc_kernel<T, D>, dim3(2 * w.pairs), kTcThreads, tc_smem<D>(), s, a, w, maps[0], maps[1],
+                                       maps[2], maps[3], maps[4]);
+    if (e != cudaSuccess) return e;
+    return start_kernel(chunk_join_kernel<T, D>, dim3(2 * kRows / kJoinWarps, w.pairs), kJoinWarps * 32, 0, s, a, w);
+  }
   const unsigned long long rows = (unsigned long long)a.n_tokens * a.nq;
   const unsigned long long grid = (rows + kRowWarps - 1) / kRowWarps, most = 16ull * num_sms();
   chunk_rows_kernel<T, D><<<(uint32_t)(grid < most ? grid : most), kRowWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t launch(const ChunkArgs &a, uint32_t D, cudaStream_t s) {
-  return D == 64 ? launch_t<T, 64>(a, s) : D == 128 ? launch_t<T, 128>(a, s) : launch_t<T, 256>(a, s);
+cudaError_t launch(const ChunkArgs &a, const ChunkWork &w, uint32_t D, cudaStream_t s) {
+  return D == 64 ? launch_t<T, 64>(a, w, s) : D == 128 ? launch_t<T, 128>(a, w, s) : launch_t<T, 256>(a, w, s);
 }
 
 const char *check(const ch_chunk_attn_args *p) {
@@ -124,7 +232,10 @@ int chunk_attention(const ch_chunk_attn_args *p, void *workspace, size_t bytes, 
   a.scale = p->scale;
   a.status = p->status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = p->dtype == CH_F16 ? launch<__half>(a, p->head_dim, s) : launch<__nv_bfloat16>(a, p->head_dim, s);
+  ChunkWork w;
+  carve(p, static_cast<uint8_t *>(workspace), &w);
+  const cudaError_t e =
+      p->dtype == CH_F16 ? launch<__half>(a, w, p->head_dim, s) : launch<__nv_bfloat16>(a, w, p->head_dim, s);
   if (e != cudaSuccess) return set_last_error(CH_ECUDA, std::string("chunk_attention: ") + cudaGetErrorString(e));
   return CH_OK;
 }
@@ -132,7 +243,9 @@ int chunk_attention(const ch_chunk_attn_args *p, void *workspace, size_t bytes, 
 }  // namespace ch
 
 extern "C" size_t ch_chunk_attention_workspace(const ch_chunk_attn_args *args) {
-  return 0;
+  if (ch::check(args) || args->n_tokens == 0 || args->n_streams == 0) return 0;
+  ch::ChunkWork w;
+  return ch::carve(args, nullptr, &w);
 }
 extern "C" int ch_chunk_attention(const ch_chunk_attn_args *args, void *workspace, size_t workspace_bytes, void *stream) {
   try {

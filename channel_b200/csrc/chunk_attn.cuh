@@ -54,20 +54,18 @@ CH_DEV int32_t chunk_parent(const ChunkArgs &a, uint32_t first, uint32_t i) {
   const int32_t p = a.parents[first + i];
   return p >= 0 && (uint32_t)p < i ? p : -1;
 }
-// what the calling CTA's threads see of starts and parents that break the rules, into the status word
+// what breaks the rules into the status word: starts (by the threads of one CTA), and the parent of
+// node i
 CH_DEV void chunk_report(const ChunkArgs &a) {
   if (!a.status) return;
   bool bad = false;
-  for (uint32_t b = threadIdx.x; b < a.n; b += blockDim.x) {
-    const long long lo = a.starts[b], hi = a.starts[b + 1];
-    bad |= lo < 0 || hi < lo || hi > (long long)a.n_tokens;
-    const ChunkStream s = chunk_stream(a, b);
-    for (uint32_t i = 0; a.parents && i < s.count; i++) {
-      const int32_t p = a.parents[s.first + i];
-      bad |= p < -1 || p >= (int32_t)i;
-    }
-  }
+  for (uint32_t b = threadIdx.x; b < a.n; b += blockDim.x)
+    bad |= a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > (long long)a.n_tokens;
   if (bad) atomicOr(a.status, DEV_ERR_BAD_LIST);
+}
+CH_DEV void chunk_report_parent(const ChunkArgs &a, uint32_t first, uint32_t i) {
+  const int32_t p = a.parents[first + i];
+  if (a.status && (p < -1 || p >= (int32_t)i)) atomicOr(a.status, DEV_ERR_BAD_LIST);
 }
 CH_DEV uint32_t chunk_depth(const ChunkArgs &a, uint32_t first, uint32_t i) {
   uint32_t d = 0;

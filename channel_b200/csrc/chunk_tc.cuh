@@ -1,0 +1,789 @@
+// chunk_tc.cuh -- ch_chunk_attention on the 5th-generation tensor cores.
+//
+// A unit is one kv head of one stream and the query rows of 2 x floor(128 / group) of its new
+// tokens, row = token * group + q head: the M = 256 rows of a CTA pair (a cluster of two, rows 0 to
+// 127 in the first).  Its keys are the 128-key tiles of the prefix, of the cached tokens and of the
+// new ones that any of its rows sees, and per tile
+//   S (256 x 128) = Q K^T,   P = 2^(scale log2(e) S - m),   O (256 x D) += P V
+// with cta_group::2 products: each CTA loads half of the tile's keys for the first and half of the
+// dims of V for the second, so a byte of K or V that reaches shared memory serves 256 rows.
+// O (D columns), and S in two buffers with P over it, lie in tensor memory; Q and a ring of K and V
+// tiles in shared memory, in the order the products take them: K_0, K_1, V_0, K_2, V_1, ...
+//
+// A softmax thread owns a row.  O is rescaled only when a row's maximum has grown by more than 2^8
+// since its last scale; a row's sum is kept in f32 before P is rounded to the type of V, which is
+// what the tensor cores take (in f16 P is 2^7 larger, so that small weights beside a large one do
+// not fall below the type's range).
+//
+// All tiles of all units, laid end to end with a unit's start counted as kUnitCost tiles, are cut
+// into equal runs, one for each pair; a unit that is cut leaves (O, m, l) of each of its parts in the
+// workspace, and chunk_join_kernel, already resident, adds them.
+//
+// Warps: 0 copies K, 1 copies V, 2 issues the products (in the second CTA: tells the first that its
+// copies have landed), 3 walks the units and looks pages up, 4 to 7 softmax and results (TMEM lanes
+// 32 * (warp % 4)), 8 copies Q.  Every wait is bounded; one that gives up sets the status word and the
+// abort flag, the roles leave their loops, and what is in flight is waited for (again with a limit).
+#pragma once
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "chunk_attn.cuh"
+
+namespace ch {
+namespace {
+constexpr uint32_t kKeys = 128, kRows = 128;  // keys of a tile; rows of a CTA
+constexpr int kTcThreads = 9 * 32;
+constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 256 and 384
+constexpr uint32_t kUnitCost = 2;
+constexpr uint32_t kItems = 2, kRecs = 6;
+constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
+template <typename T>
+constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;
+
+template <int D>
+struct Tc {
+  static constexpr int kGroups = D / 64;             // groups of 64 dims
+  static constexpr uint32_t kDv = D < 128 ? 128 : D;  // columns of O: 64 dims a CTA at least
+  static constexpr int kVGroups = kDv / 128;         // groups of 64 dims in a CTA's half of V
+  static constexpr uint32_t kQ = kRows * D * 2;
+  static constexpr uint32_t kK = kKeys / 2 * D * 2, kV = kKeys * kDv;  // bytes of a CTA's half tile
+  static constexpr uint32_t kPiece = kK > kV ? kK : kV;
+  static constexpr int kSlots = D == 256 ? 5 : 12;
+  static constexpr uint32_t kMisc = kQ + kSlots * kPiece;
+};
+
+struct Item {  // a run of one unit's tiles
+  uint32_t b, h, tok0, tok1;       // stream, kv head, the unit's new tokens [tok0, tok1)
+  uint32_t p0, np, c0, nc, n0;     // first tile of each segment and how many tiles the first two have
+  uint32_t k0, nt;                 // first tile of the run among the unit's, and how many
+  uint32_t part;                   // 0: the whole unit; 1 + slot of its part in the workspace
+};
+struct Rec {  // a tile
+  uint32_t seg, key0, z0, z1;  // segment, first key; keys [z0, z1) of the tile may be seen
+  uint32_t mask[4];            // which keys are there
+  uint32_t page[16];           // of every min(page size, 128) keys
+};
+struct TcShared {
+  uint64_t full[12], empty[12], peer[12], q_full, q_peer, q_empty, s_full[2], p_ready[2], pv_done, o_free, done;
+  uint64_t item_full[kItems], item_empty[kItems], rec_full[kRecs], rec_empty[kRecs];
+  Item items[kItems];
+  Rec recs[kRecs];
+  uint32_t v_rows[12];  // keys of a box of the V tile in a slot
+  uint32_t tmem_slot, abort_flag;
+};
+static_assert(sizeof(TcShared) <= 2048, "room beside the ring");
+
+// A unit cut between pairs: parts of it in the workspace, for the join (0: none).  Part slot 2 w is
+// the end or the middle of a unit in pair w's run, 2 w + 1 the beginning of one.
+struct Cut {
+  uint32_t b, h, tok0, tok1, parts;
+};
+struct ChunkWork {
+  Cut *cut;    // [pairs], by the pair that begins the unit
+  float *o;    // [2 * pairs][256][D]
+  float2 *ml;  // [2 * pairs][256]: maximum (log2), sum
+  uint32_t pairs;
+};
+
+// tiles of the unit of tokens [tok0, tok1)
+struct Tiles {
+  uint32_t p0, np, c0, nc, n0, nn;
+  CH_DEV uint32_t all() const { return np + nc + nn; }
+};
+CH_DEV Tiles tiles_of(const ChunkArgs &a, const ChunkStream &s, uint32_t tok0, uint32_t tok1) {
+  const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? 0u : tok0));
+  auto tiles = [](uint32_t from, uint32_t to, uint32_t &first) {
+    first = from / kKeys;
+    return to > from ? (to + kKeys - 1) / kKeys - first : 0u;
+  };
+  Tiles t;
+  t.np = tiles(lo.prefix, a.prefix, t.p0);
+  t.nc = tiles(lo.cached, s.cached, t.c0);
+  t.nn = tiles(lo.fresh, tok1, t.n0);
+  return t;
+}
+
+CH_DEV void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+CH_DEV void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// arrive on `bar` in both CTAs once every product issued so far is complete
+CH_DEV void commit2(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((unsigned short)3)
+      : "memory");
+}
+// instruction descriptor of kind::f16 with f32 sums, M = 256: A K-major, B K-major or (mn) N-major
+CH_DEV uint32_t idesc2(uint32_t n, bool bf16, bool mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((2 * kRows >> 4) << 24);
+}
+// V as the N-major operand B in the 128-byte swizzle: 64 dims x 8 keys are 1024 bytes; the
+// next 8 keys lie `keys8` bytes on (stride offset), the next 64 dims `dims64` (leading offset)
+CH_DEV uint64_t v_desc(uint32_t saddr, uint32_t dims64, uint32_t keys8) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(dims64 >> 4) << 16) | ((uint64_t)(keys8 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// bits [lo, hi) of a word, for numbers that may lie outside 0..32
+CH_DEV uint32_t bits_of(int lo, int hi) {
+  lo = max(lo, 0), hi = min(hi, 32);
+  if (hi <= lo) return 0u;
+  return (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+}
+
+template <typename T, int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+    chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w, const __grid_constant__ CUtensorMap qmap,
+                    const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const __grid_constant__ CUtensorMap kpmap, const __grid_constant__ CUtensorMap vpmap) {
+  using C = Tc<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t *sm = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
+  TcShared &sh = *reinterpret_cast<TcShared *>(sm + C::kMisc);
+  const uint32_t ring = smem_u32(sm) + C::kQ;
+  volatile uint32_t *abort = &sh.abort_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank(), pair = blockIdx.x >> 1;
+  const uint32_t tpt = kRows / a.group;  // tokens of a CTA
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1), mbar_init(&sh.peer[s], 1);
+    mbar_init(&sh.q_full, 1), mbar_init(&sh.q_peer, 1), mbar_init(&sh.q_empty, 1);
+    for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 8);
+    mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_free, 8), mbar_init(&sh.done, 1);
+    for (uint32_t s = 0; s < kItems; s++) mbar_init(&sh.item_full[s], 1), mbar_init(&sh.item_empty[s], 8);
+    for (uint32_t s = 0; s < kRecs; s++) mbar_init(&sh.rec_full[s], 1), mbar_init(&sh.rec_empty[s], 6);
+    sh.abort_flag = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+
+  grid_dep_wait();  // the kernel in front may still be running
+  // ---- what all units cost, and where this pair's run starts: the same sums in every CTA ----
+  unsigned long long *sums = reinterpret_cast<unsigned long long *>(sm);  // (before the first copy)
+  uint32_t *begin = reinterpret_cast<uint32_t *>(sm + 8 * (kTcThreads / 32));
+  const uint32_t per = (a.n + kTcThreads - 1) / kTcThreads, b0 = min(a.n, tid * per), b1 = min(a.n, b0 + per);
+  auto stream_cost = [&](uint32_t b) {  // of one kv head
+    const ChunkStream s = chunk_stream(a, b);
+    unsigned long long c = 0;
+    for (uint32_t t = 0; t < s.count; t += 2 * tpt) c += kUnitCost + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
+    return c;
+  };
+  unsigned long long mine = 0;
+  for (uint32_t b = b0; b < b1; b++) mine += stream_cost(b) * a.nkv;
+  unsigned long long at = mine, total = 0;  // at: cost of the streams before this thread's
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += u;
+  }
+  if (lane == 31) sums[warp] = at;
+  if (tid == 0) *begin = a.n;
+  if (blockIdx.x == 0) chunk_report(a);
+  __syncthreads();
+  at -= mine;
+  for (int i = 0; i < kTcThreads / 32; i++) {
+    if (i < warp) at += sums[i];
+    total += sums[i];
+  }
+  const unsigned long long run = (total + w.pairs - 1) / w.pairs;
+  const unsigned long long first = run * pair, last = min(first + run, total);
+  __syncthreads();
+  unsigned long long *found = sums;  // where the stream of the run's start begins
+  if (first < last && at <= first && first < at + mine) {
+    uint32_t b = b0;
+    for (unsigned long long c; at + (c = stream_cost(b) * a.nkv) <= first; b++) at += c;
+    *begin = b;
+    *found = at;
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // barriers initialised and tensor memory taken in both CTAs
+  tc_fence_after();
+  grid_dep_launch();
+  const uint32_t tmem = *(volatile uint32_t *)&sh.tmem_slot;
+  const uint32_t run_b = *begin;
+  const unsigned long long run_at = *found;
+  fence_proxy_async();
+  __syncthreads();  // (read before the first copy)
+
+  if (warp == 3) {
+    // ---- units and tiles of the run ----
+    Cut cut{0, 0, 0, 0, 0};
+    uint32_t n_items = 0, n_recs = 0;
+    bool ok = true;
+    unsigned long long x = run_at;  // start of the unit looked at
+    for (uint32_t b = run_b; b < a.n && x < last && ok; b++) {
+      const ChunkStream s = chunk_stream(a, b);
+      const unsigned long long c = stream_cost(b);
+      if (x + c * a.nkv <= first) {
+        x += c * a.nkv;
+        continue;
+      }
+      for (uint32_t h = 0; h < a.nkv && x < last && ok; h++) {
+        if (x + c <= first) {
+          x += c;
+          continue;
+        }
+        for (uint32_t t = 0; t < s.count && x < last && ok; t += 2 * tpt) {
+          const uint32_t tok1 = min(s.count, t + 2 * tpt);
+          const Tiles u = tiles_of(a, s, t, tok1);
+          const uint32_t all = u.all();
+          const unsigned long long k_at = x + kUnitCost;  // place of its first tile
+          const uint32_t k0 = first > k_at ? (uint32_t)min(first - k_at, (unsigned long long)all) : 0u;
+          const uint32_t k1 = last > k_at ? (uint32_t)min(last - k_at, (unsigned long long)all) : 0u;
+          x = k_at + all;
+          if (k1 <= k0) continue;
+          const uint32_t slot = n_items % kItems;
+          if (n_items >= kItems) ok = tc_wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1, abort, a.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          Item it{b, h, t, tok1, u.p0, u.np, u.c0, u.nc, u.n0, k0, k1 - k0, 0u};
+          if (k0 > 0)
+            it.part = 1 + 2 * pair;
+          else if (k1 < all) {
+            it.part = 2 + 2 * pair;
+            cut = Cut{b, h, t, tok1, 1u + (uint32_t)((x - 1) / run) - pair};
+          }
+          if (lane == 0) {
+            sh.items[slot] = it;
+            mbar_arrive(&sh.item_full[slot]);
+          }
+          __syncwarp();
+          n_items++;
+          // its tiles; a page is looked up one tile before it is used
+          const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? 0u : t));
+          const uint32_t pk = min(1u << a.shift, kKeys), pages = kKeys / pk;
+          auto seg_of = [&](uint32_t k, uint32_t &key0) {
+            if (k < u.np) {
+              key0 = (u.p0 + k) * kKeys;
+              return 0u;
+            }
+            if (k < u.np + u.nc) {
+              key0 = (u.c0 + k - u.np) * kKeys;
+              return 1u;
+            }
+            key0 = (u.n0 + k - u.np - u.nc) * kKeys;
+            return 2u;
+          };
+          auto end_of = [&](uint32_t seg) { return seg == 0 ? a.prefix : seg == 1 ? s.cached : tok1; };
+          auto look_up = [&](uint32_t k) {
+            uint32_t key0;
+            const uint32_t seg = seg_of(k, key0), j = key0 + lane * pk;
+            if (seg == 2 || lane >= (int)pages || j >= end_of(seg)) return -1;
+            return seg == 0 ? a.prefix_table[j >> a.shift] : a.table[b * a.ts + (j >> a.shift)];
+          };
+          int32_t next = look_up(k0);
+          for (uint32_t k = k0; k < k1; k++) {
+            uint32_t key0;
+            const uint32_t seg = seg_of(k, key0), end = end_of(seg);
+            const uint32_t low = seg == 0 ? lo.prefix : seg == 1 ? lo.cached : lo.fresh;
+            const int32_t page = next;
+            if (k + 1 < k1) next = look_up(k + 1);
+            const uint32_t r = n_recs % kRecs;
+            if (n_recs >= kRecs) ok = tc_wait(&sh.rec_empty[r], (n_recs / kRecs - 1) & 1, abort, a.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const bool there = seg == 2 || (page >= 0 && (uint32_t)page < a.n_pages);
+            if (!there && lane < (int)pages && key0 + lane * pk < end && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
+            Rec &rec = sh.recs[r];
+            if (lane < 16) rec.page[lane] = there ? (uint32_t)page : a.n_pages;  // past the pool: reads as zeros
+#pragma unroll
+            for (int c4 = 0; c4 < 4; c4++) {
+              const uint32_t key = c4 * 32 + lane;
+              const bool in = __shfl_sync(0xffffffffu, there, key / pk);
+              const uint32_t bits = __ballot_sync(0xffffffffu, in && key0 + key < end);
+              if (lane == 0) rec.mask[c4] = bits;
+            }
+            if (lane == 0) {
+              rec.seg = seg, rec.key0 = key0;
+              rec.z0 = low > key0 ? low - key0 : 0u;
+              rec.z1 = min(end - key0, kKeys);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.rec_full[r]);
+            n_recs++;
+          }
+        }
+      }
+    }
+    // the end: an item without tiles
+    if (ok) {
+      const uint32_t slot = n_items % kItems;
+      if (n_items >= kItems) ok = tc_wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1, abort, a.status);
+      if (__all_sync(0xffffffffu, ok) && lane == 0) {
+        sh.items[slot].nt = 0;
+        mbar_arrive(&sh.item_full[slot]);
+      }
+    }
+    if (rank == 0 && lane == 0) w.cut[pair] = cut;
+  } else {
+    // every other role walks the items
+    uint32_t n = 0;
+    Item it;
+    auto next_item = [&]() {  // false: the run is over, or a wait gave up
+      const uint32_t slot = n % kItems;
+      const bool ok = __all_sync(0xffffffffu, tc_wait(&sh.item_full[slot], (n / kItems) & 1, abort, a.status));
+      if (!ok) return false;
+      it = sh.items[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+      n++;
+      return it.nt != 0;
+    };
+    // place in the ring's order of K_i and of V_i of the item whose first piece has place `base`
+    auto k_seq = [&](uint32_t i) { return i ? 2 * i - 1 : 0u; };
+    auto v_seq = [&](uint32_t i) { return i + 1 < it.nt ? 2 * i + 2 : 2 * it.nt - 1; };
+    uint32_t base = 0, recs = 0;
+
+    if (warp == 0 || warp == 1) {
+      // ---- copies of K (this CTA's 64 keys of a tile) and V (its half of the dims) ----
+      const bool is_v = warp == 1;
+      const uint32_t ps = 1u << a.shift, pk = min(ps, kKeys), kb = min(ps, kKeys / 2);
+      uint32_t issued = 0, last_seq = 0;
+      bool ok = true;
+      while (ok && next_item()) {
+        const uint32_t row0 = chunk_stream(a, it.b).first;
+        for (uint32_t i = 0; i < it.nt && ok; i++, recs++) {
+          const uint32_t r = recs % kRecs;
+          ok = tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status);
+          const uint32_t seq = base + (is_v ? v_seq(i) : k_seq(i)), s = seq % C::kSlots;
+          if (ok && seq >= (uint32_t)C::kSlots) ok = tc_wait(&sh.empty[s], (seq / C::kSlots - 1) & 1, abort, a.status, true);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const Rec &rec = sh.recs[r];
+          const uint32_t seg = rec.seg, key0 = rec.key0, dst = ring + s * C::kPiece;
+          if (lane == 0) {
+            if (is_v) sh.v_rows[s] = seg == 2 ? kKeys : pk;
+            mbar_arrive_expect_tx(&sh.full[s], is_v ? C::kV : C::kK);
+          }
+          __syncwarp();
+          if (is_v) {
+            if (seg == 2) {
+              if (lane == 0) tma_load_4d(dst, &vmap, 0, (int)(row0 + key0), (int)(rank * C::kVGroups), (int)it.h, &sh.full[s]);
+            } else if (lane < (int)(kKeys / pk)) {
+              tma_load_5d(dst + lane * pk * C::kDv, &vpmap, 0, (int)((key0 + lane * pk) & (ps - 1)), (int)(rank * C::kVGroups),
+                          (int)it.h, (int)rec.page[lane], &sh.full[s]);
+            }
+          } else {
+            const uint32_t half = rank * (kKeys / 2);
+            if (seg == 2) {
+              if (lane == 0) tma_load_4d(dst, &kmap, 0, (int)(row0 + key0 + half), 0, (int)it.h, &sh.full[s]);
+            } else {
+              const uint32_t boxes = kKeys / 2 / kb, bx = lane % boxes, g = lane / boxes;
+              const uint32_t key = half + bx * kb;
+              if (g < (boxes == 1 ? 1u : (uint32_t)C::kGroups))
+                tma_load_5d(dst + g * (kKeys / 2 * 128) + bx * kb * 128, &kpmap, 0, (int)((key0 + key) & (ps - 1)), (int)g,
+                            (int)it.h, (int)rec.page[key / pk], &sh.full[s]);
+            }
+          }
+          issued++, last_seq = seq;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
+        }
+        base += 2 * it.nt;
+      }
+      // the last copies have landed (normally long since) before this CTA ends
+      if (issued && !ok) tc_wait(&sh.full[last_seq % C::kSlots], (last_seq / C::kSlots) & 1, nullptr, a.status);
+    } else if (warp == 8) {
+      // ---- copies of Q ----
+      uint32_t k = 0;
+      bool ok = true;
+      for (; ok && next_item(); k++) {
+        if (k > 0) ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status, true));
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
+          const uint32_t row = chunk_stream(a, it.b).first + it.tok0 + rank * tpt;
+          for (int g = 0; g < C::kGroups; g++)
+            tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)row, &sh.q_full);
+        }
+        __syncwarp();
+      }
+      if (k && !ok) tc_wait(&sh.q_full, (k - 1) & 1, nullptr, a.status);
+    } else if (warp == 2 && rank == 1) {
+      // ---- this CTA's copies have landed: tell the first CTA ----
+      const uint32_t peer = map_shared(smem_u32(sh.peer), 0), q_peer = map_shared(smem_u32(&sh.q_peer), 0);
+      bool ok = true;
+      for (uint32_t k = 0; ok && next_item(); k++) {
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_full, k & 1, abort, a.status));
+        if (ok && lane == 0) mbar_arrive_cluster(q_peer);
+        for (uint32_t i = 0; ok && i < 2 * it.nt; i++, base++) {
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.full[base % C::kSlots], (base / C::kSlots) & 1, abort, a.status));
+          if (ok && lane == 0) mbar_arrive_cluster(peer + (base % C::kSlots) * 8);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 2) {
+      // ---- products: the warp walks the loop together and one elected lane issues ----
+      const uint32_t issuer = elect_one();
+      const uint32_t s_idesc = idesc2(kKeys, kBf16, false), o_idesc = idesc2(C::kDv, kBf16, true);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(sm)), k_hi = umma_desc_sw128(0);
+      uint32_t g0 = 0, slot = 0, phase = 0;
+      bool ok = true;
+      auto take = [&]() {  // waits for the next piece of the ring, in both CTAs
+        ok = ok && tc_wait(&sh.full[slot], phase, abort, a.status) && tc_wait(&sh.peer[slot], phase, abort, a.status, true);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        return (ring + slot * C::kPiece) >> 4;
+      };
+      auto pass = [&]() {
+        if (issuer) commit2(&sh.empty[slot]);
+        __syncwarp();
+        if (++slot == (uint32_t)C::kSlots) slot = 0, phase ^= 1;
+      };
+      for (uint32_t k = 0; ok && next_item(); k++) {
+        ok = tc_wait(&sh.q_full, k & 1, abort, a.status) && tc_wait(&sh.q_peer, k & 1, abort, a.status, true);
+        ok = __all_sync(0xffffffffu, ok);
+        for (uint32_t i = 0; i <= it.nt && ok; i++) {
+          const uint32_t g = g0 + i;
+          if (i < it.nt) {
+            // S_g lies where P_{g-2} lay (of an item's first tile that is known: see below)
+            if (i > 0 && g >= 2) ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, g & 1, abort, a.status, true));
+            const uint32_t from = take();
+            if (!ok) break;
+            if (issuer) {
+              const uint32_t d = tmem + kSCol + (g & 1) * kKeys;
+#pragma unroll
+              for (int c = 0; c < D / 16; c++)
+                mma2_ss(d, q_desc + c / 4 * (kRows * 8) + 2 * (c % 4), k_hi + (from + c / 4 * (kKeys / 2 * 8) + 2 * (c % 4)), s_idesc,
+                        c != 0);
+              commit2(&sh.s_full[g & 1]);
+              if (i + 1 == it.nt) commit2(&sh.q_empty);
+            }
+            pass();
+          }
+          if (i > 0 && ok) {
+            const uint32_t gj = g - 1;
+            ok = tc_wait(&sh.p_ready[gj & 1], (gj >> 1) & 1, abort, a.status, true);
+            if (ok && i == 1 && k > 0) ok = tc_wait(&sh.o_free, (k - 1) & 1, abort, a.status, true);
+            // the next item's first S comes behind this product, when pv_done may be a phase further and
+            // the one before it cannot be asked for any more: so it is asked for here
+            if (ok && i == it.nt && gj > 0) ok = tc_wait(&sh.pv_done, (gj - 1) & 1, abort, a.status, true);
+            const uint32_t from = take();
+            if (!ok) break;
+            const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot];
+            const uint64_t v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 8u * C::kDv);
+            if (issuer) {
+              const uint32_t p = tmem + kSCol + (gj & 1) * kKeys, vs = 31 - __clz(vr);
+#pragma unroll
+              for (uint32_t c = 0; c < kKeys / 16; c++) {
+                const uint32_t box = c * 16 >> vs, in = c * 16 & (vr - 1);
+                mma2_ts(tmem, p + c * 8, v_hi + (from + box * (vr * C::kDv / 16) + in * 8), o_idesc, (i - 1) | c);
+              }
+              commit2(&sh.pv_done);
+            }
+            pass();
+          }
+        }
+        g0 += it.nt;
+      }
+      if (issuer) commit2(&sh.done);  // every product issued is complete, and its arrivals are made
+      __syncwarp();
+    } else {
+      // ---- softmax: thread = query row ----
+      const uint32_t quad = warp & 3, row = quad * 32 + lane, lanes = (quad * 32u) << 16;
+      const uint32_t p_ready = map_shared(smem_u32(sh.p_ready), 0), o_free = map_shared(smem_u32(&sh.o_free), 0);
+      const bool flip = !(a.scale > 0.f);
+      const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
+      const uint32_t token = row / a.group, qg = row % a.group;
+      uint32_t g = 0;
+      bool ok = true;
+      while (ok && next_item()) {
+        const ChunkStream st = chunk_stream(a, it.b);
+        const uint32_t i = it.tok0 + rank * tpt + token;  // this row's token
+        const bool valid = token < tpt && i < it.tok1;
+        const bool any = __any_sync(0xffffffffu, valid);
+        uint32_t depth = 0;
+        if (valid && a.parents) chunk_report_parent(a, st.first, i);
+        if (valid && a.parents && a.window) depth = chunk_depth(a, st.first, i);
+        const ChunkLow lo = chunk_low(a, st, st.before + (a.parents ? depth : i));
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
+          const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes, r = recs % kRecs;
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status));
+          if (!ok) break;
+          const uint32_t seg = sh.recs[r].seg, key0 = sh.recs[r].key0, z0 = sh.recs[r].z0, z1 = sh.recs[r].z1;
+          uint32_t mask[4];
+#pragma unroll
+          for (int c = 0; c < 4; c++) mask[c] = sh.recs[r].mask[c];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
+          if (any) {
+            // which of the tile's keys this row sees
+            if (seg == 2 && a.parents) {
+              uint32_t own[4] = {0u, 0u, 0u, 0u};
+              int32_t j = valid ? (int32_t)i : -1;
+              for (uint32_t d = depth; j >= (int32_t)key0 && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, st.first, (uint32_t)j)) {
+                const uint32_t x = (uint32_t)j - key0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) own[c] |= x / 32 == (uint32_t)c ? 1u << (x & 31) : 0u;
+              }
+#pragma unroll
+              for (int c = 0; c < 4; c++) mask[c] &= own[c];
+            } else {
+              const uint32_t from = seg == 0 ? lo.prefix : seg == 1 ? lo.cached : lo.fresh;
+              const int k0 = from > key0 ? (int)min(from - key0, kKeys) : 0;
+              const int k1 = seg < 2 ? (int)kKeys : i < key0 ? 0 : (int)min(i - key0 + 1, kKeys);
+              if (k0 > 0 || k1 < (int)kKeys) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) mask[c] &= bits_of(k0 - 32 * c, k1 - 32 * c);
+              }
+            }
+          }
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status, true));
+          if (!ok) break;
+          tc_fence_after();
+          if (any) {
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tc_ld32(scol + 32 * c, s[c]);
+            tc_wait_ld();
+            if (flip) {  // a scale that is not positive goes into the scores: below it is |scale|
+#pragma unroll
+              for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int e = 0; e < 32; e++) s[c][e] = a.scale == 0.f ? 0u : s[c][e] ^ 0x80000000u;
+            }
+            if (__any_sync(0xffffffffu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu)) {
+#pragma unroll
+              for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                  if (!((mask[c] >> e) & 1)) s[c][e] = 0xFF800000u;  // -inf
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+#pragma unroll
+              for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+            const bool grow = mx > m + kGrow || (m == -INFINITY && mx > -INFINITY);
+            const float m1 = grow ? mx : m, ref = m1 == -INFINITY ? 0.f : m1;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float keep = grow ? exp2_approx(m - ref) : 1.f;
+              l *= keep;
+              if (t > 0) {
+                ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (uint32_t c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tc_ld32(tmem + lanes + c, o);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                  tc_st32(tmem + lanes + c, o);
+                }
+              }
+            }
+            m = m1;
+            const float low = ref - kBias<T>;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              uint32_t p[32];
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                const float p0 = exp2_approx(fmaf(__uint_as_float(s[c + e / 16][2 * (e % 16)]), scale2, -low));
+                const float p1 = exp2_approx(fmaf(__uint_as_float(s[c + e / 16][2 * (e % 16) + 1]), scale2, -low));
+                sum[e & 1] += p0;
+                sum[2 + (e & 1)] += p1;
+                p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
+              }
+              tc_st32(scol + 16 * c, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_wait_st();
+          }
+          // rows of V that no row of the unit sees (before and behind its keys) are cleared: a
+          // weight of 0 must not meet stale bits
+          if (z0 > 0 || z1 < kKeys) {
+            const uint32_t seq = base + v_seq(t), slot = seq % C::kSlots;
+            ok = __all_sync(0xffffffffu, tc_wait(&sh.full[slot], (seq / C::kSlots) & 1, abort, a.status));
+            if (!ok) break;
+            const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot], n1 = kKeys - z1;
+            constexpr uint32_t kVecs = C::kDv / 16;  // 16-byte pieces of a key's dims
+            for (uint32_t x = tid - 128; x < (z0 + n1) * kVecs; x += 128) {
+              const uint32_t z = x / kVecs, v = x % kVecs, key = z < z0 ? z : z1 + (z - z0);
+              *reinterpret_cast<uint4 *>(sm + C::kQ + slot * C::kPiece + key / vr * vr * C::kDv + ((v >> 3) * vr + key % vr) * 128 +
+                                         (v & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();
+          }
+          // A barrier can only be asked for the phase that follows one known to be over, and only while
+          // the one after that cannot end.  S of this tile says that the product before the last is over;
+          // the last one is asked for while it waits for this P, so that below the item's own can be.
+          if (t + 1 == it.nt && g > 0) {
+            ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
+            if (!ok) break;
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(p_ready + (g & 1) * 8);
+        }
+        if (!ok) break;
+        base += 2 * it.nt;
+        // ---- the result, or this part of it ----
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
+        if (!ok) break;
+        tc_fence_after();
+        bool bad = false;
+        if (any && it.part) {
+          const size_t at_row = (size_t)(it.part - 1) * (2 * kRows) + rank * kRows + row;
+          if (valid) w.ml[at_row] = make_float2(m - kBias<T>, l);
+          float *po = w.o + at_row * D;
+#pragma unroll 1
+          for (uint32_t c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tc_ld32(tmem + lanes + c, o);
+            tc_wait_ld();
+            if (valid) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) st_global_32b(po + c + e, o + e);
+            }
+          }
+        } else if (any) {
+          const uint32_t hq = it.h * a.group + qg;
+          T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+          for (uint32_t c = 0; c < D; c += 32) {
+            uint32_t o[32], y[16];
+            tc_ld32(tmem + lanes + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const float x0 = __uint_as_float(o[2 * e]) * inv, x1 = __uint_as_float(o[2 * e + 1]) * inv;
+              bad |= !isfinite(x0) || !isfinite(x1);
+              y[e] = pack2(x0, x1, static_cast<const T *>(nullptr));
+            }
+            if (valid) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint4 *>(out + c + 2 * e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(o_free);
+        // A weight of 0 times a value that is not finite, at a key of the tile that this row does
+        // not see, is NaN: such a row is computed again on its own
+        uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
+        while (again) {
+          const int x = __ffs(again) - 1;
+          again &= again - 1;
+          chunk_row<T, D>(a, st, it.b, __shfl_sync(0xffffffffu, i, x), it.h * a.group + __shfl_sync(0xffffffffu, qg, x));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  // every arrival that a product makes has been made, in both CTAs, and tensor memory is at rest
+  tc_wait(&sh.done, 0, nullptr, a.status, true);
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// out = sum over a row's parts of O 2^(m - M) / sum of l 2^(m - M); a warp per row of a cut unit.
+constexpr int kJoinWarps = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w) {
+  constexpr int EPL = D / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), pair = blockIdx.y;
+  grid_dep_wait();
+  grid_dep_launch();
+  const Cut cut = w.cut[pair];
+  const uint32_t tpt = kRows / a.group, rank = row / kRows, token = row % kRows / a.group;
+  const uint32_t i = cut.tok0 + rank * tpt + token, hq = cut.h * a.group + row % kRows % a.group;
+  if (cut.parts == 0 || token >= tpt || i >= cut.tok1) return;
+  // the beginning of the unit in slot 2 pair + 1, the rest in slots 2 (pair + 1), 2 (pair + 2), ...
+  auto at = [&](uint32_t p) { return (size_t)(2 * (pair + p) + (p == 0)) * (2 * kRows) + row; };
+  float top = -INFINITY;
+  for (uint32_t p = lane; p < cut.parts; p += 32) top = fmaxf(top, w.ml[at(p)].x);
+  top = warp_max(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float o[EPL], sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; e++) o[e] = 0.f;
+  for (uint32_t p = 0; p < cut.parts; p++) {
+    const float2 ml = w.ml[at(p)];
+    const float f = exp2_approx(ml.x - ref);
+    sum = fmaf(ml.y, f, sum);
+    if (f == 0.f) continue;  // a part without a visible position has no O
+    const float *src = w.o + at(p) * D + lane * EPL;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = fmaf(src[e], f, o[e]);
+  }
+  bool bad = !isfinite(sum);
+#pragma unroll
+  for (int e = 0; e < EPL; e++) {
+    o[e] = sum == 0.f ? 0.f : o[e] / sum;
+    bad |= !isfinite(o[e]);
+  }
+  const ChunkStream st = chunk_stream(a, cut.b);
+  if (__any_sync(0xffffffffu, bad)) {
+    chunk_row<T, D>(a, st, cut.b, i, hq);
+    return;
+  }
+  T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh + lane * EPL;
+#pragma unroll
+  for (int e = 0; e < EPL; e += 2)
+    *reinterpret_cast<uint32_t *>(out + e) = pack2(o[e], o[e + 1], static_cast<const T *>(nullptr));
+}
+
+// ---------------------------------------------------------------------------
+// Host: tensor maps.  Token, head and page strides of dimensions of one element are never used and
+// may be any number, so they are replaced.
+struct MapDims {
+  uint32_t rank;
+  cuuint64_t dims[5], strides[4];  // elements; bytes from the second dimension on
+  cuuint32_t box[5];
+};
+inline cudaError_t encode_map(CUtensorMap *map, const void *base, const MapDims &d) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)
+                                                                : nullptr;
+  }();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, d.rank, const_cast<void *>(base), d.dims, d.strides, d.box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorNotSupported;
+}
+inline cuuint64_t stride_or(uint32_t n, long long elements, cuuint64_t other) {
+  return n > 1 ? (cuuint64_t)elements * 2 : other;
+}
+}  // namespace
+}  // namespace ch

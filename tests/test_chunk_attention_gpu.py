@@ -15,7 +15,11 @@ F16, BF16 = torch.float16, torch.bfloat16
 
 
 def both(s, parents=None, what="", **kw):
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    given = kw.setdefault("status", word)
     out = tree_attention(parents=parents, **s, **kw) if parents is not None else prompt_attention(**s, **kw)
+    if given is word:
+        check_status(word)
     kw.pop("out", None), kw.pop("status", None)
     check_close(out, *attend64(**s, parents=parents, **kw), what)
     return out
@@ -201,16 +205,19 @@ def test_strides_and_broadcast():
     assert torch.equal(prompt_attention(**pools), prompt_attention(**s))
 
 
-def test_long_stream():
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_stream(dim):
     """Many tiles for a row, against the same formula in 64 bits for some rows."""
-    s = make([5000, 3], [0, 0], n_q=2, n_kv=1, dim=128, dtype=BF16, seed=19)
-    out = prompt_attention(**s)
+    s = make([5000, 3], [0, 0], n_q=2, n_kv=1, dim=dim, dtype=BF16, seed=19)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = prompt_attention(status=status, **s)
+    check_status(status)
     q, k, v = (s[x].double() for x in "qkv")
-    for i in (0, 1, 127, 128, 2047, 4095, 4999):
-        z = torch.einsum("hd,kd->hk", q[i], k[:i + 1, 0]) * 128 ** -0.5
+    for i in list(range(0, 5000, 97)) + [127, 128, 2047, 4095, 4999]:
+        z = torch.einsum("hd,kd->hk", q[i], k[:i + 1, 0]) * dim ** -0.5
         p = torch.softmax(z, 1)
         ref, mass = p @ v[:i + 1, 0], p @ v[:i + 1, 0].abs()
-        drift = mass * (torch.einsum("hd,kd->hk", q[i].abs(), k[:i + 1, 0].abs()).amax(1, keepdim=True) * 128 ** -0.5)
+        drift = mass * (torch.einsum("hd,kd->hk", q[i].abs(), k[:i + 1, 0].abs()).amax(1, keepdim=True) * dim ** -0.5)
         check_close(out[i], ref, mass, drift, str(i))
 
 
@@ -219,6 +226,28 @@ def test_repeated_calls_give_the_same_bits():
     first = prompt_attention(**s)
     for _ in range(5):
         assert torch.equal(prompt_attention(**s), first)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 200])
+def test_many_units_give_the_same_bits(dim, window):
+    """More units than pairs of SMs, whole ones and cut ones, again and again: no wait gives up."""
+    s = make([16 + 37 * i % 700 for i in range(40)], [53 * i % 300 for i in range(40)], n_q=8, n_kv=4, dim=dim, dtype=BF16, seed=21)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    first = prompt_attention(status=status, window=window, **s)
+    check_status(status)
+    for _ in range(30):
+        assert torch.equal(prompt_attention(status=status, window=window, **s), first)
+    check_status(status)
+    rows = torch.arange(0, s["q"].shape[0], 61, device="cuda")
+    starts = s["starts"].tolist()
+    for r in rows.tolist():  # each as the last token of a shorter prompt
+        b = max(i for i in range(40) if starts[i] <= r)
+        one = {x: s[x][starts[b]:r + 1] for x in "qkv"}
+        one.update(starts=torch.tensor([0, r + 1 - starts[b]], dtype=torch.int32, device="cuda"), k_pool=s["k_pool"],
+                   v_pool=s["v_pool"], table=s["table"][b:b + 1], lens=s["lens"][b:b + 1])
+        alone = prompt_attention(window=window, **one)[-1].double()
+        assert (alone - first[r].double()).norm() <= 4 * torch.finfo(BF16).eps * alone.norm()
 
 
 def test_another_stream_and_two_at_once():
