@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const __grid
 
 template <int D>
 constexpr size_t tc_smem() {
-  return 1024 + Tc<D>::kMisc + sizeof(TcShared);
+  return Tc<D>::kMisc + sizeof(TcShared<D>);
 }
 static_assert(tc_smem<64>() <= 232448 && tc_smem<128>() <= 232448 && tc_smem<256>() <= 232448, "shared memory per CTA");
 

@@ -10,7 +10,9 @@
 // O (D columns), and S in two buffers with P over it, lie in tensor memory; Q and a ring of K and V
 // tiles in shared memory, in the order the products take them: K_0, K_1, V_0, K_2, V_1, ...
 //
-// A softmax thread owns a row.  O is rescaled only when a row's maximum has grown by more than 2^8
+// Two softmax threads own a row, 64 keys of a tile each: S of the tile after the next waits for the
+// product of this P (it lies over P), so the way from S to P is to be short.  (A thread for each row,
+// taking every other tile: 16,384 tokens 1.99 ms, so 1.79.)  O is rescaled only when a row's maximum has grown by more than 2^8
 // since its last scale; a row's sum is kept in f32 before P is rounded to the type of V, which is
 // what the tensor cores take (in f16 P is 2^7 larger, so that small weights beside a large one do
 // not fall below the type's range).
@@ -19,9 +21,10 @@
 // into equal runs, one for each pair; a unit that is cut leaves (O, m, l) of each of its parts in the
 // workspace, and chunk_join_kernel, already resident, adds them.
 //
-// Warps: 0 copies K, 1 copies V, 2 issues the products (in the second CTA: tells the first that its
-// copies have landed), 3 walks the units and looks pages up, 4 to 7 softmax and results (TMEM lanes
-// 32 * (warp % 4)), 8 copies Q.  Every wait is bounded; one that gives up sets the status word and the
+// Warps: 0 copies Q and K, 1 copies V, 2 issues the products (in the second CTA: tells the first that
+// its copies have landed), 3 walks the units and looks pages up, 4 to 11 softmax and results (TMEM
+// lanes 32 * (warp % 4); 8 to 11 the second half of the keys, and of
+// O's columns).  Every wait is bounded; one that gives up sets the status word and the
 // abort flag, the roles leave their loops, and what is in flight is waited for (again with a limit).
 #pragma once
 #include <cudaTypedefs.h>
@@ -33,10 +36,10 @@
 namespace ch {
 namespace {
 constexpr uint32_t kKeys = 128, kRows = 128;  // keys of a tile; rows of a CTA
-constexpr int kTcThreads = 9 * 32;
+constexpr int kSoftWarps = 8, kTcThreads = (4 + kSoftWarps) * 32;
 constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 256 and 384
 constexpr uint32_t kUnitCost = 2;
-constexpr uint32_t kItems = 2, kRecs = 6;
+constexpr uint32_t kItems = 2;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 template <typename T>
 constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;
@@ -49,7 +52,8 @@ struct Tc {
   static constexpr uint32_t kQ = kRows * D * 2;
   static constexpr uint32_t kK = kKeys / 2 * D * 2, kV = kKeys * kDv;  // bytes of a CTA's half tile
   static constexpr uint32_t kPiece = kK > kV ? kK : kV;
-  static constexpr int kSlots = D == 256 ? 5 : 12;
+  static constexpr int kSlots = D == 256 ? 5 : 11;
+  static constexpr uint32_t kRecs = D == 256 ? 4 : 6;
   static constexpr uint32_t kMisc = kQ + kSlots * kPiece;
 };
 
@@ -60,19 +64,24 @@ struct Item {  // a run of one unit's tiles
   uint32_t part;                   // 0: the whole unit; 1 + slot of its part in the workspace
 };
 struct Rec {  // a tile
-  uint32_t seg, key0, z0, z1;  // segment, first key; keys [z0, z1) of the tile may be seen
+  uint32_t seg, key0;  // segment (+ 4: every row of the unit sees every key of the tile), first key
+  uint32_t z0, z1;     // keys [z0, z1) of the tile may be seen
   uint32_t mask[4];            // which keys are there
   uint32_t page[16];           // of every min(page size, 128) keys
 };
+template <int D>
 struct TcShared {
-  uint64_t full[12], empty[12], peer[12], q_full, q_peer, q_empty, s_full[2], p_ready[2], pv_done, o_free, done;
+  static constexpr int kSlots = Tc<D>::kSlots;
+  static constexpr uint32_t kRecs = Tc<D>::kRecs;
+  uint64_t full[kSlots], empty[kSlots], q_full, q_empty, s_full[2], p_ready[2], pv_done, o_full, o_free, done;
+  alignas(16) Rec recs[kRecs];
   uint64_t item_full[kItems], item_empty[kItems], rec_full[kRecs], rec_empty[kRecs];
   Item items[kItems];
-  Rec recs[kRecs];
-  uint32_t v_rows[12];  // keys of a box of the V tile in a slot
+  uint32_t v_rows[kSlots];  // keys of a box of the V tile in a slot
   uint32_t tmem_slot, abort_flag;
+  uint32_t dead[kSoftWarps];  // a wait of the warp gave up
+  float half[2][kRows];       // what the two threads of a row tell each other
 };
-static_assert(sizeof(TcShared) <= 2048, "room beside the ring");
 
 // A unit cut between pairs: parts of it in the workspace, for the join (0: none).  Part slot 2 w is
 // the end or the middle of a unit in pair w's run, 2 w + 1 the beginning of one.
@@ -126,6 +135,12 @@ CH_DEV void commit2(uint64_t *bar) {
       "h"((unsigned short)3)
       : "memory");
 }
+// Arrive on the first CTA's barrier.  What it announces is in tensor memory (tcgen05.wait, fence) or
+// was written by copies or behind a proxy fence, so it takes no release of the cluster: that waits for
+// every access of the thread in flight (16,384 tokens took 2.6 ms with it, 2.0 without).
+CH_DEV void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // instruction descriptor of kind::f16 with f32 sums, M = 256: A K-major, B K-major or (mn) N-major
 CH_DEV uint32_t idesc2(uint32_t n, bool bf16, bool mn) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((2 * kRows >> 4) << 24);
@@ -143,6 +158,40 @@ CH_DEV uint32_t bits_of(int lo, int hi) {
   return (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
 }
 
+// barrier `id` of 64 threads, the two warps of 32 rows; pair_any: whether `p` holds in one of them
+CH_DEV void pair_sync(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+CH_DEV bool pair_any(uint32_t id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id)
+      : "memory");
+  return r != 0;
+}
+// two f32 at once
+CH_DEV uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+CH_DEV void halves(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+CH_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+CH_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CH_DEV float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T, int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w, const __grid_constant__ CUtensorMap qmap,
@@ -150,9 +199,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                     const __grid_constant__ CUtensorMap kpmap, const __grid_constant__ CUtensorMap vpmap) {
   using C = Tc<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ uint8_t smem_dyn[];
-  uint8_t *sm = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-  TcShared &sh = *reinterpret_cast<TcShared *>(sm + C::kMisc);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  TcShared<D> &sh = *reinterpret_cast<TcShared<D> *>(sm + C::kMisc);
+  constexpr uint32_t kRecs = C::kRecs;
   const uint32_t ring = smem_u32(sm) + C::kQ;
   volatile uint32_t *abort = &sh.abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -160,12 +209,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   const uint32_t tpt = kRows / a.group;  // tokens of a CTA
 
   if (tid == 0) {
-    for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1), mbar_init(&sh.peer[s], 1);
-    mbar_init(&sh.q_full, 1), mbar_init(&sh.q_peer, 1), mbar_init(&sh.q_empty, 1);
-    for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 8);
-    mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_free, 8), mbar_init(&sh.done, 1);
-    for (uint32_t s = 0; s < kItems; s++) mbar_init(&sh.item_full[s], 1), mbar_init(&sh.item_empty[s], 8);
-    for (uint32_t s = 0; s < kRecs; s++) mbar_init(&sh.rec_full[s], 1), mbar_init(&sh.rec_empty[s], 6);
+    const uint32_t ctas = rank == 0 ? 2 : 1;  // the first CTA waits for the copies of both
+    for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], ctas), mbar_init(&sh.empty[s], 1);
+    mbar_init(&sh.q_full, ctas), mbar_init(&sh.q_empty, 1);
+    for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 2 * kSoftWarps);
+    mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.o_free, 2 * kSoftWarps), mbar_init(&sh.done, 1);
+    for (int s = 0; s < kSoftWarps; s++) sh.dead[s] = 0u;
+    for (uint32_t s = 0; s < kItems; s++) mbar_init(&sh.item_full[s], 1), mbar_init(&sh.item_empty[s], 3 + kSoftWarps);
+    for (uint32_t s = 0; s < kRecs; s++) mbar_init(&sh.rec_full[s], 1), mbar_init(&sh.rec_empty[s], 2 + kSoftWarps);
     sh.abort_flag = 0u;
     fence_mbar_init();
   }
@@ -271,6 +322,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           n_items++;
           // its tiles; a page is looked up one tile before it is used
           const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? 0u : t));
+          const ChunkLow high = a.parents && a.window ? ChunkLow{~0u, ~0u, ~0u} : chunk_low(a, s, s.before + tok1 - 1);
           const uint32_t pk = min(1u << a.shift, kKeys), pages = kKeys / pk;
           auto seg_of = [&](uint32_t k, uint32_t &key0) {
             if (k < u.np) {
@@ -304,6 +356,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
             const bool there = seg == 2 || (page >= 0 && (uint32_t)page < a.n_pages);
             if (!there && lane < (int)pages && key0 + lane * pk < end && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
+            // (the last token sees from high.* on, the first one up to itself)
+            const bool all_in = seg < 2 ? key0 + kKeys <= end : !a.parents && key0 + kKeys <= t + 1;
+            const bool all_see = all_in && (seg == 0 ? high.prefix : seg == 1 ? high.cached : high.fresh) <= key0 &&
+                                 __all_sync(0xffffffffu, there || lane >= (int)pages);
             Rec &rec = sh.recs[r];
             if (lane < 16) rec.page[lane] = there ? (uint32_t)page : a.n_pages;  // past the pool: reads as zeros
 #pragma unroll
@@ -314,7 +370,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               if (lane == 0) rec.mask[c4] = bits;
             }
             if (lane == 0) {
-              rec.seg = seg, rec.key0 = key0;
+              rec.seg = seg + (all_see ? 4 : 0), rec.key0 = key0;
               rec.z0 = low > key0 ? low - key0 : 0u;
               rec.z1 = min(end - key0, kKeys);
             }
@@ -355,22 +411,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     uint32_t base = 0, recs = 0;
 
     if (warp == 0 || warp == 1) {
-      // ---- copies of K (this CTA's 64 keys of a tile) and V (its half of the dims) ----
+      // ---- copies of K (this CTA's 64 keys of a tile) and Q, and of V (its half of the dims) ----
       const bool is_v = warp == 1;
       const uint32_t ps = 1u << a.shift, pk = min(ps, kKeys), kb = min(ps, kKeys / 2);
-      uint32_t issued = 0, last_seq = 0;
+      uint32_t issued = 0, last_seq = 0, loaded_q = 0;
       bool ok = true;
-      while (ok && next_item()) {
+      for (uint32_t k = 0; ok && next_item(); k++) {
         const uint32_t row0 = chunk_stream(a, it.b).first;
         for (uint32_t i = 0; i < it.nt && ok; i++, recs++) {
           const uint32_t r = recs % kRecs;
           ok = tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status);
           const uint32_t seq = base + (is_v ? v_seq(i) : k_seq(i)), s = seq % C::kSlots;
-          if (ok && seq >= (uint32_t)C::kSlots) ok = tc_wait(&sh.empty[s], (seq / C::kSlots - 1) & 1, abort, a.status, true);
+          if (ok && seq >= (uint32_t)C::kSlots) ok = tc_wait(&sh.empty[s], (seq / C::kSlots - 1) & 1, abort, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const Rec &rec = sh.recs[r];
-          const uint32_t seg = rec.seg, key0 = rec.key0, dst = ring + s * C::kPiece;
+          const uint32_t seg = rec.seg & 3, key0 = rec.key0, dst = ring + s * C::kPiece;
           if (lane == 0) {
             if (is_v) sh.v_rows[s] = seg == 2 ? kKeys : pk;
             mbar_arrive_expect_tx(&sh.full[s], is_v ? C::kV : C::kK);
@@ -398,37 +454,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           issued++, last_seq = seq;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
+          if (!is_v && i == 0) {  // Q, behind the first K, which finds room before Q does
+            if (k > 0) ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
+              for (int g = 0; g < C::kGroups; g++)
+                tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)(row0 + it.tok0 + rank * tpt), &sh.q_full);
+            }
+            loaded_q = k + 1;
+            __syncwarp();
+          }
         }
         base += 2 * it.nt;
       }
       // the last copies have landed (normally long since) before this CTA ends
       if (issued && !ok) tc_wait(&sh.full[last_seq % C::kSlots], (last_seq / C::kSlots) & 1, nullptr, a.status);
-    } else if (warp == 8) {
-      // ---- copies of Q ----
-      uint32_t k = 0;
-      bool ok = true;
-      for (; ok && next_item(); k++) {
-        if (k > 0) ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status, true));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
-          const uint32_t row = chunk_stream(a, it.b).first + it.tok0 + rank * tpt;
-          for (int g = 0; g < C::kGroups; g++)
-            tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)row, &sh.q_full);
-        }
-        __syncwarp();
-      }
-      if (k && !ok) tc_wait(&sh.q_full, (k - 1) & 1, nullptr, a.status);
+      if (loaded_q && !ok) tc_wait(&sh.q_full, (loaded_q - 1) & 1, nullptr, a.status);
     } else if (warp == 2 && rank == 1) {
       // ---- this CTA's copies have landed: tell the first CTA ----
-      const uint32_t peer = map_shared(smem_u32(sh.peer), 0), q_peer = map_shared(smem_u32(&sh.q_peer), 0);
+      const uint32_t full0 = map_shared(smem_u32(sh.full), 0), q_full0 = map_shared(smem_u32(&sh.q_full), 0);
       bool ok = true;
       for (uint32_t k = 0; ok && next_item(); k++) {
         ok = __all_sync(0xffffffffu, tc_wait(&sh.q_full, k & 1, abort, a.status));
-        if (ok && lane == 0) mbar_arrive_cluster(q_peer);
+        if (ok && lane == 0) arrive_remote(q_full0);
         for (uint32_t i = 0; ok && i < 2 * it.nt; i++, base++) {
           ok = __all_sync(0xffffffffu, tc_wait(&sh.full[base % C::kSlots], (base / C::kSlots) & 1, abort, a.status));
-          if (ok && lane == 0) mbar_arrive_cluster(peer + (base % C::kSlots) * 8);
+          if (ok && lane == 0) arrive_remote(full0 + (base % C::kSlots) * 8);
         }
       }
       __syncwarp();
@@ -438,10 +490,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       const uint32_t s_idesc = idesc2(kKeys, kBf16, false), o_idesc = idesc2(C::kDv, kBf16, true);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(sm)), k_hi = umma_desc_sw128(0);
       uint32_t g0 = 0, slot = 0, phase = 0;
+      uint32_t v_rows = 0, v_at[kKeys / 16];  // how V lies in a slot: keys of a box, and where each 16 keys begin
+      uint64_t v_hi = 0;
       bool ok = true;
       auto take = [&]() {  // waits for the next piece of the ring, in both CTAs
-        ok = ok && tc_wait(&sh.full[slot], phase, abort, a.status) && tc_wait(&sh.peer[slot], phase, abort, a.status, true);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.full[slot], phase, abort, a.status));
         tc_fence_after();
         return (ring + slot * C::kPiece) >> 4;
       };
@@ -451,13 +504,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (++slot == (uint32_t)C::kSlots) slot = 0, phase ^= 1;
       };
       for (uint32_t k = 0; ok && next_item(); k++) {
-        ok = tc_wait(&sh.q_full, k & 1, abort, a.status) && tc_wait(&sh.q_peer, k & 1, abort, a.status, true);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_full, k & 1, abort, a.status));
         for (uint32_t i = 0; i <= it.nt && ok; i++) {
           const uint32_t g = g0 + i;
           if (i < it.nt) {
-            // S_g lies where P_{g-2} lay (of an item's first tile that is known: see below)
-            if (i > 0 && g >= 2) ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, g & 1, abort, a.status, true));
+            // S_g lies where P_{g-2} lay, whose product was issued before: the tensor cores take the
+            // products of a thread in order (waiting for it here left them idle 500 cycles a tile)
             const uint32_t from = take();
             if (!ok) break;
             if (issuer) {
@@ -473,23 +525,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           }
           if (i > 0 && ok) {
             const uint32_t gj = g - 1;
-            ok = tc_wait(&sh.p_ready[gj & 1], (gj >> 1) & 1, abort, a.status, true);
-            if (ok && i == 1 && k > 0) ok = tc_wait(&sh.o_free, (k - 1) & 1, abort, a.status, true);
-            // the next item's first S comes behind this product, when pv_done may be a phase further and
-            // the one before it cannot be asked for any more: so it is asked for here
-            if (ok && i == it.nt && gj > 0) ok = tc_wait(&sh.pv_done, (gj - 1) & 1, abort, a.status, true);
             const uint32_t from = take();
-            if (!ok) break;
-            const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot];
-            const uint64_t v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 8u * C::kDv);
-            if (issuer) {
-              const uint32_t p = tmem + kSCol + (gj & 1) * kKeys, vs = 31 - __clz(vr);
+            if (const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot]; vr != v_rows) {
+              v_rows = vr;
+              v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 8u * C::kDv);
 #pragma unroll
-              for (uint32_t c = 0; c < kKeys / 16; c++) {
-                const uint32_t box = c * 16 >> vs, in = c * 16 & (vr - 1);
-                mma2_ts(tmem, p + c * 8, v_hi + (from + box * (vr * C::kDv / 16) + in * 8), o_idesc, (i - 1) | c);
-              }
+              for (uint32_t c = 0; c < kKeys / 16; c++) v_at[c] = c * 16 / vr * (vr * C::kDv / 16) + c * 16 % vr * 8;
+            }
+            if (ok && i == 1 && k > 0) ok = tc_wait(&sh.o_free, (k - 1) & 1, abort, a.status);
+            ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.p_ready[gj & 1], (gj >> 1) & 1, abort, a.status));
+            tc_fence_after();
+            if (!ok) break;
+            if (issuer) {
+              const uint32_t p = tmem + kSCol + (gj & 1) * kKeys;
+#pragma unroll
+              for (uint32_t c = 0; c < kKeys / 16; c++) mma2_ts(tmem, p + c * 8, v_hi + (from + v_at[c]), o_idesc, (i - 1) | c);
               commit2(&sh.pv_done);
+              if (i == it.nt) commit2(&sh.o_full);
             }
             pass();
           }
@@ -499,15 +551,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       if (issuer) commit2(&sh.done);  // every product issued is complete, and its arrivals are made
       __syncwarp();
     } else {
-      // ---- softmax: thread = query row ----
-      const uint32_t quad = warp & 3, row = quad * 32 + lane, lanes = (quad * 32u) << 16;
+      // ---- softmax: two threads, half 0 and 1 of the keys, for a query row ----
+      const uint32_t quad = warp & 3, row = quad * 32 + lane, lanes = (quad * 32u) << 16, half = warp >= 8, bar = 1 + quad;
       const uint32_t p_ready = map_shared(smem_u32(sh.p_ready), 0), o_free = map_shared(smem_u32(&sh.o_free), 0);
       const bool flip = !(a.scale > 0.f);
       const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
+      const uint64_t scale22 = pair_of(scale2, scale2);
       const uint32_t token = row / a.group, qg = row % a.group;
-      uint32_t g = 0;
+      // A row's two warps wait for each other by barriers without a limit, so they leave together: one
+      // whose wait gave up goes on to the next barrier and says so there.
+      volatile uint32_t *dead = sh.dead;
+      uint32_t g = 0, items = 0;
       bool ok = true;
-      while (ok && next_item()) {
+      for (;; items++) {
+        const bool got = next_item();
+        if (pair_any(bar, !got)) break;
         const ChunkStream st = chunk_stream(a, it.b);
         const uint32_t i = it.tok0 + rank * tpt + token;  // this row's token
         const bool valid = token < tpt && i < it.tok1;
@@ -518,142 +576,153 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         const ChunkLow lo = chunk_low(a, st, st.before + (a.parents ? depth : i));
         float m = -INFINITY, l = 0.f;
         for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
-          const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes, r = recs % kRecs;
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status));
-          if (!ok) break;
-          const uint32_t seg = sh.recs[r].seg, key0 = sh.recs[r].key0, z0 = sh.recs[r].z0, z1 = sh.recs[r].z1;
-          uint32_t mask[4];
-#pragma unroll
-          for (int c = 0; c < 4; c++) mask[c] = sh.recs[r].mask[c];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
-          if (any) {
-            // which of the tile's keys this row sees
+          const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes;
+          ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status));
+          tc_fence_after();
+          uint32_t s[2][32];
+          tc_ld32(scol + half * 64, s[0]);
+          tc_ld32(scol + half * 64 + 32, s[1]);
+          // the tile's record (K was copied by it, so it is there)
+          const Rec &rec = sh.recs[recs % kRecs];
+          const uint4 head = *reinterpret_cast<const uint4 *>(&rec);
+          const uint32_t seg = head.x & 3, key0 = head.y, z0 = head.z, z1 = head.w;
+          const bool masked = any && !(head.x & 4);
+          uint32_t mask[2] = {~0u, ~0u};  // which of this thread's keys the row sees
+          if (masked) {
+            mask[0] = rec.mask[half * 2], mask[1] = rec.mask[half * 2 + 1];
+            const uint32_t at = key0 + half * 64;
             if (seg == 2 && a.parents) {
-              uint32_t own[4] = {0u, 0u, 0u, 0u};
+              uint32_t own[2] = {0u, 0u};
               int32_t j = valid ? (int32_t)i : -1;
-              for (uint32_t d = depth; j >= (int32_t)key0 && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, st.first, (uint32_t)j)) {
-                const uint32_t x = (uint32_t)j - key0;
+              for (uint32_t d = depth; j >= (int32_t)at && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, st.first, (uint32_t)j)) {
+                const uint32_t x = (uint32_t)j - at;
 #pragma unroll
-                for (int c = 0; c < 4; c++) own[c] |= x / 32 == (uint32_t)c ? 1u << (x & 31) : 0u;
+                for (int c = 0; c < 2; c++) own[c] |= x / 32 == (uint32_t)c ? 1u << (x & 31) : 0u;
               }
-#pragma unroll
-              for (int c = 0; c < 4; c++) mask[c] &= own[c];
+              mask[0] &= own[0], mask[1] &= own[1];
             } else {
               const uint32_t from = seg == 0 ? lo.prefix : seg == 1 ? lo.cached : lo.fresh;
-              const int k0 = from > key0 ? (int)min(from - key0, kKeys) : 0;
-              const int k1 = seg < 2 ? (int)kKeys : i < key0 ? 0 : (int)min(i - key0 + 1, kKeys);
-              if (k0 > 0 || k1 < (int)kKeys) {
-#pragma unroll
-                for (int c = 0; c < 4; c++) mask[c] &= bits_of(k0 - 32 * c, k1 - 32 * c);
-              }
+              const int k0 = from > at ? (int)min(from - at, 64u) : 0;
+              const int k1 = seg < 2 ? 64 : i < at ? 0 : (int)min(i - at + 1, 64u);
+              mask[0] &= bits_of(k0, k1), mask[1] &= bits_of(k0 - 32, k1 - 32);
             }
           }
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status, true));
-          if (!ok) break;
-          tc_fence_after();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.rec_empty[recs % kRecs]);
+          tc_wait_ld();
+          float mx = -INFINITY;
           if (any) {
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tc_ld32(scol + 32 * c, s[c]);
-            tc_wait_ld();
             if (flip) {  // a scale that is not positive goes into the scores: below it is |scale|
 #pragma unroll
-              for (int c = 0; c < 4; c++)
+              for (int c = 0; c < 2; c++)
 #pragma unroll
                 for (int e = 0; e < 32; e++) s[c][e] = a.scale == 0.f ? 0u : s[c][e] ^ 0x80000000u;
             }
-            if (__any_sync(0xffffffffu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu)) {
+            if (masked) {
 #pragma unroll
-              for (int c = 0; c < 4; c++)
+              for (int c = 0; c < 2; c++)
 #pragma unroll
                 for (int e = 0; e < 32; e++)
                   if (!((mask[c] >> e) & 1)) s[c][e] = 0xFF800000u;  // -inf
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; e++)
+            for (int e = 0; e < 32; e += 2)
 #pragma unroll
-              for (int c = 0; c < 4; c++) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-            const bool grow = mx > m + kGrow || (m == -INFINITY && mx > -INFINITY);
-            const float m1 = grow ? mx : m, ref = m1 == -INFINITY ? 0.f : m1;
-            if (__any_sync(0xffffffffu, grow)) {
-              const float keep = grow ? exp2_approx(m - ref) : 1.f;
-              l *= keep;
-              if (t > 0) {
-                ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (uint32_t c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tc_ld32(tmem + lanes + c, o);
-                  tc_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                  tc_st32(tmem + lanes + c, o);
-                }
-              }
-            }
+              for (int c = 0; c < 2; c++)
+                top[(e + c) & 3] = max3_nan(top[(e + c) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * scale2;
+          }
+          // (a NaN grows whatever there is, and stays)
+          auto grows = [&]() { return !(mx <= m + kGrow) && !(m == -INFINITY && mx == -INFINITY); };
+          // P of the second half lies over S of the first: both have read S behind this barrier
+          tc_fence_before();
+          if (!ok) dead[warp - 4] = 1u;
+          const bool some = pair_any(bar, !ok || grows());
+          tc_fence_after();
+          if (some) {  // a row's maximum has grown: the two halves agree on it
+            sh.half[half][row] = mx;
+            pair_sync(bar);
+            mx = max3_nan(mx, sh.half[half ^ 1][row], sh.half[half ^ 1][row]);
+            ok = !(dead[quad] | dead[4 + quad]);
+            pair_sync(bar);
+            if (!ok) break;
+            const bool grow = grows();
+            // (a score of +inf makes the row's sum NaN, as inf - inf would)
+            const float m1 = grow ? (mx == INFINITY ? NAN : mx) : m, keep = grow ? exp2_approx(m - m1) : 1.f;
             m = m1;
-            const float low = ref - kBias<T>;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            l *= keep;
+            if (t > 0) {
+              // O is rescaled behind the product of the tile before.  (A barrier can only be asked for the phase
+              // that follows one known to be over, while the one after that cannot end: S of this tile came
+              // behind the product before that one, and the next product waits for this P.)
+              ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status));
+              tc_fence_after();
+#pragma unroll 1
+              for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+                uint32_t o[32];
+                tc_ld32(tmem + lanes + c, o);
+                tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-              uint32_t p[32];
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const float p0 = exp2_approx(fmaf(__uint_as_float(s[c + e / 16][2 * (e % 16)]), scale2, -low));
-                const float p1 = exp2_approx(fmaf(__uint_as_float(s[c + e / 16][2 * (e % 16) + 1]), scale2, -low));
-                sum[e & 1] += p0;
-                sum[2 + (e & 1)] += p1;
-                p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tc_st32(tmem + lanes + c, o);
               }
-              tc_st32(scol + 16 * c, p);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          }
+          if (any) {
+            const float low = kBias<T> - (m == -INFINITY ? 0.f : m);
+            const uint64_t low2 = pair_of(low, low);
+            uint64_t sum[2] = {0ull, 0ull};
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              const uint64_t x = fma2(pair_of(__uint_as_float(s[e / 16][2 * (e % 16)]), __uint_as_float(s[e / 16][2 * (e % 16) + 1])),
+                                      scale22, low2);
+              float x0, x1;
+              halves(x, x0, x1);
+              const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
+              sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
+              p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
+            }
+            tc_st32(scol + half * 32, p);
+            float l0, l1;
+            halves(add2(sum[0], sum[1]), l0, l1);
+            l += l0 + l1;
             tc_wait_st();
           }
           // rows of V that no row of the unit sees (before and behind its keys) are cleared: a
           // weight of 0 must not meet stale bits
           if (z0 > 0 || z1 < kKeys) {
             const uint32_t seq = base + v_seq(t), slot = seq % C::kSlots;
-            ok = __all_sync(0xffffffffu, tc_wait(&sh.full[slot], (seq / C::kSlots) & 1, abort, a.status));
-            if (!ok) break;
+            ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.full[slot], (seq / C::kSlots) & 1, abort, a.status));
             const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot], n1 = kKeys - z1;
             constexpr uint32_t kVecs = C::kDv / 16;  // 16-byte pieces of a key's dims
-            for (uint32_t x = tid - 128; x < (z0 + n1) * kVecs; x += 128) {
+            for (uint32_t x = ok ? tid - 128 : ~0u; x < (z0 + n1) * kVecs; x += kSoftWarps * 32) {
               const uint32_t z = x / kVecs, v = x % kVecs, key = z < z0 ? z : z1 + (z - z0);
               *reinterpret_cast<uint4 *>(sm + C::kQ + slot * C::kPiece + key / vr * vr * C::kDv + ((v >> 3) * vr + key % vr) * 128 +
                                          (v & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async();
           }
-          // A barrier can only be asked for the phase that follows one known to be over, and only while
-          // the one after that cannot end.  S of this tile says that the product before the last is over;
-          // the last one is asked for while it waits for this P, so that below the item's own can be.
-          if (t + 1 == it.nt && g > 0) {
-            ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
-            if (!ok) break;
-          }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(p_ready + (g & 1) * 8);
+          if (lane == 0) arrive_remote(p_ready + (g & 1) * 8);
         }
-        if (!ok) break;
+        if (!ok && (dead[quad] | dead[4 + quad])) break;  // (both warps left the loop above)
         base += 2 * it.nt;
         // ---- the result, or this part of it ----
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status, true));
-        if (!ok) break;
+        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.o_full, items & 1, abort, a.status));
         tc_fence_after();
         bool bad = false;
+        sh.half[half][row] = l;
+        if (pair_any(bar, !ok)) break;
+        l += sh.half[half ^ 1][row];  // the sums of both halves
         if (any && it.part) {
           const size_t at_row = (size_t)(it.part - 1) * (2 * kRows) + rank * kRows + row;
-          if (valid) w.ml[at_row] = make_float2(m - kBias<T>, l);
+          if (valid && half == 0) w.ml[at_row] = make_float2(m - kBias<T>, l);
           float *po = w.o + at_row * D;
 #pragma unroll 1
-          for (uint32_t c = 0; c < D; c += 32) {
+          for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32];
             tc_ld32(tmem + lanes + c, o);
             tc_wait_ld();
@@ -667,7 +736,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh;
           const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-          for (uint32_t c = 0; c < D; c += 32) {
+          for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32], y[16];
             tc_ld32(tmem + lanes + c, o);
             tc_wait_ld();
@@ -686,10 +755,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(o_free);
+        if (lane == 0) arrive_remote(o_free);
         // A weight of 0 times a value that is not finite, at a key of the tile that this row does
         // not see, is NaN: such a row is computed again on its own
-        uint32_t again = __ballot_sync(0xffffffffu, bad && valid);
+        if (pair_any(bar, bad && valid)) {
+          sh.half[half][row] = bad;
+          pair_sync(bar);  // (the rows' stores come before those of the new results)
+          bad |= sh.half[half ^ 1][row] != 0.f;
+          pair_sync(bar);
+        }
+        uint32_t again = half ? 0u : __ballot_sync(0xffffffffu, bad && valid);
         while (again) {
           const int x = __ffs(again) - 1;
           again &= again - 1;
@@ -700,7 +775,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   }
   __syncwarp();
   // every arrival that a product makes has been made, in both CTAs, and tensor memory is at rest
-  tc_wait(&sh.done, 0, nullptr, a.status, true);
+  tc_wait(&sh.done, 0, nullptr, a.status);
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
