@@ -54,6 +54,9 @@ struct Tc {
   static constexpr uint32_t kPiece = kK > kV ? kK : kV;
   static constexpr int kSlots = D == 256 ? 5 : 11;
   static constexpr uint32_t kRecs = D == 256 ? 4 : 6;
+  // of 8 pairs of exponentials, how many go to the FMA pipe (8,192 tokens with D = 128: 726 us with none,
+  // 689 with 2, 758 with 4; with D = 256, whose products take twice as long, 444, 445 and 463)
+  static constexpr int kPoly = D == 256 ? 0 : 2;
   static constexpr uint32_t kMisc = kQ + kSlots * kPiece;
 };
 
@@ -190,6 +193,29 @@ CH_DEV float max3_nan(float a, float b, float c) {  // NaN if one is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// 2^x of two numbers up to 127 on the FMA pipe: the exponential's pipe takes 16 a cycle and SM, which
+// for 128 x 128 scores is as long as the products of D = 128 take.  x = n + f with |f| <= 1/2 by adding
+// and taking off 1.5 2^23; 2^f by the polynomial of degree 4 with f(0) = 1 and the least relative error
+// on [-1/2, 1/2], 2^-18.4 (a weight is rounded to 2^-9 or 2^-12 next); n into the exponent.  Below
+// -126: 2^-126, as good as nothing beside a row's largest weight of 2^-8 or more.
+CH_DEV void exp2_poly(uint64_t x, float &p0, float &p1) {
+  float x0, x1;
+  halves(x, x0, x1);
+  x = pair_of(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t n = add2(x, pair_of(12582912.f, 12582912.f)), r = add2(n, pair_of(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(r, pair_of(-1.f, -1.f), x);
+  uint64_t y = pair_of(0.009582852944731712f, 0.009582852944731712f);
+  y = fma2(y, f, pair_of(0.055906426161527634f, 0.055906426161527634f));
+  y = fma2(y, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
+  y = fma2(y, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
+  y = fma2(y, f, pair_of(1.f, 1.f));
+  float n0, n1;
+  halves(n, n0, n1);
+  halves(y, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
 }
 
 template <typename T, int D>
@@ -577,7 +603,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         float m = -INFINITY, l = 0.f;
         for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
           const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes;
-          ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status));
+          ok = ok && tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status);
+          __syncwarp();
           tc_fence_after();
           uint32_t s[2][32];
           tc_ld32(scol + half * 64, s[0]);
@@ -678,9 +705,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             for (int e = 0; e < 32; e++) {
               const uint64_t x = fma2(pair_of(__uint_as_float(s[e / 16][2 * (e % 16)]), __uint_as_float(s[e / 16][2 * (e % 16) + 1])),
                                       scale22, low2);
-              float x0, x1;
-              halves(x, x0, x1);
-              const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
+              float p0, p1;
+              if (e % 8 < C::kPoly) {
+                exp2_poly(x, p0, p1);
+              } else {
+                halves(x, p0, p1);
+                p0 = exp2_approx(p0), p1 = exp2_approx(p1);
+              }
               sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
               p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
             }
@@ -716,7 +747,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         bool bad = false;
         sh.half[half][row] = l;
         if (pair_any(bar, !ok)) break;
-        l += sh.half[half ^ 1][row];  // the sums of both halves
+        l = m == -INFINITY ? 0.f : l + sh.half[half ^ 1][row];  // the sums of both halves
         if (any && it.part) {
           const size_t at_row = (size_t)(it.part - 1) * (2 * kRows) + rank * kRows + row;
           if (valid && half == 0) w.ml[at_row] = make_float2(m - kBias<T>, l);

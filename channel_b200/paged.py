@@ -254,7 +254,12 @@ def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table,
         _fail(f"{name}: starts has one number more than there are streams")
     n = starts.shape[0] - 1
     p_starts = _vec(starts, n + 1, at, "starts")
-    p_parents = 0 if parents is None else _vec(parents, rows, at, "parents")
+    p_parents = 0
+    if parents is not None:  # rows behind the last parent belong to no stream
+        p_parents = _vec(parents, -1, at, "parents")
+        if parents.shape[0] > rows:
+            _fail(f"{name}: parents has more rows than q")
+        rows = parents.shape[0]
     if prefix_len < 0 or window < 0:
         _fail(f"{name}: negative size")
     p_k = p_v = p_table = p_lens = p_prefix = 0
@@ -328,7 +333,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: to
                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``prompt_attention`` where a stream's new tokens are nodes of a tree: parents[row] is the
-    node of the stream (an earlier one) that the row's token follows, -1 at a root.  A node sees
+    node of the stream (an earlier one) that the row's token follows, -1 at a root; rows behind the
+    last parent belong to no stream.  A node sees
     the prefix, the stream's cached tokens and the nodes on its path, itself among them; it is as
     many positions behind the cached tokens as there are nodes above it."""
     if parents is None:

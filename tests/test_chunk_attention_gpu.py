@@ -115,6 +115,7 @@ def test_what_no_token_owns_is_not_seen(stale, dim):
     s = make(new, [30, 17, 0], prefix=21, dim=dim, pad=70, seed=10, stale=stale)
     both(s)
     both(s, torch.cat([random_parents(new, 10), torch.zeros(70, dtype=torch.int32, device="cuda")]))
+    both(s, random_parents(new, 10))  # (no parents for the padding)
 
 
 @pytest.mark.parametrize("what", ["k", "v"])

@@ -95,7 +95,7 @@ def test_chunk_attention_tensors(kw):
 
 
 def test_tree_tensors():
-    for parents in (None, torch.zeros(5).int(), torch.zeros(6), torch.zeros(6, 1).int()):
+    for parents in (None, torch.zeros(7).int(), torch.zeros(6), torch.zeros(6, 1).int()):
         with pytest.raises(ChannelError):
             tree_attention(parents=parents, **tensors())
 
