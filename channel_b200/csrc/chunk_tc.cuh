@@ -172,29 +172,6 @@ CH_DEV bool pair_any(uint32_t id, bool p) {
       : "memory");
   return r != 0;
 }
-// two f32 at once
-CH_DEV uint64_t pair_of(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-CH_DEV void halves(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-CH_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-CH_DEV uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-CH_DEV float max3_nan(float a, float b, float c) {  // NaN if one is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // 2^x of two numbers up to 127 on the FMA pipe: the exponential's pipe takes 16 a cycle and SM, which
 // for 128 x 128 scores is as long as the products of D = 128 take.  x = n + f with |f| <= 1/2 by adding
 // and taking off 1.5 2^23; 2^f by the polynomial of degree 4 with f(0) = 1 and the least relative error

@@ -570,7 +570,7 @@ typedef struct {
 int ch_accept_drafts(const ch_accept_args *args, void *stream);
 
 /* Log-probabilities of given tokens.  Per row of logits (as for ch_sample_rows: f32, f16 or
- * bf16, vocab <= 262144, x = softcap * tanh(logit / softcap), softcap >= 0 with 0 for the logit;
+ * bf16, vocab <= 262144, x = softcap * tanh(logit / softcap), softcap 1e-30 to 1e30 or 0 for the logit;
  * NaN, -inf and the type's lowest value mask a token) and p = softmax(x):
  *   logprobs [n_rows]  log p of targets[row]; -inf when it is masked; 0 for a target that is
  *                      negative (nothing asked) or not below vocab (status bit 1)

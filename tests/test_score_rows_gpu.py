@@ -125,6 +125,14 @@ def test_large_and_small_logits():
     x = torch.randn(4, 3000, generator=g, device="cuda") * torch.tensor([[1e-6], [1.0], [1e3], [1e30]], device="cuda")
     check(x, torch.zeros(4, dtype=torch.int32, device="cuda"), 5, 30.0)
     check(x[:2].contiguous(), torch.zeros(2, dtype=torch.int32, device="cuda"), 5, 0.0)
+    # without a cap: one token has all the weight, and the others' log-probabilities are differences of logits
+    for big in (1e6, 1e30, 3e38):
+        y = torch.zeros(1, 3000, device="cuda")
+        y[0, 7], y[0, 9], y[0, 11] = big, big / 2, -big / 8
+        r = score_rows(y, torch.tensor([9], dtype=torch.int32, device="cuda"), top=3)
+        assert r.top_ids.tolist() == [[7, 9, 0]] and r.entropy.item() == 0 and r.ranks.item() == 2
+        want = torch.tensor([0.0, big / 2 - big, -big])
+        assert torch.allclose(r.top_logprobs[0].cpu(), want, rtol=2.0 ** -22) and abs(r.logprobs.item() - want[1]) <= 2.0 ** -22 * big
 
 
 def test_targets_outside():
