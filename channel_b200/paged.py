@@ -240,19 +240,18 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
 
 def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table, lens, prefix_table, prefix_len, window,
                      scale, out, status) -> torch.Tensor:
-    at, shape, kind = q.get_device(), q.shape, q.dtype
-    if len(shape) != 3 or len(k.shape) != 3 or k.shape != v.shape or k.shape[0] != shape[0] or k.shape[2] != shape[2] or \
+    at, kind, shape, kv_shape = q.get_device(), q.dtype, q.shape, k.shape
+    q_strides, k_strides, v_strides = q.stride(), k.stride(), v.stride()
+    if len(shape) != 3 or len(kv_shape) != 3 or kv_shape != v.shape or kv_shape[0] != shape[0] or kv_shape[2] != shape[2] or \
             k.dtype is not kind or v.dtype is not kind or k.get_device() != at or v.get_device() != at or \
-            q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+            q_strides[2] != 1 or k_strides[2] != 1 or v_strides[2] != 1:
         _fail(f"{name}: q is [tokens, n_q, head_dim], k and v are [tokens, n_kv, head_dim], of one type and device and dense "
               "in the last dimension")
-    if q.requires_grad or k.requires_grad or v.requires_grad:
-        _no_graph()
     rows, n_q, dim = shape
-    n_kv = k.shape[1]
-    if starts.dim() != 1 or starts.shape[0] < 1:
+    n_kv = kv_shape[1]
+    n = starts.numel() - 1
+    if n < 0:
         _fail(f"{name}: starts has one number more than there are streams")
-    n = starts.shape[0] - 1
     p_starts = _vec(starts, n + 1, at, "starts")
     p_parents = 0
     if parents is not None:  # rows behind the last parent belong to no stream
@@ -264,48 +263,53 @@ def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table,
         _fail(f"{name}: negative size")
     p_k = p_v = p_table = p_lens = p_prefix = 0
     pages = page = cols = ps = ts = hs = row = 0
-    if k_pool is not None or v_pool is not None:
-        if k_pool is None or v_pool is None:
-            _fail(f"{name}: k_pool and v_pool go together")
+    grad = q.requires_grad or k.requires_grad or v.requires_grad
+    if k_pool is not None and v_pool is not None:
         (pages, page, pool_kv, pool_dim), (ps, ts, hs, _) = _pools(k_pool, v_pool, at)
         if k_pool.dtype is not kind or pool_kv != n_kv or pool_dim != dim:
             _fail(f"{name}: the pools have the type, kv heads and head_dim of k and v")
-        if k_pool.requires_grad or v_pool.requires_grad:
-            _no_graph()
+        grad = grad or k_pool.requires_grad or v_pool.requires_grad
         p_k, p_v = k_pool.data_ptr(), v_pool.data_ptr()
-        if (table is None) != (lens is None):
-            _fail(f"{name}: table and lens go together")
-        if table is not None:
+        if table is not None and lens is not None:
             p_table, p_lens = _table(table, n, at, "table"), _vec(lens, n, at, "lens")
             cols, row = table.shape[1], table.stride(0)
-        p_prefix = 0 if prefix_table is None else _vec(prefix_table, -1, at, "prefix_table")
+        elif table is not None or lens is not None:
+            _fail(f"{name}: table and lens go together")
+        if prefix_table is not None:
+            p_prefix = _vec(prefix_table, -1, at, "prefix_table")
         if prefix_len and (prefix_table is None or prefix_table.shape[0] * page < prefix_len):
             _fail(f"{name}: prefix_table is shorter than prefix_len")
+    elif k_pool is not None or v_pool is not None:
+        _fail(f"{name}: k_pool and v_pool go together")
     elif table is not None or lens is not None or prefix_table is not None or prefix_len:
         _fail(f"{name}: a cache needs k_pool and v_pool")
     if out is None:
-        out = torch.empty(shape, dtype=kind, device=q.device)
-    elif out.shape != shape or out.dtype is not kind or out.get_device() != at or out.stride(2) != 1:
-        _fail(f"{name}: out is like q")
-    elif out.requires_grad:
+        out = q.new_empty(shape)
+        os, oh = n_q * dim, dim
+    else:
+        (os, oh, od) = out.stride() if out.dim() == 3 else (0, 0, 0)
+        if out.shape != shape or out.dtype is not kind or out.get_device() != at or od != 1:
+            _fail(f"{name}: out is like q")
+        grad = grad or out.requires_grad
+    if grad:
         _no_graph()
-    _device(q)
-    (qs, qh, _), (os, oh, _), (ks, kh, _), (vs, vh, _) = q.stride(), out.stride(), k.stride(), v.stride()
+    if at < 0:
+        _device(q)
     if scale is None:
         scale = dim ** -0.5
     elif not abs(scale) <= _F32_MAX:  # packing would make it infinite
         _fail(f"{name}: scale is out of range")
     try:
         args = _CHUNK.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p_starts, p_parents, p_k, p_v, p_prefix,
-                           p_table, p_lens, qs, qh, ks, kh, vs, vh, os, oh, ps, ts, hs, row, rows, n, n_q, n_kv, dim, page,
-                           pages, cols, prefix_len, window, scale, _DTYPES.get(kind, -1), _status(status, at))
+                           p_table, p_lens, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0], v_strides[1],
+                           os, oh, ps, ts, hs, row, rows, n, n_q, n_kv, dim, page, pages, cols, prefix_len, window, scale,
+                           _DTYPES.get(kind, -1), _status(status, at))
     except struct.error as e:
         _out_of_range(name, e)
     lib = L.load()
     need = lib.ch_chunk_attention_workspace(args)
     if need:  # torch's caching allocator hands the workspace out in the stream's order
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _run(lib.ch_chunk_attention, at, args, work.data_ptr(), need)
+        _run(lib.ch_chunk_attention, at, args, q.new_empty(need, dtype=torch.uint8).data_ptr(), need)
     else:  # nothing to do, or sizes the call refuses
         _run(lib.ch_chunk_attention, at, args, None, 0)
     return out
