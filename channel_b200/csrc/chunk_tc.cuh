@@ -17,7 +17,7 @@
 // what the tensor cores take (in f16 P is 2^7 larger, so that small weights beside a large one do
 // not fall below the type's range).
 //
-// All tiles of all units, laid end to end with a unit's start counted as kUnitCost tiles, are cut
+// All tiles of all units, laid end to end with a unit's start counted as some tiles, are cut
 // into equal runs, one for each pair; a unit that is cut leaves (O, m, l) of each of its parts in the
 // workspace, and chunk_join_kernel, already resident, adds them.
 //
@@ -38,7 +38,10 @@ namespace {
 constexpr uint32_t kKeys = 128, kRows = 128;  // keys of a tile; rows of a CTA
 constexpr int kSoftWarps = 8, kTcThreads = (4 + kSoftWarps) * 32;
 constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 256 and 384
-constexpr uint32_t kUnitCost = 2;
+// (a 16K prompt of 256-dim heads 1,770 us with 2, 1,719 with 4, 1,738 with 6; 8,192 tokens of 128-dim heads 657 with 3,
+// 664 with 4)
+template <int D>
+constexpr uint32_t kUnitCost = D == 256 ? 4 : 3;
 constexpr uint32_t kItems = 2;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 template <typename T>
@@ -61,6 +64,7 @@ struct Tc {
 };
 
 struct Item {  // a run of one unit's tiles
+  ChunkStream s;
   uint32_t b, h, tok0, tok1;       // stream, kv head, the unit's new tokens [tok0, tok1)
   uint32_t p0, np, c0, nc, n0;     // first tile of each segment and how many tiles the first two have
   uint32_t k0, nt;                 // first tile of the run among the unit's, and how many
@@ -80,7 +84,7 @@ struct TcShared {
   alignas(16) Rec recs[kRecs];
   uint64_t item_full[kItems], item_empty[kItems], rec_full[kRecs], rec_empty[kRecs];
   Item items[kItems];
-  uint32_t v_rows[kSlots];  // keys of a box of the V tile in a slot
+  uint32_t v_info[kSlots];  // of the V tile in a slot: keys of a box, first and last 16 keys of use (in bytes 2 and 3)
   uint32_t tmem_slot, abort_flag;
   uint32_t dead[kSoftWarps];  // a wait of the warp gave up
   float half[2][kRows];       // what the two threads of a row tell each other
@@ -238,11 +242,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   auto stream_cost = [&](uint32_t b) {  // of one kv head
     const ChunkStream s = chunk_stream(a, b);
     unsigned long long c = 0;
-    for (uint32_t t = 0; t < s.count; t += 2 * tpt) c += kUnitCost + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
+    for (uint32_t t = 0; t < s.count; t += 2 * tpt) c += kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
     return c;
   };
-  unsigned long long mine = 0;
-  for (uint32_t b = b0; b < b1; b++) mine += stream_cost(b) * a.nkv;
+  unsigned long long mine = 0, cost = 0;  // cost: of the thread's last stream
+  for (uint32_t b = b0; b < b1; b++) mine += (cost = stream_cost(b)) * a.nkv;
   unsigned long long at = mine, total = 0;  // at: cost of the streams before this thread's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -261,12 +265,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   const unsigned long long run = (total + w.pairs - 1) / w.pairs;
   const unsigned long long first = run * pair, last = min(first + run, total);
   __syncthreads();
-  unsigned long long *found = sums;  // where the stream of the run's start begins
+  unsigned long long *found = sums;  // where the stream of the run's start begins, and its cost
   if (first < last && at <= first && first < at + mine) {
     uint32_t b = b0;
-    for (unsigned long long c; at + (c = stream_cost(b) * a.nkv) <= first; b++) at += c;
+    if (per > 1)
+      for (; at + (cost = stream_cost(b)) * a.nkv <= first; b++) at += cost * a.nkv;
     *begin = b;
-    *found = at;
+    found[0] = at, found[1] = cost;
   }
   __syncwarp();
   tc_fence_before();
@@ -275,7 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   grid_dep_launch();
   const uint32_t tmem = *(volatile uint32_t *)&sh.tmem_slot;
   const uint32_t run_b = *begin;
-  const unsigned long long run_at = *found;
+  const unsigned long long run_at = found[0], run_cost = found[1];
   fence_proxy_async();
   __syncthreads();  // (read before the first copy)
 
@@ -287,21 +292,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     unsigned long long x = run_at;  // start of the unit looked at
     for (uint32_t b = run_b; b < a.n && x < last && ok; b++) {
       const ChunkStream s = chunk_stream(a, b);
-      const unsigned long long c = stream_cost(b);
-      if (x + c * a.nkv <= first) {
-        x += c * a.nkv;
-        continue;
+      uint32_t h = 0;
+      if (b == run_b) {  // the run starts in it
+        h = (uint32_t)((first - x) / run_cost);
+        x += h * run_cost;
       }
-      for (uint32_t h = 0; h < a.nkv && x < last && ok; h++) {
-        if (x + c <= first) {
-          x += c;
-          continue;
-        }
+      for (; h < a.nkv && x < last && ok; h++) {
         for (uint32_t t = 0; t < s.count && x < last && ok; t += 2 * tpt) {
           const uint32_t tok1 = min(s.count, t + 2 * tpt);
           const Tiles u = tiles_of(a, s, t, tok1);
           const uint32_t all = u.all();
-          const unsigned long long k_at = x + kUnitCost;  // place of its first tile
+          const unsigned long long k_at = x + kUnitCost<D>;  // place of its first tile
           const uint32_t k0 = first > k_at ? (uint32_t)min(first - k_at, (unsigned long long)all) : 0u;
           const uint32_t k1 = last > k_at ? (uint32_t)min(last - k_at, (unsigned long long)all) : 0u;
           x = k_at + all;
@@ -310,7 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (n_items >= kItems) ok = tc_wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1, abort, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          Item it{b, h, t, tok1, u.p0, u.np, u.c0, u.nc, u.n0, k0, k1 - k0, 0u};
+          Item it{s, b, h, t, tok1, u.p0, u.np, u.c0, u.nc, u.n0, k0, k1 - k0, 0u};
           if (k0 > 0)
             it.part = 1 + 2 * pair;
           else if (k1 < all) {
@@ -419,8 +420,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       const uint32_t ps = 1u << a.shift, pk = min(ps, kKeys), kb = min(ps, kKeys / 2);
       uint32_t issued = 0, last_seq = 0, loaded_q = 0;
       bool ok = true;
+      auto load_q = [&](uint32_t row0) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
+          for (int g = 0; g < C::kGroups; g++)
+            tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)(row0 + it.tok0 + rank * tpt), &sh.q_full);
+        }
+        loaded_q++;
+        __syncwarp();
+      };
       for (uint32_t k = 0; ok && next_item(); k++) {
-        const uint32_t row0 = chunk_stream(a, it.b).first;
+        const uint32_t row0 = it.s.first;
+        if (!is_v && k == 0) load_q(row0);
         for (uint32_t i = 0; i < it.nt && ok; i++, recs++) {
           const uint32_t r = recs % kRecs;
           ok = tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status);
@@ -431,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           const Rec &rec = sh.recs[r];
           const uint32_t seg = rec.seg & 3, key0 = rec.key0, dst = ring + s * C::kPiece;
           if (lane == 0) {
-            if (is_v) sh.v_rows[s] = seg == 2 ? kKeys : pk;
+            if (is_v) sh.v_info[s] = (seg == 2 ? kKeys : pk) | rec.z0 / 16 << 16 | (rec.z1 + 15) / 16 << 24;
             mbar_arrive_expect_tx(&sh.full[s], is_v ? C::kV : C::kK);
           }
           __syncwarp();
@@ -457,16 +468,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           issued++, last_seq = seq;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
-          if (!is_v && i == 0) {  // Q, behind the first K, which finds room before Q does
-            if (k > 0) ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status));
+          // Q of a later item behind its first K, which finds room before Q does
+          if (!is_v && i == 0 && k > 0) {
+            ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status));
             if (!ok) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
-              for (int g = 0; g < C::kGroups; g++)
-                tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)(row0 + it.tok0 + rank * tpt), &sh.q_full);
-            }
-            loaded_q = k + 1;
-            __syncwarp();
+            load_q(row0);
           }
         }
         base += 2 * it.nt;
@@ -529,7 +535,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (i > 0 && ok) {
             const uint32_t gj = g - 1;
             const uint32_t from = take();
-            if (const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot]; vr != v_rows) {
+            const uint32_t info = *(volatile uint32_t *)&sh.v_info[slot], c0 = info >> 16 & 0xFF, c1 = info >> 24;
+            if (const uint32_t vr = info & 0xFFFF; vr != v_rows) {
               v_rows = vr;
               v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 8u * C::kDv);
 #pragma unroll
@@ -541,8 +548,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
             if (issuer) {
               const uint32_t p = tmem + kSCol + (gj & 1) * kKeys;
+              if (info >> 16 == (kKeys / 16) << 8) {
 #pragma unroll
-              for (uint32_t c = 0; c < kKeys / 16; c++) mma2_ts(tmem, p + c * 8, v_hi + (from + v_at[c]), o_idesc, (i - 1) | c);
+                for (uint32_t c = 0; c < kKeys / 16; c++) mma2_ts(tmem, p + c * 8, v_hi + (from + v_at[c]), o_idesc, (i - 1) | c);
+              } else {  // keys that no row sees are left out, 16 at a time
+#pragma unroll
+                for (uint32_t c = 0; c < kKeys / 16; c++)
+                  if (c >= c0 && c < c1) mma2_ts(tmem, p + c * 8, v_hi + (from + v_at[c]), o_idesc, (i - 1) | (c - c0));
+              }
               commit2(&sh.pv_done);
               if (i == it.nt) commit2(&sh.o_full);
             }
@@ -569,13 +582,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       for (;; items++) {
         const bool got = next_item();
         if (pair_any(bar, !got)) break;
-        const ChunkStream st = chunk_stream(a, it.b);
+        const ChunkStream st = it.s;
         const uint32_t i = it.tok0 + rank * tpt + token;  // this row's token
         const bool valid = token < tpt && i < it.tok1;
         const bool any = __any_sync(0xffffffffu, valid);
-        uint32_t depth = 0;
-        if (valid && a.parents) chunk_report_parent(a, st.first, i);
-        if (valid && a.parents && a.window) depth = chunk_depth(a, st.first, i);
+        const uint32_t depth = valid && a.parents && a.window ? chunk_depth(a, st.first, i) : 0u;
         const ChunkLow lo = chunk_low(a, st, st.before + (a.parents ? depth : i));
         float m = -INFINITY, l = 0.f;
         for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
@@ -596,9 +607,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             mask[0] = rec.mask[half * 2], mask[1] = rec.mask[half * 2 + 1];
             const uint32_t at = key0 + half * 64;
             if (seg == 2 && a.parents) {
+              if (valid && half == 0) chunk_report_parent(a, st.first, i);
               uint32_t own[2] = {0u, 0u};
               int32_t j = valid ? (int32_t)i : -1;
-              for (uint32_t d = depth; j >= (int32_t)at && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, st.first, (uint32_t)j)) {
+              for (uint32_t d = depth; j >= (int32_t)at && (!a.window || d >= lo.fresh); d--, j = chunk_parent(a, st.first, (uint32_t)j)) {
                 const uint32_t x = (uint32_t)j - at;
 #pragma unroll
                 for (int c = 0; c < 2; c++) own[c] |= x / 32 == (uint32_t)c ? 1u << (x & 31) : 0u;
@@ -698,15 +710,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             l += l0 + l1;
             tc_wait_st();
           }
-          // rows of V that no row of the unit sees (before and behind its keys) are cleared: a
-          // weight of 0 must not meet stale bits
-          if (z0 > 0 || z1 < kKeys) {
+          // rows of V that no row of the unit sees but are in the product, up to 15 before and behind its
+          // keys, are cleared: a weight of 0 must not meet stale bits
+          const uint32_t y0 = z0 & 15, y1 = -z1 & 15;
+          if (y0 | y1) {
             const uint32_t seq = base + v_seq(t), slot = seq % C::kSlots;
             ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.full[slot], (seq / C::kSlots) & 1, abort, a.status));
-            const uint32_t vr = *(volatile uint32_t *)&sh.v_rows[slot], n1 = kKeys - z1;
+            const uint32_t vr = *(volatile uint32_t *)&sh.v_info[slot] & 0xFFFF;
             constexpr uint32_t kVecs = C::kDv / 16;  // 16-byte pieces of a key's dims
-            for (uint32_t x = ok ? tid - 128 : ~0u; x < (z0 + n1) * kVecs; x += kSoftWarps * 32) {
-              const uint32_t z = x / kVecs, v = x % kVecs, key = z < z0 ? z : z1 + (z - z0);
+            for (uint32_t x = ok ? tid - 128 : ~0u; x < (y0 + y1) * kVecs; x += kSoftWarps * 32) {
+              const uint32_t y = x / kVecs, v = x % kVecs, key = y < y0 ? z0 - y0 + y : z1 + (y - y0);
               *reinterpret_cast<uint4 *>(sm + C::kQ + slot * C::kPiece + key / vr * vr * C::kDv + ((v >> 3) * vr + key % vr) * 128 +
                                          (v & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -743,6 +756,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           const uint32_t hq = it.h * a.group + qg;
           T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh;
           const float inv = l == 0.f ? 0.f : 1.f / l;
+          float most = 0.f;
 #pragma unroll 1
           for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32], y[16];
@@ -751,7 +765,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const float x0 = __uint_as_float(o[2 * e]) * inv, x1 = __uint_as_float(o[2 * e + 1]) * inv;
-              bad |= !isfinite(x0) || !isfinite(x1);
+              most = max3_nan(most, fabsf(x0), fabsf(x1));
               y[e] = pack2(x0, x1, static_cast<const T *>(nullptr));
             }
             if (valid) {
@@ -760,6 +774,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                 *reinterpret_cast<uint4 *>(out + c + 2 * e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
             }
           }
+          bad = !(most < INFINITY);
         }
         tc_fence_before();
         __syncwarp();
@@ -794,52 +809,83 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// out = sum over a row's parts of O 2^(m - M) / sum of l 2^(m - M); a warp per row of a cut unit.
-constexpr int kJoinWarps = 8;
+// out = sum over a row's parts of O 2^(m - M) / sum of l 2^(m - M); a warp per row of a cut unit,
+// the loads of its first parts on their way before the maxima are known.
+constexpr int kJoinWarps = 8, kJoinRows = 32;  // of a CTA
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w) {
   constexpr int EPL = D / 32;
+  constexpr uint32_t kU = 4;  // parts whose loads are in flight together
   const int lane = threadIdx.x & 31;
-  const uint32_t row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), pair = blockIdx.y;
+  const uint32_t pair = blockIdx.y;
   grid_dep_wait();
   grid_dep_launch();
   const Cut cut = w.cut[pair];
-  const uint32_t tpt = kRows / a.group, rank = row / kRows, token = row % kRows / a.group;
-  const uint32_t i = cut.tok0 + rank * tpt + token, hq = cut.h * a.group + row % kRows % a.group;
-  if (cut.parts == 0 || token >= tpt || i >= cut.tok1) return;
-  // the beginning of the unit in slot 2 pair + 1, the rest in slots 2 (pair + 1), 2 (pair + 2), ...
-  auto at = [&](uint32_t p) { return (size_t)(2 * (pair + p) + (p == 0)) * (2 * kRows) + row; };
-  float top = -INFINITY;
-  for (uint32_t p = lane; p < cut.parts; p += 32) top = fmaxf(top, w.ml[at(p)].x);
-  top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float o[EPL], sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < EPL; e++) o[e] = 0.f;
-  for (uint32_t p = 0; p < cut.parts; p++) {
-    const float2 ml = w.ml[at(p)];
-    const float f = exp2_approx(ml.x - ref);
-    sum = fmaf(ml.y, f, sum);
-    if (f == 0.f) continue;  // a part without a visible position has no O
-    const float *src = w.o + at(p) * D + lane * EPL;
-#pragma unroll
-    for (int e = 0; e < EPL; e++) o[e] = fmaf(src[e], f, o[e]);
-  }
-  bool bad = !isfinite(sum);
-#pragma unroll
-  for (int e = 0; e < EPL; e++) {
-    o[e] = sum == 0.f ? 0.f : o[e] / sum;
-    bad |= !isfinite(o[e]);
-  }
+  if (cut.parts == 0) return;
   const ChunkStream st = chunk_stream(a, cut.b);
-  if (__any_sync(0xffffffffu, bad)) {
-    chunk_row<T, D>(a, st, cut.b, i, hq);
-    return;
-  }
-  T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh + lane * EPL;
+  const uint32_t tpt = kRows / a.group;
+  for (uint32_t row = blockIdx.x * kJoinRows + (threadIdx.x >> 5); row < (blockIdx.x + 1) * kJoinRows; row += kJoinWarps) {
+    const uint32_t rank = row / kRows, token = row % kRows / a.group;
+    const uint32_t i = cut.tok0 + rank * tpt + token, hq = cut.h * a.group + row % kRows % a.group;
+    if (token >= tpt || i >= cut.tok1) continue;
+    // the beginning of the unit in slot 2 pair + 1, the rest in slots 2 (pair + 1), 2 (pair + 2), ...
+    auto at = [&](uint32_t p) { return (size_t)(2 * (pair + p) + (p == 0)) * (2 * kRows) + row; };
+    float v[kU][EPL];
+    auto load = [&](uint32_t p0) {
 #pragma unroll
-  for (int e = 0; e < EPL; e += 2)
-    *reinterpret_cast<uint32_t *>(out + e) = pack2(o[e], o[e + 1], static_cast<const T *>(nullptr));
+      for (uint32_t u = 0; u < kU; u++) {
+        if (p0 + u >= cut.parts) break;
+        const float *src = w.o + at(p0 + u) * D + lane * EPL;
+        if constexpr (EPL == 2) {
+          *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4 *>(&v[u][e]) = *reinterpret_cast<const float4 *>(src + e);
+        }
+      }
+    };
+    load(0);
+    float top = -INFINITY;
+    for (uint32_t p = lane; p < cut.parts; p += 32) top = fmaxf(top, w.ml[at(p)].x);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float o[EPL], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = 0.f;
+    for (uint32_t p0 = 0; p0 < cut.parts; p0 += 32) {
+      float f = 0.f;
+      if (p0 + lane < cut.parts) {
+        const float2 ml = w.ml[at(p0 + lane)];
+        f = exp2_approx(ml.x - ref);
+        sum = fmaf(ml.y, f, sum);
+      }
+      for (uint32_t k = 0; k < 32 && p0 + k < cut.parts; k += kU) {
+        if (p0 + k) load(p0 + k);
+#pragma unroll
+        for (uint32_t u = 0; u < kU; u++) {
+          const float fk = __shfl_sync(0xffffffffu, f, k + u);  // 0 past the last part
+          if (fk == 0.f) continue;  // a part without a visible position has no O
+#pragma unroll
+          for (int e = 0; e < EPL; e++) o[e] = fmaf(v[u][e], fk, o[e]);
+        }
+      }
+    }
+    sum = warp_sum(sum);
+    bool bad = !isfinite(sum);
+#pragma unroll
+    for (int e = 0; e < EPL; e++) {
+      o[e] = sum == 0.f ? 0.f : o[e] / sum;
+      bad |= !isfinite(o[e]);
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+      chunk_row<T, D>(a, st, cut.b, i, hq);
+      continue;
+    }
+    T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh + lane * EPL;
+#pragma unroll
+    for (int e = 0; e < EPL; e += 2)
+      *reinterpret_cast<uint32_t *>(out + e) = pack2(o[e], o[e + 1], static_cast<const T *>(nullptr));
+  }
 }
 
 // ---------------------------------------------------------------------------
