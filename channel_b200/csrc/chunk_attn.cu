@@ -19,7 +19,8 @@ namespace {
 constexpr uint32_t kMaxStreams = 4096;
 
 // ---------------------------------------------------------------------------
-// A warp per (new token, q head): tensors that no tensor map can describe.
+// A warp per (new token, q head): for tensors that no tensor map can describe, and scales that are not
+// positive (the maximum of scale s is not that of s).
 constexpr int kRowWarps = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const __grid_constant__ ChunkArgs a) {
@@ -140,7 +141,7 @@ bool encode_maps(const ChunkArgs &a, CUtensorMap (&maps)[5]) {
 template <typename T, int D>
 cudaError_t launch_t(const ChunkArgs &a, const ChunkWork &w, cudaStream_t s) {
   alignas(64) CUtensorMap maps[5];
-  if (w.pairs && encode_maps<D>(a, maps)) {
+  if (w.pairs && a.scale > 0.f && encode_maps<D>(a, maps)) {
     const cudaError_t e = start_kernel(chunk_tc_kernel<T, D>, dim3(2 * w.pairs), kTcThreads, tc_smem<D>(), s, a, w, maps[0], maps[1],
                                        maps[2], maps[3], maps[4]);
     if (e != cudaSuccess) return e;

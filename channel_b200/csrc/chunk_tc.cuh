@@ -57,9 +57,6 @@ struct Tc {
   static constexpr uint32_t kPiece = kK > kV ? kK : kV;
   static constexpr int kSlots = D == 256 ? 5 : 11;
   static constexpr uint32_t kRecs = D == 256 ? 4 : 6;
-  // of 8 pairs of exponentials, how many go to the FMA pipe (8,192 tokens with D = 128: 726 us with none,
-  // 689 with 2, 758 with 4; with D = 256, whose products take twice as long, 444, 445 and 463)
-  static constexpr int kPoly = D == 256 ? 0 : 2;
   static constexpr uint32_t kMisc = kQ + kSlots * kPiece;
 };
 
@@ -97,10 +94,17 @@ struct Cut {
 };
 struct ChunkWork {
   Cut *cut;    // [pairs], by the pair that begins the unit
-  float *o;    // [2 * pairs][256][D]
+  float *o;    // [2 * pairs] parts of 256 rows (part_at)
   float2 *ml;  // [2 * pairs][256]: maximum (log2), sum
   uint32_t pairs;
 };
+
+// place of column c (a multiple of 8) of a row in a part of O: [D / 8][256][8], so that a warp stores
+// 32 rows' 32 bytes in one piece
+template <int D>
+CH_DEV size_t part_at(uint32_t slot, uint32_t row, uint32_t c) {
+  return (((size_t)slot * (D / 8) + c / 8) * (2 * kRows) + row) * 8 + c % 8;
+}
 
 // tiles of the unit of tokens [tok0, tok1)
 struct Tiles {
@@ -176,29 +180,6 @@ CH_DEV bool pair_any(uint32_t id, bool p) {
       : "memory");
   return r != 0;
 }
-// 2^x of two numbers up to 127 on the FMA pipe: the exponential's pipe takes 16 a cycle and SM, which
-// for 128 x 128 scores is as long as the products of D = 128 take.  x = n + f with |f| <= 1/2 by adding
-// and taking off 1.5 2^23; 2^f by the polynomial of degree 4 with f(0) = 1 and the least relative error
-// on [-1/2, 1/2], 2^-18.4 (a weight is rounded to 2^-9 or 2^-12 next); n into the exponent.  Below
-// -126: 2^-126, as good as nothing beside a row's largest weight of 2^-8 or more.
-CH_DEV void exp2_poly(uint64_t x, float &p0, float &p1) {
-  float x0, x1;
-  halves(x, x0, x1);
-  x = pair_of(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t n = add2(x, pair_of(12582912.f, 12582912.f)), r = add2(n, pair_of(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(r, pair_of(-1.f, -1.f), x);
-  uint64_t y = pair_of(0.009582852944731712f, 0.009582852944731712f);
-  y = fma2(y, f, pair_of(0.055906426161527634f, 0.055906426161527634f));
-  y = fma2(y, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
-  y = fma2(y, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
-  y = fma2(y, f, pair_of(1.f, 1.f));
-  float n0, n1;
-  halves(n, n0, n1);
-  halves(y, p0, p1);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
-}
-
 template <typename T, int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     chunk_tc_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w, const __grid_constant__ CUtensorMap qmap,
@@ -570,8 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       // ---- softmax: two threads, half 0 and 1 of the keys, for a query row ----
       const uint32_t quad = warp & 3, row = quad * 32 + lane, lanes = (quad * 32u) << 16, half = warp >= 8, bar = 1 + quad;
       const uint32_t p_ready = map_shared(smem_u32(sh.p_ready), 0), o_free = map_shared(smem_u32(&sh.o_free), 0);
-      const bool flip = !(a.scale > 0.f);
-      const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
+      const float scale2 = a.scale * 1.44269504088896341f;  // (positive)
       const uint64_t scale22 = pair_of(scale2, scale2);
       const uint32_t token = row / a.group, qg = row % a.group;
       // A row's two warps wait for each other by barriers without a limit, so they leave together: one
@@ -628,12 +608,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           tc_wait_ld();
           float mx = -INFINITY;
           if (any) {
-            if (flip) {  // a scale that is not positive goes into the scores: below it is |scale|
-#pragma unroll
-              for (int c = 0; c < 2; c++)
-#pragma unroll
-                for (int e = 0; e < 32; e++) s[c][e] = a.scale == 0.f ? 0u : s[c][e] ^ 0x80000000u;
-            }
             if (masked) {
 #pragma unroll
               for (int c = 0; c < 2; c++)
@@ -695,12 +669,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               const uint64_t x = fma2(pair_of(__uint_as_float(s[e / 16][2 * (e % 16)]), __uint_as_float(s[e / 16][2 * (e % 16) + 1])),
                                       scale22, low2);
               float p0, p1;
-              if (e % 8 < C::kPoly) {
-                exp2_poly(x, p0, p1);
-              } else {
-                halves(x, p0, p1);
-                p0 = exp2_approx(p0), p1 = exp2_approx(p1);
-              }
+              halves(x, p0, p1);
+              p0 = exp2_approx(p0), p1 = exp2_approx(p1);
               sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
               p[e] = pack2(p0, p1, static_cast<const T *>(nullptr));
             }
@@ -741,7 +711,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (any && it.part) {
           const size_t at_row = (size_t)(it.part - 1) * (2 * kRows) + rank * kRows + row;
           if (valid && half == 0) w.ml[at_row] = make_float2(m - kBias<T>, l);
-          float *po = w.o + at_row * D;
 #pragma unroll 1
           for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32];
@@ -749,30 +718,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             tc_wait_ld();
             if (valid) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) st_global_32b(po + c + e, o + e);
+              for (int e = 0; e < 32; e += 8) st_global_32b(w.o + part_at<D>(it.part - 1, rank * kRows + row, c + e), o + e);
             }
           }
         } else if (any) {
-          const uint32_t hq = it.h * a.group + qg;
-          T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh;
+          // four lanes write 64 bytes of a row (with a lane to a row the stores took 7,000 cycles a unit)
+          T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + (it.h * a.group + qg) * a.oh;
+          if (!valid) out = nullptr;
+          T *rows[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) rows[r] = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)out, (lane & 28) + r));
           const float inv = l == 0.f ? 0.f : 1.f / l;
           float most = 0.f;
 #pragma unroll 1
           for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-            uint32_t o[32], y[16];
+            uint32_t o[32], y[4][4];
             tc_ld32(tmem + lanes + c, o);
             tc_wait_ld();
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const float x0 = __uint_as_float(o[2 * e]) * inv, x1 = __uint_as_float(o[2 * e + 1]) * inv;
               most = max3_nan(most, fabsf(x0), fabsf(x1));
-              y[e] = pack2(x0, x1, static_cast<const T *>(nullptr));
+              y[e / 4][e % 4] = pack2(x0, x1, static_cast<const T *>(nullptr));
             }
-            if (valid) {
+            // 4 x 4 pieces of 16 bytes turned over: y[r] becomes this lane's quarter of row r
 #pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<uint4 *>(out + c + 2 * e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            for (int step = 1; step <= 2; step++) {
+              const bool odd = lane & step;
+#pragma unroll
+              for (int q = 0; q < 2; q++) {
+                const int p = step == 1 ? 2 * q : q;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? y[p][e] : y[p + step][e], step);
+                  if (odd) y[p][e] = got; else y[p + step][e] = got;
+                }
+              }
             }
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              if (rows[r]) *reinterpret_cast<uint4 *>(rows[r] + c + (lane & 3) * 8) = make_uint4(y[r][0], y[r][1], y[r][2], y[r][3]);
           }
           bad = !(most < INFINITY);
         }
@@ -829,13 +814,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __gri
     const uint32_t i = cut.tok0 + rank * tpt + token, hq = cut.h * a.group + row % kRows % a.group;
     if (token >= tpt || i >= cut.tok1) continue;
     // the beginning of the unit in slot 2 pair + 1, the rest in slots 2 (pair + 1), 2 (pair + 2), ...
-    auto at = [&](uint32_t p) { return (size_t)(2 * (pair + p) + (p == 0)) * (2 * kRows) + row; };
+    auto slot = [&](uint32_t p) { return 2 * (pair + p) + (p == 0); };
+    auto at = [&](uint32_t p) { return (size_t)slot(p) * (2 * kRows) + row; };
     float v[kU][EPL];
     auto load = [&](uint32_t p0) {
 #pragma unroll
       for (uint32_t u = 0; u < kU; u++) {
         if (p0 + u >= cut.parts) break;
-        const float *src = w.o + at(p0 + u) * D + lane * EPL;
+        const float *src = w.o + part_at<D>(slot(p0 + u), row, lane * EPL);
         if constexpr (EPL == 2) {
           *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
         } else {
