@@ -12,10 +12,10 @@
 //
 // Two softmax threads own a row, 64 keys of a tile each: S of the tile after the next waits for the
 // product of this P (it lies over P), so the way from S to P is to be short.  (A thread for each row,
-// taking every other tile: 16,384 tokens 1.99 ms, so 1.79.)  O is rescaled only when a row's maximum has grown by more than 2^8
-// since its last scale; a row's sum is kept in f32 before P is rounded to the type of V, which is
-// what the tensor cores take (in f16 P is 2^7 larger, so that small weights beside a large one do
-// not fall below the type's range).
+// taking every other tile: 16,384 tokens 1.99 ms, so 1.79.)  O is rescaled only when a row's maximum
+// has grown by more than 2^8 since its last scale; a row's sum is kept in f32 before P is rounded to
+// the type of V, which is what the tensor cores take (in f16 P is 2^7 larger, so that small weights
+// beside a large one do not fall below the type's range).
 //
 // All tiles of all units, laid end to end with a unit's start counted as some tiles, are cut
 // into equal runs, one for each pair; a unit that is cut leaves (O, m, l) of each of its parts in the
@@ -23,9 +23,16 @@
 //
 // Warps: 0 copies Q and K, 1 copies V, 2 issues the products (in the second CTA: tells the first that
 // its copies have landed), 3 walks the units and looks pages up, 4 to 11 softmax and results (TMEM
-// lanes 32 * (warp % 4); 8 to 11 the second half of the keys, and of
-// O's columns).  Every wait is bounded; one that gives up sets the status word and the
-// abort flag, the roles leave their loops, and what is in flight is waited for (again with a limit).
+// lanes 32 * (warp % 4); 8 to 11 the second half of the keys, and of O's columns).  Every wait is
+// bounded; one that gives up sets the status word and the abort flag, the roles leave their loops,
+// and what is in flight is waited for (again with a limit).
+//
+// Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
+// 256 dims on 8, bf16, 1,706 us (1,290 TFLOP/s; 2,060 us again and again, when the 1,000 W limit
+// holds the clocks at 1,150 MHz); 64 prompts of 37 to 2,048 tokens behind a prefix of 2,048, 818 us
+// (790); 8,192 tokens, 32 q heads of 128 dims on 8, 632 us (870).  A tile's products take 2,048
+// cycles of 256 dims and 1,024 of 128, its softmax from S to P 2,450 of two tiles' overlap: below
+// 256 dims, and where units are short, the softmax threads are what bounds it.
 #pragma once
 #include <cudaTypedefs.h>
 
@@ -38,8 +45,8 @@ namespace {
 constexpr uint32_t kKeys = 128, kRows = 128;  // keys of a tile; rows of a CTA
 constexpr int kSoftWarps = 8, kTcThreads = (4 + kSoftWarps) * 32;
 constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 256 and 384
-// (a 16K prompt of 256-dim heads 1,770 us with 2, 1,719 with 4, 1,738 with 6; 8,192 tokens of 128-dim heads 657 with 3,
-// 664 with 4)
+// what a unit's start costs, in tiles (a 16K prompt of 256-dim heads 1,770 us with 2, 1,719 with 4,
+// 1,738 with 6; 8,192 tokens of 128-dim heads 657 with 3, 664 with 4)
 template <int D>
 constexpr uint32_t kUnitCost = D == 256 ? 4 : 3;
 constexpr uint32_t kItems = 2;
@@ -77,7 +84,7 @@ template <int D>
 struct TcShared {
   static constexpr int kSlots = Tc<D>::kSlots;
   static constexpr uint32_t kRecs = Tc<D>::kRecs;
-  uint64_t full[kSlots], empty[kSlots], q_full, q_empty, s_full[2], p_ready[2], pv_done, o_full, o_free, done;
+  uint64_t full[kSlots], empty[kSlots], q_here, q_full, q_empty, s_full[2], p_ready[2], pv_done, o_full, o_free, done;
   alignas(16) Rec recs[kRecs];
   uint64_t item_full[kItems], item_empty[kItems], rec_full[kRecs], rec_empty[kRecs];
   Item items[kItems];
@@ -199,7 +206,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   if (tid == 0) {
     const uint32_t ctas = rank == 0 ? 2 : 1;  // the first CTA waits for the copies of both
     for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], ctas), mbar_init(&sh.empty[s], 1);
-    mbar_init(&sh.q_full, ctas), mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.q_here, 1), mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1);
     for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 2 * kSoftWarps);
     mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.o_free, 2 * kSoftWarps), mbar_init(&sh.done, 1);
     for (int s = 0; s < kSoftWarps; s++) sh.dead[s] = 0u;
@@ -394,6 +401,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     auto k_seq = [&](uint32_t i) { return i ? 2 * i - 1 : 0u; };
     auto v_seq = [&](uint32_t i) { return i + 1 < it.nt ? 2 * i + 2 : 2 * it.nt - 1; };
     uint32_t base = 0, recs = 0;
+    // The rows of Q behind the unit's last are zeros: products of zeros take less power, and where few
+    // rows are of use the clocks follow from it (64 trees of 16 nodes, again and again: 324 us, so 280).
+    uint32_t zero_from = kRows;  // rows from here on are zeros already
+    auto clear_q = [&]() {       // by the warp that tells that Q is here
+      const uint32_t tok = min(it.tok0 + rank * tpt, it.tok1), used = min(it.tok1 - tok, tpt) * a.group;
+      if (used) zero_from = min(max(zero_from, tpt * a.group), kRows);  // the copy has written the others
+      if (used >= zero_from) return;
+      for (int g = 0; g < C::kGroups; g++)
+        for (uint32_t x = used * 8 + lane; x < zero_from * 8; x += 32)
+          *reinterpret_cast<uint4 *>(sm + g * kRows * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+      zero_from = used;
+      fence_proxy_async();
+      __syncwarp();
+    };
 
     if (warp == 0 || warp == 1) {
       // ---- copies of K (this CTA's 64 keys of a tile) and Q, and of V (its half of the dims) ----
@@ -403,9 +424,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       bool ok = true;
       auto load_q = [&](uint32_t row0) {
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh.q_full, C::kGroups * tpt * a.group * 128);
-          for (int g = 0; g < C::kGroups; g++)
-            tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)(row0 + it.tok0 + rank * tpt), &sh.q_full);
+          if (it.tok0 + rank * tpt < it.tok1) {
+            mbar_arrive_expect_tx(&sh.q_here, C::kGroups * tpt * a.group * 128);
+            for (int g = 0; g < C::kGroups; g++)
+              tma_load_3d(sm + g * kRows * 128, &qmap, g * 64, (int)(it.h * a.group), (int)(row0 + it.tok0 + rank * tpt), &sh.q_here);
+          } else {  // no row of this CTA's
+            mbar_arrive(&sh.q_here);
+          }
         }
         loaded_q++;
         __syncwarp();
@@ -460,14 +485,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       }
       // the last copies have landed (normally long since) before this CTA ends
       if (issued && !ok) tc_wait(&sh.full[last_seq % C::kSlots], (last_seq / C::kSlots) & 1, nullptr, a.status);
-      if (loaded_q && !ok) tc_wait(&sh.q_full, (loaded_q - 1) & 1, nullptr, a.status);
+      if (loaded_q && !ok) tc_wait(&sh.q_here, (loaded_q - 1) & 1, nullptr, a.status);
     } else if (warp == 2 && rank == 1) {
       // ---- this CTA's copies have landed: tell the first CTA ----
       const uint32_t full0 = map_shared(smem_u32(sh.full), 0), q_full0 = map_shared(smem_u32(&sh.q_full), 0);
       bool ok = true;
       for (uint32_t k = 0; ok && next_item(); k++) {
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_full, k & 1, abort, a.status));
-        if (ok && lane == 0) arrive_remote(q_full0);
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
+        if (ok) clear_q();
+        if (ok && lane == 0)  // (once a unit: the zeros are to be seen before the first CTA's products)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(q_full0) : "memory");
         for (uint32_t i = 0; ok && i < 2 * it.nt; i++, base++) {
           ok = __all_sync(0xffffffffu, tc_wait(&sh.full[base % C::kSlots], (base / C::kSlots) & 1, abort, a.status));
           if (ok && lane == 0) arrive_remote(full0 + (base % C::kSlots) * 8);
@@ -494,7 +521,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (++slot == (uint32_t)C::kSlots) slot = 0, phase ^= 1;
       };
       for (uint32_t k = 0; ok && next_item(); k++) {
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_full, k & 1, abort, a.status));
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
+        if (ok) clear_q();
+        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.q_full, k & 1, abort, a.status));
         for (uint32_t i = 0; i <= it.nt && ok; i++) {
           const uint32_t g = g0 + i;
           if (i < it.nt) {
@@ -568,7 +597,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         const bool any = __any_sync(0xffffffffu, valid);
         const uint32_t depth = valid && a.parents && a.window ? chunk_depth(a, st.first, i) : 0u;
         const ChunkLow lo = chunk_low(a, st, st.before + (a.parents ? depth : i));
-        float m = -INFINITY, l = 0.f;
+        float m = valid ? -INFINITY : INFINITY, l = 0.f;  // (other rows: weights of 0, see clear_q)
         for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
           const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes;
           ok = ok && tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status);
