@@ -85,6 +85,7 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
 #pragma unroll
   for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[e]), o[e] = 0.f;
   auto key = [&](const T *k, const T *v) {
+    if (sum != sum) return;  // all of the row is NaN
     float x = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; e++) x = fmaf(qr[e], to_f32(k[lane * EPL + e]), x);
