@@ -28,9 +28,9 @@
 // and what is in flight is waited for (again with a limit).
 //
 // Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
-// 256 dims on 8, bf16, 1,706 us (1,290 TFLOP/s; 2,060 us again and again, when the 1,000 W limit
+// 256 dims on 8, bf16, 1,706 us (1,290 TFLOP/s; 2,010 us again and again, when the 1,000 W limit
 // holds the clocks at 1,150 MHz); 64 prompts of 37 to 2,048 tokens behind a prefix of 2,048, 818 us
-// (790); 8,192 tokens, 32 q heads of 128 dims on 8, 632 us (870).  A tile's products take 2,048
+// (790); 8,192 tokens, 32 q heads of 128 dims on 8, 614 us (895).  A tile's products take 2,048
 // cycles of 256 dims and 1,024 of 128, its softmax from S to P 2,450 of two tiles' overlap: below
 // 256 dims, and where units are short, the softmax threads are what bounds it.
 #pragma once
@@ -226,15 +226,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   // ---- what all units cost, and where this pair's run starts: the same sums in every CTA ----
   unsigned long long *sums = reinterpret_cast<unsigned long long *>(sm);  // (before the first copy)
   uint32_t *begin = reinterpret_cast<uint32_t *>(sm + 8 * (kTcThreads / 32));
-  const uint32_t per = (a.n + kTcThreads - 1) / kTcThreads, b0 = min(a.n, tid * per), b1 = min(a.n, b0 + per);
-  auto stream_cost = [&](uint32_t b) {  // of one kv head
+  // a thread takes a stream or several; a warp one, where there are enough (with both this and the start
+  // of the run found by a warp's lanes together, 16,384 tokens of 16 q heads on one kv head take 1,530 us;
+  // unit after unit by one thread 1,670)
+  const bool by_warp = a.n <= kTcThreads / 32;
+  const uint32_t per = (a.n + kTcThreads - 1) / kTcThreads;
+  const uint32_t b0 = by_warp ? min(a.n, (uint32_t)warp) : min(a.n, tid * per), b1 = min(a.n, b0 + per);
+  auto stream_cost = [&](uint32_t b, uint32_t u, uint32_t step) {  // of one kv head, of units u, u + step, ...
     const ChunkStream s = chunk_stream(a, b);
     unsigned long long c = 0;
-    for (uint32_t t = 0; t < s.count; t += 2 * tpt) c += kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
+    for (uint32_t t = u * 2 * tpt; t < s.count; t += step * 2 * tpt)
+      c += kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
     return c;
   };
   unsigned long long mine = 0, cost = 0;  // cost: of the thread's last stream
-  for (uint32_t b = b0; b < b1; b++) mine += (cost = stream_cost(b)) * a.nkv;
+  if (by_warp) {
+    if (b0 < b1) cost = stream_cost(b0, lane, 32);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+    if (lane == 0) mine = cost * a.nkv;
+  } else {
+    for (uint32_t b = b0; b < b1; b++) mine += (cost = stream_cost(b, 0, 1)) * a.nkv;
+  }
   unsigned long long at = mine, total = 0;  // at: cost of the streams before this thread's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -257,7 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   if (first < last && at <= first && first < at + mine) {
     uint32_t b = b0;
     if (per > 1)
-      for (; at + (cost = stream_cost(b)) * a.nkv <= first; b++) at += cost * a.nkv;
+      for (; at + (cost = stream_cost(b, 0, 1)) * a.nkv <= first; b++) at += cost * a.nkv;
     *begin = b;
     found[0] = at, found[1] = cost;
   }
@@ -280,13 +293,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     unsigned long long x = run_at;  // start of the unit looked at
     for (uint32_t b = run_b; b < a.n && x < last && ok; b++) {
       const ChunkStream s = chunk_stream(a, b);
-      uint32_t h = 0;
-      if (b == run_b) {  // the run starts in it
+      uint32_t h = 0, t0 = 0;
+      if (b == run_b) {  // the run starts in it; units that end before are left out, 32 at a time
         h = (uint32_t)((first - x) / run_cost);
         x += h * run_cost;
+        for (uint32_t out = 32; out == 32 && t0 < s.count;) {
+          const uint32_t t = t0 + lane * 2 * tpt;
+          const uint32_t c = t < s.count ? kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all() : 0u;
+          uint32_t end = c;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += u;
+          }
+          out = __popc(__ballot_sync(0xffffffffu, c && x + end <= first));
+          if (out) x += __shfl_sync(0xffffffffu, end, out - 1);
+          t0 += out * 2 * tpt;
+        }
       }
-      for (; h < a.nkv && x < last && ok; h++) {
-        for (uint32_t t = 0; t < s.count && x < last && ok; t += 2 * tpt) {
+      for (; h < a.nkv && x < last && ok; h++, t0 = 0) {
+        for (uint32_t t = t0; t < s.count && x < last && ok; t += 2 * tpt) {
           const uint32_t tok1 = min(s.count, t + 2 * tpt);
           const Tiles u = tiles_of(a, s, t, tok1);
           const uint32_t all = u.all();
