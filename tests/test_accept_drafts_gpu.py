@@ -103,3 +103,8 @@ def test_captured():
     torch.cuda.synchronize()
     want = walk(*other)
     assert r.counts.tolist() == want[0] and r.next_tokens.tolist() == want[1] and r.kept.tolist() == want[2]
+
+
+@pytest.mark.parametrize("n", [32, 33, 64, 65, 128, 129, 256, 257, 1023, 1024, 1025, 2049])
+def test_stream_counts(n):
+    run(*random_case([(5 * i) % 7 for i in range(n)], n, 2, pad=n % 3))
