@@ -284,7 +284,7 @@ def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table,
     elif table is not None or lens is not None or prefix_table is not None or prefix_len:
         _fail(f"{name}: a cache needs k_pool and v_pool")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os, oh = n_q * dim, dim
     else:
         (os, oh, od) = out.stride() if out.dim() == 3 else (0, 0, 0)
