@@ -145,7 +145,7 @@ cudaError_t launch_t(const ChunkArgs &a, const ChunkWork &w, cudaStream_t s) {
     const cudaError_t e = start_kernel(chunk_tc_kernel<T, D>, dim3(2 * w.pairs), kTcThreads, tc_smem<D>(), s, a, w, maps[0], maps[1],
                                        maps[2], maps[3], maps[4]);
     if (e != cudaSuccess) return e;
-    return start_kernel(chunk_join_kernel<T, D>, dim3(2 * kRows / kJoinRows, w.pairs), kJoinWarps * 32, 0, s, a, w);
+    return start_kernel(chunk_join_kernel<T, D>, dim3(2 * kRows / kJoinRows, w.pairs), kJoinThreads<D>, 0, s, a, w);
   }
   const unsigned long long rows = (unsigned long long)a.n_tokens * a.nq;
   const unsigned long long grid = (rows + kRowWarps - 1) / kRowWarps, most = 16ull * num_sms();
