@@ -45,10 +45,9 @@ namespace {
 constexpr uint32_t kKeys = 128, kRows = 128;  // keys of a tile; rows of a CTA
 constexpr int kSoftWarps = 8, kTcThreads = (4 + kSoftWarps) * 32;
 constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 256 and 384
-// what a unit's start costs, in tiles (a 16K prompt of 256-dim heads 1,770 us with 2, 1,719 with 4,
-// 1,738 with 6; 8,192 tokens of 128-dim heads 657 with 3, 664 with 4)
-template <int D>
-constexpr uint32_t kUnitCost = D == 256 ? 4 : 3;
+// what a unit's start costs, in tiles (256-dim heads: 64 prompts 796 us with 3, 809 with 4, 814 with 6; 128-dim
+// heads: 21 chunks 793 us with 2, 782 with 3, 788 with 5)
+constexpr uint32_t kUnitCost = 3;
 constexpr uint32_t kItems = 2;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 template <typename T>
@@ -236,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     const ChunkStream s = chunk_stream(a, b);
     unsigned long long c = 0;
     for (uint32_t t = u * 2 * tpt; t < s.count; t += step * 2 * tpt)
-      c += kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
+      c += kUnitCost + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all();
     return c;
   };
   unsigned long long mine = 0, cost = 0;  // cost: of the thread's last stream
@@ -299,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         x += h * run_cost;
         for (uint32_t out = 32; out == 32 && t0 < s.count;) {
           const uint32_t t = t0 + lane * 2 * tpt;
-          const uint32_t c = t < s.count ? kUnitCost<D> + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all() : 0u;
+          const uint32_t c = t < s.count ? kUnitCost + tiles_of(a, s, t, min(s.count, t + 2 * tpt)).all() : 0u;
           uint32_t end = c;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -316,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           const uint32_t tok1 = min(s.count, t + 2 * tpt);
           const Tiles u = tiles_of(a, s, t, tok1);
           const uint32_t all = u.all();
-          const unsigned long long k_at = x + kUnitCost<D>;  // place of its first tile
+          const unsigned long long k_at = x + kUnitCost;  // place of its first tile
           const uint32_t k0 = first > k_at ? (uint32_t)min(first - k_at, (unsigned long long)all) : 0u;
           const uint32_t k1 = last > k_at ? (uint32_t)min(last - k_at, (unsigned long long)all) : 0u;
           x = k_at + all;
