@@ -15,7 +15,8 @@
 //
 // Bound: the pass by HBM (a block of 512 f32 logits takes an SM 77 cycles, its share of the bandwidth 85),
 // the rest by latency: the blocks read again come behind what the other CTAs stream.  512 rows of 262,144
-// capped f32 logits 109 us (537 MB, 4.9 TB/s), 777 rows of 100,003 bf16 66 us, one row 17 us a call.
+// capped f32 logits 109 us (537 MB, 4.9 TB/s), 777 rows of 100,003 bf16 61 us, one row 17 us a call;
+// without the cap 512 f32 rows 87 us (6.2 TB/s).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -37,7 +38,7 @@ constexpr uint32_t kMaxBlocks = kMaxVocab / kBlock, kMaxParts = 16, kNear = 512;
 constexpr uint32_t kParts = 8;
 // What a part costs beside its blocks (first loads, the cluster; reading again for the alternatives), in
 // blocks.  512 capped f32 rows of 262,144 with 5 alternatives take 123, 109, 125 and 155 us in 1, 2, 4
-// and 8 parts; 777 16-bit rows of 100,003 with 20 alternatives 68, 78, 112 and 193; one row 47, 30, 22, 20.
+// and 8 parts; 777 16-bit rows of 100,003 with 20 alternatives 60, 71, 102 and 185; one row 47, 30, 22, 20.
 constexpr uint32_t kPartCost = 90, kTopCost = 7;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -322,7 +323,6 @@ __global__ void __launch_bounds__(kThreads, ctas_of(CAP)) score_rows_kernel(cons
   const uint64_t log2e2 = pair_of(kLog2e, kLog2e);
   float m = -INFINITY, s = 0.f, t = 0.f;
   uint32_t before = 0, infinite = 0;
-  constexpr int kU = sizeof(T) == 4 ? 1 : 2;  // blocks whose loads are in flight together
   constexpr int kN = kLane * kRuns;
   auto raise = [&](float m1) {  // m1: largest of the lane's
     if (!(m1 > m)) return;
@@ -412,16 +412,15 @@ __global__ void __launch_bounds__(kThreads, ctas_of(CAP)) score_rows_kernel(cons
     halves(s2, lo, hi), s += lo + hi;
     halves(t2, lo, hi), t += lo + hi;
   };
-  // the next blocks are on their way while these are added
-  Raw<T> next[kU][kRuns];
+  // a warp's next block is on its way while this one is added (two at a time: 777 16-bit rows 67.5 us, so
+  // 61; 512 capped 16-bit rows of 262,144 116 us, so 105: twice the code)
+  Raw<T> next[kRuns];
   auto fetch = [&](uint32_t b) {
+    if (b < blocks) {
 #pragma unroll
-    for (int u = 0; u < kU; u++)
-      if (b + u * kWarps < blocks) {
-#pragma unroll
-        for (int c = 0; c < (int)kRuns; c++)
-          load8(row, (first + b + u * kWarps) * kBlock + c * (kBlock / kRuns) + lane * kLane, a.vocab, vec, next[u][c]);
-      }
+      for (int c = 0; c < (int)kRuns; c++)
+        load8(row, (first + b) * kBlock + c * (kBlock / kRuns) + lane * kLane, a.vocab, vec, next[c]);
+    }
   };
   fetch(warp);
   // (behind the first loads: the target's logit takes two more on end)
@@ -432,21 +431,12 @@ __global__ void __launch_bounds__(kThreads, ctas_of(CAP)) score_rows_kernel(cons
   own_block = at / kBlock;
   given = asked ? clean(value(row[at]), a.lowest) : INFINITY;
   least = asked && given > -INFINITY ? nextafterf(given, -INFINITY) : INFINITY;
-  for (uint32_t b = warp; b < blocks; b += kU * kWarps) {
-    Raw<T> now[kU][kRuns];
+  for (uint32_t b = warp; b < blocks; b += kWarps) {
+    float x[kN];
 #pragma unroll
-    for (int u = 0; u < kU; u++)
-#pragma unroll
-      for (int c = 0; c < (int)kRuns; c++) now[u][c] = next[u][c];
-    fetch(b + kU * kWarps);
-#pragma unroll
-    for (int u = 0; u < kU; u++) {
-      if (b + u * kWarps >= blocks) break;
-      float x[kN];
-#pragma unroll
-      for (int c = 0; c < (int)kRuns; c++) values(now[u][c], x + c * kLane);
-      block(b + u * kWarps, x);
-    }
+    for (int c = 0; c < (int)kRuns; c++) values(next[c], x + c * kLane);
+    fetch(b + kWarps);
+    block(b, x);
   }
 
   // ---- the part's sums ----
