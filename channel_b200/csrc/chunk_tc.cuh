@@ -28,9 +28,9 @@
 // and what is in flight is waited for (again with a limit).
 //
 // Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
-// 256 dims on 8, f16, 1,704 us (1,291 TFLOP/s; 2,010 us again and again, when the 1,000 W limit holds
-// the clocks at 1,150 MHz); 64 prompts of 16 to 2,048 tokens in a window of 1,024, bf16, 816 us (793);
-// 8,192 tokens, 32 q heads of 128 dims on 8, 614 us (895).  A tile's products take 2,048 cycles of
+// 256 dims on 8, f16, 1,688 us (1,303 TFLOP/s; 1,955 us again and again, when the 1,000 W limit holds
+// the clocks at 1,150 MHz); 64 prompts of 16 to 2,048 tokens in a window of 1,024, bf16, 798 us (810);
+// 8,192 tokens, 32 q heads of 128 dims on 8, 624 us (882).  A tile's products take 2,048 cycles of
 // 256 dims and 1,024 of 128, its way from S to P 2,450: below 256 dims, and where units are short,
 // the softmax threads are what bounds it.
 #pragma once

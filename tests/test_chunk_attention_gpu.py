@@ -308,3 +308,12 @@ def test_requires_grad_is_refused():
 def test_many_streams():
     new = [(7 * i) % 5 for i in range(300)]
     both(make(new, [(11 * i) % 40 for i in range(300)], n_q=4, n_kv=1, dim=64, seed=28))
+
+
+@pytest.mark.parametrize("streams", [1, 2, 12, 13])
+@pytest.mark.parametrize("n_q,n_kv,dim", [(16, 1, 64), (8, 2, 128)])
+def test_runs_that_start_far_into_a_stream(streams, n_q, n_kv, dim):
+    """Streams of many units, more of them than a warp has lanes: each pair finds its own first one."""
+    new = [(1100, 7, 640, 0, 333)[i % 5] for i in range(streams)]
+    both(make(new, [(0, 290, 31)[i % 3] for i in range(streams)], prefix=40, n_q=n_q, n_kv=n_kv, dim=dim, dtype=BF16, seed=29))
+    both(make(new, n_q=n_q, n_kv=n_kv, dim=dim, dtype=BF16, seed=30), window=150)
