@@ -230,6 +230,7 @@ int chunk_attention(const ch_chunk_attn_args *p, void *workspace, size_t bytes, 
   a.cols = p->table_cols;
   a.prefix = p->prefix_len;
   a.window = p->window;
+  a.most = p->parents ? kMaxNodes : ~0u;
   a.scale = p->scale;
   a.status = p->status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -7,13 +7,17 @@
 
 namespace ch {
 
+// Nodes of a stream's tree (`most`, where there are parents).  A row walks its path anew for every
+// tile of new keys, so a chain costs the square of its length; a larger tree is reported and left out.
+constexpr uint32_t kMaxNodes = 4096;
+
 struct ChunkArgs {
   const void *q, *k, *v, *k_pool, *v_pool;
   void *out;
   const int32_t *starts, *parents, *prefix_table, *table, *lens;
   long long qs, qh, ks, kh, vs, vh, os, oh;  // token and head strides
   long long page, token, head, ts;           // pool and table strides
-  uint32_t n_tokens, n, nq, nkv, group, shift, n_pages, cols, prefix, window;
+  uint32_t n_tokens, n, nq, nkv, group, shift, n_pages, cols, prefix, window, most;
   float scale;
   uint32_t *status;
 };
@@ -30,6 +34,7 @@ CH_DEV ChunkStream chunk_stream(const ChunkArgs &a, uint32_t b) {
   s.first = (uint32_t)min(max(lo, 0ll), top);
   const uint32_t end = (uint32_t)min(max(hi, 0ll), top);
   s.count = end > s.first ? end - s.first : 0u;
+  if (s.count > a.most) s.count = 0u;
   const long long len = a.lens ? max(a.lens[b], 0) : 0;
   s.cached = (uint32_t)min(len, (long long)a.cols << a.shift);
   s.before = a.prefix + len;
@@ -60,7 +65,8 @@ CH_DEV void chunk_report(const ChunkArgs &a) {
   if (!a.status) return;
   bool bad = false;
   for (uint32_t b = threadIdx.x; b < a.n; b += blockDim.x)
-    bad |= a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > (long long)a.n_tokens;
+    bad |= a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > (long long)a.n_tokens ||
+           (long long)a.starts[b + 1] - a.starts[b] > (long long)a.most;
   if (bad) atomicOr(a.status, DEV_ERR_BAD_LIST);
 }
 CH_DEV void chunk_report_parent(const ChunkArgs &a, uint32_t first, uint32_t i) {

@@ -338,9 +338,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: to
                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``prompt_attention`` where a stream's new tokens are nodes of a tree: parents[row] is the
     node of the stream (an earlier one) that the row's token follows, -1 at a root; rows behind the
-    last parent belong to no stream.  A node sees
-    the prefix, the stream's cached tokens and the nodes on its path, itself among them; it is as
-    many positions behind the cached tokens as there are nodes above it."""
+    last parent belong to no stream.  A node sees the prefix, the stream's cached tokens and the
+    nodes on its path, itself among them; it is as many positions behind the cached tokens as there
+    are nodes above it.  A stream has at most 4096 nodes."""
     if parents is None:
         _fail("tree_attention: parents are needed")
     return _chunk_attention("tree_attention", q, k, v, starts, parents, k_pool, v_pool, table, lens, prefix_table, prefix_len,

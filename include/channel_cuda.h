@@ -521,7 +521,8 @@ int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
  *   parents [n_tokens]: the new tokens are nodes of a tree, parents[row] the node (counted in the
  *     stream, before its own) that a node follows, -1 at a root (status bit 2 for others).  A
  *     node at depth d (0 at a root) is at position t = prefix_len + lens[b] + d and attends to the
- *     prefix, the cached tokens and the nodes on its path, itself among them, in the window.
+ *     prefix, the cached tokens and the nodes on its path, itself among them, in the window.  A
+ *     stream has at most 4096 nodes; one with more is left out (status bit 2).
  * out = softmax(scale q.k) v over these, q head h on kv head h / (n_q / n_kv); zeros when no
  * position is visible.  A position whose score is -inf counts as one that is not.  Rows of no stream are
  * neither read as keys nor written.  out must not overlap q, k or v.

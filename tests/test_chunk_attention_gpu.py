@@ -317,3 +317,20 @@ def test_runs_that_start_far_into_a_stream(streams, n_q, n_kv, dim):
     new = [(1100, 7, 640, 0, 333)[i % 5] for i in range(streams)]
     both(make(new, [(0, 290, 31)[i % 3] for i in range(streams)], prefix=40, n_q=n_q, n_kv=n_kv, dim=dim, dtype=BF16, seed=29))
     both(make(new, n_q=n_q, n_kv=n_kv, dim=dim, dtype=BF16, seed=30), window=150)
+
+
+def test_the_largest_tree_and_a_larger_one():
+    s = make([4096, 5], n_q=1, n_kv=1, dim=64, seed=31)
+    chain = torch.cat([torch.arange(-1, 4095), torch.arange(-1, 4)]).int().cuda()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, b = tree_attention(parents=chain, status=status, **s).double(), prompt_attention(**s).double()
+    check_status(status)
+    assert (a - b).norm() <= 4 * torch.finfo(F16).eps * b.norm()
+    s = make([4097, 5], n_q=1, n_kv=1, dim=64, seed=32)
+    chain = torch.cat([torch.arange(-1, 4096), torch.arange(-1, 4)]).int().cuda()
+    out = torch.full_like(s["q"], 7.0)
+    tree_attention(parents=chain, status=status, out=out, **s)
+    with pytest.raises(ChannelError):
+        check_status(status)
+    b = prompt_attention(**s).double()
+    assert (out[:4097] == 7.0).all() and (out[4097:].double() - b[4097:]).norm() <= 4 * torch.finfo(F16).eps * b[4097:].norm()
