@@ -308,8 +308,9 @@ def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table,
         _out_of_range(name, e)
     lib = L.load()
     need = lib.ch_chunk_attention_workspace(args)
-    if need:  # torch's caching allocator hands the workspace out in the stream's order
-        _run(lib.ch_chunk_attention, at, args, q.new_empty(need, dtype=torch.uint8).data_ptr(), need)
+    if need:  # torch's caching allocator hands the workspace out in the stream's order, once it is let go of
+        work = q.new_empty(need, dtype=torch.uint8)
+        _run(lib.ch_chunk_attention, at, args, work.data_ptr(), need)
     else:  # nothing to do, or sizes the call refuses
         _run(lib.ch_chunk_attention, at, args, None, 0)
     return out
