@@ -110,6 +110,21 @@ def _run(fn, at: int, *args) -> None:
         L.check(rc)
 
 
+def _run_with_workspace(size_of, fn, at: int, t: torch.Tensor, args) -> None:
+    """fn(args, workspace, its bytes, stream) on t's device `at` and its current torch stream."""
+    if at != torch.cuda.current_device():  # the size depends on the device
+        with torch.cuda.device(at):
+            return _run_with_workspace(size_of, fn, at, t, args)
+    need = size_of(args)
+    if need:  # torch's caching allocator hands the workspace out in the stream's order, once it is let go of
+        work = t.new_empty(need, dtype=torch.uint8)
+        rc = fn(args, work.data_ptr(), need, _stream_of(at))
+    else:  # nothing to do, or sizes the call refuses
+        rc = fn(args, None, 0, _stream_of(at))
+    if rc:
+        L.check(rc)
+
+
 def _device(t: torch.Tensor) -> int:
     at = t.get_device()
     if at < 0:
@@ -229,12 +244,7 @@ def prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     except struct.error as e:
         _out_of_range("prefix_attention", e)
     lib = L.load()
-    need = lib.ch_prefix_attention_workspace(args)
-    if need:  # torch's caching allocator hands the workspace out in the stream's order
-        work = q.new_empty(need, dtype=torch.uint8)
-        _run(lib.ch_prefix_attention, at, args, work.data_ptr(), need)
-    else:  # sizes the call refuses
-        _run(lib.ch_prefix_attention, at, args, None, 0)
+    _run_with_workspace(lib.ch_prefix_attention_workspace, lib.ch_prefix_attention, at, q, args)
     return out
 
 
@@ -307,12 +317,7 @@ def _chunk_attention(name: str, q, k, v, starts, parents, k_pool, v_pool, table,
     except struct.error as e:
         _out_of_range(name, e)
     lib = L.load()
-    need = lib.ch_chunk_attention_workspace(args)
-    if need:  # torch's caching allocator hands the workspace out in the stream's order, once it is let go of
-        work = q.new_empty(need, dtype=torch.uint8)
-        _run(lib.ch_chunk_attention, at, args, work.data_ptr(), need)
-    else:  # nothing to do, or sizes the call refuses
-        _run(lib.ch_chunk_attention, at, args, None, 0)
+    _run_with_workspace(lib.ch_chunk_attention_workspace, lib.ch_chunk_attention, at, q, args)
     return out
 
 

@@ -461,7 +461,7 @@ int ch_paged_kv_write(const ch_kv_write_args *args, void *stream);
  * in [0, n_pages) are left out (status bit 2); own positions past table_cols pages are left
  * out too (the window still ends at T), a negative length counts as 0.
  * The shared pages are read once for the whole batch.  workspace: at least
- * ch_prefix_attention_workspace(args) bytes (0 when a size is invalid), 16-byte aligned,
+ * ch_prefix_attention_workspace(args) bytes (of the current device, 0 when a size is invalid), 16-byte aligned,
  * contents irrelevant; calls that may overlap need one each. */
 typedef struct {
   const void *q, *k_pool, *v_pool;
@@ -534,8 +534,8 @@ int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
  * pools 16-byte aligned.  Positions whose page index is not in [0, n_pages) are left out (status
  * bit 2); cached positions past table_cols pages too (the new tokens' positions stay), and a
  * negative length counts as 0.
- * workspace: at least ch_chunk_attention_workspace(args) bytes (0 when a size is invalid),
- * 16-byte aligned, contents irrelevant; calls that may overlap need one each. */
+ * workspace: at least ch_chunk_attention_workspace(args) bytes (of the current device, 0 when a size
+ * is invalid), 16-byte aligned, contents irrelevant; calls that may overlap need one each. */
 typedef struct {
   const void *q, *k, *v;
   void *out;

@@ -66,3 +66,25 @@ def test_the_workspace_lives_until_the_call_returns(call, name, library, monkeyp
     lib = library(lambda: [t() is not None for t in OnDevice.made])
     call()
     assert lib.seen[name] == [True]
+
+
+@pytest.mark.parametrize("call,name", [(chunk_call, "ch_chunk_attention"), (prefix_call, "ch_prefix_attention")])
+def test_the_workspace_is_that_of_the_tensors_device(call, name, library, monkeypatch):
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *why):
+            current[0] = self.before
+
+    monkeypatch.setattr(OnDevice, "index", 1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    lib = library(lambda: current[0])
+    call()
+    assert lib.seen == {f"{name}_workspace": 1, name: 1} and current == [0]
