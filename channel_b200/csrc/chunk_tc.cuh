@@ -677,8 +677,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                 top[(e + c) & 3] = max3_nan(top[(e + c) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
             mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * scale2;
           }
-          // (a NaN grows whatever there is, and stays)
-          auto grows = [&]() { return !(mx <= m + kGrow) && !(m == -INFINITY && mx == -INFINITY); };
+          // (a NaN grows whatever there is, and its sum stays NaN; a tile without a visible key leaves all as it is)
+          auto grows = [&]() { return !(mx <= m + kGrow) && mx != -INFINITY; };
           // P of the second half lies over S of the first: both have read S behind this barrier
           tc_fence_before();
           if (!ok) dead[warp - 4] = 1u;
@@ -902,8 +902,8 @@ __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
       for (uint32_t u = 0; u < kU; u++) {
         if (p0 + u >= cut.parts) break;
         const float2 ml = ml_of(p0 + u);
-        const float f = exp2_approx(ml.x - ref);
-        if (f == 0.f) continue;  // a part without a visible position has no O
+        if (ml.x == -INFINITY) continue;  // a part without a visible position has no O
+        const float f = exp2_approx(ml.x - ref);  // (0 of a part that is not finite is NaN)
         sum = fmaf(ml.y, f, sum);
 #pragma unroll
         for (uint32_t e = 0; e < kJoinCols; e++) o[e] = fmaf(v[u][e], f, o[e]);
