@@ -6,6 +6,7 @@
 // over the visible positions j; m is the running maximum, and sums are f32.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cstring>
 #include <string>
 
@@ -20,7 +21,7 @@ constexpr uint32_t kMaxStreams = 4096;
 
 // ---------------------------------------------------------------------------
 // A warp per (new token, q head): for tensors that no tensor map can describe, and scales that are not
-// positive (the maximum of scale s is not that of s).
+// positive (the maximum of scale s is not that of s) or whose product with log2(e) is not finite.
 constexpr int kRowWarps = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const __grid_constant__ ChunkArgs a) {
@@ -141,7 +142,7 @@ bool encode_maps(const ChunkArgs &a, CUtensorMap (&maps)[5]) {
 template <typename T, int D>
 cudaError_t launch_t(const ChunkArgs &a, const ChunkWork &w, cudaStream_t s) {
   alignas(64) CUtensorMap maps[5];
-  if (w.pairs && a.scale > 0.f && encode_maps<D>(a, maps)) {
+  if (w.pairs && a.scale > 0.f && a.scale < FLT_MAX / kLog2e && encode_maps<D>(a, maps)) {
     const cudaError_t e = start_kernel(chunk_tc_kernel<T, D>, dim3(2 * w.pairs), kTcThreads, tc_smem<D>(), s, a, w, maps[0], maps[1],
                                        maps[2], maps[3], maps[4]);
     if (e != cudaSuccess) return e;

@@ -49,6 +49,7 @@ constexpr uint32_t kTmemCols = 512, kSCol = 256;  // O: columns 0 .. DV - 1; S: 
 // heads: 21 chunks 793 us with 2, 782 with 3, 788 with 5)
 constexpr uint32_t kUnitCost = 3;
 constexpr uint32_t kItems = 2;
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kGrow = 8.f;  // log2 of the growth of a maximum that O is not rescaled for
 template <typename T>
 constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;
@@ -605,7 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       // ---- softmax: two threads, half 0 and 1 of the keys, for a query row ----
       const uint32_t quad = warp & 3, row = quad * 32 + lane, lanes = (quad * 32u) << 16, half = warp >= 8, bar = 1 + quad;
       const uint32_t p_ready = map_shared(smem_u32(sh.p_ready), 0), o_free = map_shared(smem_u32(&sh.o_free), 0);
-      const float scale2 = a.scale * 1.44269504088896341f;  // (positive)
+      const float scale2 = a.scale * kLog2e;  // (positive and finite)
       const uint64_t scale22 = pair_of(scale2, scale2);
       const uint32_t token = row / a.group, qg = row % a.group;
       // A row's two warps wait for each other by barriers without a limit, so they leave together: one

@@ -42,3 +42,16 @@ def test_a_nan_beside_far_larger_scores(dim):
     assert bool(call(s, scale=1.0).isfinite().all())
     s["k_pool"][pages[1], 5] = math.nan  # (with tiles of finite scores behind it in its part)
     assert bool(call(s, scale=1.0).isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [1e38, 2.3e38, 2.4e38, 3.4e38])
+def test_scales_near_the_end_of_f32(scale, dtype):
+    """Scores of -2^-10 scale, 0 and -2^-8 scale: the largest has all the weight."""
+    s = make([3], n_q=1, n_kv=1, dim=64, dtype=dtype, seed=3)
+    s["q"] = torch.zeros_like(s["q"])
+    s["k"] = torch.zeros_like(s["k"])
+    s["q"][..., 0] = 2.0 ** -5
+    s["k"][:, 0, 0] = torch.tensor([-2.0 ** -5, 0.0, -2.0 ** -3])
+    out = call(s, scale=scale)
+    assert torch.equal(out, s["v"][[0, 1, 1]])
