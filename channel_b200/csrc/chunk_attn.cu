@@ -74,7 +74,7 @@ uint32_t tc_pairs() {
   return c > 0 ? (uint32_t)c : 0u;
 }
 
-// workspace: w.cut | w.ml | w.o, each on 256 bytes (parts of O are stored 32 bytes at a time); the
+// workspace: w.cut | w.bad | w.ml | w.o, each on 256 bytes (parts of O are stored 32 bytes at a time); the
 // caller's base is on 16 only, so there is room to align it
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 size_t carve(const ch_chunk_attn_args *p, uint8_t *base, ChunkWork *w) {
@@ -88,6 +88,7 @@ size_t carve(const ch_chunk_attn_args *p, uint8_t *base, ChunkWork *w) {
     return r;
   };
   w->cut = reinterpret_cast<Cut *>(take(w->pairs * sizeof(Cut)));
+  w->bad = reinterpret_cast<uint2 *>(take(w->pairs * 2 * sizeof(uint2)));
   w->ml = reinterpret_cast<float2 *>(take(rows * sizeof(float2)));
   w->o = reinterpret_cast<float *>(take(rows * p->head_dim * sizeof(float)));
   return at + 256 - 16;

@@ -79,6 +79,41 @@ CH_DEV uint32_t chunk_depth(const ChunkArgs &a, uint32_t first, uint32_t i) {
   return d;
 }
 
+// K and V rows of a position for one kv head; null where its page is not in the pool (which is reported)
+template <typename T>
+struct ChunkKey {
+  const T *k, *v;
+};
+// at(x), x = 0 .. n - 1, of every run of positions that new token i of stream s sees: run(n, at) returns
+// false to end the walk.  The last run is the stream's new tokens, in a tree one run per node.
+template <typename T, typename F>
+CH_DEV void chunk_visible(const ChunkArgs &a, const ChunkStream &s, uint32_t b, uint32_t i, uint32_t h, F run) {
+  auto paged = [&](const int32_t *table, uint32_t j) {
+    const int32_t page = table[j >> a.shift];
+    if (page < 0 || (uint32_t)page >= a.n_pages) {
+      if (a.status && (threadIdx.x & 31) == 0) atomicOr(a.status, DEV_ERR_BAD_LIST);
+      return ChunkKey<T>{nullptr, nullptr};
+    }
+    const long long at = page * a.page + (long long)(j & ((1u << a.shift) - 1)) * a.token + h * a.head;
+    return ChunkKey<T>{static_cast<const T *>(a.k_pool) + at, static_cast<const T *>(a.v_pool) + at};
+  };
+  auto fresh = [&](uint32_t j) {
+    const long long at = (long long)s.first + j;
+    return ChunkKey<T>{static_cast<const T *>(a.k) + at * a.ks + h * a.kh, static_cast<const T *>(a.v) + at * a.vs + h * a.vh};
+  };
+  const uint32_t depth = a.parents && a.window ? chunk_depth(a, s.first, i) : 0u;
+  const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? depth : i));
+  if (!run(a.prefix - lo.prefix, [&](uint32_t x) { return paged(a.prefix_table, lo.prefix + x); })) return;
+  if (!run(s.cached - lo.cached, [&](uint32_t x) { return paged(a.table + b * a.ts, lo.cached + x); })) return;
+  if (a.parents) {  // the path to the root, down to the first depth in the window
+    int32_t j = (int32_t)i;
+    for (uint32_t d = depth; j >= 0 && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, s.first, (uint32_t)j))
+      if (!run(1u, [&](uint32_t) { return fresh((uint32_t)j); })) return;
+  } else {
+    run(i + 1 - lo.fresh, [&](uint32_t x) { return fresh(lo.fresh + x); });
+  }
+}
+
 // out row of new token i of stream s and q head hq, by one warp, key after key from the visible
 // ones only: EPL dims per lane.
 template <typename T, int D>
@@ -103,30 +138,11 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
     for (int e = 0; e < EPL; e++) o[e] = fmaf(p, to_f32(v[lane * EPL + e]), o[e] * c);
     m = m1;
   };
-  auto paged = [&](const int32_t *table, uint32_t j) {
-    const int32_t page = table[j >> a.shift];
-    if (page < 0 || (uint32_t)page >= a.n_pages) {
-      if (a.status && lane == 0) atomicOr(a.status, DEV_ERR_BAD_LIST);
-      return;
-    }
-    const long long at = page * a.page + (long long)(j & ((1u << a.shift) - 1)) * a.token + h * a.head;
-    key(static_cast<const T *>(a.k_pool) + at, static_cast<const T *>(a.v_pool) + at);
-  };
-  auto fresh = [&](uint32_t j) {
-    const long long at = (long long)s.first + j;
-    key(static_cast<const T *>(a.k) + at * a.ks + h * a.kh, static_cast<const T *>(a.v) + at * a.vs + h * a.vh);
-  };
-  const uint32_t depth = a.parents && a.window ? chunk_depth(a, s.first, i) : 0u;
-  const ChunkLow lo = chunk_low(a, s, s.before + (a.parents ? depth : i));
-  for (uint32_t j = lo.prefix; j < a.prefix; j++) paged(a.prefix_table, j);
-  for (uint32_t j = lo.cached; j < s.cached; j++) paged(a.table + b * a.ts, j);
-  if (a.parents) {  // the path to the root, down to the first depth in the window
-    int32_t j = (int32_t)i;
-    for (uint32_t d = depth; j >= 0 && (!a.window || d + 1 > lo.fresh); d--, j = chunk_parent(a, s.first, (uint32_t)j))
-      fresh((uint32_t)j);
-  } else {
-    for (uint32_t j = lo.fresh; j <= i; j++) fresh(j);
-  }
+  chunk_visible<T>(a, s, b, i, h, [&](uint32_t n, auto at) {
+    for (uint32_t x = 0; x < n; x++)
+      if (const ChunkKey<T> at_x = at(x); at_x.k) key(at_x.k, at_x.v);
+    return true;
+  });
   T *out = static_cast<T *>(a.out) + row * a.os + hq * a.oh + lane * EPL;
   uint32_t packed[EPL / 2];
 #pragma unroll
@@ -140,6 +156,69 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
     *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
   else
     *reinterpret_cast<uint32_t *>(out) = packed[0];
+}
+
+// Column after column of an out row that the tensor cores left NaN although its sum is not, by one
+// warp.  There a weight of 0 met a value that is not finite: of a key that the row sees (its weight was
+// below the type's range) or of another one of the tile.  What the row sees says what is right: NaN for a NaN or
+// infinities of both signs, otherwise the infinity; without any the row is computed again.  Only values
+// are read until all columns are settled: with one NaN at the start of a prompt of 2,048 tokens, which
+// every row sees, that is a few keys a row.
+template <typename T, int D>
+__device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s, uint32_t b, uint32_t i, uint32_t hq) {
+  constexpr int EPL = D / 32;
+  constexpr uint32_t kAhead = 4;  // keys whose values are on their way together
+  struct alignas(2 * EPL) Vec {
+    uint32_t w[EPL / 2];
+  };
+  const int lane = threadIdx.x & 31;
+  const uint32_t h = hq / a.group, row = s.first + i;
+  T *out = static_cast<T *>(a.out) + row * a.os + hq * a.oh + lane * EPL;
+  uint32_t open = 0, up = 0, down = 0, nan = 0;  // of this lane's columns: to be settled; what was seen
+#pragma unroll
+  for (int e = 0; e < EPL; e++) open |= isnan(to_f32(out[e])) ? 1u << e : 0u;
+  if (!__any_sync(0xffffffffu, open)) return;
+  auto look = [&](const ChunkKey<T> &key) {
+    const T *q = static_cast<const T *>(a.q) + row * a.qs + hq * a.qh + lane * EPL;
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) x = fmaf(to_f32(q[e]), to_f32(key.k[lane * EPL + e]), x);
+    if (warp_sum(x) * a.scale == -INFINITY) return;  // (counts as a key that is not seen)
+#pragma unroll
+    for (int e = 0; e < EPL; e++) {
+      const float v = to_f32(key.v[lane * EPL + e]);
+      nan |= isnan(v) ? 1u << e : 0u, up |= v == INFINITY ? 1u << e : 0u, down |= v == -INFINITY ? 1u << e : 0u;
+    }
+  };
+  chunk_visible<T>(a, s, b, i, h, [&](uint32_t n, auto at) {
+    for (uint32_t x0 = 0; x0 < n; x0 += kAhead) {
+      Vec v[kAhead];
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; u++) {
+        const ChunkKey<T> key = x0 + u < n ? at(x0 + u) : ChunkKey<T>{nullptr, nullptr};
+        v[u] = key.v ? *reinterpret_cast<const Vec *>(key.v + lane * EPL) : Vec{};
+      }
+      uint32_t hits = 0;
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; u++)
+#pragma unroll
+        for (int e = 0; e < EPL; e++)
+          if ((open >> e & 1) && !isfinite(to_f32(reinterpret_cast<const T *>(v[u].w)[e]))) hits |= 1u << u;
+      hits = __reduce_or_sync(0xffffffffu, hits);
+      if (!hits) continue;
+      for (; hits; hits &= hits - 1) look(at(x0 + __ffs(hits) - 1));
+      if (!__any_sync(0xffffffffu, open & ~(nan | (up & down)))) return false;
+    }
+    return true;
+  });
+  if (__any_sync(0xffffffffu, open & ~(nan | up | down))) chunk_row<T, D>(a, s, b, i, hq);
+  const uint32_t one = open & ~nan & (up ^ down);
+#pragma unroll
+  for (int e = 0; e < EPL; e++)
+    if (one >> e & 1) {
+      const uint32_t word = pack2(up >> e & 1 ? INFINITY : -INFINITY, 0.f, static_cast<const T *>(nullptr));
+      *reinterpret_cast<uint16_t *>(out + e) = (uint16_t)word;
+    }
 }
 
 }  // namespace ch

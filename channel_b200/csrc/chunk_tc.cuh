@@ -91,6 +91,7 @@ struct TcShared {
   uint32_t v_info[kSlots];  // of the V tile in a slot: keys of a box, first and last 16 keys of use (in bytes 2 and 3)
   uint32_t tmem_slot, abort_flag;
   uint32_t dead[kSoftWarps];  // a wait of the warp gave up
+  uint32_t bad[2];            // first item, and the one behind the last, with a row for chunk_mend
   float half[2][kRows];       // what the two threads of a row tell each other
 };
 
@@ -98,9 +99,11 @@ struct TcShared {
 // the end or the middle of a unit in pair w's run, 2 w + 1 the beginning of one.
 struct Cut {
   uint32_t b, h, tok0, tok1, parts;
+  uint32_t run_b, run_h, run_tok;  // the first unit of the pair's run
 };
 struct ChunkWork {
   Cut *cut;    // [pairs], by the pair that begins the unit
+  uint2 *bad;  // [pairs][2 CTAs]: TcShared::bad
   float *o;    // [2 * pairs] parts of 256 rows (part_at)
   float2 *ml;  // [2 * pairs][256]: maximum (log2), sum
   uint32_t pairs;
@@ -210,6 +213,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 2 * kSoftWarps);
     mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.o_free, 2 * kSoftWarps), mbar_init(&sh.done, 1);
     for (int s = 0; s < kSoftWarps; s++) sh.dead[s] = 0u;
+    sh.bad[0] = ~0u, sh.bad[1] = 0u;
     for (uint32_t s = 0; s < kItems; s++) mbar_init(&sh.item_full[s], 1), mbar_init(&sh.item_empty[s], 3 + kSoftWarps);
     for (uint32_t s = 0; s < kRecs; s++) mbar_init(&sh.rec_full[s], 1), mbar_init(&sh.rec_empty[s], 2 + kSoftWarps);
     sh.abort_flag = 0u;
@@ -287,7 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 
   if (warp == 3) {
     // ---- units and tiles of the run ----
-    Cut cut{0, 0, 0, 0, 0};
+    Cut cut{};
     uint32_t n_items = 0, n_recs = 0;
     bool ok = true;
     unsigned long long x = run_at;  // start of the unit looked at
@@ -330,8 +334,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             it.part = 1 + 2 * pair;
           else if (k1 < all) {
             it.part = 2 + 2 * pair;
-            cut = Cut{b, h, t, tok1, 1u + (uint32_t)((x - 1) / run) - pair};
+            cut.b = b, cut.h = h, cut.tok0 = t, cut.tok1 = tok1, cut.parts = 1u + (uint32_t)((x - 1) / run) - pair;
           }
+          if (n_items == 0) cut.run_b = b, cut.run_h = h, cut.run_tok = t;
           if (lane == 0) {
             sh.items[slot] = it;
             mbar_arrive(&sh.item_full[slot]);
@@ -693,8 +698,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             pair_sync(bar);
             if (!ok) break;
             const bool grow = grows();
-            // (a score of +inf makes the row's sum NaN, as inf - inf would)
-            const float m1 = grow ? (mx == INFINITY ? NAN : mx) : m, keep = grow ? exp2_approx(m - m1) : 1.f;
+            // (with a maximum of +inf the result is NaN, as inf - inf would be: see chunk_mend)
+            const float m1 = grow ? mx : m, keep = grow ? exp2_approx(m - m1) : 1.f;
             m = m1;
             l *= keep;
             if (t > 0) {
@@ -783,7 +788,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           T *rows[4];
 #pragma unroll
           for (int r = 0; r < 4; r++) rows[r] = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, (unsigned long long)out, (lane & 28) + r));
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = m == INFINITY ? NAN : l == 0.f ? 0.f : 1.f / l;
           float most = 0.f;
 #pragma unroll 1
           for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
@@ -814,25 +819,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             for (int r = 0; r < 4; r++)
               if (rows[r]) *reinterpret_cast<uint4 *>(rows[r] + c + (lane & 3) * 8) = make_uint4(y[r][0], y[r][1], y[r][2], y[r][3]);
           }
-          bad = !(most < INFINITY);
+          // NaN beside a sum that is not, or a maximum that is infinite in the power of 2 only: chunk_mend
+          bad = valid && isnan(most) && (!isnan(l) || m == INFINITY);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_remote(o_free);
-        // A weight of 0 times a value that is not finite, at a key of the tile that this row does
-        // not see, is NaN: such a row is computed again on its own
-        if (pair_any(bar, bad && valid)) {
-          sh.half[half][row] = bad;
-          pair_sync(bar);  // (the rows' stores come before those of the new results)
-          bad |= sh.half[half ^ 1][row] != 0.f;
-          pair_sync(bar);
-        }
-        uint32_t again = half ? 0u : __ballot_sync(0xffffffffu, bad && valid);
-        while (again) {
-          const int x = __ffs(again) - 1;
-          again &= again - 1;
-          chunk_row<T, D>(a, st, it.b, __shfl_sync(0xffffffffu, i, x), it.h * a.group + __shfl_sync(0xffffffffu, qg, x));
-        }
+        // (by the join kernel: here it would keep the other roles waiting)
+        if (__any_sync(0xffffffffu, bad) && lane == 0) atomicMin(&sh.bad[0], items), atomicMax(&sh.bad[1], items + 1);
       }
     }
   }
@@ -842,6 +836,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
+  if (tid == 0) w.bad[blockIdx.x] = make_uint2(sh.bad[0], sh.bad[1]);
   if (warp == 2) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
@@ -853,9 +848,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 // a thread 16 columns of one: a warp reads a part's rows as they lie, and all loads of a unit's first
 // parts are in flight at once.  (A warp per row, one row after the other, took 11.6 us behind the
 // main kernel of 64 trees of 16 nodes, this 7.0; of 21 chunks 15.2 and 7.9.)
-constexpr uint32_t kJoinRows = 32, kJoinCols = 16;
+constexpr uint32_t kJoinRows = 32, kJoinCols = 16;  // (a lane to a row)
 template <int D>
-constexpr uint32_t kJoinThreads = kJoinRows * (D / kJoinCols);
+constexpr uint32_t kJoinWarps = D / kJoinCols;
+template <int D>
+constexpr uint32_t kJoinThreads = 32 * kJoinWarps<D>;
+// A CTA's rows with a NaN that need a second look (chunk_mend), a warp each: `again` of the pair's cut
+// unit, and those of its whole ones.  The kernel waits for nobody here, however long a row takes.
+template <typename T, int D>
+__device__ __noinline__ void chunk_mend_rows(const ChunkArgs &a, const ChunkWork &w, uint32_t again) {
+  const uint32_t warp = threadIdx.x >> 5, row0 = blockIdx.x * kJoinRows, rank = row0 / kRows, tpt = kRows / a.group;
+  const Cut &cut = w.cut[blockIdx.y];
+  auto mend = [&](const ChunkStream &s, uint32_t b, uint32_t h, uint32_t t, uint32_t x) {  // row x of the unit at token t
+    const uint32_t at = (row0 + x) % kRows, i = t + rank * tpt + at / a.group;
+    if (at / a.group < tpt && i < min(s.count, t + 2 * tpt)) chunk_mend<T, D>(a, s, b, i, h * a.group + at % a.group);
+  };
+  if (again) {
+    const ChunkStream s = chunk_stream(a, cut.b);
+    for (uint32_t x = warp; x < kJoinRows; x += kJoinWarps<D>)
+      if (again >> x & 1) mend(s, cut.b, cut.h, cut.tok0, x);
+  }
+  const uint2 items = w.bad[2 * blockIdx.y + rank];
+  if (items.x >= items.y) return;
+  uint32_t b = cut.run_b, h = cut.run_h, t = cut.run_tok;
+  ChunkStream s = chunk_stream(a, b);
+  for (uint32_t n = 0; n < items.y; n++) {
+    for (uint32_t x = warp; n >= items.x && x < kJoinRows; x += kJoinWarps<D>) mend(s, b, h, t, x);
+    t += 2 * tpt;
+    if (t < s.count) continue;
+    t = 0;
+    if (++h < a.nkv) continue;
+    h = 0;
+    do {
+      if (++b >= a.n) return;
+      s = chunk_stream(a, b);
+    } while (!s.count);
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
     chunk_join_kernel(const __grid_constant__ ChunkArgs a, const ChunkWork w) {
@@ -871,7 +901,8 @@ __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
   const uint32_t rank = row / kRows, token = row % kRows / a.group;
   const uint32_t i = cut.tok0 + rank * tpt + token, hq = cut.h * a.group + row % kRows % a.group;
   const bool valid = cut.parts && token < tpt && i < cut.tok1;
-  if (!__any_sync(0xffffffffu, valid)) return;  // (the same in all warps)
+  const uint2 items = w.bad[2 * pair + rank];
+  if (!__any_sync(0xffffffffu, valid) && items.x >= items.y) return;  // (the same in all warps)
   // the beginning of the unit in slot 2 pair + 1, the rest in slots 2 (pair + 1), 2 (pair + 2), ...
   auto slot = [&](uint32_t p) { return 2 * (pair + p) + (p == 0); };
   float v[kU][kJoinCols];
@@ -910,19 +941,12 @@ __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
         for (uint32_t e = 0; e < kJoinCols; e++) o[e] = fmaf(v[u][e], f, o[e]);
       }
     }
-    bad = !isfinite(sum);
 #pragma unroll
     for (uint32_t e = 0; e < kJoinCols; e++) {
       o[e] = sum == 0.f ? 0.f : o[e] / sum;
-      bad |= !isfinite(o[e]);
+      bad |= isnan(o[e]);
     }
-  }
-  const uint32_t mine = __ballot_sync(0xffffffffu, bad);
-  __syncthreads();
-  if (mine && lane == 0) atomicOr(&bad_rows, mine);
-  __syncthreads();
-  uint32_t again = bad_rows;
-  if (valid && !((again >> lane) & 1)) {
+    bad = bad && (!isnan(sum) || top == INFINITY);
     T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh + col;
 #pragma unroll
     for (uint32_t e = 0; e < kJoinCols; e += 8)
@@ -931,13 +955,11 @@ __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
                      pack2(o[e + 4], o[e + 5], static_cast<const T *>(nullptr)),
                      pack2(o[e + 6], o[e + 7], static_cast<const T *>(nullptr)));
   }
-  // a row that is not finite is computed again on its own, a warp each
-  for (uint32_t n = 0; again; n++) {
-    const int x = __ffs(again) - 1;
-    again &= again - 1;
-    if (n % (kJoinThreads<D> / 32) == warp)
-      chunk_row<T, D>(a, st, cut.b, __shfl_sync(0xffffffffu, i, x), __shfl_sync(0xffffffffu, hq, x));
-  }
+  const uint32_t mine = __ballot_sync(0xffffffffu, bad);
+  __syncthreads();
+  if (mine && lane == 0) atomicOr(&bad_rows, mine);
+  __syncthreads();
+  if (bad_rows || items.x < items.y) chunk_mend_rows<T, D>(a, w, bad_rows);
 }
 
 // ---------------------------------------------------------------------------
