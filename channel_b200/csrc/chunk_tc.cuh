@@ -360,17 +360,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             return 2u;
           };
           auto end_of = [&](uint32_t seg) { return seg == 0 ? a.prefix : seg == 1 ? s.cached : tok1; };
+          auto low_of = [&](uint32_t seg) { return seg == 0 ? lo.prefix : seg == 1 ? lo.cached : lo.fresh; };
+          // this lane's page of a tile: one that the unit's rows see something of (those ahead of a window may be gone)
+          auto in_use = [&](uint32_t seg, uint32_t key0) {
+            const uint32_t j = key0 + lane * pk;
+            return seg < 2 && lane < (int)pages && j < end_of(seg) && j + pk > low_of(seg);
+          };
           auto look_up = [&](uint32_t k) {
             uint32_t key0;
             const uint32_t seg = seg_of(k, key0), j = key0 + lane * pk;
-            if (seg == 2 || lane >= (int)pages || j >= end_of(seg)) return -1;
+            if (!in_use(seg, key0)) return -1;
             return seg == 0 ? a.prefix_table[j >> a.shift] : a.table[b * a.ts + (j >> a.shift)];
           };
           int32_t next = look_up(k0);
           for (uint32_t k = k0; k < k1; k++) {
             uint32_t key0;
             const uint32_t seg = seg_of(k, key0), end = end_of(seg);
-            const uint32_t low = seg == 0 ? lo.prefix : seg == 1 ? lo.cached : lo.fresh;
+            const uint32_t low = low_of(seg);
             const int32_t page = next;
             if (k + 1 < k1) next = look_up(k + 1);
             const uint32_t r = n_recs % kRecs;
@@ -378,7 +384,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const bool there = seg == 2 || (page >= 0 && (uint32_t)page < a.n_pages);
-            if (!there && lane < (int)pages && key0 + lane * pk < end && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
+            if (!there && in_use(seg, key0) && a.status) atomicOr(a.status, DEV_ERR_BAD_LIST);
             // (the last token sees from high.* on, the first one up to itself)
             const bool all_in = seg < 2 ? key0 + kKeys <= end : !a.parents && key0 + kKeys <= t + 1;
             const bool all_see = all_in && (seg == 0 ? high.prefix : seg == 1 ? high.cached : high.fresh) <= key0 &&
