@@ -88,7 +88,9 @@ struct TcShared {
   alignas(16) Rec recs[kRecs];
   uint64_t item_full[kItems], item_empty[kItems], rec_full[kRecs], rec_empty[kRecs];
   Item items[kItems];
-  uint32_t v_info[kSlots];  // of the V tile in a slot: keys of a box, first and last 16 keys of use (in bytes 2 and 3)
+  // of the V tile in a slot: keys of a box; how many rows ahead of its keys and behind them are to be zeros (bits
+  // 8 and 12 on); first and last 16 keys of use (bytes 2 and 3)
+  uint32_t v_info[kSlots];
   uint32_t tmem_slot, abort_flag;
   uint32_t dead[kSoftWarps];  // a wait of the warp gave up
   uint32_t bad[2];            // first item, and the one behind the last, with a row for chunk_mend
@@ -157,8 +159,9 @@ CH_DEV void commit2(uint64_t *bar) {
       : "memory");
 }
 // Arrive on the first CTA's barrier.  What it announces is in tensor memory (tcgen05.wait, fence) or
-// was written by copies or behind a proxy fence, so it takes no release of the cluster: that waits for
-// every access of the thread in flight (16,384 tokens took 2.6 ms with it, 2.0 without).
+// was written by copies, so it takes no release of the cluster: that waits for every access of the
+// thread in flight (16,384 tokens took 2.6 ms with it, 2.0 without).  The zeros that threads of the second
+// CTA write into Q and V are announced by mbar_arrive_cluster, and waited for by an acquire of the cluster.
 CH_DEV void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -453,6 +456,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       __syncwarp();
     };
 
+    // Rows of V that no row of the unit sees but are in the product, up to 15 ahead of its keys and
+    // behind them, are zeros: a weight of 0 must not meet stale bits.  (By the same warp, ahead of its wait
+    // for P: by the softmax warps it was on the way from S to P.)
+    auto clear_v = [&](uint32_t slot, uint32_t info) {
+      const uint32_t vr = info & 0xFF, y0 = info >> 8 & 15, y1 = info >> 12 & 15, z0 = (info >> 16 & 0xFF) * 16, z1 = (info >> 24) * 16 - y1;
+      constexpr uint32_t kVecs = C::kDv / 16;  // 16-byte pieces of a key's dims
+      for (uint32_t x = lane; x < (y0 + y1) * kVecs; x += 32) {
+        const uint32_t y = x / kVecs, v = x % kVecs, key = y < y0 ? z0 + y : z1 + (y - y0);
+        *reinterpret_cast<uint4 *>(sm + C::kQ + slot * C::kPiece + key / vr * vr * C::kDv + ((v >> 3) * vr + key % vr) * 128 +
+                                   (v & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      __syncwarp();
+    };
+
     if (warp == 0 || warp == 1) {
       // ---- copies of K (this CTA's 64 keys of a tile) and Q, and of V (its half of the dims) ----
       const bool is_v = warp == 1;
@@ -485,7 +503,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           const Rec &rec = sh.recs[r];
           const uint32_t seg = rec.seg & 3, key0 = rec.key0, dst = ring + s * C::kPiece;
           if (lane == 0) {
-            if (is_v) sh.v_info[s] = (seg == 2 ? kKeys : pk) | rec.z0 / 16 << 16 | (rec.z1 + 15) / 16 << 24;
+            if (is_v)
+              sh.v_info[s] = (seg == 2 ? kKeys : pk) | (rec.z0 & 15) << 8 | (-rec.z1 & 15) << 12 | rec.z0 / 16 << 16 | (rec.z1 + 15) / 16 << 24;
             mbar_arrive_expect_tx(&sh.full[s], is_v ? C::kV : C::kK);
           }
           __syncwarp();
@@ -530,11 +549,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       for (uint32_t k = 0; ok && next_item(); k++) {
         ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
         if (ok) clear_q();
-        if (ok && lane == 0)  // (once a unit: the zeros are to be seen before the first CTA's products)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(q_full0) : "memory");
+        if (ok && lane == 0) mbar_arrive_cluster(q_full0);
         for (uint32_t i = 0; ok && i < 2 * it.nt; i++, base++) {
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.full[base % C::kSlots], (base / C::kSlots) & 1, abort, a.status));
-          if (ok && lane == 0) arrive_remote(full0 + (base % C::kSlots) * 8);
+          const uint32_t slot = base % C::kSlots;
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.full[slot], (base / C::kSlots) & 1, abort, a.status));
+          if (!ok) break;
+          const bool is_v = i + 1 == 2 * it.nt || (i > 0 && i % 2 == 0);
+          const uint32_t info = is_v ? *(volatile uint32_t *)&sh.v_info[slot] : 0u;
+          if (info & 0xFF00) clear_v(slot, info);
+          if (lane == 0) {
+            if (info & 0xFF00) mbar_arrive_cluster(full0 + slot * 8);
+            else arrive_remote(full0 + slot * 8);
+          }
         }
       }
       __syncwarp();
@@ -561,6 +587,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
         if (ok) clear_q();
         ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.q_full, k & 1, abort, a.status));
+        if (ok) (void)mbar_try_wait_cluster(&sh.q_full, k & 1);  // (it is over: acquires the second CTA's zeros)
         for (uint32_t i = 0; i <= it.nt && ok; i++) {
           const uint32_t g = g0 + i;
           if (i < it.nt) {
@@ -583,7 +610,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             const uint32_t gj = g - 1;
             const uint32_t from = take();
             const uint32_t info = *(volatile uint32_t *)&sh.v_info[slot], c0 = info >> 16 & 0xFF, c1 = info >> 24;
-            if (const uint32_t vr = info & 0xFFFF; vr != v_rows) {
+            if (ok && (info & 0xFF00)) {
+              (void)mbar_try_wait_cluster(&sh.full[slot], phase);  // (it is over: acquires the second CTA's zeros)
+              clear_v(slot, info);
+            }
+            if (const uint32_t vr = info & 0xFF; vr != v_rows) {
               v_rows = vr;
               v_hi = v_desc(0, vr * 128, vr > 8 ? 1024u : 8u * C::kDv);
 #pragma unroll
@@ -645,8 +676,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           tc_ld32(scol + half * 64 + 32, s[1]);
           // the tile's record (K was copied by it, so it is there)
           const Rec &rec = sh.recs[recs % kRecs];
-          const uint4 head = *reinterpret_cast<const uint4 *>(&rec);
-          const uint32_t seg = head.x & 3, key0 = head.y, z0 = head.z, z1 = head.w;
+          const uint2 head = *reinterpret_cast<const uint2 *>(&rec);
+          const uint32_t seg = head.x & 3, key0 = head.y;
           const bool masked = any && !(head.x & 4);
           uint32_t mask[2] = {~0u, ~0u};  // which of this thread's keys the row sees
           if (masked) {
@@ -746,27 +777,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             l += l0 + l1;
             tc_wait_st();
           }
-          // rows of V that no row of the unit sees but are in the product, up to 15 before and behind its
-          // keys, are cleared: a weight of 0 must not meet stale bits
-          const uint32_t y0 = z0 & 15, y1 = -z1 & 15;
-          if (y0 | y1) {
-            const uint32_t seq = base + v_seq(t), slot = seq % C::kSlots;
-            ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.full[slot], (seq / C::kSlots) & 1, abort, a.status));
-            const uint32_t vr = *(volatile uint32_t *)&sh.v_info[slot] & 0xFFFF;
-            constexpr uint32_t kVecs = C::kDv / 16;  // 16-byte pieces of a key's dims
-            for (uint32_t x = ok ? tid - 128 : ~0u; x < (y0 + y1) * kVecs; x += kSoftWarps * 32) {
-              const uint32_t y = x / kVecs, v = x % kVecs, key = y < y0 ? z0 - y0 + y : z1 + (y - y0);
-              *reinterpret_cast<uint4 *>(sm + C::kQ + slot * C::kPiece + key / vr * vr * C::kDv + ((v >> 3) * vr + key % vr) * 128 +
-                                         (v & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async();
-          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_remote(p_ready + (g & 1) * 8);
         }
         if (!ok && (dead[quad] | dead[4 + quad])) break;  // (both warps left the loop above)
-        base += 2 * it.nt;
         // ---- the result, or this part of it ----
         ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.o_full, items & 1, abort, a.status));
         tc_fence_after();

@@ -42,3 +42,23 @@ def test_pages_ahead_of_the_window_may_be_gone(page, window, form):
         with pytest.raises(ChannelError):
             check_status(status)
         table[col] = kept
+
+
+@pytest.mark.parametrize("dim,n_q", [(64, 4), (128, 4), (256, 2)])
+@pytest.mark.parametrize("window", [0, 77])
+def test_stale_rows_change_no_bit(dim, n_q, window):
+    """What no token owns, and positions ahead of the window, hold zeros, infinities or NaN: the
+    tensor cores see zeros there, in both CTAs of a pair, so that the results are the same bits."""
+    new, old, prefix = [3, 40, 131, 9] * 10, [300, 129, 7, 601] * 10, 150
+    outs = []
+    for stale in (0.0, float("inf"), float("nan")):
+        s = make(new, old, prefix=prefix, n_q=n_q, n_kv=2, dim=dim, pad=70, seed=11, stale=stale)
+        first = [max(0, prefix + n + 1 - window) if window else 0 for n in old]
+        for b, at in enumerate(first):
+            j = torch.arange(max(0, at - prefix), device="cuda")
+            for p in (s["k_pool"], s["v_pool"]):
+                p[s["table"][b, j // 16].long(), j % 16] = stale
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        outs += [prompt_attention(window=window, status=status, **s)[:sum(new)] for _ in range(5)]
+        check_status(status)
+    assert bool(outs[0].isfinite().all()) and all(torch.equal(x, outs[0]) for x in outs)
