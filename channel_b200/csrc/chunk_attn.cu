@@ -18,6 +18,7 @@ int set_last_error(int code, const std::string &msg);
 
 namespace {
 constexpr uint32_t kMaxStreams = 4096;
+std::atomic<uint64_t> wait_ns{kWaitNs};
 
 // ---------------------------------------------------------------------------
 // A warp per (new token, q head): for tensors that no tensor map can describe, and scales that are not
@@ -235,6 +236,7 @@ int chunk_attention(const ch_chunk_attn_args *p, void *workspace, size_t bytes, 
   a.most = p->parents ? kMaxNodes : ~0u;
   a.scale = p->scale;
   a.status = p->status;
+  a.wait_ns = wait_ns.load(std::memory_order_relaxed);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ChunkWork w;
   carve(p, static_cast<uint8_t *>(workspace), &w);
@@ -258,3 +260,5 @@ extern "C" int ch_chunk_attention(const ch_chunk_attn_args *args, void *workspac
     return CH_ENOMEM;
   }
 }
+// For tests: sets after how many nanoseconds the kernel's waits give up, and returns what was set.
+extern "C" uint64_t ch_test_chunk_wait_ns(uint64_t ns) { return ch::wait_ns.exchange(ns); }

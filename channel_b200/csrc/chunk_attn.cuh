@@ -20,6 +20,7 @@ struct ChunkArgs {
   uint32_t n_tokens, n, nq, nkv, group, shift, n_pages, cols, prefix, window, most;
   float scale;
   uint32_t *status;
+  uint64_t wait_ns;  // after which a wait inside the kernel gives up
 };
 
 // A stream's new tokens [first, first + count) of the packed rows and its cached ones: `cached` of

@@ -25,7 +25,7 @@
 // its copies have landed), 3 walks the units and looks pages up, 4 to 11 softmax and results (TMEM
 // lanes 32 * (warp % 4); 8 to 11 the second half of the keys, and of O's columns).  Every wait is
 // bounded; one that gives up sets the status word and the abort flag, the roles leave their loops,
-// and what is in flight is waited for (again with a limit).
+// and what is in flight, the last copy into each slot among it, is waited for (again with a limit).
 //
 // Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
 // 256 dims on 8, f16, 1,688 us (1,303 TFLOP/s; 1,955 us again and again, when the 1,000 W limit holds
@@ -92,7 +92,9 @@ struct TcShared {
   // 8 and 12 on); first and last 16 keys of use (bytes 2 and 3)
   uint32_t v_info[kSlots];
   uint32_t tmem_slot, abort_flag;
+  uint64_t wait_ns;
   uint32_t dead[kSoftWarps];  // a wait of the warp gave up
+  uint32_t fills[kSlots], q_loads;  // copies into a slot, and of Q, that were issued
   uint32_t bad[2];            // first item, and the one behind the last, with a row for chunk_mend
   float half[2][kRows];       // what the two threads of a row tell each other
 };
@@ -205,13 +207,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   constexpr uint32_t kRecs = C::kRecs;
   const uint32_t ring = smem_u32(sm) + C::kQ;
   volatile uint32_t *abort = &sh.abort_flag;
+  auto wait = [&](uint64_t *bar, uint32_t parity) {  // (the limit is looked up once a wait is not over already)
+    if (mbar_try_wait(bar, parity)) return true;
+    return tc_wait(bar, parity, abort, a.status, false, *(volatile uint64_t *)&sh.wait_ns);
+  };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), pair = blockIdx.x >> 1;
   const uint32_t tpt = kRows / a.group;  // tokens of a CTA
 
   if (tid == 0) {
     const uint32_t ctas = rank == 0 ? 2 : 1;  // the first CTA waits for the copies of both
-    for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], ctas), mbar_init(&sh.empty[s], 1);
+    for (int s = 0; s < C::kSlots; s++) mbar_init(&sh.full[s], ctas), mbar_init(&sh.empty[s], 1), sh.fills[s] = 0u;
     mbar_init(&sh.q_here, 1), mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1);
     for (int s = 0; s < 2; s++) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], 2 * kSoftWarps);
     mbar_init(&sh.pv_done, 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.o_free, 2 * kSoftWarps), mbar_init(&sh.done, 1);
@@ -219,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     sh.bad[0] = ~0u, sh.bad[1] = 0u;
     for (uint32_t s = 0; s < kItems; s++) mbar_init(&sh.item_full[s], 1), mbar_init(&sh.item_empty[s], 3 + kSoftWarps);
     for (uint32_t s = 0; s < kRecs; s++) mbar_init(&sh.rec_full[s], 1), mbar_init(&sh.rec_empty[s], 2 + kSoftWarps);
-    sh.abort_flag = 0u;
+    sh.abort_flag = 0u, sh.q_loads = 0u, sh.wait_ns = a.wait_ns;
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -329,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           x = k_at + all;
           if (k1 <= k0) continue;
           const uint32_t slot = n_items % kItems;
-          if (n_items >= kItems) ok = tc_wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1, abort, a.status);
+          if (n_items >= kItems) ok = wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           Item it{s, b, h, t, tok1, u.p0, u.np, u.c0, u.nc, u.n0, k0, k1 - k0, 0u};
@@ -383,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             const int32_t page = next;
             if (k + 1 < k1) next = look_up(k + 1);
             const uint32_t r = n_recs % kRecs;
-            if (n_recs >= kRecs) ok = tc_wait(&sh.rec_empty[r], (n_recs / kRecs - 1) & 1, abort, a.status);
+            if (n_recs >= kRecs) ok = wait(&sh.rec_empty[r], (n_recs / kRecs - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const bool there = seg == 2 || (page >= 0 && (uint32_t)page < a.n_pages);
@@ -416,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     // the end: an item without tiles
     if (ok) {
       const uint32_t slot = n_items % kItems;
-      if (n_items >= kItems) ok = tc_wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1, abort, a.status);
+      if (n_items >= kItems) ok = wait(&sh.item_empty[slot], (n_items / kItems - 1) & 1);
       if (__all_sync(0xffffffffu, ok) && lane == 0) {
         sh.items[slot].nt = 0;
         mbar_arrive(&sh.item_full[slot]);
@@ -429,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     Item it;
     auto next_item = [&]() {  // false: the run is over, or a wait gave up
       const uint32_t slot = n % kItems;
-      const bool ok = __all_sync(0xffffffffu, tc_wait(&sh.item_full[slot], (n / kItems) & 1, abort, a.status));
+      const bool ok = __all_sync(0xffffffffu, wait(&sh.item_full[slot], (n / kItems) & 1));
       if (!ok) return false;
       it = sh.items[slot];
       __syncwarp();
@@ -475,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       // ---- copies of K (this CTA's 64 keys of a tile) and Q, and of V (its half of the dims) ----
       const bool is_v = warp == 1;
       const uint32_t ps = 1u << a.shift, pk = min(ps, kKeys), kb = min(ps, kKeys / 2);
-      uint32_t issued = 0, last_seq = 0, loaded_q = 0;
+      uint32_t loaded_q = 0;
       bool ok = true;
       auto load_q = [&](uint32_t row0) {
         if (lane == 0) {
@@ -495,9 +501,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (!is_v && k == 0) load_q(row0);
         for (uint32_t i = 0; i < it.nt && ok; i++, recs++) {
           const uint32_t r = recs % kRecs;
-          ok = tc_wait(&sh.rec_full[r], (recs / kRecs) & 1, abort, a.status);
+          ok = wait(&sh.rec_full[r], (recs / kRecs) & 1);
           const uint32_t seq = base + (is_v ? v_seq(i) : k_seq(i)), s = seq % C::kSlots;
-          if (ok && seq >= (uint32_t)C::kSlots) ok = tc_wait(&sh.empty[s], (seq / C::kSlots - 1) & 1, abort, a.status);
+          if (ok && seq >= (uint32_t)C::kSlots) ok = wait(&sh.empty[s], (seq / C::kSlots - 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const Rec &rec = sh.recs[r];
@@ -505,6 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (lane == 0) {
             if (is_v)
               sh.v_info[s] = (seg == 2 ? kKeys : pk) | (rec.z0 & 15) << 8 | (-rec.z1 & 15) << 12 | rec.z0 / 16 << 16 | (rec.z1 + 15) / 16 << 24;
+            sh.fills[s] = seq / C::kSlots + 1;
             mbar_arrive_expect_tx(&sh.full[s], is_v ? C::kV : C::kK);
           }
           __syncwarp();
@@ -527,32 +534,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                             (int)it.h, (int)rec.page[key / pk], &sh.full[s]);
             }
           }
-          issued++, last_seq = seq;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.rec_empty[r]);
           // Q of a later item behind its first K, which finds room before Q does
           if (!is_v && i == 0 && k > 0) {
-            ok = __all_sync(0xffffffffu, tc_wait(&sh.q_empty, (k - 1) & 1, abort, a.status));
+            ok = __all_sync(0xffffffffu, wait(&sh.q_empty, (k - 1) & 1));
             if (!ok) break;
             load_q(row0);
           }
         }
         base += 2 * it.nt;
       }
-      // the last copies have landed (normally long since) before this CTA ends
-      if (issued && !ok) tc_wait(&sh.full[last_seq % C::kSlots], (last_seq / C::kSlots) & 1, nullptr, a.status);
-      if (loaded_q && !ok) tc_wait(&sh.q_here, (loaded_q - 1) & 1, nullptr, a.status);
+      if (!is_v && lane == 0) sh.q_loads = loaded_q;
     } else if (warp == 2 && rank == 1) {
       // ---- this CTA's copies have landed: tell the first CTA ----
       const uint32_t full0 = map_shared(smem_u32(sh.full), 0), q_full0 = map_shared(smem_u32(&sh.q_full), 0);
       bool ok = true;
       for (uint32_t k = 0; ok && next_item(); k++) {
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
+        ok = __all_sync(0xffffffffu, wait(&sh.q_here, k & 1));
         if (ok) clear_q();
         if (ok && lane == 0) mbar_arrive_cluster(q_full0);
         for (uint32_t i = 0; ok && i < 2 * it.nt; i++, base++) {
           const uint32_t slot = base % C::kSlots;
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.full[slot], (base / C::kSlots) & 1, abort, a.status));
+          ok = __all_sync(0xffffffffu, wait(&sh.full[slot], (base / C::kSlots) & 1));
           if (!ok) break;
           const bool is_v = i + 1 == 2 * it.nt || (i > 0 && i % 2 == 0);
           const uint32_t info = is_v ? *(volatile uint32_t *)&sh.v_info[slot] : 0u;
@@ -574,7 +578,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       uint64_t v_hi = 0;
       bool ok = true;
       auto take = [&]() {  // waits for the next piece of the ring, in both CTAs
-        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.full[slot], phase, abort, a.status));
+        ok = __all_sync(0xffffffffu, ok && wait(&sh.full[slot], phase));
         tc_fence_after();
         return (ring + slot * C::kPiece) >> 4;
       };
@@ -584,9 +588,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (++slot == (uint32_t)C::kSlots) slot = 0, phase ^= 1;
       };
       for (uint32_t k = 0; ok && next_item(); k++) {
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.q_here, k & 1, abort, a.status));
+        ok = __all_sync(0xffffffffu, wait(&sh.q_here, k & 1));
         if (ok) clear_q();
-        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.q_full, k & 1, abort, a.status));
+        ok = __all_sync(0xffffffffu, ok && wait(&sh.q_full, k & 1));
         if (ok) (void)mbar_try_wait_cluster(&sh.q_full, k & 1);  // (it is over: acquires the second CTA's zeros)
         for (uint32_t i = 0; i <= it.nt && ok; i++) {
           const uint32_t g = g0 + i;
@@ -620,8 +624,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (uint32_t c = 0; c < kKeys / 16; c++) v_at[c] = c * 16 / vr * (vr * C::kDv / 16) + c * 16 % vr * 8;
             }
-            if (ok && i == 1 && k > 0) ok = tc_wait(&sh.o_free, (k - 1) & 1, abort, a.status);
-            ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.p_ready[gj & 1], (gj >> 1) & 1, abort, a.status));
+            if (ok && i == 1 && k > 0) ok = wait(&sh.o_free, (k - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok && wait(&sh.p_ready[gj & 1], (gj >> 1) & 1));
             tc_fence_after();
             if (!ok) break;
             if (issuer) {
@@ -668,7 +672,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         float m = valid ? -INFINITY : INFINITY, l = 0.f;  // (other rows: weights of 0, see clear_q)
         for (uint32_t t = 0; t < it.nt; t++, g++, recs++) {
           const uint32_t scol = tmem + kSCol + (g & 1) * kKeys + lanes;
-          ok = ok && tc_wait(&sh.s_full[g & 1], (g >> 1) & 1, abort, a.status);
+          ok = ok && wait(&sh.s_full[g & 1], (g >> 1) & 1);
           __syncwarp();
           tc_fence_after();
           uint32_t s[2][32];
@@ -743,7 +747,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               // O is rescaled behind the product of the tile before.  (A barrier can only be asked for the phase
               // that follows one known to be over, while the one after that cannot end: S of this tile came
               // behind the product before that one, and the next product waits for this P.)
-              ok = __all_sync(0xffffffffu, tc_wait(&sh.pv_done, (g - 1) & 1, abort, a.status));
+              ok = __all_sync(0xffffffffu, wait(&sh.pv_done, (g - 1) & 1));
               tc_fence_after();
 #pragma unroll 1
               for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
@@ -783,7 +787,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         }
         if (!ok && (dead[quad] | dead[4 + quad])) break;  // (both warps left the loop above)
         // ---- the result, or this part of it ----
-        ok = __all_sync(0xffffffffu, ok && tc_wait(&sh.o_full, items & 1, abort, a.status));
+        ok = __all_sync(0xffffffffu, ok && wait(&sh.o_full, items & 1));
         tc_fence_after();
         bool bad = false;
         sh.half[half][row] = l;
@@ -854,6 +858,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   __syncwarp();
   // every arrival that a product makes has been made, in both CTAs, and tensor memory is at rest
   tc_wait(&sh.done, 0, nullptr, a.status);
+  __syncthreads();
+  if (*abort) {  // and so are copies that no product has waited for (the second CTA may not have told of its own)
+    if (tid < C::kSlots && sh.fills[tid]) tc_wait(&sh.full[tid], (sh.fills[tid] - 1) & 1, nullptr, a.status, false, kWaitNs / 20);
+    if (tid == 32 && sh.q_loads) tc_wait(&sh.q_here, (sh.q_loads - 1) & 1, nullptr, a.status, false, kWaitNs / 20);
+  }
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();

@@ -80,7 +80,9 @@ CH_DEV void cluster_sync_all() {
 // Bounded mbarrier wait (cluster: acquire at cluster scope, for barriers the other
 // CTA arrives at).  With `abort` it also gives up as soon as another role has
 // aborted; a wait that runs out of time raises the abort flag and the error.
-CH_DEV bool tc_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, bool cluster = false) {
+constexpr uint64_t kWaitNs = 2000000000ull;
+CH_DEV bool tc_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, bool cluster = false,
+                    uint64_t limit = kWaitNs) {
   auto poll = [&]() { return cluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
   if (poll()) return true;
   const uint64_t t0 = globaltimer_ns();
@@ -88,7 +90,7 @@ CH_DEV bool tc_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, ui
     for (int i = 0; i < 32; i++)
       if (poll()) return true;
     if (abort && *abort) return false;
-    if (globaltimer_ns() - t0 > 2000000000ull) break;
+    if (globaltimer_ns() - t0 > limit) break;
   }
   if (abort) *abort = 1u;
   if (err) atomicOr(err, DEV_ERR_TMA_TIMEOUT);
