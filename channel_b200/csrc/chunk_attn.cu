@@ -210,7 +210,7 @@ int chunk_attention(const ch_chunk_attn_args *p, void *workspace, size_t bytes, 
   a.parents = p->parents;
   a.prefix_table = p->prefix_table;
   a.table = p->table;
-  a.lens = p->table_cols ? p->lens : nullptr;
+  a.lens = paged ? p->lens : nullptr;  // (positions count without columns too)
   a.qs = p->q_token_stride;
   a.qh = p->q_head_stride;
   a.ks = p->k_token_stride;

@@ -533,7 +533,7 @@ int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
  * Strides are multiples of 8 elements (any number where the dimension is 1), q, k, v, out and the
  * pools 16-byte aligned.  Positions whose page index is not in [0, n_pages) are left out (status
  * bit 2); cached positions past table_cols pages too (the new tokens' positions stay), and a
- * negative length counts as 0.
+ * negative length counts as 0.  lens may be NULL (all 0) when table_cols is 0.
  * workspace: at least ch_chunk_attention_workspace(args) bytes (of the current device, 0 when a size
  * is invalid), 16-byte aligned, contents irrelevant; calls that may overlap need one each. */
 typedef struct {

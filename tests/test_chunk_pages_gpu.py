@@ -62,3 +62,14 @@ def test_stale_rows_change_no_bit(dim, n_q, window):
         outs += [prompt_attention(window=window, status=status, **s)[:sum(new)] for _ in range(5)]
         check_status(status)
     assert bool(outs[0].isfinite().all()) and all(torch.equal(x, outs[0]) for x in outs)
+
+
+@pytest.mark.parametrize("window", [0, 25, 60])
+def test_lengths_count_without_columns(window):
+    """A table without columns holds no cached token, but the new ones keep their positions."""
+    s = make([10, 3], [0, 0], prefix=50, dim=64, seed=12)
+    s["table"] = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    s["lens"] = torch.tensor([30, 7], dtype=torch.int32, device="cuda")
+    check_close(prompt_attention(window=window, **s), *attend64(**s, window=window))
+    parents = random_parents([10, 3], 12)
+    check_close(tree_attention(parents=parents, window=window, **s), *attend64(**s, parents=parents, window=window))
