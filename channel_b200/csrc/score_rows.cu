@@ -4,8 +4,8 @@
 // With x the (capped) logits of a row, m their maximum, S = sum e^(x - m), T = sum (x - m) e^(x - m):
 //   log p_t = x_t - m - log S,   entropy = -sum p log p = log S - T / S.
 // One pass over the row, cut into equal parts for the CTAs of a cluster: a thread keeps its own
-// running m, S and T (rescaled when its m grows; sums of all threads in 64 bits)
-// and the count of logits in front of the given one.  The alternatives need no second pass: a warp
+// running m, S and T (rescaled when its m grows; f32, as are the sums of a warp's lanes, and those of the
+// warps and parts in 64 bits) and the count of logits in front of the given one.  The alternatives need no second pass: a warp
 // keeps the largest logit of each block of 512, and the k largest logits of a part (equal ones by
 // index) lie in the k blocks with the largest maxima (equal ones by index): if a block is not among
 // them, k blocks each hold a logit that comes before all of its own.  Those blocks are read again for
@@ -577,8 +577,10 @@ __global__ void __launch_bounds__(kThreads, ctas_of(CAP)) score_rows_kernel(cons
   auto logprob = [&](float x) {
     if (x == -INFINITY || (x < INFINITY && all.m == INFINITY)) return -INFINITY;
     if (!CAP && x == INFINITY) return (float)-log_s;
-    const float y = CAP ? a.cap * tanhf(x / a.cap) : x;
-    return (float)((double)y - all.m - log_s);
+    // the cap as the pass computed it, so that the maximum's is m itself; a block takes the polynomial and `any`
+    // does not where x is a rounding away from the border, so not above 0 all the same
+    const float y = CAP ? cap.any(x) : x;
+    return (float)fmin((double)y - all.m - log_s, 0.);
   };
   if (tid == 0) {
     a.logprobs[r] = asked ? logprob(given) : 0.f;
