@@ -132,6 +132,13 @@ class SharedPromptDecoder:
         logits.record_stream(caller)
         return logits
 
+    def _handed_over(self, result: torch.Tensor) -> torch.Tensor:
+        """A result of the context's stream whose memory waits for what the caller queues on its own"""
+        caller = torch.cuda.current_stream(self.device)
+        if caller != self.stream:
+            result.record_stream(caller)
+        return result
+
     def _forward(self, tokens: torch.Tensor, positions: torch.Tensor, attend) -> torch.Tensor:
         """Logits of tokens at positions; attend(layer, q, k, v) gives a layer's attention of f16 q
         over the cache and f32 k, v."""
@@ -210,8 +217,9 @@ class SharedPromptDecoder:
                     found[b].append(rows)
                 lens = plan.lens
             check_status(self.status)
+            scores = [RowScores(*(torch.cat(x) for x in zip(*rows))) for rows in found]
         self.stream.synchronize()
-        return [RowScores(*(torch.cat(x) for x in zip(*rows))) for rows in found]
+        return [RowScores(*map(self._handed_over, x)) for x in scores]
 
     def decode_drafted(self, prompt, streams: int, n_tokens: int, temperature: float = 0.0, seed: int = 1, depth: int = 4,
                        branches: int = 2, chunk: int = 256, **filters) -> list:
@@ -350,7 +358,7 @@ class SharedPromptDecoder:
             if int(result.min()) < 0:  # and what followed took another token's embedding
                 raise L.ChannelError(L.CH_EDEVICE, "decode: a row of logits had nothing to choose from (NaN or -inf throughout)")
         self.stream.synchronize()
-        return result
+        return self._handed_over(result)
 
 
 def main() -> None:

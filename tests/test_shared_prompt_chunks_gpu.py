@@ -130,3 +130,30 @@ def test_drafts_are_accepted(decoder):
     finally:
         SharedPromptDecoder._draft = real
     assert calls == [1]  # one step for the five tokens after the first
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["score", "decode"])
+def test_results_outlive_the_next_call(decoder, what):
+    """Results read by work that is still queued on the caller's stream when they are let go of and
+    the decoder is called again."""
+    def call(seed):
+        texts = [[(seed * 31 + 7 * b + 13 * i) % 4096 for i in range(40)] for b in range(6)]
+        if what == "score":
+            return [t for r in decoder.score(texts, top=3) for t in r]
+        return [decoder.decode(texts[0], 6, 24, chunk=40, temperature=1.0, seed=seed)]
+
+    want = [t.clone() for t in call(1)]
+    call(2)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(400_000_000)  # 0.2 s: longer than the next calls
+            results = call(1)
+            got = [t.clone() for t in results]
+            del results
+            call(2)
+            call(3)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
