@@ -35,6 +35,7 @@ from . import _lib as L
 _DTYPES = {torch.float32: L.CH_F32, torch.float16: L.CH_F16, torch.bfloat16: L.CH_BF16}
 _I32 = torch.int32
 _F32_MAX = torch.finfo(torch.float32).max
+TREE_NODES = 4096  # that a stream's tree may have (tree_attention)
 _NO_PAGES, _BAD = 1 << 5, (1 << 1) | (1 << 2)
 
 # A step makes these calls once per layer, so their host time counts: the argument records
@@ -139,7 +140,8 @@ def check_status(status: torch.Tensor) -> None:
     if bits & _NO_PAGES:
         raise L.ChannelError(L.CH_ENOMEM, "a page plan ran out of pages, table columns, token rows or slot numbers")
     if bits & _BAD:
-        raise L.ChannelError(L.CH_EDEVICE, "a kernel saw a slot or page outside its pool")
+        raise L.ChannelError(L.CH_EDEVICE, "a kernel saw a slot or page outside its pool, a token outside the vocabulary, rows of a "
+                             "stream that fall or end past the last, a parent that is no earlier node, or a tree that is too large")
     if bits:
         raise L.ChannelError(L.CH_ETIMEOUT, "a bounded device wait gave up")
 
@@ -346,7 +348,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: to
     node of the stream (an earlier one) that the row's token follows, -1 at a root; rows behind the
     last parent belong to no stream.  A node sees the prefix, the stream's cached tokens and the
     nodes on its path, itself among them; it is as many positions behind the cached tokens as there
-    are nodes above it.  A stream has at most 4096 nodes."""
+    are nodes above it.  A stream has at most ``TREE_NODES`` nodes."""
     if parents is None:
         _fail("tree_attention: parents are needed")
     return _chunk_attention("tree_attention", q, k, v, starts, parents, k_pool, v_pool, table, lens, prefix_table, prefix_len,

@@ -23,7 +23,7 @@ import torch
 
 from . import _lib as L
 from .engine import GpuContext
-from .paged import PagePlan, _fail, check_status, kv_write, plan_pages, prefix_attention, prompt_attention, tree_attention
+from .paged import TREE_NODES, PagePlan, _fail, check_status, kv_write, plan_pages, prefix_attention, prompt_attention, tree_attention
 from .sampling import RowScores, accept_drafts, sample_rows, score_rows
 
 
@@ -251,6 +251,7 @@ class SharedPromptDecoder:
             end = len(prompt) + n_tokens
             while min(len(x) for x in texts) < end:
                 if min(x[-1] for x in texts) < 0:
+                    check_status(self.status)
                     raise L.ChannelError(L.CH_EDEVICE, "decode_drafted: a row of logits had nothing to choose from")
                 trees = [self._draft(x, depth, branches) if len(x) < end else ([], [], []) for x in texts]
                 tokens, parents, depths, starts = [], [], [], [0]
@@ -288,7 +289,7 @@ class SharedPromptDecoder:
     @staticmethod
     def _draft(text: list, depth: int, branches: int):
         """Tokens, parents and depths of a tree after the text's last token, its root: what followed
-        that token earlier, latest first, paths that begin alike shared."""
+        that token earlier, latest first, paths that begin alike shared; no more than a tree may have."""
         tokens, parents, depths = [text[-1]], [-1], [0]
         found = 0
         for i in range(len(text) - 2, -1, -1):
@@ -303,6 +304,8 @@ class SharedPromptDecoder:
                 if known:
                     at = known[0]
                     continue
+                if len(tokens) == TREE_NODES:
+                    return tokens, parents, depths
                 tokens.append(token)
                 parents.append(at)
                 depths.append(depths[at] + 1)

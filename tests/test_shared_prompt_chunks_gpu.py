@@ -30,6 +30,15 @@ def test_drafts_share_what_begins_alike():
     assert SharedPromptDecoder._draft([1, 2, 3], 3, 2) == ([3], [-1], [0])
 
 
+@pytest.mark.parametrize("depth,branches", [(5000, 2), (3000, 3), (4095, 1), (4096, 1)])
+def test_drafts_are_no_larger_than_a_tree_may_be(depth, branches):
+    body = [9] + list(range(10, 4010))
+    text = sum((body + [4000 + j, *range(10, 3000), j] for j in range(3)), []) + [9]
+    tokens, parents, depths = SharedPromptDecoder._draft(text, depth, branches)
+    assert 1 + min(depth, 4095) <= len(tokens) == len(parents) == len(depths) <= 4096
+    assert parents[0] == -1 and all(0 <= p < i and depths[i] == depths[p] + 1 for i, p in enumerate(parents) if i)
+
+
 @pytest.fixture(scope="module")
 def decoder(ctx):
     return SharedPromptDecoder(ctx, DecoderShape(), 600)
