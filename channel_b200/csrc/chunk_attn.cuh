@@ -162,9 +162,10 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
 // Column after column of an out row that the tensor cores left NaN although its sum is not, by one
 // warp.  There a weight of 0 met a value that is not finite: of a key that the row sees (its weight was
 // below the type's range) or of another one of the tile.  What the row sees says what is right: NaN for a NaN or
-// infinities of both signs, otherwise the infinity; without any the row is computed again.  Only values
-// are read until all columns are settled: with one NaN at the start of a prompt of 2,048 tokens, which
-// every row sees, that is a few keys a row.
+// infinities of both signs, otherwise the infinity; without any the row is computed again.  A row of NaN
+// throughout may have a sum that is NaN, and then no infinity: unless it is to be NaN either way it is
+// computed again too.  Only values are read until all columns are settled: with one NaN at the start of a
+// prompt, which every row sees, that is a few keys a row.
 template <typename T, int D>
 __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s, uint32_t b, uint32_t i, uint32_t hq) {
   constexpr int EPL = D / 32;
@@ -179,6 +180,7 @@ __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s
 #pragma unroll
   for (int e = 0; e < EPL; e++) open |= isnan(to_f32(out[e])) ? 1u << e : 0u;
   if (!__any_sync(0xffffffffu, open)) return;
+  const bool whole = __all_sync(0xffffffffu, open == (1u << EPL) - 1);
   auto look = [&](const ChunkKey<T> &key) {
     const T *q = static_cast<const T *>(a.q) + row * a.qs + hq * a.qh + lane * EPL;
     float x = 0.f;
@@ -212,8 +214,8 @@ __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s
     }
     return true;
   });
-  if (__any_sync(0xffffffffu, open & ~(nan | up | down))) chunk_row<T, D>(a, s, b, i, hq);
-  const uint32_t one = open & ~nan & (up ^ down);
+  const uint32_t one = whole ? 0u : open & ~nan & (up ^ down);
+  if (__any_sync(0xffffffffu, open & ~(nan | one | (up & down)))) chunk_row<T, D>(a, s, b, i, hq);
 #pragma unroll
   for (int e = 0; e < EPL; e++)
     if (one >> e & 1) {

@@ -189,3 +189,25 @@ def test_a_bad_value_behind_a_long_cache(value, at):
         s = poison(s, "new", 150, value)
         ref[150:, :, 3] = value
     check_values(call(s), ref, mass, drift)
+
+
+@pytest.mark.parametrize("form", ["prompt", "tree"])
+@pytest.mark.parametrize("n_q,n_kv,dim", [(2, 1, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("score", [math.nan, math.inf])
+@pytest.mark.parametrize("streams", [1, 90])
+def test_scores_and_values_that_are_not_finite_together(form, n_q, n_kv, dim, score, streams):
+    """Rows that see a score that is not finite are NaN throughout, whatever the values of other keys."""
+    new = [110] * streams if streams == 1 else [41 + i % 7 for i in range(streams)]
+    s = make(new, [30] * streams, n_q=n_q, n_kv=n_kv, dim=dim, seed=13)
+    starts = s["starts"].tolist()
+    s["k"], s["v"] = s["k"].clone(), s["v"].clone()
+    s["q"] = s["q"].clone()
+    s["q"][..., 1] = 0.5  # (the infinity alone decides the score)
+    for at in starts[:-1:max(1, streams // 6)]:
+        s["k"][at + 20, :, 1] = score
+        s["v"][at + 10, :, 3] = math.inf
+        s["v"][at + 20, :, 4:] = -math.inf
+        s["v"][at + 35, :, :] = math.inf
+    parents = random_parents(new, 13) if form == "tree" else None
+    nan = dict(s, k=torch.where(s["k"].isinf(), math.nan, s["k"]))
+    check_values(call(s, parents), *attend64(**nan, parents=parents))
