@@ -136,7 +136,10 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
     const float m1 = fmaxf(m, x), c = m1 == m ? 1.f : expf(m - m1), p = expf(x - m1);
     sum = sum * c + p;
 #pragma unroll
-    for (int e = 0; e < EPL; e++) o[e] = fmaf(p, to_f32(v[lane * EPL + e]), o[e] * c);
+    for (int e = 0; e < EPL; e++) {  // (an infinity stays one, however small its weight)
+      const float y = to_f32(v[lane * EPL + e]), kept = isinf(o[e]) ? o[e] : o[e] * c;
+      o[e] = isinf(y) ? kept + y : fmaf(p, y, kept);
+    }
     m = m1;
   };
   chunk_visible<T>(a, s, b, i, h, [&](uint32_t n, auto at) {
@@ -215,7 +218,10 @@ __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s
     return true;
   });
   const uint32_t one = whole ? 0u : open & ~nan & (up ^ down);
-  if (__any_sync(0xffffffffu, open & ~(nan | one | (up & down)))) chunk_row<T, D>(a, s, b, i, hq);
+  if (__any_sync(0xffffffffu, open & ~(nan | one | (up & down)))) {
+    chunk_row<T, D>(a, s, b, i, hq);
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < EPL; e++)
     if (one >> e & 1) {

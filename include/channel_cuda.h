@@ -524,8 +524,9 @@ int ch_sample_rows(const ch_sample_rows_args *args, void *stream);
  *     prefix, the cached tokens and the nodes on its path, itself among them, in the window.  A
  *     stream has at most 4096 nodes; one with more is left out (status bit 2).
  * out = softmax(scale q.k) v over these, q head h on kv head h / (n_q / n_kv); zeros when no
- * position is visible.  A position whose score is -inf counts as one that is not.  Rows of no stream are
- * neither read as keys nor written.  out must not overlap q, k or v.
+ * position is visible.  A position whose score is -inf counts as one that is not; a score of +inf or NaN makes
+ * the row NaN, and an infinite value the result's dim infinite, however small its weight (NaN beside one of
+ * the other sign).  Rows of no stream are neither read as keys nor written.  out must not overlap q, k or v.
  * q, k, v, out: element (row, head, d) at row * token_stride + head * head_stride + d.  Without
  * a cache prefix_len and table_cols are 0, and the pools, the tables, lens and the page fields are not looked at.
  * head_dim 64, 128 or 256; n_q / n_kv at most 16, n_q at most 1024; n_streams at most 4096;

@@ -211,3 +211,22 @@ def test_scores_and_values_that_are_not_finite_together(form, n_q, n_kv, dim, sc
     parents = random_parents(new, 13) if form == "tree" else None
     nan = dict(s, k=torch.where(s["k"].isinf(), math.nan, s["k"]))
     check_values(call(s, parents), *attend64(**nan, parents=parents))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("below", [25.0, 150.0, 600.0])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+def test_a_token_of_infinities_with_a_small_weight(below, scale, dtype):
+    """All of a key's values are infinite, of alternating sign: so is the result."""
+    s = make([70, 9], [40, 3], n_q=2, n_kv=1, dim=64, dtype=dtype, seed=14)
+    for x in "qk":
+        s[x] = torch.zeros_like(s[x])
+    s["k_pool"] = torch.zeros_like(s["k_pool"])
+    s["q"][..., 0] = 1.0
+    s["k"][20, 0, 0] = -below * scale
+    s["v"] = s["v"].clone()
+    s["v"][20, 0, 0::2], s["v"][20, 0, 1::2] = math.inf, -math.inf
+    s["v"][73, 0, :] = math.inf
+    out = call(s, scale=scale)
+    check_values(out, *attend64(**s, scale=scale))
+    assert bool((out[20:70, :, 0::2] == math.inf).all()) and bool((out[20:70, :, 1::2] == -math.inf).all())
