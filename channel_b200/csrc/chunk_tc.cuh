@@ -207,7 +207,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   constexpr uint32_t kRecs = C::kRecs;
   const uint32_t ring = smem_u32(sm) + C::kQ;
   volatile uint32_t *abort = &sh.abort_flag;
-  auto wait = [&](uint64_t *bar, uint32_t parity) {  // (the limit is looked up once a wait is not over already)
+  // The limit of a wait is a parameter, or looked up in shared memory once the wait is not over at once: the
+  // loops' speed hangs on the code around them (8,192 tokens, 64-dim heads 569 us with the first, 690 with
+  // the second; 128 dims 671 and 621, 256 dims 430 and 414).
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if constexpr (D == 64) return tc_wait(bar, parity, abort, a.status, false, a.wait_ns);
     if (mbar_try_wait(bar, parity)) return true;
     return tc_wait(bar, parity, abort, a.status, false, *(volatile uint64_t *)&sh.wait_ns);
   };
