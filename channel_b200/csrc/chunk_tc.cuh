@@ -22,17 +22,20 @@
 // workspace, and chunk_join_kernel, already resident, adds them.
 //
 // Warps: 0 copies Q and K, 1 copies V, 2 issues the products (in the second CTA: tells the first that
-// its copies have landed), 3 walks the units and looks pages up, 4 to 11 softmax and results (TMEM
+// its copies have landed; in both it clears what of Q and V is to be zeros), 3 walks the units and looks pages up, 4 to 11 softmax and results (TMEM
 // lanes 32 * (warp % 4); 8 to 11 the second half of the keys, and of O's columns).  Every wait is
 // bounded; one that gives up sets the status word and the abort flag, the roles leave their loops,
 // and what is in flight, the last copy into each slot among it, is waited for (again with a limit).
 //
+// A row that sees a value that is not finite, or whose tiles hold one, may come out NaN: such rows are
+// settled by the join kernel (chunk_mend), which waits for nobody.
+//
 // Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
-// 256 dims on 8, f16, 1,688 us (1,303 TFLOP/s; 1,955 us again and again, when the 1,000 W limit holds
-// the clocks at 1,150 MHz); 64 prompts of 16 to 2,048 tokens in a window of 1,024, bf16, 798 us (810);
-// 8,192 tokens, 32 q heads of 128 dims on 8, 624 us (882).  A tile's products take 2,048 cycles of
-// 256 dims and 1,024 of 128, its way from S to P 2,450: below 256 dims, and where units are short,
-// the softmax threads are what bounds it.
+// 256 dims on 8, f16, 1,684 us (1,306 TFLOP/s; 1,937 us again and again, when the 1,000 W limit holds
+// the clocks at 1,150 MHz); 64 prompts of 16 to 2,048 tokens in a window of 1,024, bf16, 788 us (820);
+// 8,192 tokens, 32 q heads on 8, bf16: of 128 dims 622 us (885), of 64 dims 569 (483; half of the second
+// product is zeros).  A tile's products take 2,048 cycles of 256 dims and 1,024 of 128, its way from S to
+// P 2,450: below 256 dims, and where units are short, the softmax threads are what bounds it.
 #pragma once
 #include <cudaTypedefs.h>
 
@@ -880,7 +883,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 // out = sum over a row's parts of O 2^(m - M) / sum of l 2^(m - M).  A CTA takes 32 rows of a cut unit,
 // a thread 16 columns of one: a warp reads a part's rows as they lie, and all loads of a unit's first
-// parts are in flight at once.  (A warp per row, one row after the other, took 11.6 us behind the
+// parts are in flight at once; 20 to 28 bytes spill at 64 registers.  (A warp per row, one row after the other, took 11.6 us behind the
 // main kernel of 64 trees of 16 nodes, this 7.0; of 21 chunks 15.2 and 7.9.)
 constexpr uint32_t kJoinRows = 32, kJoinCols = 16;  // (a lane to a row)
 template <int D>

@@ -15,7 +15,7 @@
 //
 // Bound: the pass by HBM (a block of 512 f32 logits takes an SM 77 cycles, its share of the bandwidth 85),
 // the rest by latency: the blocks read again come behind what the other CTAs stream.  512 rows of 262,144
-// capped f32 logits 109 us (537 MB, 4.9 TB/s), 777 rows of 100,003 bf16 61 us, one row 17 us a call;
+// capped f32 logits 117 us (537 MB, 4.6 TB/s), 777 rows of 100,003 bf16 61 us, one row 17 us a call;
 // without the cap 512 f32 rows 87 us (6.2 TB/s).
 #include <cuda_bf16.h>
 
@@ -42,7 +42,8 @@ constexpr uint32_t kParts = 8;
 constexpr uint32_t kPartCost = 90, kTopCost = 7;
 constexpr float kLog2e = 1.44269504088896341f;
 
-// CTAs on an SM: the polynomial of the cap wants 80 registers
+// CTAs on an SM: the polynomial of the cap wants 80 registers (24 to 28 bytes spill; without it, at 64
+// registers, 64 to 76 bytes)
 constexpr int ctas_of(bool cap) { return cap ? 3 : 4; }
 
 struct ScoreArgs {
