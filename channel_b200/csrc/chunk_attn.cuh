@@ -115,17 +115,24 @@ CH_DEV void chunk_visible(const ChunkArgs &a, const ChunkStream &s, uint32_t b, 
   }
 }
 
+// Whether a row of results up to x in magnitude needs a second look: NaN, or past the type's largest number.
+// An infinity of f16 results is one of the values; the sums of bf16 ones may have left f32.
+CH_DEV bool suspect(float x, const __half *) { return !(x <= 65504.f) && x != INFINITY; }
+CH_DEV bool suspect(float x, const __nv_bfloat16 *) { return !(x <= 3.38953139e38f); }
+
 // out row of new token i of stream s and q head hq, by one warp, key after key from the visible
-// ones only: EPL dims per lane.
+// ones only: EPL dims per lane.  Where the sum of weighted values leaves f32, which bf16 values can make
+// it do, it is taken again of values 2^32 smaller.
 template <typename T, int D>
 __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s, uint32_t b, uint32_t i, uint32_t hq) {
   constexpr int EPL = D / 32;
   const int lane = threadIdx.x & 31;
   const uint32_t h = hq / a.group, row = s.first + i;
   const T *q = static_cast<const T *>(a.q) + row * a.qs + hq * a.qh + lane * EPL;
-  float qr[EPL], o[EPL], m = -INFINITY, sum = 0.f;
+  float qr[EPL], o[EPL], m, sum, shrink = 1.f;
+  uint32_t odd;  // columns with a value that is not finite
 #pragma unroll
-  for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[e]), o[e] = 0.f;
+  for (int e = 0; e < EPL; e++) qr[e] = to_f32(q[e]);
   auto key = [&](const T *k, const T *v) {
     if (sum != sum) return;  // all of the row is NaN
     float x = 0.f;
@@ -137,21 +144,32 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
     sum = sum * c + p;
 #pragma unroll
     for (int e = 0; e < EPL; e++) {  // (an infinity stays one, however small its weight)
-      const float y = to_f32(v[lane * EPL + e]), kept = isinf(o[e]) ? o[e] : o[e] * c;
+      const float y = to_f32(v[lane * EPL + e]) * shrink, kept = isinf(o[e]) ? o[e] : o[e] * c;
       o[e] = isinf(y) ? kept + y : fmaf(p, y, kept);
+      odd |= isfinite(y) ? 0u : 1u << e;
     }
     m = m1;
   };
-  chunk_visible<T>(a, s, b, i, h, [&](uint32_t n, auto at) {
-    for (uint32_t x = 0; x < n; x++)
-      if (const ChunkKey<T> at_x = at(x); at_x.k) key(at_x.k, at_x.v);
-    return true;
-  });
+  for (;;) {
+    m = -INFINITY, sum = 0.f, odd = 0u;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) o[e] = 0.f;
+    chunk_visible<T>(a, s, b, i, h, [&](uint32_t n, auto at) {
+      for (uint32_t x = 0; x < n; x++)
+        if (const ChunkKey<T> at_x = at(x); at_x.k) key(at_x.k, at_x.v);
+      return true;
+    });
+    bool over = false;
+#pragma unroll
+    for (int e = 0; e < EPL; e++) over |= sum == sum && !isfinite(o[e]) && !(odd >> e & 1);
+    if (shrink != 1.f || !__any_sync(0xffffffffu, over)) break;
+    shrink = 0x1p-32f;
+  }
   T *out = static_cast<T *>(a.out) + row * a.os + hq * a.oh + lane * EPL;
   uint32_t packed[EPL / 2];
 #pragma unroll
   for (int e = 0; e < EPL / 2; e++) {
-    const float x = sum == 0.f ? 0.f : o[2 * e] / sum, y = sum == 0.f ? 0.f : o[2 * e + 1] / sum;
+    const float x = sum == 0.f ? 0.f : o[2 * e] / sum / shrink, y = sum == 0.f ? 0.f : o[2 * e + 1] / sum / shrink;
     packed[e] = pack2(x, y, static_cast<const T *>(nullptr));
   }
   if constexpr (EPL == 8)
@@ -162,10 +180,11 @@ __device__ __noinline__ void chunk_row(const ChunkArgs &a, const ChunkStream &s,
     *reinterpret_cast<uint32_t *>(out) = packed[0];
 }
 
-// Column after column of an out row that the tensor cores left NaN although its sum is not, by one
-// warp.  There a weight of 0 met a value that is not finite: of a key that the row sees (its weight was
-// below the type's range) or of another one of the tile.  What the row sees says what is right: NaN for a NaN or
-// infinities of both signs, otherwise the infinity; without any the row is computed again.  A row of NaN
+// Columns of an out row that the tensor cores left NaN or infinite although its sum is finite, by one
+// warp.  In one of NaN a weight of 0 met a value that is not finite: of a key that the row sees (its weight
+// was below the type's range) or of another one of the tile.  What the row sees says what is right: NaN for
+// a NaN or infinities of both signs, otherwise the infinity.  Without any (an infinite column then is one
+// whose sum left f32, or left the type's range by the rounding of the weights) the row is computed again.  A row of NaN
 // throughout may have a sum that is NaN, and then no infinity: unless it is to be NaN either way it is
 // computed again too.  Only values are read until all columns are settled: with one NaN at the start of a
 // prompt, which every row sees, that is a few keys a row.
@@ -179,11 +198,15 @@ __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s
   const int lane = threadIdx.x & 31;
   const uint32_t h = hq / a.group, row = s.first + i;
   T *out = static_cast<T *>(a.out) + row * a.os + hq * a.oh + lane * EPL;
-  uint32_t open = 0, up = 0, down = 0, nan = 0;  // of this lane's columns: to be settled; what was seen
+  uint32_t lost = 0, far = 0, up = 0, down = 0, nan = 0;  // of this lane's columns: NaN, infinite; what was seen
 #pragma unroll
-  for (int e = 0; e < EPL; e++) open |= isnan(to_f32(out[e])) ? 1u << e : 0u;
+  for (int e = 0; e < EPL; e++) {
+    const float x = to_f32(out[e]);
+    lost |= isnan(x) ? 1u << e : 0u, far |= isinf(x) ? 1u << e : 0u;
+  }
+  const uint32_t open = lost | far;
   if (!__any_sync(0xffffffffu, open)) return;
-  const bool whole = __all_sync(0xffffffffu, open == (1u << EPL) - 1);
+  const bool whole = __all_sync(0xffffffffu, lost == (1u << EPL) - 1);
   auto look = [&](const ChunkKey<T> &key) {
     const T *q = static_cast<const T *>(a.q) + row * a.qs + hq * a.qh + lane * EPL;
     float x = 0.f;
@@ -213,7 +236,7 @@ __device__ __noinline__ void chunk_mend(const ChunkArgs &a, const ChunkStream &s
       hits = __reduce_or_sync(0xffffffffu, hits);
       if (!hits) continue;
       for (; hits; hits &= hits - 1) look(at(x0 + __ffs(hits) - 1));
-      if (!__any_sync(0xffffffffu, open & ~(nan | (up & down)))) return false;
+      if (!__any_sync(0xffffffffu, (lost & ~(nan | (up & down))) | (far & ~(nan | up | down)))) return false;
     }
     return true;
   });

@@ -27,8 +27,8 @@
 // bounded; one that gives up sets the status word and the abort flag, the roles leave their loops,
 // and what is in flight, the last copy into each slot among it, is waited for (again with a limit).
 //
-// A row that sees a value that is not finite, or whose tiles hold one, may come out NaN: such rows are
-// settled by the join kernel (chunk_mend), which waits for nobody.
+// A row that sees a value that is not finite, or whose tiles hold one, may come out NaN: rows that are not
+// finite are settled by the join kernel (chunk_mend), which waits for nobody.
 //
 // Measured, at full clocks, of the products' 1,637 TFLOP/s: a prompt of 16,384 tokens, 16 q heads of
 // 256 dims on 8, f16, 1,684 us (1,306 TFLOP/s; 1,937 us again and again, when the 1,000 W limit holds
@@ -851,8 +851,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             for (int r = 0; r < 4; r++)
               if (rows[r]) *reinterpret_cast<uint4 *>(rows[r] + c + (lane & 3) * 8) = make_uint4(y[r][0], y[r][1], y[r][2], y[r][3]);
           }
-          // NaN beside a sum that is not, or a maximum that is infinite in the power of 2 only: chunk_mend
-          bad = valid && isnan(most) && (!isnan(l) || m == INFINITY);
+          // not finite beside a sum that is, or a maximum that is infinite in the power of 2 only: chunk_mend
+          bad = valid && suspect(most, static_cast<const T *>(nullptr)) && (!isnan(l) || m == INFINITY);
         }
         tc_fence_before();
         __syncwarp();
@@ -890,7 +890,7 @@ template <int D>
 constexpr uint32_t kJoinWarps = D / kJoinCols;
 template <int D>
 constexpr uint32_t kJoinThreads = 32 * kJoinWarps<D>;
-// A CTA's rows with a NaN that need a second look (chunk_mend), a warp each: `again` of the pair's cut
+// A CTA's rows that are not finite and need a second look (chunk_mend), a warp each: `again` of the pair's cut
 // unit, and those of its whole ones.  The kernel waits for nobody here, however long a row takes.
 template <typename T, int D>
 __device__ __noinline__ void chunk_mend_rows(const ChunkArgs &a, const ChunkWork &w, uint32_t again) {
@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(kJoinThreads<D>, 1024 / kJoinThreads<D>)
 #pragma unroll
     for (uint32_t e = 0; e < kJoinCols; e++) {
       o[e] = sum == 0.f ? 0.f : o[e] / sum;
-      bad |= isnan(o[e]);
+      bad |= suspect(fabsf(o[e]), static_cast<const T *>(nullptr));
     }
     bad = bad && (!isnan(sum) || top == INFINITY);
     T *out = static_cast<T *>(a.out) + (long long)(st.first + i) * a.os + hq * a.oh + col;

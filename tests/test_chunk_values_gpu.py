@@ -230,3 +230,30 @@ def test_a_token_of_infinities_with_a_small_weight(below, scale, dtype):
     out = call(s, scale=scale)
     check_values(out, *attend64(**s, scale=scale))
     assert bool((out[20:70, :, 0::2] == math.inf).all()) and bool((out[20:70, :, 1::2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype,most", [(F16, 65504.0), (BF16, torch.finfo(BF16).max)])
+@pytest.mark.parametrize("scale", [None, -0.1])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_values_at_the_end_of_the_type(dtype, most, scale, dim):
+    """Values of the type's largest magnitude: a mean of them is no larger, neither by the rounding of
+    the weights nor because a sum of weighted values leaves f32."""
+    s = make([200, 31], [300, 5], n_q=4, n_kv=2, dim=dim, dtype=dtype, seed=15)
+    for x in ("v", "v_pool"):
+        s[x] = torch.full_like(s[x], most)
+        s[x][..., 1::2] = -most
+        s[x][..., 4] = 0.5
+    out = call(s, scale=scale)
+    ref = s["v"][:, :1].expand_as(out)
+    assert bool(((out.double() - ref.double()).abs() <= 2.5 * torch.finfo(dtype).eps * ref.double().abs()).all())
+    assert bool(out.isfinite().all())
+
+
+def test_a_large_value_with_a_large_weight():
+    """bf16 values whose sum of weights times values would leave f32, under scores that grow."""
+    s = make([60], [200], n_q=2, n_kv=1, dim=128, dtype=BF16, seed=16)
+    s["v"] = (s["v"].float() * 1e36).to(BF16)
+    s["v_pool"] = (s["v_pool"].float() * 1e36).to(BF16)
+    check_values(call(s), *attend64(**s))
+    s["v"], s["v_pool"] = (x.float().clamp(-3e36, 3e36).mul(1e2).to(BF16) for x in (s["v"], s["v_pool"]))
+    check_values(call(s), *attend64(**s))
