@@ -896,9 +896,10 @@ template <typename T, int D>
 __device__ __noinline__ void chunk_mend_rows(const ChunkArgs &a, const ChunkWork &w, uint32_t again) {
   const uint32_t warp = threadIdx.x >> 5, row0 = blockIdx.x * kJoinRows, rank = row0 / kRows, tpt = kRows / a.group;
   const Cut &cut = w.cut[blockIdx.y];
+  ChunkKey<T> hint{nullptr, nullptr};
   auto mend = [&](const ChunkStream &s, uint32_t b, uint32_t h, uint32_t t, uint32_t x) {  // row x of the unit at token t
     const uint32_t at = (row0 + x) % kRows, i = t + rank * tpt + at / a.group;
-    if (at / a.group < tpt && i < min(s.count, t + 2 * tpt)) chunk_mend<T, D>(a, s, b, i, h * a.group + at % a.group);
+    if (at / a.group < tpt && i < min(s.count, t + 2 * tpt)) chunk_mend<T, D>(a, s, b, i, h * a.group + at % a.group, hint);
   };
   if (again) {
     const ChunkStream s = chunk_stream(a, cut.b);
@@ -907,6 +908,7 @@ __device__ __noinline__ void chunk_mend_rows(const ChunkArgs &a, const ChunkWork
   }
   const uint2 items = w.bad[2 * blockIdx.y + rank];
   if (items.x >= items.y) return;
+  hint = ChunkKey<T>{nullptr, nullptr};  // (of later tokens than these)
   uint32_t b = cut.run_b, h = cut.run_h, t = cut.run_tok;
   ChunkStream s = chunk_stream(a, b);
   for (uint32_t n = 0; n < items.y; n++) {
@@ -914,6 +916,7 @@ __device__ __noinline__ void chunk_mend_rows(const ChunkArgs &a, const ChunkWork
     t += 2 * tpt;
     if (t < s.count) continue;
     t = 0;
+    hint = ChunkKey<T>{nullptr, nullptr};
     if (++h < a.nkv) continue;
     h = 0;
     do {
